@@ -486,6 +486,32 @@ typedef struct sana_block_args {
 size_t sana_hip_block_scratch_bytes(const sana_block_args* args); /* 0: sizes that cannot be */
 int sana_hip_block(const sana_block_args* args, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Linear attention with a decay for each head (causal), for streams whose memory must not grow:
+ *
+ *   S_t = exp(log_decay[h]) * S_{t-1} + v_t k_t^T,   out_t = scale * S_t q_t,   S [d of v][d of k] per (batch, head),
+ *
+ * the products `v @ k` of the streaming cache (slot "vk" [B][h][d][d] of CachedCausalAttention,
+ * diffusion/model/nets/sana_blocks.py:498-572) with a memory that fades, without a feature map or a denominator (which the
+ * caller applies where a model has them).  A prompt of N tokens, or N = 1: one token of each stream.
+ *   q, k, v, out  [B][N][H*d] views, bf16 or f16; each its own strides (batch, token)
+ *   log_decay     fp32 [H], at most 0 (-inf: no memory)
+ *   state_in      fp32 [B][H][d][d] in front of the first token, or NULL: zeros
+ *   state_out     fp32 [B][H][d][d] behind the last token; may be state_in itself
+ *   lengths       int32 [B] or NULL: entry b has lengths[b] tokens (0 .. N, values outside are clamped); what lies behind is
+ *                 neither read nor written, and a stream of 0 tokens keeps its state
+ *   workspace     at least sana_hip_decay_attention_workspace_bytes(...) bytes, 16-byte aligned (NULL where that is 0)
+ * d % 8 == 0, d <= 128; B * H <= 2^24; q, k, v and the states 16-byte aligned, out 8; token strides from H*d to 2^23 - 1.
+ * The state is summed in fp32 in a fixed order.  out must not overlap q, k or v.  A token's inf or NaN reaches its own
+ * output, later ones, and those of up to 63 tokens in front of it.
+ */
+size_t sana_hip_decay_attention_workspace_bytes(int B, int N, int H, int d);
+int sana_hip_decay_attention(const void* q, const void* k, const void* v, const float* log_decay, const float* state_in,
+                             float* state_out, void* out, const int32_t* lengths, void* workspace, size_t workspace_bytes,
+                             int B, int N, int H, int d, int64_t q_stride_b, int64_t q_stride_n, int64_t k_stride_b,
+                             int64_t k_stride_n, int64_t v_stride_b, int64_t v_stride_n, int64_t o_stride_b,
+                             int64_t o_stride_n, float scale, int io_dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -107,6 +107,10 @@ SIGNATURES = {
                                              c_int64, c_int64, c_int64, c_int64, c_float, c_void_p]),
     "sana_hip_block_scratch_bytes": (c_size_t, [c_void_p]),
     "sana_hip_block": (c_int, [c_void_p, c_void_p]),
+    "sana_hip_decay_attention_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "sana_hip_decay_attention": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                         c_void_p, c_size_t, c_int, c_int, c_int, c_int, c_int64, c_int64, c_int64, c_int64,
+                                         c_int64, c_int64, c_int64, c_int64, c_float, c_int, c_void_p]),
     "sana_hip_layernorm_modulate": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int,
                                             c_int64, c_int64, c_int, c_int64, c_float, c_int, c_void_p]),
 }

@@ -1,0 +1,531 @@
+// Linear attention with a decay for each head, causal, bf16 or f16 in and out, the state in fp32:
+//
+//   S_t = exp(g_h) S_{t-1} + v_t k_t^T,   o_t = scale * S_t q_t,   S [d of v][d of k] per (batch, head).
+//
+// One token (the serving loop) is the recurrence itself: the state is read and written once, nothing else is of any size.
+// A prompt goes in chunks of C = 64 tokens.  With a = exp(g_h), token t of a chunk and S0 the state in front of it,
+//
+//   o_t = scale * (a^(t+1) S0 q_t + sum_{j <= t} a^(t-j) (q_t . k_j) v_j),     S = a^C S0 + sum_j a^(C-1-j) v_j k_j^T:
+//
+// four products of 64 rows on the matrix pipes, 4 C d + 4 d^2 operations a token and head against 8 d bytes of memory.
+#include <type_traits>
+
+#include "common.h"
+
+namespace sana {
+namespace {
+
+constexpr int DC = 64;  // tokens of a chunk
+
+struct DecayArgs {
+  const uint16_t *q, *k, *v;
+  uint16_t* out;
+  const float *log_decay, *state_in;
+  float *state_out, *segments;  // segments: [B * H][nseg][d * d], the states in front of each segment
+  const int* lengths;
+  int N, H, d, nseg, seg_tokens, items;
+  int64_t q_b, q_n, k_b, k_n, v_b, v_n, o_b, o_n;
+  float scale;
+};
+
+// 16-byte slots of an LDS row of DK * 64 bytes are exchanged by a key of the row: 16 consecutive rows of one slot, and the 16 rows of a
+// transposing read, cover all banks.  The key of row 16 i + r is that of r.
+template <int DK>
+__device__ __forceinline__ int dc_key(int row) {
+  return DK == 4 ? (row & 15) : DK == 2 ? ((row >> 1) & 7) : ((row >> 2) & 3);
+}
+__device__ __forceinline__ u32x2_t dc_read_tr(uint32_t lds) {  // 4 tokens x 16 channels -> this lane's channel, 4 tokens
+  typedef short s16x4_t __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(size_t)lds));
+}
+__device__ __forceinline__ u32x4_t dc_read(uint32_t lds) {
+  return *(__attribute__((address_space(3))) const u32x4_t*)(size_t)lds;
+}
+// What this wave wrote to LDS is there and what it reads from there has come; loads from memory stay in flight.
+__device__ __forceinline__ void dc_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+// exp(g) as a power of two; below 2^-256 a decay is 0 in every power but the 0th, and -inf * 0 must not be NaN
+__device__ __forceinline__ float dc_log2(float g) {
+  const float g2 = g * 1.44269504088896341f;
+  return g2 < -256.0f ? -256.0f : g2;
+}
+__device__ __forceinline__ float dc_pow(float g2, int n) { return __builtin_amdgcn_exp2f(g2 * (float)n); }
+// the power of two that takes a maximum to 2^14 .. 2^15 (f16 ends at 2^16), within 2^-90 .. 2^40
+__device__ __forceinline__ float dc_fit(float most) {
+  const int e = (int)((__float_as_uint(most) >> 23) & 255u);  // 255: inf or NaN stay what they are
+  const int f = e == 255 ? 127 : min(max(127 + 14 + 127 - e, 37), 167);
+  return __uint_as_float((uint32_t)f << 23);
+}
+
+// One workgroup takes a (batch, head, segment) through its chunks; NW waves, each of which owns 32 channels of v: their
+// columns of the state stay in its registers (fp32) from chunk to chunk.  The waves share the scores, 64 / NW queries each, through LDS.
+// The operands of the MFMAs (16 x 16 x 32):
+//   scores^T = K Q^T   both from LDS as they lie;
+//   out^T    = S Q^T   S as its own accumulators hold it (row v of the product: lane; a lane's 8 values of k: the accumulators of two
+//                      tiles, whose rows are channels 32 s + 8 g + {0..3} and + {4..7}, by the addresses of the transposing read below);
+//   out^T   += V^T P^T V by transposing reads, P^T from LDS in the key order that these give;
+//   S       += K^T V   both by transposing reads.
+// Roundings: P to 16 bits (as it enters the product).  S and the weighted values a^(C-1-j) v_j enter their products as the sum
+// of two 16-bit values, which keeps the state that is carried at fp32's accuracy (one of 16 bits would leave 2^-9 of each term), f16's
+// second value times 2^11, so that it stays a normal number.  f16 ends at 65504: S goes in scaled by a power of two for each wave, P for each query.
+template <typename T, int DK, int NW, bool OUT>
+__global__ __launch_bounds__(64 * NW, 2) void decay_chunk_kernel(const DecayArgs a) {
+  constexpr int PITCH = DK * 64, TILE = DC * PITCH, KT = 2 * DK;  // LDS row / tensor in bytes; 16-row tiles of k
+  constexpr int NT = 64 * NW, PIECES = DC * DK * 4 / NT;
+  static_assert(DC * DK * 4 % NT == 0 && 4 % NW == 0, "");
+  constexpr int QW = 4 / NW;  // query tiles of a wave
+  constexpr bool F = is_f16<T>;
+  __shared__ __attribute__((aligned(16))) unsigned char smem[(OUT ? 3 : 2) * TILE + (OUT ? DC * 128 + DC * 4 : 0)];
+  const uint32_t sk = (uint32_t)(size_t)(__attribute__((address_space(3))) unsigned char*)smem;
+  const uint32_t sv = sk + TILE, sq = sk + 2 * TILE, sp = sk + 3 * TILE;
+  float* fit = reinterpret_cast<float*>(smem + 3 * TILE + DC * 128);  // f16: the scale of a query's P
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, fr = lane & 15, fg = lane >> 4;
+
+  // neighbouring heads, whose rows share cache lines, on one XCD
+  const int per = (a.items + 7) >> 3, item = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if (item >= a.items) return;
+  const int h = item % a.H, rest = item / a.H, seg = rest % a.nseg, b = rest / a.nseg, d = a.d, bh = b * a.H + h;
+  const int n = a.lengths ? min(max(a.lengths[b], 0), a.N) : a.N;
+  const int first = seg * a.seg_tokens, last = min(n, first + a.seg_tokens);  // (host: seg * seg_tokens < N)
+  if (OUT ? (seg > 0 && first >= n) : first + a.seg_tokens >= n) return;  // nothing of this segment is asked for
+  const float g2 = dc_log2(a.log_decay[h]);
+
+  // ---- the state: st[vt][kt][r] = row v = 32 wave + 16 vt + fr, column k = 32 (kt / 2) + 8 fg + 4 (kt & 1) + r
+  f32x4_t st[2][KT];
+  const float* s0 = !OUT ? nullptr : a.nseg > 1 ? a.segments + ((int64_t)bh * a.nseg + seg) * d * d : a.state_in ? a.state_in + (int64_t)bh * d * d : nullptr;
+#pragma unroll
+  for (int vt = 0; vt < 2; ++vt)
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) {
+      const int v = 32 * wave + 16 * vt + fr, k = 32 * (kt >> 1) + 8 * fg + 4 * (kt & 1);
+      st[vt][kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      if (s0 && v < d && k < d) st[vt][kt] = *reinterpret_cast<const f32x4_t*>(s0 + v * d + k);
+    }
+
+  // ---- what does not change from chunk to chunk
+  float within[OUT ? QW : 1][4][4], since[4];  // scale * a^(t - j) (0 where j > t); scale * a^(t + 1)
+  if constexpr (OUT) {
+#pragma unroll
+    for (int i = 0; i < QW; ++i)
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int apart = 16 * (wave + NW * i) + fr - (16 * kt + 4 * fg + r);
+          within[i][kt][r] = apart >= 0 ? a.scale * dc_pow(g2, apart) : 0.f;
+        }
+#pragma unroll
+    for (int qt = 0; qt < 4; ++qt) since[qt] = a.scale * dc_pow(g2, 16 * qt + fr + 1);
+  }
+  float to_end[2][8];  // a^(C - 1 - t) of the tokens of this lane's transposed values; tokens past the end are zeros
+  auto weights = [&](int count) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) to_end[s][e] = dc_pow(g2, max(count - 1 - (32 * s + 4 * fg + (e & 3) + 16 * (e >> 2)), 0));
+  };
+  weights(DC);
+  float over = dc_pow(g2, DC);
+
+  // ---- a chunk's rows: requested into registers a chunk ahead, then to LDS
+  u32x4_t rk[PIECES], rv[PIECES], rq[OUT ? PIECES : 1];
+  const uint32_t k2 = 2 * (uint32_t)a.k_n, v2 = 2 * (uint32_t)a.v_n, q2 = 2 * (uint32_t)a.q_n;
+  auto request = [&](int at) {
+    const int count = min(last - at, DC);
+    auto rows = [&](const uint16_t* base, uint32_t ld2, u32x4_t* r) {
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base), 0, (int)((uint32_t)(count - 1) * ld2 + 2 * d), 0x00020000);
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        const int idx = tid + NT * i, row = idx / (DK * 4), c = idx - row * (DK * 4);
+        const uint32_t off = 8 * c < d ? (uint32_t)row * ld2 + 16 * c : 0x80000000u;  // (outside: zeros)
+        r[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rs, (int)off, 0, 0));
+      }
+    };
+    rows(a.k + b * a.k_b + (int64_t)at * a.k_n + h * d, k2, rk);
+    rows(a.v + b * a.v_b + (int64_t)at * a.v_n + h * d, v2, rv);
+    if constexpr (OUT) rows(a.q + b * a.q_b + (int64_t)at * a.q_n + h * d, q2, rq);
+  };
+  if (first < last) request(first);
+
+  // ---- this lane's places in LDS
+  const int key = dc_key<DK>(fr);
+  uint32_t row16[DK];  // row fr, k = 32 s + 8 fg
+#pragma unroll
+  for (int s = 0; s < DK; ++s) row16[s] = fr * PITCH + (((4 * s + fg) ^ key) << 4);
+  const int trow = 4 * fg + (fr >> 2), tkey = dc_key<DK>(trow), piece = fr & 3;  // of a transposing read
+  uint32_t vt_at[2], kt_at[DK];
+#pragma unroll
+  for (int vt = 0; vt < 2; ++vt) vt_at[vt] = sv + trow * PITCH + (((2 * (2 * wave + vt) + (piece >> 1)) ^ tkey) << 4) + 8 * (piece & 1);
+#pragma unroll
+  for (int s = 0; s < DK; ++s) kt_at[s] = sk + trow * PITCH + (((4 * s + piece) ^ tkey) << 4);
+  const bool own = 32 * wave < 32 * DK;  // (DK = 3: the fourth wave has no channels of v, and its reads would leave the rows)
+
+#pragma unroll 1
+  for (int at = first; at < last; at += DC) {
+    const int count = min(last - at, DC);
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const int idx = tid + NT * i, row = idx / (DK * 4), c = idx - row * (DK * 4);
+      const uint32_t to = row * PITCH + ((c ^ dc_key<DK>(row)) << 4);
+      *reinterpret_cast<u32x4_t*>(smem + to) = rk[i];
+      *reinterpret_cast<u32x4_t*>(smem + TILE + to) = rv[i];
+      if constexpr (OUT) *reinterpret_cast<u32x4_t*>(smem + 2 * TILE + to) = rq[i];
+    }
+    dc_barrier();
+    if (at + DC < last) request(at + DC);
+    if (count < DC) {
+      weights(count);
+      over = dc_pow(g2, count);
+    }
+    f32x4_t oc[2][4];  // out^T: channel 32 wave + 16 vt + 4 fg + r, query 16 qt + fr
+    u32x4_t vf[2][2];  // values of two ranges of 32 tokens
+    if constexpr (OUT) {
+      // ---- scores, decayed, to LDS: row = query, 16-byte slot 4 s + g = keys 32 s + 4 g + {0..3}, + 16
+#pragma unroll
+      for (int i = 0; i < QW; ++i) {
+        const int qt = wave + NW * i;
+        f32x4_t sc[4];
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt) sc[kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < DK; ++s) {
+          const u32x4_t qf = dc_read(sq + 16 * qt * PITCH + row16[s]);
+#pragma unroll
+          for (int kt = 0; kt < 4; ++kt)
+            if (kt <= qt) sc[kt] = mfma_16x16x32<T>(dc_read(sk + 16 * kt * PITCH + row16[s]), qf, sc[kt]);
+        }
+        float most = 0.f, f = 1.f;
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            sc[kt][r] = 16 * kt + 4 * fg + r <= 16 * qt + fr ? sc[kt][r] * within[i][kt][r] : 0.f;
+            if constexpr (F) most = fmaxf(most, fabsf(sc[kt][r]));
+          }
+        if constexpr (F) {
+          most = fmaxf(most, __shfl_xor(most, 16));
+          most = fmaxf(most, __shfl_xor(most, 32));
+          f = dc_fit(most);
+          if (fg == 0) fit[16 * qt + fr] = f;
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const int q = 16 * qt + fr;
+          u32x4_t p;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const f32x4_t x = sc[2 * s + (e >> 1)];
+            p[e] = F ? pk16<T>(x[2 * (e & 1)] * f, x[2 * (e & 1) + 1] * f) : pk16<T>(x[2 * (e & 1)], x[2 * (e & 1) + 1]);
+          }
+          *reinterpret_cast<u32x4_t*>(smem + 3 * TILE + q * 128 + (((4 * s + fg) ^ ((q >> 1) & 7)) << 4)) = p;
+        }
+      }
+      // ---- the state in front of the chunk
+      float sfit = 1.f;
+      if constexpr (F) {
+        float most = 0.f;
+#pragma unroll
+        for (int vt = 0; vt < 2; ++vt)
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(st[vt][kt][r]));
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) most = fmaxf(most, __shfl_xor(most, m));
+        sfit = dc_fit(most);
+      }
+#pragma unroll
+      for (int vt = 0; vt < 2; ++vt)
+#pragma unroll
+        for (int qt = 0; qt < 4; ++qt) oc[vt][qt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < DK; ++s) {
+        u32x4_t hi[2], lo[2];
+#pragma unroll
+        for (int vt = 0; vt < 2; ++vt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const f32x4_t x = st[vt][2 * s + (e >> 1)];
+            const float x0 = F ? x[2 * (e & 1)] * sfit : x[2 * (e & 1)], x1 = F ? x[2 * (e & 1) + 1] * sfit : x[2 * (e & 1) + 1];
+            hi[vt][e] = pk16<T>(x0, x1);
+            lo[vt][e] = pk16<T>(x0 - lo16<T>(hi[vt][e]), x1 - hi16<T>(hi[vt][e]));
+          }
+#pragma unroll
+        for (int qt = 0; qt < 4; ++qt) {
+          const u32x4_t qf = dc_read(sq + 16 * qt * PITCH + row16[s]);
+#pragma unroll
+          for (int vt = 0; vt < 2; ++vt) {
+            oc[vt][qt] = mfma_16x16x32<T>(hi[vt], qf, oc[vt][qt]);
+            oc[vt][qt] = mfma_16x16x32<T>(lo[vt], qf, oc[vt][qt]);
+          }
+        }
+      }
+      dc_barrier();
+      float pfit[4];
+#pragma unroll
+      for (int qt = 0; qt < 4; ++qt) {
+        pfit[qt] = F ? fit[16 * qt + fr] : 1.f;
+        const float m = F ? since[qt] * pfit[qt] / sfit : since[qt];
+#pragma unroll
+        for (int vt = 0; vt < 2; ++vt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) oc[vt][qt][r] *= m;
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int vt = 0; vt < 2; ++vt) {
+        vf[s][vt] = u32x4_t{0u, 0u, 0u, 0u};
+        if (own) {
+          const u32x2_t x = dc_read_tr(vt_at[vt] + 32 * s * PITCH), y = dc_read_tr(vt_at[vt] + (32 * s + 16) * PITCH);
+          vf[s][vt] = u32x4_t{x.x, x.y, y.x, y.y};
+        }
+      }
+    if constexpr (OUT) {
+      // ---- the scores' part
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int qt = 2 * s; qt < 4; ++qt) {  // (queries of the first 32 see none of the second 32 tokens)
+          const int q = 16 * qt + fr;
+          const u32x4_t pf = dc_read(sp + q * 128 + (((4 * s + fg) ^ ((q >> 1) & 7)) << 4));
+#pragma unroll
+          for (int vt = 0; vt < 2; ++vt) oc[vt][qt] = mfma_16x16x32<T>(vf[s][vt], pf, oc[vt][qt]);
+        }
+      uint16_t* o = a.out + b * a.o_b + (int64_t)at * a.o_n + h * d;
+#pragma unroll
+      for (int qt = 0; qt < 4; ++qt) {
+        const int q = 16 * qt + fr;
+        const float m = F ? 1.0f / fit[q] : 1.f;
+#pragma unroll
+        for (int vt = 0; vt < 2; ++vt) {
+          const int c = 32 * wave + 16 * vt + 4 * fg;
+          const f32x4_t x = oc[vt][qt];
+          if (q < count && c < d)
+            *reinterpret_cast<u32x2_t*>(o + (int64_t)q * a.o_n + c) =
+                F ? u32x2_t{pk16<T>(x[0] * m, x[1] * m), pk16<T>(x[2] * m, x[3] * m)} : u32x2_t{pk16<T>(x[0], x[1]), pk16<T>(x[2], x[3])};
+        }
+      }
+    }
+    // ---- the state behind the chunk
+    if (own) {
+      u32x4_t hi[2][2], lo[2][2];
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int vt = 0; vt < 2; ++vt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x0 = lo16<T>(vf[s][vt][e]) * to_end[s][2 * e], x1 = hi16<T>(vf[s][vt][e]) * to_end[s][2 * e + 1];
+            hi[s][vt][e] = pk16<T>(x0, x1);
+            const float y0 = x0 - lo16<T>(hi[s][vt][e]), y1 = x1 - hi16<T>(hi[s][vt][e]);
+            lo[s][vt][e] = F ? pk16<T>(y0 * 2048.f, y1 * 2048.f) : pk16<T>(y0, y1);
+          }
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) {
+        u32x4_t kf[2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const uint32_t from = kt_at[kt >> 1] + 8 * (kt & 1) + 32 * s * PITCH;
+          const u32x2_t x = dc_read_tr(from), y = dc_read_tr(from + 16 * PITCH);
+          kf[s] = u32x4_t{x.x, x.y, y.x, y.y};
+        }
+#pragma unroll
+        for (int vt = 0; vt < 2; ++vt) {
+          f32x4_t x = st[vt][kt];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[r] *= over;
+          if constexpr (F) {
+            f32x4_t y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+              x = mfma_16x16x32<T>(kf[s], hi[s][vt], x);
+              y = mfma_16x16x32<T>(kf[s], lo[s][vt], y);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[r] = fmaf(y[r], 1.0f / 2048.f, x[r]);
+          } else {
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+              x = mfma_16x16x32<T>(kf[s], hi[s][vt], x);
+              x = mfma_16x16x32<T>(kf[s], lo[s][vt], x);
+            }
+          }
+          st[vt][kt] = x;
+        }
+      }
+    }
+    dc_barrier();
+  }
+  // ---- the state behind the last token: of the whole stream, or of this segment
+  float* to = !OUT ? a.segments + ((int64_t)bh * a.nseg + seg) * d * d : last == n ? a.state_out + (int64_t)bh * d * d : nullptr;
+  if (to)
+#pragma unroll
+    for (int vt = 0; vt < 2; ++vt)
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) {
+        const int v = 32 * wave + 16 * vt + fr, k = 32 * (kt >> 1) + 8 * fg + 4 * (kt & 1);
+        if (v < d && k < d) *reinterpret_cast<f32x4_t*>(to + v * d + k) = st[vt][kt];
+      }
+}
+
+// The segments' own sums -> the states in front of them: run = S0; run = a^L run + sum_s.  Four values a thread.
+__global__ __launch_bounds__(256) void decay_scan_kernel(const DecayArgs a) {
+  const int bh = blockIdx.y, b = bh / a.H, i = blockIdx.x * 256 + threadIdx.x, dd4 = a.d * a.d / 4;
+  if (i >= dd4) return;
+  const int n = a.lengths ? min(max(a.lengths[b], 0), a.N) : a.N;
+  const float over = dc_pow(dc_log2(a.log_decay[bh % a.H]), a.seg_tokens);
+  f32x4_t* s = reinterpret_cast<f32x4_t*>(a.segments) + (int64_t)bh * a.nseg * dd4 + i;
+  f32x4_t run = {0.f, 0.f, 0.f, 0.f};
+  if (a.state_in) run = reinterpret_cast<const f32x4_t*>(a.state_in)[(int64_t)bh * dd4 + i];
+  for (int seg = 0;; ++seg) {
+    const bool more = seg + 1 < a.nseg && (int64_t)(seg + 1) * a.seg_tokens < n;
+    const f32x4_t own = more ? s[(int64_t)seg * dd4] : f32x4_t{0.f, 0.f, 0.f, 0.f};
+    s[(int64_t)seg * dd4] = run;
+    if (!more) break;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) run[r] = fmaf(run[r], over, own[r]);
+  }
+}
+
+// One token of each stream.  A row of the state is d floats in LPR lanes of four; a wave holds 64 / LPR rows at a time.
+template <typename T, int LPR>
+__global__ __launch_bounds__(256) void decay_step_kernel(const DecayArgs a) {
+  constexpr int RW = 64 / LPR;  // rows of a wave
+  const int bh = blockIdx.x, b = bh / a.H, h = bh - b * a.H, d = a.d;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = 4 * (lane % LPR);
+  const bool idle = a.lengths && a.lengths[b] <= 0;
+  const float decay = idle ? 1.f : dc_pow(dc_log2(a.log_decay[h]), 1);
+  const uint16_t *qp = a.q + b * a.q_b + h * d, *kp = a.k + b * a.k_b + h * d, *vp = a.v + b * a.v_b + h * d;
+  uint16_t* op = a.out + b * a.o_b + h * d;
+  float q[4], k[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) q[e] = k[e] = 0.f;
+  if (c < d && !idle) {
+    const u32x2_t x = *reinterpret_cast<const u32x2_t*>(qp + c), y = *reinterpret_cast<const u32x2_t*>(kp + c);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      q[2 * e] = a.scale * lo16<T>(x[e]), q[2 * e + 1] = a.scale * hi16<T>(x[e]);
+      k[2 * e] = lo16<T>(y[e]), k[2 * e + 1] = hi16<T>(y[e]);
+    }
+  }
+  const int64_t base = (int64_t)bh * d * d;
+  for (int row = (blockIdx.y * 4 + wave) * RW + lane / LPR; row - lane / LPR < d; row += 4 * RW * gridDim.y) {
+    f32x4_t s = {0.f, 0.f, 0.f, 0.f};
+    const bool in = row < d && c < d;
+    if (in && a.state_in) s = *reinterpret_cast<const f32x4_t*>(a.state_in + base + row * d + c);
+    float v = 0.f;
+    if (row < d && !idle) v = lo16<T>(vp[row]);
+    float o = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      s[e] = fmaf(decay, s[e], v * k[e]);
+      o = fmaf(q[e], s[e], o);
+    }
+#pragma unroll
+    for (int m = 1; m < LPR; m <<= 1) o += __shfl_xor(o, m);
+    if (in) *reinterpret_cast<f32x4_t*>(a.state_out + base + row * d + c) = s;
+    if (row < d && c == 0 && !idle) op[row] = (uint16_t)pk16<T>(o, 0.f);
+  }
+}
+
+// Segments of a stream: none for a state alone; otherwise whole chunks.
+int segment_count(int B, int N, int H, int* tokens) {
+  const int chunks = (N + DC - 1) / DC;
+  const int64_t heads = (int64_t)B * H;
+  int want = 1;
+  if (heads < 256 && chunks >= 16) want = (int)((512 + heads - 1) / heads);
+  want = want > chunks / 4 ? (chunks / 4 > 1 ? chunks / 4 : 1) : want;
+  const int per = (chunks + want - 1) / want;
+  *tokens = per * DC;
+  return (chunks + per - 1) / per;
+}
+
+template <typename T, int DK, int NW>
+int launch_chunks(const DecayArgs& a, int B, hipStream_t s) {
+  const int64_t items = (int64_t)B * a.H * a.nseg;
+  if (items > 0x7ffffff0) return SANA_ERR_SHAPE;
+  DecayArgs args = a;
+  args.items = (int)items;
+  const dim3 grid((unsigned)((items + 7) / 8 * 8)), block(64 * NW);
+  if (a.nseg > 1) {
+    hipLaunchKernelGGL((decay_chunk_kernel<T, DK, NW, false>), grid, block, 0, s, args);
+    hipLaunchKernelGGL(decay_scan_kernel, dim3((unsigned)((a.d * a.d / 4 + 255) / 256), (unsigned)(B * a.H)), dim3(256), 0, s, args);
+  }
+  hipLaunchKernelGGL((decay_chunk_kernel<T, DK, NW, true>), grid, block, 0, s, args);
+  return hipGetLastError() == hipSuccess ? SANA_OK : SANA_ERR_LAUNCH;
+}
+
+template <typename T>
+int launch_step(const DecayArgs& a, int B, hipStream_t s) {
+  const dim3 grid((unsigned)(B * a.H), a.d > 64 ? 2 : 1), block(256);
+  if (a.d > 64) hipLaunchKernelGGL((decay_step_kernel<T, 32>), grid, block, 0, s, a);
+  else if (a.d > 32) hipLaunchKernelGGL((decay_step_kernel<T, 16>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((decay_step_kernel<T, 8>), grid, block, 0, s, a);
+  return hipGetLastError() == hipSuccess ? SANA_OK : SANA_ERR_LAUNCH;
+}
+
+template <typename T>
+int decay_attention(const DecayArgs& a, int B, hipStream_t s) {
+  if (a.N == 1) return launch_step<T>(a, B, s);
+  if (a.d <= 32) return launch_chunks<T, 1, 1>(a, B, s);
+  if (a.d <= 64) return launch_chunks<T, 2, 2>(a, B, s);
+  if (a.d <= 96) return launch_chunks<T, 3, 4>(a, B, s);
+  return launch_chunks<T, 4, 4>(a, B, s);
+}
+
+}  // namespace
+}  // namespace sana
+
+using namespace sana;
+
+#define SANA_API extern "C" __attribute__((visibility("default")))
+
+SANA_API size_t sana_hip_decay_attention_workspace_bytes(int B, int N, int H, int d) {
+  if (B <= 0 || N <= 1 || H <= 0 || d <= 0 || d > 128 || (int64_t)B * H > (1 << 24)) return 0;
+  int tokens;
+  const int nseg = segment_count(B, N, H, &tokens);
+  return nseg > 1 ? (size_t)B * H * nseg * d * d * sizeof(float) : 0;
+}
+
+SANA_API int sana_hip_decay_attention(const void* q, const void* k, const void* v, const float* log_decay, const float* state_in,
+                                      float* state_out, void* out, const int32_t* lengths, void* workspace, size_t workspace_bytes,
+                                      int B, int N, int H, int d, int64_t q_stride_b, int64_t q_stride_n, int64_t k_stride_b,
+                                      int64_t k_stride_n, int64_t v_stride_b, int64_t v_stride_n, int64_t o_stride_b,
+                                      int64_t o_stride_n, float scale, int io_dtype, void* stream) {
+  if (!q || !k || !v || !log_decay || !state_out || !out || B <= 0 || N <= 0 || H <= 0 || d <= 0) return SANA_ERR_ARG;
+  if (io_dtype != SANA_DT_BF16 && io_dtype != SANA_DT_F16) return SANA_ERR_DTYPE;
+  if (d % 8 || d > 128 || (int64_t)B * H > (1 << 24) || N > (1 << 30)) return SANA_ERR_SHAPE;
+  for (const int64_t ld : {q_stride_n, k_stride_n, v_stride_n, o_stride_n}) {
+    if (ld < (int64_t)H * d) return SANA_ERR_ARG;
+    if (ld >= (1 << 23)) return SANA_ERR_SHAPE;  // 32-bit byte offsets within a chunk
+  }
+  for (const int64_t sb : {q_stride_b, k_stride_b, v_stride_b, o_stride_b})
+    if (sb < 0) return SANA_ERR_ARG;
+  for (const void* p : {q, k, v, (const void*)state_in, (const void*)state_out})
+    if (!aligned16(p)) return SANA_ERR_ALIGN;
+  for (const int64_t st : {q_stride_b, q_stride_n, k_stride_b, k_stride_n, v_stride_b, v_stride_n})
+    if (st % 8) return SANA_ERR_ALIGN;
+  if ((reinterpret_cast<uintptr_t>(out) & 7u) || o_stride_b % 4 || o_stride_n % 4 || (reinterpret_cast<uintptr_t>(log_decay) & 3u) ||
+      (reinterpret_cast<uintptr_t>(lengths) & 3u))
+    return SANA_ERR_ALIGN;
+  DecayArgs a;
+  a.q = static_cast<const uint16_t*>(q), a.k = static_cast<const uint16_t*>(k), a.v = static_cast<const uint16_t*>(v);
+  a.out = static_cast<uint16_t*>(out);
+  a.log_decay = log_decay, a.state_in = state_in, a.state_out = state_out, a.segments = nullptr, a.lengths = lengths;
+  a.N = N, a.H = H, a.d = d, a.nseg = 1, a.seg_tokens = N, a.items = 0;
+  a.q_b = q_stride_b, a.q_n = q_stride_n, a.k_b = k_stride_b, a.k_n = k_stride_n, a.v_b = v_stride_b, a.v_n = v_stride_n;
+  a.o_b = o_stride_b, a.o_n = o_stride_n, a.scale = scale;
+  if (N > 1) a.nseg = segment_count(B, N, H, &a.seg_tokens);
+  if (a.nseg > 1) {
+    if (!workspace || workspace_bytes < sana_hip_decay_attention_workspace_bytes(B, N, H, d)) return SANA_ERR_WORKSPACE;
+    if (!aligned16(workspace)) return SANA_ERR_ALIGN;
+    a.segments = static_cast<float*>(workspace);
+  }
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return io_dtype == SANA_DT_F16 ? decay_attention<F16>(a, B, s) : decay_attention<BF16>(a, B, s);
+}

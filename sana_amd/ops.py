@@ -870,3 +870,97 @@ def gate_residual(y: torch.Tensor, gate: torch.Tensor, residual: torch.Tensor) -
                                               ldy, ldr, C, Ntok // groups, gstride, _dt(y), _stream())
     _lib.check(code, "sana_hip_gate_residual")
     return out.view(B, Ntok, C)
+
+
+# --------------------------------------------------------------------------- streams whose memory does not grow
+
+def _here(first: torch.Tensor, others, what: str) -> int:
+    """The device index of ``first``, on which all tensors of the call have to be (None entries aside)."""
+    _need_cuda(first, *others)
+    dev = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            raise SanaHipError(f"{what}: all tensors must be on one device")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (first, *others)):
+        raise SanaHipError(f"{what} is forward only: call it under torch.no_grad() or on detached tensors")
+    return dev
+
+
+def _token_rows(t: torch.Tensor, what: str) -> Tuple[int, int]:
+    """:func:`_token_major_view` of [B, N, C] whose strides along axes of length 1 say nothing."""
+    sb, sn = _token_major_view(t, what) if t.shape[2] != 1 else (t.stride(0), t.stride(1))
+    return (sb if t.shape[0] > 1 else 0), (sn if t.shape[1] > 1 else t.shape[2])
+
+
+def _lengths_arg(t: Optional[torch.Tensor], B: int, what: str = "lengths") -> Optional[int]:
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or tuple(t.shape) != (B,) or not t.is_contiguous():
+        raise SanaHipError(f"{what} must be contiguous int32 [{B}], got {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _call_scratch(device: torch.device, nbytes: int) -> Optional[torch.Tensor]:
+    """Scratch that holds nothing between calls: the stream's buffer, or, under capture and where it is too large to be kept,
+    one of this call's own (graphs that are captured on one stream and replayed side by side must not share it)."""
+    if nbytes and (nbytes > STATE_SCRATCH_KEPT or torch._C._cuda_isCurrentStreamCapturing()):
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return _workspace(device, nbytes)
+
+
+def decay_linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, scale: float = 1.0,
+                           state: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
+                           out: Optional[torch.Tensor] = None,
+                           state_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Causal linear attention with a decay for each head: ``S_t = exp(log_decay[h]) S_{t-1} + v_t k_t^T``,
+    ``out_t = scale * S_t q_t``.  q, k, v: [B, N, C] token-major views, bf16 or fp16 of one dtype; log_decay: fp32 [H], at
+    most 0, C = H * head_dim, head_dim a multiple of 8 up to 128.  Many tokens run in chunks, N = 1 as the recurrence itself
+    (a serving loop's token).
+
+    ``state``: fp32 [B, H, d, d] (rows of v, columns of k) in front of the first token, None for zeros.  Returns
+    (out [B, N, C], the state behind the last token); ``state_out`` receives the latter and may be ``state`` itself, else
+    it is a new tensor.  ``lengths``: int32 [B] on the device, the tokens that each batch entry really has (clamped to 0 .. N);
+    rows behind them are not read, and stay in ``out`` as they were (zeros in a new one); an entry without tokens
+    keeps its state.  ``out`` must not overlap the inputs.  Forward only."""
+    dev = _here(q, (k, v, log_decay, state, lengths, out, state_out), "decay_linear_attention")
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            return decay_linear_attention(q, k, v, log_decay, scale, state, lengths, out, state_out)
+    if q.dim() != 3 or q.dtype not in IO16 or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise SanaHipError(f"decay_linear_attention needs bf16 or fp16 q, k and v [B, N, C] of one dtype, got {q.dtype}, {k.dtype}, {v.dtype}")
+    if k.shape != q.shape or v.shape != q.shape:
+        raise SanaHipError(f"q, k and v must share their shape: {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    B, N, C = q.shape
+    H = log_decay.numel()
+    if log_decay.dtype != torch.float32 or log_decay.dim() != 1 or not log_decay.is_contiguous() or H == 0 or C % H:
+        raise SanaHipError(f"log_decay must be contiguous fp32 [H] with H dividing C={C}, got {log_decay.dtype} {tuple(log_decay.shape)}")
+    d = C // H
+    if d % 8 or not 0 < d <= 128:
+        raise SanaHipError(f"head_dim {d} has no kernel (multiples of 8 up to 128)")
+    for name, t in (("state", state), ("state_out", state_out)):
+        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (B, H, d, d) or not t.is_contiguous()):
+            raise SanaHipError(f"{name} must be contiguous fp32 {(B, H, d, d)}, got {t.dtype} {tuple(t.shape)}")
+    length_ptr = _lengths_arg(lengths, B)
+    if out is None:
+        out = (torch.empty if lengths is None else torch.zeros)((B, N, C), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise SanaHipError("out has the wrong shape or dtype")
+    if state_out is None:
+        state_out = torch.empty((B, H, d, d), dtype=torch.float32, device=q.device)
+    if B * N == 0:
+        if state is None:
+            state_out.zero_()
+        elif state_out is not state:
+            state_out.copy_(state)
+        return out, state_out
+    strides = [s for t, name in ((q, "q"), (k, "k"), (v, "v"), (out, "out")) for s in _token_rows(t, name)]
+    lib = _lib.load()
+    nbytes = lib.sana_hip_decay_attention_workspace_bytes(B, N, H, d) if N > 1 else 0
+    ws = _call_scratch(q.device, nbytes)
+    code = lib.sana_hip_decay_attention(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), None if state is None else state.data_ptr(),
+        state_out.data_ptr(), out.data_ptr(), length_ptr, None if ws is None else ws.data_ptr(), nbytes, B, N, H, d, *strides,
+        float(scale), _DT[q.dtype], _stream())
+    if code:
+        _lib.check(code, "sana_hip_decay_attention")
+    return out, state_out
