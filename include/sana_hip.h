@@ -512,6 +512,48 @@ int sana_hip_decay_attention(const void* q, const void* k, const void* v, const 
                              int64_t k_stride_n, int64_t v_stride_b, int64_t v_stride_n, int64_t o_stride_b,
                              int64_t o_stride_n, float scale, int io_dtype, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Softmax attention over a sliding window and the first tokens (sinks), causal; key heads may be shared (H % Hkv == 0).
+ * The query at position p sees key j where j <= p and (p - j < window or j < sinks).  The queries are the last N of the Nk
+ * keys: query i is at position Nk - N + i.  (Of a longer past only the sinks and the window - 1 keys in front of the first query
+ * need to be among the rows, in order.)  The softmax core that the `flash` blocks take from
+ * F.scaled_dot_product_attention (diffusion/model/nets/sana_blocks.py:86-92), for streams whose memory must not grow.
+ *   q, out  [B][N][H*d] views, k, v [B][Nk][Hkv*d] views, bf16 or f16; each its own strides (batch, token)
+ *   lengths int32 [B] or NULL: entry b has lengths[b] queries (0 .. N, values outside are clamped) and the keys up to its last;
+ *           what lies behind is neither read nor written
+ *   workspace  at least sana_hip_window_attention_workspace_bytes(...) bytes, 16-byte aligned (NULL where that is 0): few queries
+ *           of many keys are split over the keys
+ * scale > 0; window >= 1; d % 8 == 0, d <= 128; q, k, v 16-byte aligned, out 8; token strides of k and v below 2^23.
+ * Probabilities are rounded to the io dtype before they multiply v; maxima, sums and outputs are fp32.  A key whose value is
+ * inf or NaN may reach the queries that see any of the 64 aligned keys around it.
+ */
+size_t sana_hip_window_attention_workspace_bytes(int B, int N, int Nk, int H, int d, int window, int sinks);
+int sana_hip_window_attention(const void* q, const void* k, const void* v, void* out, const int32_t* lengths, void* workspace,
+                              size_t workspace_bytes, int B, int N, int Nk, int H, int Hkv, int d, int window, int sinks,
+                              int64_t q_stride_b, int64_t q_stride_n, int64_t k_stride_b, int64_t k_stride_n,
+                              int64_t v_stride_b, int64_t v_stride_n, int64_t o_stride_b, int64_t o_stride_n, float scale,
+                              int io_dtype, void* stream);
+
+/* The cache of such a stream: sinks + window rows of keys and of values; the token at position p is row p for p < sinks, else
+ * row sinks + (p - sinks) % window.  Appends N new tokens (lengths[b] of them) at positions[b], positions[b] + 1, ...
+ *   cache_k, cache_v [B][sinks + window][C], k, v [B][N][C] views, 16-bit; C % 8 == 0, all 16-byte aligned; B <= 65535
+ *   positions int32 [B]: tokens that the stream has seen before; negative: an idle stream, nothing is written
+ * Rows of positions that hold no token yet, and tokens that later ones of the call push out, are not written. */
+int sana_hip_window_cache_append(void* cache_k, void* cache_v, const void* k, const void* v, const int32_t* positions,
+                                 const int32_t* lengths, int B, int N, int C, int window, int sinks, int64_t ck_stride_b,
+                                 int64_t ck_stride_n, int64_t cv_stride_b, int64_t cv_stride_n, int64_t k_stride_b,
+                                 int64_t k_stride_n, int64_t v_stride_b, int64_t v_stride_n, int io_dtype, void* stream);
+
+/* One token of each stream: its key and value go into the cache as above (position positions[b]), and its queries attend to
+ * what the cache then holds.  q, out [B][H*d] rows, k, v [B][Hkv*d] rows; an idle stream (negative position) gets zeros and its
+ * cache is left alone.  Workspace, types and alignment as in sana_hip_window_attention. */
+size_t sana_hip_window_step_workspace_bytes(int B, int H, int Hkv, int d, int window, int sinks);
+int sana_hip_window_step(const void* q, const void* k, const void* v, void* cache_k, void* cache_v, const int32_t* positions,
+                         void* out, void* workspace, size_t workspace_bytes, int B, int H, int Hkv, int d, int window,
+                         int sinks, int64_t q_stride_b, int64_t k_stride_b, int64_t v_stride_b, int64_t ck_stride_b,
+                         int64_t ck_stride_n, int64_t cv_stride_b, int64_t cv_stride_n, int64_t o_stride_b, float scale,
+                         int io_dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -111,6 +111,17 @@ SIGNATURES = {
     "sana_hip_decay_attention": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                          c_void_p, c_size_t, c_int, c_int, c_int, c_int, c_int64, c_int64, c_int64, c_int64,
                                          c_int64, c_int64, c_int64, c_int64, c_float, c_int, c_void_p]),
+    "sana_hip_window_attention_workspace_bytes": (c_size_t, [c_int] * 7),
+    "sana_hip_window_attention": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
+                                          c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int64, c_int64, c_int64,
+                                          c_int64, c_int64, c_int64, c_int64, c_int64, c_float, c_int, c_void_p]),
+    "sana_hip_window_cache_append": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                             c_int, c_int, c_int, c_int, c_int, c_int64, c_int64, c_int64, c_int64, c_int64,
+                                             c_int64, c_int64, c_int64, c_int, c_void_p]),
+    "sana_hip_window_step_workspace_bytes": (c_size_t, [c_int] * 6),
+    "sana_hip_window_step": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
+                                     c_int, c_int, c_int, c_int, c_int, c_int, c_int64, c_int64, c_int64, c_int64, c_int64,
+                                     c_int64, c_int64, c_int64, c_float, c_int, c_void_p]),
     "sana_hip_layernorm_modulate": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int,
                                             c_int64, c_int64, c_int, c_int64, c_float, c_int, c_void_p]),
 }

@@ -68,9 +68,10 @@ __device__ __forceinline__ float dc_fit(float most) {
 //                      tiles, whose rows are channels 32 s + 8 g + {0..3} and + {4..7}, by the addresses of the transposing read below);
 //   out^T   += V^T P^T V by transposing reads, P^T from LDS in the key order that these give;
 //   S       += K^T V   both by transposing reads.
-// Roundings: P to 16 bits (as it enters the product).  S and the weighted values a^(C-1-j) v_j enter their products as the sum
-// of two 16-bit values, which keeps the state that is carried at fp32's accuracy (one of 16 bits would leave 2^-9 of each term), f16's
-// second value times 2^11, so that it stays a normal number.  f16 ends at 65504: S goes in scaled by a power of two for each wave, P for each query.
+// Roundings: P to 16 bits, as it enters its product.  S enters its product with q as the sum of two 16-bit values.  The weighted values
+// a^(C-1-j) v_j enter theirs as the sum of three bf16 values or two f16 ones (22 bits and more: the state that is carried keeps
+// fp32's accuracy; of a 32760-token stream it is 1.3e-6 off with two bf16 values), f16's second value times 2^11, so that it stays a
+// normal number.  f16 ends at 65504: S goes in scaled by a power of two for each wave, P for each query.
 template <typename T, int DK, int NW, bool OUT>
 __global__ __launch_bounds__(64 * NW, 2) void decay_chunk_kernel(const DecayArgs a) {
   constexpr int PITCH = DK * 64, TILE = DC * PITCH, KT = 2 * DK;  // LDS row / tensor in bytes; 16-row tiles of k
@@ -313,49 +314,44 @@ __global__ __launch_bounds__(64 * NW, 2) void decay_chunk_kernel(const DecayArgs
     }
     // ---- the state behind the chunk
     if (own) {
-      u32x4_t hi[2][2], lo[2][2];
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
+      for (int s = 0; s < 2; ++s) {
+        constexpr int TERMS = F ? 2 : 3;
+        u32x4_t w[TERMS][2];
 #pragma unroll
         for (int vt = 0; vt < 2; ++vt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float x0 = lo16<T>(vf[s][vt][e]) * to_end[s][2 * e], x1 = hi16<T>(vf[s][vt][e]) * to_end[s][2 * e + 1];
-            hi[s][vt][e] = pk16<T>(x0, x1);
-            const float y0 = x0 - lo16<T>(hi[s][vt][e]), y1 = x1 - hi16<T>(hi[s][vt][e]);
-            lo[s][vt][e] = F ? pk16<T>(y0 * 2048.f, y1 * 2048.f) : pk16<T>(y0, y1);
+            float x0 = lo16<T>(vf[s][vt][e]) * to_end[s][2 * e], x1 = hi16<T>(vf[s][vt][e]) * to_end[s][2 * e + 1];
+#pragma unroll
+            for (int i = 0; i < TERMS; ++i) {
+              w[i][vt][e] = pk16<T>(x0, x1);
+              x0 -= lo16<T>(w[i][vt][e]), x1 -= hi16<T>(w[i][vt][e]);
+              if constexpr (F) x0 *= 2048.f, x1 *= 2048.f;
+            }
           }
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt) {
-        u32x4_t kf[2];
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
+        for (int kt = 0; kt < KT; ++kt) {
           const uint32_t from = kt_at[kt >> 1] + 8 * (kt & 1) + 32 * s * PITCH;
-          const u32x2_t x = dc_read_tr(from), y = dc_read_tr(from + 16 * PITCH);
-          kf[s] = u32x4_t{x.x, x.y, y.x, y.y};
-        }
+          const u32x2_t lo = dc_read_tr(from), hi = dc_read_tr(from + 16 * PITCH);
+          const u32x4_t kf = {lo.x, lo.y, hi.x, hi.y};
 #pragma unroll
-        for (int vt = 0; vt < 2; ++vt) {
-          f32x4_t x = st[vt][kt];
+          for (int vt = 0; vt < 2; ++vt) {
+            f32x4_t x = st[vt][kt];
+            if (s == 0)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) x[r] *= over;
-          if constexpr (F) {
-            f32x4_t y = {0.f, 0.f, 0.f, 0.f};
+              for (int r = 0; r < 4; ++r) x[r] *= over;
+            if constexpr (F) {
+              const f32x4_t y = mfma_16x16x32<T>(kf, w[1][vt], f32x4_t{0.f, 0.f, 0.f, 0.f});
+              x = mfma_16x16x32<T>(kf, w[0][vt], x);
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-              x = mfma_16x16x32<T>(kf[s], hi[s][vt], x);
-              y = mfma_16x16x32<T>(kf[s], lo[s][vt], y);
+              for (int r = 0; r < 4; ++r) x[r] = fmaf(y[r], 1.0f / 2048.f, x[r]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < TERMS; ++i) x = mfma_16x16x32<T>(kf, w[i][vt], x);
             }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) x[r] = fmaf(y[r], 1.0f / 2048.f, x[r]);
-          } else {
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-              x = mfma_16x16x32<T>(kf[s], hi[s][vt], x);
-              x = mfma_16x16x32<T>(kf[s], lo[s][vt], x);
-            }
+            st[vt][kt] = x;
           }
-          st[vt][kt] = x;
         }
       }
     }

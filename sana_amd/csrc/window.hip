@@ -1,0 +1,646 @@
+// Softmax attention over a sliding window and a few first tokens (sinks), causal, bf16 or f16; key heads may be shared by
+// several query heads.  Query at position p sees key j where j <= p and (p - j < window or j < sinks):
+//
+//   out_p = sum_j softmax_j(scale * q_p . k_j) v_j
+//
+// in one pass over the keys with a running maximum m and sum l: of a block of scores s (in powers of two, scale * log2(e) inside),
+// m' = max(m, max s), p = 2^(s - m'), l' = 2^(m - m') l + sum p, o' = 2^(m - m') o + p v; out = o / l.
+// What a stream keeps of its past is a cache of sinks + window rows: row p for a position p below the sinks, then a ring.
+// The order of the keys does not matter to the sum, so a token's attention reads the rows as they lie.
+#include <initializer_list>
+
+#include "common.h"
+
+namespace sana {
+namespace {
+
+constexpr int WK = 64;            // keys of a tile
+constexpr int WA_MAX_SPLITS = 32;  // parts that the keys of a query are split into
+
+struct WindowArgs {
+  const uint16_t *q, *k, *v;
+  uint16_t *out, *cache_k, *cache_v;
+  const int *lengths, *positions;
+  float *part_o, *part_ml;  // parts: [splits][B * N * H][d] and [splits][B * N * H][2] (maximum, sum)
+  int B, N, Nk, H, Hkv, d, window, sinks, splits, qblocks, items;
+  int64_t q_b, q_n, k_b, k_n, v_b, v_n, o_b, o_n, ck_b, ck_n, cv_b, cv_n;
+  float scale_log2e;
+};
+
+// 16-byte slots of an LDS row of DK * 64 bytes are exchanged by a key of the row: 16 consecutive rows of one slot, and the 16 rows of a
+// transposing read, cover all banks.  The key of row 16 i + r is that of r.
+template <int DK>
+__device__ __forceinline__ int wa_key(int row) {
+  return DK == 4 ? (row & 15) : DK == 2 ? ((row >> 1) & 7) : ((row >> 2) & 3);
+}
+__device__ __forceinline__ u32x2_t wa_read_tr(uint32_t lds) {  // 4 keys x 16 channels -> this lane's channel, 4 keys
+  typedef short s16x4_t __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(size_t)lds));
+}
+__device__ __forceinline__ u32x4_t wa_read(uint32_t lds) {
+  return *(__attribute__((address_space(3))) const u32x4_t*)(size_t)lds;
+}
+// What this wave wrote to LDS is there and what it reads from there has come; loads from memory stay in flight.
+__device__ __forceinline__ void wa_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+template <typename T> inline constexpr float kShift = is_f16<T> ? 6.f : 0.f;
+__device__ __forceinline__ float wa_max_groups(float x) {  // over the four lane groups that share a query
+  x = fmaxf(x, __shfl_xor(x, 16));
+  return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ float wa_sum_groups(float x) {
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
+}
+
+// A prompt or a chunk: the queries are the last N of Nk keys.  A workgroup takes NW * 16 * QT queries of one head through its
+// tiles of 64 keys, the tiles of the sinks first; K and V go to LDS through registers, a tile ahead.  scores^T = K Q^T: a lane
+// owns a query (its column) and four keys of every 16; the probabilities are fed back from the accumulators, V by transposing reads in the
+// order of keys that this gives.  The running maximum moves only when some score is 2^8 above it: until then p <= 2^8 and
+// nothing is rescaled (the 16-bit p keeps its relative step, l and o are fp32).  f16: p times 2^6, the small ones away from its
+// subnormal numbers.
+template <typename T, int DK, int DT, int QT, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void window_attn_kernel(const WindowArgs a) {
+  constexpr int PITCH = DK * 64, TILE = WK * PITCH, NT = 64 * NW, PIECES = WK * DK * 4 / NT, QB = NW * 16 * QT;
+  static_assert(WK * DK * 4 % NT == 0 && DT <= 2 * DK, "");
+  __shared__ __attribute__((aligned(16))) unsigned char smem[4 * TILE];  // two buffers of K, V
+  const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) unsigned char*)smem;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, fr = lane & 15, fg = lane >> 4;
+
+  // the blocks of one head, which read the same keys, on one XCD
+  const int per = (a.items + 7) >> 3, item = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per || item >= a.items) return;
+  const int split = item % a.splits, r1 = item / a.splits, qb = a.qblocks - 1 - r1 % a.qblocks, bh = r1 / a.qblocks;
+  const int b = bh / a.H, h = bh - b * a.H, hk = h / (a.H / a.Hkv), d = a.d;
+  const int queries = a.lengths ? min(max(a.lengths[b], 0), a.N) : a.N;  // that there are
+  const int q0 = qb * QB;
+  if (q0 >= queries) return;
+  const int past = a.Nk - a.N, keys = past + queries;
+  const int p0 = past + q0, p1 = past + min(q0 + QB, queries) - 1;  // positions of the block
+  const int band = max(p0 - a.window + 1, 0);                       // first key of any window
+  // tiles: those of the sinks, then from the band's first on
+  const int last_tile = p1 / WK, sink_tiles = min((a.sinks + WK - 1) / WK, last_tile + 1);
+  const int band_tile = max(band / WK, sink_tiles), tiles = sink_tiles + max(last_tile + 1 - band_tile, 0);
+  const int t0 = (int)((int64_t)tiles * split / a.splits), t1 = (int)((int64_t)tiles * (split + 1) / a.splits);
+
+  // ---- queries: column operand, lane -> query fr, k = 32 s + 8 fg .. + 7
+  const int w0 = q0 + 16 * QT * wave;  // this wave's first query
+  u32x4_t qf[QT][DK];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const uint16_t* row = a.q + b * a.q_b + (int64_t)min(w0 + 16 * t + fr, queries - 1) * a.q_n + h * d;
+#pragma unroll
+    for (int s = 0; s < DK; ++s) {
+      qf[t][s] = *reinterpret_cast<const u32x4_t*>(row + (32 * s + 8 * fg < d ? 32 * s + 8 * fg : 0));
+      if (32 * s + 8 * fg >= d) qf[t][s] = u32x4_t{0u, 0u, 0u, 0u};
+    }
+  }
+  const int wp0 = past + w0, wp1 = min(wp0 + 16 * QT - 1, p1);
+
+  u32x4_t rk[PIECES], rv[PIECES];
+  const uint16_t* kb = a.k + b * a.k_b + hk * d;
+  const uint16_t* vb = a.v + b * a.v_b + hk * d;
+  const uint32_t k2 = 2 * (uint32_t)a.k_n, v2 = 2 * (uint32_t)a.v_n;
+  auto tile_of = [&](int t) { return t < sink_tiles ? t : band_tile + (t - sink_tiles); };
+  auto request = [&](int t) {
+    const int j0 = tile_of(t) * WK, count = min(keys - j0, WK);
+    auto rows = [&](const uint16_t* base, uint32_t ld2, u32x4_t* r) {
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base), 0, (int)((uint32_t)(count - 1) * ld2 + 2 * d), 0x00020000);
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        const int idx = tid + NT * i, row = idx / (DK * 4), c = idx - row * (DK * 4);
+        const uint32_t off = 8 * c < d ? (uint32_t)row * ld2 + 16 * c : 0x80000000u;  // (outside: zeros)
+        r[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rs, (int)off, 0, 0));
+      }
+    };
+    rows(kb + (int64_t)j0 * a.k_n, k2, rk);
+    rows(vb + (int64_t)j0 * a.v_n, v2, rv);
+  };
+
+  const int key = wa_key<DK>(fr), trow = 4 * fg + (fr >> 2), tkey = wa_key<DK>(trow), piece = fr & 3;
+  uint32_t k_at[DK];
+#pragma unroll
+  for (int s = 0; s < DK; ++s) k_at[s] = fr * PITCH + (((4 * s + fg) ^ key) << 4);
+  auto v_at = [&](int dt) { return (uint32_t)(TILE + trow * PITCH + (((2 * dt + (piece >> 1)) ^ tkey) << 4) + 8 * (piece & 1)); };
+
+  f32x4_t oc[QT][DT];  // out^T: channel 16 dt + 4 fg + r, query fr
+  float mx[QT], sub[QT], sum[QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    mx[t] = -INFINITY, sub[t] = 0.f, sum[t] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) oc[t][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+
+  if (t0 < t1) request(t0);
+#pragma unroll 1
+  for (int t = t0; t < t1; ++t) {
+    const uint32_t buf = (t - t0) & 1 ? 2 * TILE : 0;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const int idx = tid + NT * i, row = idx / (DK * 4), c = idx - row * (DK * 4);
+      const uint32_t to = buf + row * PITCH + ((c ^ wa_key<DK>(row)) << 4);
+      *reinterpret_cast<u32x4_t*>(smem + to) = rk[i];
+      *reinterpret_cast<u32x4_t*>(smem + to + TILE) = rv[i];
+    }
+    wa_barrier();  // (also: everyone is done with the tile before the last, whose buffer is written next)
+    if (t + 1 < t1) request(t + 1);
+    const int j0 = tile_of(t) * WK, j1 = j0 + WK - 1;
+    if (w0 >= queries || j0 > wp1 || (wp0 - j1 >= a.window && j0 >= a.sinks)) continue;  // (uniform; no barrier below)
+    const bool whole = j1 <= wp0 && (j1 < a.sinks || wp1 - j0 < a.window);
+    // ---- scores
+    f32x4_t sc[QT][4];
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt) {
+#pragma unroll
+      for (int q = 0; q < QT; ++q) sc[q][kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < DK; ++s) {
+        const u32x4_t kf = wa_read(lds0 + buf + 16 * kt * PITCH + k_at[s]);
+#pragma unroll
+        for (int q = 0; q < QT; ++q) sc[q][kt] = mfma_16x16x32<T>(kf, qf[q][s], sc[q][kt]);
+      }
+    }
+    // ---- softmax
+    u32x2_t pk[QT][4];
+#pragma unroll
+    for (int q = 0; q < QT; ++q) {
+      if (!whole) {
+        const int p = past + w0 + 16 * q + fr;
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int j = j0 + 16 * kt + 4 * fg + r;
+            if (!(j <= p && (p - j < a.window || j < a.sinks))) sc[q][kt][r] = -INFINITY;
+          }
+      }
+      // (the scale is positive: the maximum of the scaled scores is the scaled maximum)
+      float most = -INFINITY;
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) most = fmaxf(most, sc[q][kt][r]);
+      most *= a.scale_log2e;
+      if (__any(most > mx[q] + 8.f)) {
+        const float now = fmaxf(mx[q], wa_max_groups(most));
+        const float f = __builtin_amdgcn_exp2f(mx[q] - (now == -INFINITY ? 0.f : now));  // (nothing yet: 0)
+        mx[q] = now, sub[q] = now == -INFINITY ? 0.f : now - kShift<T>;
+        sum[q] *= f;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) oc[q][dt][r] *= f;
+      }
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt) {
+        float p[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          p[r] = __builtin_amdgcn_exp2f(fmaf(sc[q][kt][r], a.scale_log2e, -sub[q]));
+          sum[q] += p[r];
+        }
+        pk[q][kt] = u32x2_t{pk16<T>(p[0], p[1]), pk16<T>(p[2], p[3])};
+      }
+    }
+    // ---- values
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const uint32_t from = lds0 + buf + v_at(dt) + 32 * s * PITCH;
+        const u32x2_t x = wa_read_tr(from), y = wa_read_tr(from + 16 * PITCH);
+        const u32x4_t vf = {x.x, x.y, y.x, y.y};
+#pragma unroll
+        for (int q = 0; q < QT; ++q)
+          oc[q][dt] = mfma_16x16x32<T>(vf, u32x4_t{pk[q][2 * s].x, pk[q][2 * s].y, pk[q][2 * s + 1].x, pk[q][2 * s + 1].y}, oc[q][dt]);
+      }
+  }
+  // ---- out, or this part's
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int qi = w0 + 16 * t + fr;
+    const float l = wa_sum_groups(sum[t]);
+    if (qi >= queries) continue;
+    if (a.splits == 1) {
+      const float inv = 1.0f / l;
+      uint16_t* row = a.out + b * a.o_b + (int64_t)qi * a.o_n + h * d;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const int c = 16 * dt + 4 * fg;
+        if (c < d) *reinterpret_cast<u32x2_t*>(row + c) = u32x2_t{pk16<T>(oc[t][dt][0] * inv, oc[t][dt][1] * inv), pk16<T>(oc[t][dt][2] * inv, oc[t][dt][3] * inv)};
+      }
+    } else {
+      const int64_t at = ((int64_t)split * a.B * a.N + (int64_t)b * a.N + qi) * a.H + h;
+      if (fg == 0) a.part_ml[2 * at] = mx[t], a.part_ml[2 * at + 1] = l;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const int c = 16 * dt + 4 * fg;
+        if (c < d) *reinterpret_cast<f32x4_t*>(a.part_o + at * d + c) = oc[t][dt];
+      }
+    }
+  }
+}
+
+// The parts of a query and head: weights 2^(m_s - m), sums and outputs added up in the order of the parts.  A wave a (query, head), four
+// channels a lane.
+template <typename T>
+__global__ __launch_bounds__(256) void window_join_kernel(const WindowArgs a) {
+  const int64_t rows = (int64_t)a.B * a.N * a.H, row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const int c = 4 * (threadIdx.x & 31);
+  const int64_t bn = row / a.H;
+  const int h = (int)(row - bn * a.H), b = (int)(bn / a.N), i = (int)(bn - (int64_t)b * a.N);
+  if ((a.lengths && i >= a.lengths[b]) || (a.positions && a.positions[b] < 0)) return;
+  float m = -INFINITY;
+  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[2 * (s * rows + row)]);
+  float l = 0.f;
+  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < a.splits; ++s) {
+    const int64_t at = s * rows + row;
+    const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * at] - m);
+    l = fmaf(f, a.part_ml[2 * at + 1], l);
+    if (c < a.d) {
+      const f32x4_t x = *reinterpret_cast<const f32x4_t*>(a.part_o + at * a.d + c);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[r] = fmaf(f, x[r], o[r]);
+    }
+  }
+  const float inv = 1.0f / l;
+  if (c < a.d)
+    *reinterpret_cast<u32x2_t*>(a.out + b * a.o_b + (int64_t)i * a.o_n + h * a.d + c) =
+        u32x2_t{pk16<T>(o[0] * inv, o[1] * inv), pk16<T>(o[2] * inv, o[3] * inv)};
+}
+
+__device__ __forceinline__ int wa_slot(int64_t p, int sinks, int window) { return (int)(p < sinks ? p : sinks + (p - sinks) % window); }
+
+// One token of each stream over its cache.  A workgroup takes a part of the rows of one (stream, key head), its waves every fourth
+// tile of 32 rows; the query heads that share the key head are the 16 columns of the products (more than 16 in further workgroups).  K comes
+// from memory as the operand it is, V through the wave's own LDS to be transposed.  The new token's row is taken from k and v, wherever its
+// slot is met, and written to the cache by the workgroup whose part holds the slot: nobody reads that row of the cache.
+template <typename T, int DK, int DT>
+__global__ __launch_bounds__(256) void window_step_kernel(const WindowArgs a) {
+  constexpr int PITCH = DK * 64, TILE = 32 * PITCH, PV = DK * 2;  // PV: 16-byte pieces of V a lane
+  __shared__ __attribute__((aligned(16))) unsigned char smem[4 * (TILE > 16 * 16 * DT * 4 + 128 ? TILE : 16 * 16 * DT * 4 + 128)];
+  constexpr int OWN = sizeof(smem) / 4;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, fr = lane & 15, fg = lane >> 4;
+  unsigned char* mine = smem + wave * OWN;
+  const uint32_t lds = (uint32_t)(size_t)(__attribute__((address_space(3))) unsigned char*)mine;
+  const int G = a.H / a.Hkv, blocks = (G + 15) / 16, d = a.d;
+  const int split = blockIdx.y, gb = blockIdx.x % blocks, bk = blockIdx.x / blocks, b = bk / a.Hkv, hk = bk - b * a.Hkv;
+  const int pos = a.positions[b];
+  if (pos < 0) {  // an idle stream: zeros
+    if (split == 0 && gb == 0)
+      for (int c = tid; c < G * d; c += 256) a.out[b * a.o_b + hk * G * d + c] = 0;
+    return;
+  }
+  const int rows = a.window + a.sinks, count = pos < rows ? pos + 1 : rows, slot = wa_slot(pos, a.sinks, a.window);
+  const int tiles = (count + 31) / 32, t0 = (int)((int64_t)tiles * split / a.splits), t1 = (int)((int64_t)tiles * (split + 1) / a.splits);
+
+  const int head = 16 * gb + fr, h = hk * G + min(head, G - 1);
+  u32x4_t qf[DK];
+#pragma unroll
+  for (int s = 0; s < DK; ++s) {
+    qf[s] = *reinterpret_cast<const u32x4_t*>(a.q + b * a.q_b + h * d + (32 * s + 8 * fg < d ? 32 * s + 8 * fg : 0));
+    if (32 * s + 8 * fg >= d) qf[s] = u32x4_t{0u, 0u, 0u, 0u};
+  }
+  const uint16_t *new_k = a.k + b * a.k_b + hk * d, *new_v = a.v + b * a.v_b + hk * d;
+  uint16_t *ck = a.cache_k + b * a.ck_b + hk * d, *cv = a.cache_v + b * a.cv_b + hk * d;
+  if (gb == 0 && slot / 32 >= t0 && slot / 32 < t1 && tid < 32 * DK / 4) {  // (t0 <= slot's tile < t1 holds for one part)
+    const int c = 8 * (tid % (4 * DK));
+    if (c < d) {
+      const bool of_v = tid >= 4 * DK;
+      *reinterpret_cast<u32x4_t*>((of_v ? cv + (int64_t)slot * a.cv_n : ck + (int64_t)slot * a.ck_n) + c) =
+          *reinterpret_cast<const u32x4_t*>((of_v ? new_v : new_k) + c);
+    }
+  }
+
+  u32x4_t rk[2][DK], rv[PV];
+  auto request = [&](int t) {
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      const int row = min(32 * t + 16 * kt + fr, count - 1);
+      const uint16_t* from = row == slot ? new_k : ck + (int64_t)row * a.ck_n;
+#pragma unroll
+      for (int s = 0; s < DK; ++s) rk[kt][s] = *reinterpret_cast<const u32x4_t*>(from + (32 * s + 8 * fg < d ? 32 * s + 8 * fg : 0));
+    }
+#pragma unroll
+    for (int i = 0; i < PV; ++i) {
+      const int idx = lane + 64 * i, r = idx / (DK * 4), c = idx - r * (DK * 4), row = min(32 * t + r, count - 1);
+      const uint16_t* from = row == slot ? new_v : cv + (int64_t)row * a.cv_n;
+      rv[i] = *reinterpret_cast<const u32x4_t*>(from + (8 * c < d ? 8 * c : 0));
+    }
+  };
+  f32x4_t oc[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) oc[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  float mx = -INFINITY, sub = 0.f, sum = 0.f;
+  const int trow = 4 * fg + (fr >> 2), tkey = wa_key<DK>(trow), piece = fr & 3;
+  if (t0 + wave < t1) request(t0 + wave);
+#pragma unroll 1
+  for (int t = t0 + wave; t < t1; t += 4) {
+    f32x4_t sc[2];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      sc[kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < DK; ++s) {  // (channels past d: K repeats others there, q is zero; an inf there must not count)
+        u32x4_t kf = rk[kt][s];
+        if (32 * s + 8 * fg >= d) kf = u32x4_t{0u, 0u, 0u, 0u};
+        sc[kt] = mfma_16x16x32<T>(kf, qf[s], sc[kt]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < PV; ++i) {
+      const int idx = lane + 64 * i, r = idx / (DK * 4), c = idx - r * (DK * 4);
+      *reinterpret_cast<u32x4_t*>(mine + r * PITCH + ((c ^ wa_key<DK>(r)) << 4)) = rv[i];
+    }
+    if (t + 4 < t1) request(t + 4);
+    float most = -INFINITY;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        sc[kt][r] = 32 * t + 16 * kt + 4 * fg + r < count ? sc[kt][r] * a.scale_log2e : -INFINITY;
+        most = fmaxf(most, sc[kt][r]);
+      }
+    if (__any(most > mx + 8.f)) {
+      const float now = fmaxf(mx, wa_max_groups(most));
+      const float f = __builtin_amdgcn_exp2f(mx - (now == -INFINITY ? 0.f : now));
+      mx = now, sub = now == -INFINITY ? 0.f : now - kShift<T>;
+      sum *= f;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) oc[dt][r] *= f;
+    }
+    u32x4_t pf;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      float p[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        p[r] = __builtin_amdgcn_exp2f(sc[kt][r] - sub);
+        sum += p[r];
+      }
+      pf[2 * kt] = pk16<T>(p[0], p[1]), pf[2 * kt + 1] = pk16<T>(p[2], p[3]);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the wave's own V is there)
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      const uint32_t from = lds + trow * PITCH + (((2 * dt + (piece >> 1)) ^ tkey) << 4) + 8 * (piece & 1);
+      const u32x2_t x = wa_read_tr(from), y = wa_read_tr(from + 16 * PITCH);
+      oc[dt] = mfma_16x16x32<T>(u32x4_t{x.x, x.y, y.x, y.y}, pf, oc[dt]);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+  // ---- the waves' parts, through LDS: [channel][head], then the maxima and sums
+  sum = wa_sum_groups(sum);
+  float* po = reinterpret_cast<float*>(mine);
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) po[(16 * dt + 4 * fg + r) * 16 + fr] = oc[dt][r];
+  if (fg == 0) po[16 * 16 * DT + fr] = mx, po[16 * 16 * DT + 16 + fr] = sum;
+  wa_barrier();
+  auto part = [&](int w) { return reinterpret_cast<const float*>(smem + w * OWN); };
+  const int col = tid & 15, g = 16 * gb + col;
+  float m = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) m = fmaxf(m, part(w)[16 * 16 * DT + col]);
+  const float base = m == -INFINITY ? 0.f : m;
+  float f[4], l = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    f[w] = __builtin_amdgcn_exp2f(part(w)[16 * 16 * DT + col] - base);
+    l = fmaf(f[w], part(w)[16 * 16 * DT + 16 + col], l);
+  }
+  if (g >= G) return;
+  const int64_t at = ((int64_t)split * a.B + b) * a.H + hk * G + g;
+  const float inv = 1.0f / l;
+  for (int c = tid >> 4; c < d; c += 16) {
+    float o = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) o = fmaf(f[w], part(w)[c * 16 + col], o);
+    if (a.splits == 1) a.out[b * a.o_b + (hk * G + g) * d + c] = (uint16_t)pk16<T>(o * inv, 0.f);
+    else a.part_o[at * d + c] = o;
+  }
+  if (a.splits > 1 && tid < 16) a.part_ml[2 * at] = m, a.part_ml[2 * at + 1] = l;
+}
+
+// New tokens into the caches, 16 bytes a thread; a token that later ones of the same call push out is not written, so no row is
+// written twice.
+__global__ __launch_bounds__(256) void window_append_kernel(const WindowArgs a) {
+  const int width = a.d / 8;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (int64_t)a.N * width) return;
+  const int t = (int)(i / width), c = 8 * (int)(i - (int64_t)t * width), b = blockIdx.y;
+  const int n = a.lengths ? min(max(a.lengths[b], 0), a.N) : a.N;
+  const int64_t pos = a.positions[b], p = pos + t;
+  if (pos < 0 || t >= n || (p >= a.sinks && t < n - a.window)) return;
+  const int slot = wa_slot(p, a.sinks, a.window);
+  *reinterpret_cast<u32x4_t*>(a.cache_k + b * a.ck_b + (int64_t)slot * a.ck_n + c) =
+      *reinterpret_cast<const u32x4_t*>(a.k + b * a.k_b + (int64_t)t * a.k_n + c);
+  *reinterpret_cast<u32x4_t*>(a.cache_v + b * a.cv_b + (int64_t)slot * a.cv_n + c) =
+      *reinterpret_cast<const u32x4_t*>(a.v + b * a.v_b + (int64_t)t * a.v_n + c);
+}
+
+constexpr int WA_QT = 2, WA_NW = 4, WA_QB = WA_NW * 16 * WA_QT;
+
+// Parts of a prompt's keys: where the blocks of queries leave compute units idle and have keys enough.
+int prompt_splits(int B, int N, int Nk, int H, int window, int sinks) {
+  const int64_t blocks = (int64_t)B * H * ((N + WA_QB - 1) / WA_QB);
+  const int64_t seen = (int64_t)window + WA_QB + sinks;
+  const int tiles = (int)((seen < Nk ? seen : Nk) / WK);
+  if (blocks >= 256 || tiles < 8) return 1;
+  int64_t want = 512 / blocks;
+  want = want > tiles / 4 ? tiles / 4 : want;
+  return (int)(want < 1 ? 1 : want > WA_MAX_SPLITS ? WA_MAX_SPLITS : want);
+}
+// Parts of a cache's rows for one token: four tiles of 32 rows a workgroup at least.
+int step_splits(int B, int H, int Hkv, int rows) {
+  const int64_t groups = (int64_t)B * Hkv * ((H / Hkv + 15) / 16);
+  const int tiles = (rows + 31) / 32;
+  int64_t want = (1024 + groups - 1) / groups;
+  want = want > tiles / 4 ? tiles / 4 : want;
+  return (int)(want < 1 ? 1 : want > WA_MAX_SPLITS ? WA_MAX_SPLITS : want);
+}
+size_t part_bytes(int splits, int64_t rows, int d) { return splits > 1 ? (size_t)splits * rows * (d + 2) * sizeof(float) : 0; }
+
+template <typename T>
+int launch_join(const WindowArgs& a, hipStream_t s) {
+  const int64_t groups = ((int64_t)a.B * a.N * a.H + 7) / 8;
+  if (groups > 0x7fffffff) return SANA_ERR_SHAPE;
+  hipLaunchKernelGGL(window_join_kernel<T>, dim3((unsigned)groups), dim3(256), 0, s, a);
+  return SANA_OK;
+}
+
+template <typename T, int DK, int DT>
+int launch_prompt(WindowArgs a, hipStream_t s) {
+  a.qblocks = (a.N + WA_QB - 1) / WA_QB;
+  const int64_t items = (int64_t)a.B * a.H * a.qblocks * a.splits;
+  if (items > 0x7ffffff0) return SANA_ERR_SHAPE;
+  a.items = (int)items;
+  hipLaunchKernelGGL((window_attn_kernel<T, DK, DT, WA_QT, WA_NW>), dim3((unsigned)((items + 7) / 8 * 8)), dim3(64 * WA_NW), 0, s, a);
+  if (a.splits > 1) {
+    const int rc = launch_join<T>(a, s);
+    if (rc != SANA_OK) return rc;
+  }
+  return hipGetLastError() == hipSuccess ? SANA_OK : SANA_ERR_LAUNCH;
+}
+
+template <typename T, int DK, int DT>
+int launch_step(const WindowArgs& a, hipStream_t s) {
+  const int64_t groups = (int64_t)a.B * a.Hkv * ((a.H / a.Hkv + 15) / 16);
+  if (groups > 0x7fffffff) return SANA_ERR_SHAPE;
+  hipLaunchKernelGGL((window_step_kernel<T, DK, DT>), dim3((unsigned)groups, (unsigned)a.splits), dim3(256), 0, s, a);
+  if (a.splits > 1) {
+    const int rc = launch_join<T>(a, s);
+    if (rc != SANA_OK) return rc;
+  }
+  return hipGetLastError() == hipSuccess ? SANA_OK : SANA_ERR_LAUNCH;
+}
+
+// head dims in classes: 32-channel steps of the scores, 16-channel tiles of the values
+#define SANA_WA_DIMS(F, ...)                     \
+  (a.d <= 32   ? F<T, 1, 2>(__VA_ARGS__)         \
+   : a.d <= 64 ? F<T, 2, 4>(__VA_ARGS__)         \
+   : a.d <= 80 ? F<T, 3, 5>(__VA_ARGS__)         \
+   : a.d <= 96 ? F<T, 3, 6>(__VA_ARGS__)         \
+   : a.d <= 112 ? F<T, 4, 7>(__VA_ARGS__)        \
+                : F<T, 4, 8>(__VA_ARGS__))
+template <typename T>
+int prompt_of(const WindowArgs& a, hipStream_t s) { return SANA_WA_DIMS(launch_prompt, a, s); }
+template <typename T>
+int step_of(const WindowArgs& a, hipStream_t s) { return SANA_WA_DIMS(launch_step, a, s); }
+
+bool misaligned(std::initializer_list<const void*> rows, std::initializer_list<int64_t> strides) {
+  for (const void* p : rows)
+    if (!aligned16(p)) return true;
+  for (const int64_t s : strides)
+    if (s % 8) return true;
+  return false;
+}
+bool off4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) != 0; }
+
+// sizes that all three calls share
+int check_sizes(int B, int N, int H, int Hkv, int d, int window, int sinks, int io_dtype) {
+  if (B <= 0 || N <= 0 || H <= 0 || Hkv <= 0 || d <= 0 || window <= 0 || sinks < 0 || H % Hkv) return SANA_ERR_ARG;
+  if (io_dtype != SANA_DT_BF16 && io_dtype != SANA_DT_F16) return SANA_ERR_DTYPE;
+  if (d % 8 || d > 128 || N > (1 << 30) || window > (1 << 30) || sinks > (1 << 30) || (int64_t)H * d > (1 << 22)) return SANA_ERR_SHAPE;
+  return SANA_OK;
+}
+
+}  // namespace
+}  // namespace sana
+
+using namespace sana;
+
+#define SANA_API extern "C" __attribute__((visibility("default")))
+
+SANA_API size_t sana_hip_window_attention_workspace_bytes(int B, int N, int Nk, int H, int d, int window, int sinks) {
+  if (B <= 0 || N <= 0 || Nk < N || H <= 0 || d <= 0 || window <= 0 || sinks < 0) return 0;
+  return part_bytes(prompt_splits(B, N, Nk, H, window, sinks), (int64_t)B * N * H, d);
+}
+
+SANA_API int sana_hip_window_attention(const void* q, const void* k, const void* v, void* out, const int32_t* lengths, void* workspace,
+                                       size_t workspace_bytes, int B, int N, int Nk, int H, int Hkv, int d, int window, int sinks,
+                                       int64_t q_stride_b, int64_t q_stride_n, int64_t k_stride_b, int64_t k_stride_n,
+                                       int64_t v_stride_b, int64_t v_stride_n, int64_t o_stride_b, int64_t o_stride_n, float scale,
+                                       int io_dtype, void* stream) {
+  if (!q || !k || !v || !out || Nk < N || !(scale > 0.f)) return SANA_ERR_ARG;
+  const int rc = check_sizes(B, N, H, Hkv, d, window, sinks, io_dtype);
+  if (rc != SANA_OK) return rc;
+  if (Nk > (1 << 30)) return SANA_ERR_SHAPE;
+  if (q_stride_n < (int64_t)H * d || o_stride_n < (int64_t)H * d || k_stride_n < (int64_t)Hkv * d || v_stride_n < (int64_t)Hkv * d)
+    return SANA_ERR_ARG;
+  for (const int64_t sb : {q_stride_b, k_stride_b, v_stride_b, o_stride_b})
+    if (sb < 0) return SANA_ERR_ARG;
+  if (k_stride_n >= (1 << 23) || v_stride_n >= (1 << 23)) return SANA_ERR_SHAPE;  // 32-bit byte offsets within a tile
+  if (misaligned({q, k, v}, {q_stride_b, q_stride_n, k_stride_b, k_stride_n, v_stride_b, v_stride_n}) ||
+      (reinterpret_cast<uintptr_t>(out) & 7u) || o_stride_b % 4 || o_stride_n % 4 || off4(lengths))
+    return SANA_ERR_ALIGN;
+  WindowArgs a = {};
+  a.q = static_cast<const uint16_t*>(q), a.k = static_cast<const uint16_t*>(k), a.v = static_cast<const uint16_t*>(v);
+  a.out = static_cast<uint16_t*>(out), a.lengths = lengths;
+  a.B = B, a.N = N, a.Nk = Nk, a.H = H, a.Hkv = Hkv, a.d = d, a.window = window, a.sinks = sinks;
+  a.q_b = q_stride_b, a.q_n = q_stride_n, a.k_b = k_stride_b, a.k_n = k_stride_n, a.v_b = v_stride_b, a.v_n = v_stride_n;
+  a.o_b = o_stride_b, a.o_n = o_stride_n, a.scale_log2e = scale * 1.44269504088896341f;
+  a.splits = prompt_splits(B, N, Nk, H, window, sinks);
+  const int64_t rows = (int64_t)B * N * H;
+  if (a.splits > 1) {
+    if (!workspace || workspace_bytes < part_bytes(a.splits, rows, d)) return SANA_ERR_WORKSPACE;
+    if (!aligned16(workspace)) return SANA_ERR_ALIGN;
+    a.part_o = static_cast<float*>(workspace), a.part_ml = a.part_o + a.splits * rows * d;
+  }
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return io_dtype == SANA_DT_F16 ? prompt_of<F16>(a, s) : prompt_of<BF16>(a, s);
+}
+
+SANA_API int sana_hip_window_cache_append(void* cache_k, void* cache_v, const void* k, const void* v, const int32_t* positions,
+                                          const int32_t* lengths, int B, int N, int C, int window, int sinks,
+                                          int64_t ck_stride_b, int64_t ck_stride_n, int64_t cv_stride_b, int64_t cv_stride_n,
+                                          int64_t k_stride_b, int64_t k_stride_n, int64_t v_stride_b, int64_t v_stride_n,
+                                          int io_dtype, void* stream) {
+  if (!cache_k || !cache_v || !k || !v || !positions) return SANA_ERR_ARG;
+  const int rc = check_sizes(B, N, 1, 1, 8, window, sinks, io_dtype);
+  if (rc != SANA_OK) return rc;
+  if (C <= 0) return SANA_ERR_ARG;
+  const int64_t groups = ((int64_t)N * (C / 8) + 255) / 256;
+  if (ck_stride_n < C || cv_stride_n < C || k_stride_n < C || v_stride_n < C) return SANA_ERR_ARG;
+  for (const int64_t sb : {ck_stride_b, cv_stride_b, k_stride_b, v_stride_b})
+    if (sb < 0) return SANA_ERR_ARG;
+  if (C % 8 || groups > 0x7fffffff || B > 65535) return SANA_ERR_SHAPE;
+  if (misaligned({cache_k, cache_v, k, v}, {ck_stride_b, ck_stride_n, cv_stride_b, cv_stride_n, k_stride_b, k_stride_n, v_stride_b, v_stride_n}) ||
+      off4(positions) || off4(lengths))
+    return SANA_ERR_ALIGN;
+  WindowArgs a = {};
+  a.cache_k = static_cast<uint16_t*>(cache_k), a.cache_v = static_cast<uint16_t*>(cache_v);
+  a.k = static_cast<const uint16_t*>(k), a.v = static_cast<const uint16_t*>(v), a.positions = positions, a.lengths = lengths;
+  a.B = B, a.N = N, a.d = C, a.window = window, a.sinks = sinks;
+  a.ck_b = ck_stride_b, a.ck_n = ck_stride_n, a.cv_b = cv_stride_b, a.cv_n = cv_stride_n;
+  a.k_b = k_stride_b, a.k_n = k_stride_n, a.v_b = v_stride_b, a.v_n = v_stride_n;
+  hipLaunchKernelGGL(window_append_kernel, dim3((unsigned)groups, (unsigned)B), dim3(256), 0, static_cast<hipStream_t>(stream), a);
+  return hipGetLastError() == hipSuccess ? SANA_OK : SANA_ERR_LAUNCH;
+}
+
+SANA_API size_t sana_hip_window_step_workspace_bytes(int B, int H, int Hkv, int d, int window, int sinks) {
+  if (B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || d <= 0 || window <= 0 || window > (1 << 30) || sinks < 0 || sinks > (1 << 30)) return 0;
+  return part_bytes(step_splits(B, H, Hkv, window + sinks), (int64_t)B * H, d);
+}
+
+SANA_API int sana_hip_window_step(const void* q, const void* k, const void* v, void* cache_k, void* cache_v, const int32_t* positions,
+                                  void* out, void* workspace, size_t workspace_bytes, int B, int H, int Hkv, int d, int window,
+                                  int sinks, int64_t q_stride_b, int64_t k_stride_b, int64_t v_stride_b, int64_t ck_stride_b,
+                                  int64_t ck_stride_n, int64_t cv_stride_b, int64_t cv_stride_n, int64_t o_stride_b, float scale,
+                                  int io_dtype, void* stream) {
+  if (!q || !k || !v || !cache_k || !cache_v || !positions || !out || !(scale > 0.f)) return SANA_ERR_ARG;
+  const int rc = check_sizes(B, 1, H, Hkv, d, window, sinks, io_dtype);
+  if (rc != SANA_OK) return rc;
+  const int64_t C = (int64_t)Hkv * d;
+  if (ck_stride_n < C || cv_stride_n < C) return SANA_ERR_ARG;
+  for (const int64_t sb : {q_stride_b, k_stride_b, v_stride_b, ck_stride_b, cv_stride_b, o_stride_b})
+    if (sb < 0) return SANA_ERR_ARG;
+  if (misaligned({q, k, v, cache_k, cache_v}, {q_stride_b, k_stride_b, v_stride_b, ck_stride_b, ck_stride_n, cv_stride_b, cv_stride_n}) ||
+      (reinterpret_cast<uintptr_t>(out) & 7u) || o_stride_b % 4 || off4(positions))
+    return SANA_ERR_ALIGN;
+  WindowArgs a = {};
+  a.q = static_cast<const uint16_t*>(q), a.k = static_cast<const uint16_t*>(k), a.v = static_cast<const uint16_t*>(v);
+  a.out = static_cast<uint16_t*>(out), a.cache_k = static_cast<uint16_t*>(cache_k), a.cache_v = static_cast<uint16_t*>(cache_v);
+  a.positions = positions, a.B = B, a.N = 1, a.Nk = 1, a.H = H, a.Hkv = Hkv, a.d = d, a.window = window, a.sinks = sinks;
+  a.q_b = q_stride_b, a.k_b = k_stride_b, a.v_b = v_stride_b, a.o_b = o_stride_b;
+  a.ck_b = ck_stride_b, a.ck_n = ck_stride_n, a.cv_b = cv_stride_b, a.cv_n = cv_stride_n;
+  a.scale_log2e = scale * 1.44269504088896341f;
+  a.splits = step_splits(B, H, Hkv, window + sinks);
+  const int64_t rows = (int64_t)B * H;
+  if (a.splits > 1) {
+    if (!workspace || workspace_bytes < part_bytes(a.splits, rows, d)) return SANA_ERR_WORKSPACE;
+    if (!aligned16(workspace)) return SANA_ERR_ALIGN;
+    a.part_o = static_cast<float*>(workspace), a.part_ml = a.part_o + a.splits * rows * d;
+  }
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return io_dtype == SANA_DT_F16 ? step_of<F16>(a, s) : step_of<BF16>(a, s);
+}

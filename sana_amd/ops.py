@@ -964,3 +964,133 @@ def decay_linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lo
     if code:
         _lib.check(code, "sana_hip_decay_attention")
     return out, state_out
+
+
+def _window_shapes(q, k, v, num_heads: int, window: int, sinks: int, scale: Optional[float], what: str) -> Tuple[int, int, float]:
+    """-> (head_dim, key heads, scale) of [B, N, H*d] queries and [B, Nk, Hkv*d] keys and values."""
+    if q.dim() != 3 or k.dim() != 3 or q.dtype not in IO16 or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise SanaHipError(f"{what} needs bf16 or fp16 q [B, N, H*d], k and v [B, Nk, Hkv*d] of one dtype, got {q.dtype}, {k.dtype}, {v.dtype}")
+    C = q.shape[2]
+    if num_heads < 1 or C % num_heads or C == 0:
+        raise SanaHipError(f"{C} channels are not {num_heads} heads")
+    d = C // num_heads
+    if d % 8 or d > 128:
+        raise SanaHipError(f"head_dim {d} has no kernel (multiples of 8 up to 128)")
+    if k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] == 0 or k.shape[2] % d or num_heads % (k.shape[2] // d):
+        raise SanaHipError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not match q {tuple(q.shape)} with {num_heads} heads of {d}")
+    if not 1 <= window <= 1 << 30 or not 0 <= sinks <= 1 << 30:
+        raise SanaHipError(f"window must be at least 1 and sinks at least 0, got {window} and {sinks}")
+    scale = float(d ** -0.5 if scale is None else scale)
+    if not scale > 0.0:
+        raise SanaHipError(f"scale must be positive, got {scale}")
+    return d, k.shape[2] // d, scale
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, num_heads: int, window: int, sinks: int = 0,
+                     scale: Optional[float] = None, lengths: Optional[torch.Tensor] = None,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal softmax attention in which a query sees the last ``window`` keys up to its own and the first ``sinks`` keys.
+    q: [B, N, H*d], k, v: [B, Nk, Hkv*d] token-major views, bf16 or fp16 of one dtype, H a multiple of Hkv (consecutive query
+    heads share a key head), d a multiple of 8 up to 128; the queries are the last N of the Nk keys.  Of a past that is longer than
+    what is kept, k and v hold the sinks and then, in order, at least the last window - 1 tokens in front of the queries.
+    ``lengths``: int32 [B] on the device, the queries that each batch entry really has (clamped to 0 .. N; its keys end with its
+    last query); rows behind them are not read, and stay in ``out`` as they were (zeros in a new one).
+    Returns [B, N, H*d].  ``out`` must not overlap the inputs.  Forward only."""
+    dev = _here(q, (k, v, lengths, out), "window_attention")
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            return window_attention(q, k, v, num_heads, window, sinks, scale, lengths, out)
+    d, Hkv, scale = _window_shapes(q, k, v, num_heads, window, sinks, scale, "window_attention")
+    B, N, C = q.shape
+    Nk = k.shape[1]
+    if Nk < N:
+        raise SanaHipError(f"the {N} queries are the last of the keys, of which there are {Nk}")
+    length_ptr = _lengths_arg(lengths, B)
+    if out is None:
+        out = (torch.empty if lengths is None else torch.zeros)((B, N, C), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise SanaHipError("out has the wrong shape or dtype")
+    if B * N == 0:
+        return out
+    strides = [s for t, name in ((q, "q"), (k, "k"), (v, "v"), (out, "out")) for s in _token_rows(t, name)]
+    lib = _lib.load()
+    nbytes = lib.sana_hip_window_attention_workspace_bytes(B, N, Nk, num_heads, d, window, sinks)
+    ws = _call_scratch(q.device, nbytes)
+    code = lib.sana_hip_window_attention(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), length_ptr, None if ws is None else ws.data_ptr(), nbytes,
+        B, N, Nk, num_heads, Hkv, d, window, sinks, *strides, scale, _DT[q.dtype], _stream())
+    if code:
+        _lib.check(code, "sana_hip_window_attention")
+    return out
+
+
+def _cache_rows(cache_k: torch.Tensor, cache_v: torch.Tensor, k: torch.Tensor, sinks: int, what: str) -> int:
+    """The window of a cache [B, sinks + window, C] for new tokens ``k`` [B, N, C]."""
+    if cache_k.dim() != 3 or cache_k.shape != cache_v.shape or cache_k.dtype != k.dtype or cache_v.dtype != k.dtype or \
+            cache_k.shape[0] != k.shape[0] or cache_k.shape[2] != k.shape[2]:
+        raise SanaHipError(f"{what}: the caches {tuple(cache_k.shape)}, {tuple(cache_v.shape)} do not match new tokens {tuple(k.shape)}")
+    if not 0 <= sinks < cache_k.shape[1]:
+        raise SanaHipError(f"{what}: a cache of {cache_k.shape[1]} rows holds {sinks} sinks and no window")
+    return cache_k.shape[1] - sinks
+
+
+def window_cache_append_(cache_k: torch.Tensor, cache_v: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
+                         sinks: int = 0, lengths: Optional[torch.Tensor] = None) -> None:
+    """New tokens' keys and values into the caches of :func:`window_attention_step_`: [B, sinks + window, C] rows, a token at
+    position p in row p below ``sinks``, else in row ``sinks + (p - sinks) % window``.  k, v: [B, N, C] (any N); ``positions``: int32
+    [B] on the device, the tokens that each stream has seen before (negative: idle, nothing is written), which the
+    caller advances; ``lengths``: int32 [B], the tokens that each stream really adds.  bf16 or fp16, C a multiple of 8.  The
+    caches must not overlap k and v, and no two streams may share rows."""
+    dev = _here(cache_k, (cache_v, k, v, positions, lengths), "window_cache_append_")
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            return window_cache_append_(cache_k, cache_v, k, v, positions, sinks, lengths)
+    if k.dim() != 3 or k.shape != v.shape or k.dtype not in IO16 or v.dtype != k.dtype:
+        raise SanaHipError(f"window_cache_append_ needs bf16 or fp16 k and v [B, N, C] of one dtype, got {tuple(k.shape)}, {tuple(v.shape)}")
+    window = _cache_rows(cache_k, cache_v, k, sinks, "window_cache_append_")
+    B, N, C = k.shape
+    position_ptr, length_ptr = _lengths_arg(positions, B, "positions"), _lengths_arg(lengths, B)
+    if B * N * C == 0:
+        return
+    strides = [s for t, name in ((cache_k, "cache_k"), (cache_v, "cache_v"), (k, "k"), (v, "v")) for s in _token_rows(t, name)]
+    code = _lib.load().sana_hip_window_cache_append(cache_k.data_ptr(), cache_v.data_ptr(), k.data_ptr(), v.data_ptr(), position_ptr,
+                                                    length_ptr, B, N, C, window, sinks, *strides, _DT[k.dtype], _stream())
+    if code:
+        _lib.check(code, "sana_hip_window_cache_append")
+
+
+def window_attention_step_(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tensor,
+                           positions: torch.Tensor, num_heads: int, sinks: int = 0, scale: Optional[float] = None,
+                           out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One token of each stream: q [B, 1, H*d], k, v [B, 1, Hkv*d].  The key and the value go into the caches
+    [B, sinks + window, Hkv*d] (:func:`window_cache_append_`) at ``positions`` [B] (int32, on the device: the tokens seen before,
+    which the caller advances once all layers are through), and the token attends to what the caches then hold: the last
+    ``window`` tokens up to itself and the first ``sinks``.  A stream with a negative position is idle: its caches stay as they are, its
+    output is zero.  Returns [B, 1, H*d].  Forward only."""
+    dev = _here(q, (k, v, cache_k, cache_v, positions, out), "window_attention_step_")
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            return window_attention_step_(q, k, v, cache_k, cache_v, positions, num_heads, sinks, scale, out)
+    if k.dim() != 3 or q.dim() != 3 or q.shape[1] != 1 or k.shape[1] != 1:
+        raise SanaHipError(f"window_attention_step_ takes one token of each stream, got q {tuple(q.shape)}, k {tuple(k.shape)}")
+    window = _cache_rows(cache_k, cache_v, k, sinks, "window_attention_step_")
+    d, Hkv, scale = _window_shapes(q, k, v, num_heads, window, sinks, scale, "window_attention_step_")
+    B, _, C = q.shape
+    position_ptr = _lengths_arg(positions, B, "positions")
+    if out is None:
+        out = torch.empty((B, 1, C), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise SanaHipError("out has the wrong shape or dtype")
+    if B == 0:
+        return out
+    (qb, _), (kb, _), (vb, _), (ob, _) = (_token_rows(t, name) for t, name in ((q, "q"), (k, "k"), (v, "v"), (out, "out")))
+    (ckb, ckn), (cvb, cvn) = _token_rows(cache_k, "cache_k"), _token_rows(cache_v, "cache_v")
+    lib = _lib.load()
+    nbytes = lib.sana_hip_window_step_workspace_bytes(B, num_heads, Hkv, d, window, sinks)
+    ws = _call_scratch(q.device, nbytes)
+    code = lib.sana_hip_window_step(q.data_ptr(), k.data_ptr(), v.data_ptr(), cache_k.data_ptr(), cache_v.data_ptr(), position_ptr,
+                                    out.data_ptr(), None if ws is None else ws.data_ptr(), nbytes, B, num_heads, Hkv, d, window,
+                                    sinks, qb, kb, vb, ckb, ckn, cvb, cvn, ob, scale, _DT[q.dtype], _stream())
+    if code:
+        _lib.check(code, "sana_hip_window_step")
+    return out

@@ -254,13 +254,13 @@ def test_refusals(cuda):
            lambda: call(q[..., :84], k[..., :84], v[..., :84], g), lambda: call(*[t[:, :, ::2] for t in (q, k, v)], g),
            lambda: call(*[t[:1].expand(2, 8, 96)[:, :1].expand(2, 8, 96) for t in (q, k, v)], g),
            lambda: call(*[torch.zeros(2 * 8 * 96 + 1, dtype=BF16, device="cuda")[1:].view(2, 8, 96)] * 3, g),
-           lambda: call(q, k, v.requires_grad_(), g)]
+           lambda: call(q, k, v.clone().requires_grad_(), g)]
     for i, f in enumerate(bad):
         with pytest.raises(sana_amd.SanaHipError):
             f()
             pytest.fail(f"case {i} was taken")
     with torch.no_grad():
-        call(q, k, v, g)   # (leaves that want gradients are fine where none are recorded)
+        call(q, k, v.clone().requires_grad_(), g)   # (leaves that want gradients are fine where none are recorded)
 
 
 def test_c_entry_refuses_before_any_launch():
