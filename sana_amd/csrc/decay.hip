@@ -60,30 +60,35 @@ __device__ __forceinline__ float dc_fit(float most) {
   return __uint_as_float((uint32_t)f << 23);
 }
 
-// One workgroup takes a (batch, head, segment) through its chunks; NW waves, each of which owns 32 channels of v: their
-// columns of the state stay in its registers (fp32) from chunk to chunk.  The waves share the scores, 64 / NW queries each, through LDS.
+// What a launch of the chunks gives: the sums of a segment alone, the outputs of segments whose states are known, or both for whole streams.
+enum { DC_SUMS, DC_OUT, DC_WHOLE };
+
+// One workgroup of four waves takes a (batch, head, segment) through its chunks.  NV of its waves share the channels of v, 16 VT
+// each, whose columns of the state stay in their registers (fp32) from chunk to chunk; where the head has fewer channels, 4 / NV waves
+// with the same ones share the queries.  Each wave scores 16 queries for all, through LDS.
 // The operands of the MFMAs (16 x 16 x 32):
 //   scores^T = K Q^T   both from LDS as they lie;
 //   out^T    = S Q^T   S as its own accumulators hold it (row v of the product: lane; a lane's 8 values of k: the accumulators of two
 //                      tiles, whose rows are channels 32 s + 8 g + {0..3} and + {4..7}, by the addresses of the transposing read below);
 //   out^T   += V^T P^T V by transposing reads, P^T from LDS in the key order that these give;
 //   S       += K^T V   both by transposing reads.
-// Roundings: P to 16 bits, as it enters its product.  S enters its product with q as the sum of two 16-bit values.  The weighted values
-// a^(C-1-j) v_j enter theirs as the sum of three bf16 values or two f16 ones (22 bits and more: the state that is carried keeps
-// fp32's accuracy; of a 32760-token stream it is 1.3e-6 off with two bf16 values), f16's second value times 2^11, so that it stays a
-// normal number.  f16 ends at 65504: S goes in scaled by a power of two for each wave, P for each query.
-template <typename T, int DK, int NW, bool OUT>
-__global__ __launch_bounds__(64 * NW, 2) void decay_chunk_kernel(const DecayArgs a) {
+// Roundings.  Each product of the output has one operand of 16 bits that is rounded, P or S, as attention kernels round P: with the rounding of
+// the result the error is 1.4 times that of the result's rounding alone.  The weighted values a^(C-1-j) v_j enter the state as a sum of
+// 16-bit values: three of bf16 where the state is given back (fp32's accuracy; with two it is 1.3e-6 off after 32760
+// tokens), two of bf16 where it only goes on to outputs, two of f16 (22 bits), the second times 2^11, so that it stays a normal number.
+// f16 ends at 65504: S goes in scaled by a power of two for each wave, P for each query.
+template <typename T, int DK, int VT, int NV, int MODE>
+__global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) {
+  constexpr bool OUT = MODE != DC_SUMS, F = is_f16<T>;
   constexpr int PITCH = DK * 64, TILE = DC * PITCH, KT = 2 * DK;  // LDS row / tensor in bytes; 16-row tiles of k
-  constexpr int NT = 64 * NW, PIECES = DC * DK * 4 / NT;
-  static_assert(DC * DK * 4 % NT == 0 && 4 % NW == 0, "");
-  constexpr int QW = 4 / NW;  // query tiles of a wave
-  constexpr bool F = is_f16<T>;
+  constexpr int NT = 256, PIECES = DC * DK * 4 / NT, TERMS = F || MODE == DC_OUT ? 2 : 3;
+  constexpr int NQ = 4 / NV, QN = 4 / NQ;  // shares of the queries, query tiles of a share
   __shared__ __attribute__((aligned(16))) unsigned char smem[(OUT ? 3 : 2) * TILE + (OUT ? DC * 128 + DC * 4 : 0)];
   const uint32_t sk = (uint32_t)(size_t)(__attribute__((address_space(3))) unsigned char*)smem;
   const uint32_t sv = sk + TILE, sq = sk + 2 * TILE, sp = sk + 3 * TILE;
   float* fit = reinterpret_cast<float*>(smem + 3 * TILE + DC * 128);  // f16: the scale of a query's P
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, fr = lane & 15, fg = lane >> 4;
+  const int v0 = 16 * VT * (wave % NV), qt0 = QN * (wave / NV);
 
   // neighbouring heads, whose rows share cache lines, on one XCD
   const int per = (a.items + 7) >> 3, item = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
@@ -91,63 +96,66 @@ __global__ __launch_bounds__(64 * NW, 2) void decay_chunk_kernel(const DecayArgs
   const int h = item % a.H, rest = item / a.H, seg = rest % a.nseg, b = rest / a.nseg, d = a.d, bh = b * a.H + h;
   const int n = a.lengths ? min(max(a.lengths[b], 0), a.N) : a.N;
   const int first = seg * a.seg_tokens, last = min(n, first + a.seg_tokens);  // (host: seg * seg_tokens < N)
-  if (OUT ? (seg > 0 && first >= n) : first + a.seg_tokens >= n) return;  // nothing of this segment is asked for
+  if (MODE != DC_WHOLE && first >= n) return;
   const float g2 = dc_log2(a.log_decay[h]);
 
-  // ---- the state: st[vt][kt][r] = row v = 32 wave + 16 vt + fr, column k = 32 (kt / 2) + 8 fg + 4 (kt & 1) + r
-  f32x4_t st[2][KT];
-  const float* s0 = !OUT ? nullptr : a.nseg > 1 ? a.segments + ((int64_t)bh * a.nseg + seg) * d * d : a.state_in ? a.state_in + (int64_t)bh * d * d : nullptr;
+  // ---- the state: st[vt][kt][r] = row v = v0 + 16 vt + fr, column k = 32 (kt / 2) + 8 fg + 4 (kt & 1) + r
+  f32x4_t st[VT][KT];
+  const float* s0 = MODE == DC_SUMS ? nullptr : MODE == DC_OUT ? a.segments + ((int64_t)bh * a.nseg + seg) * d * d : a.state_in ? a.state_in + (int64_t)bh * d * d : nullptr;
 #pragma unroll
-  for (int vt = 0; vt < 2; ++vt)
+  for (int vt = 0; vt < VT; ++vt)
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
-      const int v = 32 * wave + 16 * vt + fr, k = 32 * (kt >> 1) + 8 * fg + 4 * (kt & 1);
+      const int v = v0 + 16 * vt + fr, k = 32 * (kt >> 1) + 8 * fg + 4 * (kt & 1);
       st[vt][kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
       if (s0 && v < d && k < d) st[vt][kt] = *reinterpret_cast<const f32x4_t*>(s0 + v * d + k);
     }
 
-  // ---- what does not change from chunk to chunk
-  float within[OUT ? QW : 1][4][4], since[4];  // scale * a^(t - j) (0 where j > t); scale * a^(t + 1)
+  // ---- powers of the decay.  A chunk of fewer than 64 tokens fills the last rows of its tile, zeros in front of it, so only `since`
+  // and `over` depend on how many there are.  Exponents are split into a part of the lane and one of the tile, none below 0.
+  auto uniform = [](float x) { return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x))); };
+  const float lane12 = dc_pow(g2, 12 - 4 * fg);
+  float to_end[2][8];  // a^(C - 1 - t) of the tokens of this lane's transposed values, less 12 - 4 fg
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) to_end[s][e] = uniform(dc_pow(g2, 63 - 12 - 32 * s - 16 * (e >> 2) - (e & 3)));
+  // scale * a^(t - j): of the tile on the diagonal (0 where j > t); in front of it the lane's part, that of the tile's row
+  float diagonal[4], before = 0.f, row4[4], step16 = 0.f;
   if constexpr (OUT) {
+    before = a.scale * lane12 * dc_pow(g2, fr);
+    step16 = uniform(dc_pow(g2, 16));
 #pragma unroll
-    for (int i = 0; i < QW; ++i)
-#pragma unroll
-      for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int apart = 16 * (wave + NW * i) + fr - (16 * kt + 4 * fg + r);
-          within[i][kt][r] = apart >= 0 ? a.scale * dc_pow(g2, apart) : 0.f;
-        }
-#pragma unroll
-    for (int qt = 0; qt < 4; ++qt) since[qt] = a.scale * dc_pow(g2, 16 * qt + fr + 1);
+    for (int r = 0; r < 4; ++r) {
+      diagonal[r] = fr >= 4 * fg + r ? a.scale * dc_pow(g2, fr - 4 * fg - r) : 0.f;
+      row4[r] = uniform(dc_pow(g2, 4 - r));
+    }
   }
-  float to_end[2][8];  // a^(C - 1 - t) of the tokens of this lane's transposed values; tokens past the end are zeros
-  auto weights = [&](int count) {
+  float since[QN], over;  // scale * a^(t + 1); a^count
+  auto counted = [&](int count) {
+    over = dc_pow(g2, count);
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) to_end[s][e] = dc_pow(g2, max(count - 1 - (32 * s + 4 * fg + (e & 3) + 16 * (e >> 2)), 0));
+    for (int q = 0; q < QN; ++q) since[q] = a.scale * dc_pow(g2, max(16 * (qt0 + q) + fr + 1 - (DC - count), 0));
   };
-  weights(DC);
-  float over = dc_pow(g2, DC);
+  counted(DC);
 
   // ---- a chunk's rows: requested into registers a chunk ahead, then to LDS
   u32x4_t rk[PIECES], rv[PIECES], rq[OUT ? PIECES : 1];
   const uint32_t k2 = 2 * (uint32_t)a.k_n, v2 = 2 * (uint32_t)a.v_n, q2 = 2 * (uint32_t)a.q_n;
   auto request = [&](int at) {
-    const int count = min(last - at, DC);
+    const int count = min(last - at, DC), empty = DC - count;
     auto rows = [&](const uint16_t* base, uint32_t ld2, u32x4_t* r) {
       const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base), 0, (int)((uint32_t)(count - 1) * ld2 + 2 * d), 0x00020000);
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
         const int idx = tid + NT * i, row = idx / (DK * 4), c = idx - row * (DK * 4);
-        const uint32_t off = 8 * c < d ? (uint32_t)row * ld2 + 16 * c : 0x80000000u;  // (outside: zeros)
+        const uint32_t off = 8 * c < d ? (uint32_t)(row - empty) * ld2 + 16 * c : 0x80000000u;  // (outside, as rows below 0 are: zeros)
         r[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rs, (int)off, 0, 0));
       }
     };
     rows(a.k + b * a.k_b + (int64_t)at * a.k_n + h * d, k2, rk);
-    rows(a.v + b * a.v_b + (int64_t)at * a.v_n + h * d, v2, rv);
     if constexpr (OUT) rows(a.q + b * a.q_b + (int64_t)at * a.q_n + h * d, q2, rq);
+    rows(a.v + b * a.v_b + (int64_t)at * a.v_n + h * d, v2, rv);
   };
   if (first < last) request(first);
 
@@ -157,12 +165,12 @@ __global__ __launch_bounds__(64 * NW, 2) void decay_chunk_kernel(const DecayArgs
 #pragma unroll
   for (int s = 0; s < DK; ++s) row16[s] = fr * PITCH + (((4 * s + fg) ^ key) << 4);
   const int trow = 4 * fg + (fr >> 2), tkey = dc_key<DK>(trow), piece = fr & 3;  // of a transposing read
-  uint32_t vt_at[2], kt_at[DK];
+  uint32_t vt_at[VT], kt_at[DK];
 #pragma unroll
-  for (int vt = 0; vt < 2; ++vt) vt_at[vt] = sv + trow * PITCH + (((2 * (2 * wave + vt) + (piece >> 1)) ^ tkey) << 4) + 8 * (piece & 1);
+  for (int vt = 0; vt < VT; ++vt) vt_at[vt] = sv + trow * PITCH + (((v0 / 8 + 2 * vt + (piece >> 1)) ^ tkey) << 4) + 8 * (piece & 1);
 #pragma unroll
   for (int s = 0; s < DK; ++s) kt_at[s] = sk + trow * PITCH + (((4 * s + piece) ^ tkey) << 4);
-  const bool own = 32 * wave < 32 * DK;  // (DK = 3: the fourth wave has no channels of v, and its reads would leave the rows)
+  const bool own = v0 < 32 * DK;  // (DK = 3: the fourth wave has no channels of v, and its reads would leave the rows)
 
 #pragma unroll 1
   for (int at = first; at < last; at += DC) {
@@ -172,64 +180,62 @@ __global__ __launch_bounds__(64 * NW, 2) void decay_chunk_kernel(const DecayArgs
       const int idx = tid + NT * i, row = idx / (DK * 4), c = idx - row * (DK * 4);
       const uint32_t to = row * PITCH + ((c ^ dc_key<DK>(row)) << 4);
       *reinterpret_cast<u32x4_t*>(smem + to) = rk[i];
-      *reinterpret_cast<u32x4_t*>(smem + TILE + to) = rv[i];
       if constexpr (OUT) *reinterpret_cast<u32x4_t*>(smem + 2 * TILE + to) = rq[i];
+      *reinterpret_cast<u32x4_t*>(smem + TILE + to) = rv[i];
     }
     dc_barrier();
     if (at + DC < last) request(at + DC);
-    if (count < DC) {
-      weights(count);
-      over = dc_pow(g2, count);
-    }
-    f32x4_t oc[2][4];  // out^T: channel 32 wave + 16 vt + 4 fg + r, query 16 qt + fr
-    u32x4_t vf[2][2];  // values of two ranges of 32 tokens
+    if (count < DC) counted(count);
+    f32x4_t oc[VT][QN];  // out^T: channel v0 + 16 vt + 4 fg + r, query 16 (qt0 + q) + fr
+    u32x4_t vf[2][VT];   // values of two ranges of 32 tokens
     if constexpr (OUT) {
       // ---- scores, decayed, to LDS: row = query, 16-byte slot 4 s + g = keys 32 s + 4 g + {0..3}, + 16
+      f32x4_t sc[4];
 #pragma unroll
-      for (int i = 0; i < QW; ++i) {
-        const int qt = wave + NW * i;
-        f32x4_t sc[4];
+      for (int kt = 0; kt < 4; ++kt) sc[kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int kt = 0; kt < 4; ++kt) sc[kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s < DK; ++s) {
-          const u32x4_t qf = dc_read(sq + 16 * qt * PITCH + row16[s]);
-#pragma unroll
-          for (int kt = 0; kt < 4; ++kt)
-            if (kt <= qt) sc[kt] = mfma_16x16x32<T>(dc_read(sk + 16 * kt * PITCH + row16[s]), qf, sc[kt]);
-        }
-        float most = 0.f, f = 1.f;
+      for (int s = 0; s < DK; ++s) {
+        const u32x4_t qf = dc_read(sq + 16 * wave * PITCH + row16[s]);
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            sc[kt][r] = 16 * kt + 4 * fg + r <= 16 * qt + fr ? sc[kt][r] * within[i][kt][r] : 0.f;
-            if constexpr (F) most = fmaxf(most, fabsf(sc[kt][r]));
-          }
-        if constexpr (F) {
-          most = fmaxf(most, __shfl_xor(most, 16));
-          most = fmaxf(most, __shfl_xor(most, 32));
-          f = dc_fit(most);
-          if (fg == 0) fit[16 * qt + fr] = f;
-        }
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const int q = 16 * qt + fr;
-          u32x4_t p;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const f32x4_t x = sc[2 * s + (e >> 1)];
-            p[e] = F ? pk16<T>(x[2 * (e & 1)] * f, x[2 * (e & 1) + 1] * f) : pk16<T>(x[2 * (e & 1)], x[2 * (e & 1) + 1]);
-          }
-          *reinterpret_cast<u32x4_t*>(smem + 3 * TILE + q * 128 + (((4 * s + fg) ^ ((q >> 1) & 7)) << 4)) = p;
-        }
+          if (kt <= wave) sc[kt] = mfma_16x16x32<T>(dc_read(sk + 16 * kt * PITCH + row16[s]), qf, sc[kt]);
       }
+      float most = 0.f, f = 1.f;
+      float ahead = before;  // of tile kt: a^(16 (wave - 1 - kt)), from the last in front of the diagonal on
+#pragma unroll
+      for (int kt = 3; kt >= 0; --kt) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (kt < wave) sc[kt][r] *= ahead * row4[r];
+          else sc[kt][r] = kt == wave && fr >= 4 * fg + r ? sc[kt][r] * diagonal[r] : 0.f;
+          if constexpr (F) most = fmaxf(most, fabsf(sc[kt][r]));
+        }
+        if (kt < wave) ahead *= step16;
+      }
+      if constexpr (F) {
+        most = fmaxf(most, __shfl_xor(most, 16));
+        most = fmaxf(most, __shfl_xor(most, 32));
+        f = dc_fit(most);
+        if (fg == 0) fit[16 * wave + fr] = f;
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int q = 16 * wave + fr;
+        u32x4_t p;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const f32x4_t x = sc[2 * s + (e >> 1)];
+          p[e] = F ? pk16<T>(x[2 * (e & 1)] * f, x[2 * (e & 1) + 1] * f) : pk16<T>(x[2 * (e & 1)], x[2 * (e & 1) + 1]);
+        }
+        *reinterpret_cast<u32x4_t*>(smem + 3 * TILE + q * 128 + (((4 * s + fg) ^ ((q >> 1) & 7)) << 4)) = p;
+      }
+      __builtin_amdgcn_sched_barrier(0);
       // ---- the state in front of the chunk
       float sfit = 1.f;
       if constexpr (F) {
         float most = 0.f;
 #pragma unroll
-        for (int vt = 0; vt < 2; ++vt)
+        for (int vt = 0; vt < VT; ++vt)
 #pragma unroll
           for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
@@ -239,47 +245,41 @@ __global__ __launch_bounds__(64 * NW, 2) void decay_chunk_kernel(const DecayArgs
         sfit = dc_fit(most);
       }
 #pragma unroll
-      for (int vt = 0; vt < 2; ++vt)
+      for (int vt = 0; vt < VT; ++vt)
 #pragma unroll
-        for (int qt = 0; qt < 4; ++qt) oc[vt][qt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        for (int q = 0; q < QN; ++q) oc[vt][q] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int s = 0; s < DK; ++s) {
-        u32x4_t hi[2], lo[2];
+        u32x4_t sf[VT];
 #pragma unroll
-        for (int vt = 0; vt < 2; ++vt)
+        for (int vt = 0; vt < VT; ++vt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const f32x4_t x = st[vt][2 * s + (e >> 1)];
-            const float x0 = F ? x[2 * (e & 1)] * sfit : x[2 * (e & 1)], x1 = F ? x[2 * (e & 1) + 1] * sfit : x[2 * (e & 1) + 1];
-            hi[vt][e] = pk16<T>(x0, x1);
-            lo[vt][e] = pk16<T>(x0 - lo16<T>(hi[vt][e]), x1 - hi16<T>(hi[vt][e]));
+            sf[vt][e] = F ? pk16<T>(x[2 * (e & 1)] * sfit, x[2 * (e & 1) + 1] * sfit) : pk16<T>(x[2 * (e & 1)], x[2 * (e & 1) + 1]);
           }
 #pragma unroll
-        for (int qt = 0; qt < 4; ++qt) {
-          const u32x4_t qf = dc_read(sq + 16 * qt * PITCH + row16[s]);
+        for (int q = 0; q < QN; ++q) {
+          const u32x4_t qf = dc_read(sq + 16 * (qt0 + q) * PITCH + row16[s]);
 #pragma unroll
-          for (int vt = 0; vt < 2; ++vt) {
-            oc[vt][qt] = mfma_16x16x32<T>(hi[vt], qf, oc[vt][qt]);
-            oc[vt][qt] = mfma_16x16x32<T>(lo[vt], qf, oc[vt][qt]);
-          }
+          for (int vt = 0; vt < VT; ++vt) oc[vt][q] = mfma_16x16x32<T>(sf[vt], qf, oc[vt][q]);
         }
       }
       dc_barrier();
-      float pfit[4];
 #pragma unroll
-      for (int qt = 0; qt < 4; ++qt) {
-        pfit[qt] = F ? fit[16 * qt + fr] : 1.f;
-        const float m = F ? since[qt] * pfit[qt] / sfit : since[qt];
+      for (int q = 0; q < QN; ++q) {
+        const float m = F ? since[q] * fit[16 * (qt0 + q) + fr] / sfit : since[q];
 #pragma unroll
-        for (int vt = 0; vt < 2; ++vt)
+        for (int vt = 0; vt < VT; ++vt)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) oc[vt][qt][r] *= m;
+          for (int r = 0; r < 4; ++r) oc[vt][q][r] *= m;
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int vt = 0; vt < 2; ++vt) {
+      for (int vt = 0; vt < VT; ++vt) {
         vf[s][vt] = u32x4_t{0u, 0u, 0u, 0u};
         if (own) {
           const u32x2_t x = dc_read_tr(vt_at[vt] + 32 * s * PITCH), y = dc_read_tr(vt_at[vt] + (32 * s + 16) * PITCH);
@@ -291,38 +291,40 @@ __global__ __launch_bounds__(64 * NW, 2) void decay_chunk_kernel(const DecayArgs
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
-        for (int qt = 2 * s; qt < 4; ++qt) {  // (queries of the first 32 see none of the second 32 tokens)
-          const int q = 16 * qt + fr;
-          const u32x4_t pf = dc_read(sp + q * 128 + (((4 * s + fg) ^ ((q >> 1) & 7)) << 4));
+        for (int q = 0; q < QN; ++q) {
+          if (NQ == 1 && 2 * s > q) continue;  // (queries of the first 32 see none of the second 32 tokens)
+          const int row = 16 * (qt0 + q) + fr;
+          const u32x4_t pf = dc_read(sp + row * 128 + (((4 * s + fg) ^ ((row >> 1) & 7)) << 4));
 #pragma unroll
-          for (int vt = 0; vt < 2; ++vt) oc[vt][qt] = mfma_16x16x32<T>(vf[s][vt], pf, oc[vt][qt]);
+          for (int vt = 0; vt < VT; ++vt) oc[vt][q] = mfma_16x16x32<T>(vf[s][vt], pf, oc[vt][q]);
         }
       uint16_t* o = a.out + b * a.o_b + (int64_t)at * a.o_n + h * d;
 #pragma unroll
-      for (int qt = 0; qt < 4; ++qt) {
-        const int q = 16 * qt + fr;
-        const float m = F ? 1.0f / fit[q] : 1.f;
+      for (int q = 0; q < QN; ++q) {
+        const int row = 16 * (qt0 + q) + fr;
+        const float m = F ? 1.0f / fit[row] : 1.f;
 #pragma unroll
-        for (int vt = 0; vt < 2; ++vt) {
-          const int c = 32 * wave + 16 * vt + 4 * fg;
-          const f32x4_t x = oc[vt][qt];
-          if (q < count && c < d)
-            *reinterpret_cast<u32x2_t*>(o + (int64_t)q * a.o_n + c) =
+        for (int vt = 0; vt < VT; ++vt) {
+          const int c = v0 + 16 * vt + 4 * fg;
+          const f32x4_t x = oc[vt][q];
+          if (row >= DC - count && c < d)
+            *reinterpret_cast<u32x2_t*>(o + (int64_t)(row - (DC - count)) * a.o_n + c) =
                 F ? u32x2_t{pk16<T>(x[0] * m, x[1] * m), pk16<T>(x[2] * m, x[3] * m)} : u32x2_t{pk16<T>(x[0], x[1]), pk16<T>(x[2], x[3])};
         }
       }
     }
     // ---- the state behind the chunk
+    __builtin_amdgcn_sched_barrier(0);
     if (own) {
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        constexpr int TERMS = F ? 2 : 3;
-        u32x4_t w[TERMS][2];
+        __builtin_amdgcn_sched_barrier(0);
+        u32x4_t w[TERMS][VT];
 #pragma unroll
-        for (int vt = 0; vt < 2; ++vt)
+        for (int vt = 0; vt < VT; ++vt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            float x0 = lo16<T>(vf[s][vt][e]) * to_end[s][2 * e], x1 = hi16<T>(vf[s][vt][e]) * to_end[s][2 * e + 1];
+            float x0 = lo16<T>(vf[s][vt][e]) * (lane12 * to_end[s][2 * e]), x1 = hi16<T>(vf[s][vt][e]) * (lane12 * to_end[s][2 * e + 1]);
 #pragma unroll
             for (int i = 0; i < TERMS; ++i) {
               w[i][vt][e] = pk16<T>(x0, x1);
@@ -336,7 +338,7 @@ __global__ __launch_bounds__(64 * NW, 2) void decay_chunk_kernel(const DecayArgs
           const u32x2_t lo = dc_read_tr(from), hi = dc_read_tr(from + 16 * PITCH);
           const u32x4_t kf = {lo.x, lo.y, hi.x, hi.y};
 #pragma unroll
-          for (int vt = 0; vt < 2; ++vt) {
+          for (int vt = 0; vt < VT; ++vt) {
             f32x4_t x = st[vt][kt];
             if (s == 0)
 #pragma unroll
@@ -357,35 +359,45 @@ __global__ __launch_bounds__(64 * NW, 2) void decay_chunk_kernel(const DecayArgs
     }
     dc_barrier();
   }
-  // ---- the state behind the last token: of the whole stream, or of this segment
-  float* to = !OUT ? a.segments + ((int64_t)bh * a.nseg + seg) * d * d : last == n ? a.state_out + (int64_t)bh * d * d : nullptr;
-  if (to)
+  // ---- the state behind the last token, or the segment's sum
+  if (MODE != DC_OUT && qt0 == 0) {
+    float* to = MODE == DC_SUMS ? a.segments + ((int64_t)bh * a.nseg + seg) * d * d : a.state_out + (int64_t)bh * d * d;
 #pragma unroll
-    for (int vt = 0; vt < 2; ++vt)
+    for (int vt = 0; vt < VT; ++vt)
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) {
-        const int v = 32 * wave + 16 * vt + fr, k = 32 * (kt >> 1) + 8 * fg + 4 * (kt & 1);
+        const int v = v0 + 16 * vt + fr, k = 32 * (kt >> 1) + 8 * fg + 4 * (kt & 1);
         if (v < d && k < d) *reinterpret_cast<f32x4_t*>(to + v * d + k) = st[vt][kt];
       }
+  }
 }
 
-// The segments' own sums -> the states in front of them: run = S0; run = a^L run + sum_s.  Four values a thread.
-__global__ __launch_bounds__(256) void decay_scan_kernel(const DecayArgs a) {
-  const int bh = blockIdx.y, b = bh / a.H, i = blockIdx.x * 256 + threadIdx.x, dd4 = a.d * a.d / 4;
+// The segments' own sums -> the states in front of them, and the one behind the last: run = S0; run = a^(tokens) run + sum.  Four
+// values a thread, eight segments requested at a time.
+__global__ __launch_bounds__(64) void decay_scan_kernel(const DecayArgs a) {
+  constexpr int AHEAD = 8;
+  const int bh = blockIdx.y, b = bh / a.H, i = blockIdx.x * 64 + threadIdx.x, dd4 = a.d * a.d / 4;
   if (i >= dd4) return;
   const int n = a.lengths ? min(max(a.lengths[b], 0), a.N) : a.N;
-  const float over = dc_pow(dc_log2(a.log_decay[bh % a.H]), a.seg_tokens);
+  const float g2 = dc_log2(a.log_decay[bh % a.H]);
   f32x4_t* s = reinterpret_cast<f32x4_t*>(a.segments) + (int64_t)bh * a.nseg * dd4 + i;
   f32x4_t run = {0.f, 0.f, 0.f, 0.f};
   if (a.state_in) run = reinterpret_cast<const f32x4_t*>(a.state_in)[(int64_t)bh * dd4 + i];
-  for (int seg = 0;; ++seg) {
-    const bool more = seg + 1 < a.nseg && (int64_t)(seg + 1) * a.seg_tokens < n;
-    const f32x4_t own = more ? s[(int64_t)seg * dd4] : f32x4_t{0.f, 0.f, 0.f, 0.f};
-    s[(int64_t)seg * dd4] = run;
-    if (!more) break;
+  const int used = (n + a.seg_tokens - 1) / a.seg_tokens;
+  for (int seg = 0; seg < used; seg += AHEAD) {
+    f32x4_t own[AHEAD];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) run[r] = fmaf(run[r], over, own[r]);
+    for (int j = 0; j < AHEAD; ++j) own[j] = s[(int64_t)min(seg + j, used - 1) * dd4];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      if (seg + j >= used) break;
+      s[(int64_t)(seg + j) * dd4] = run;
+      const float over = dc_pow(g2, min(n - (seg + j) * a.seg_tokens, a.seg_tokens));
+#pragma unroll
+      for (int r = 0; r < 4; ++r) run[r] = fmaf(run[r], over, own[j][r]);
+    }
   }
+  reinterpret_cast<f32x4_t*>(a.state_out)[(int64_t)bh * dd4 + i] = run;
 }
 
 // One token of each stream.  A row of the state is d floats in LPR lanes of four; a wave holds 64 / LPR rows at a time.
@@ -434,25 +446,27 @@ int segment_count(int B, int N, int H, int* tokens) {
   const int chunks = (N + DC - 1) / DC;
   const int64_t heads = (int64_t)B * H;
   int want = 1;
-  if (heads < 256 && chunks >= 16) want = (int)((512 + heads - 1) / heads);
+  if (heads < 256 && chunks >= 16) want = (int)(512 / heads);
   want = want > chunks / 4 ? (chunks / 4 > 1 ? chunks / 4 : 1) : want;
   const int per = (chunks + want - 1) / want;
   *tokens = per * DC;
   return (chunks + per - 1) / per;
 }
 
-template <typename T, int DK, int NW>
+template <typename T, int DK, int VT, int NV>
 int launch_chunks(const DecayArgs& a, int B, hipStream_t s) {
   const int64_t items = (int64_t)B * a.H * a.nseg;
   if (items > 0x7ffffff0) return SANA_ERR_SHAPE;
   DecayArgs args = a;
   args.items = (int)items;
-  const dim3 grid((unsigned)((items + 7) / 8 * 8)), block(64 * NW);
+  const dim3 grid((unsigned)((items + 7) / 8 * 8)), block(256);
   if (a.nseg > 1) {
-    hipLaunchKernelGGL((decay_chunk_kernel<T, DK, NW, false>), grid, block, 0, s, args);
-    hipLaunchKernelGGL(decay_scan_kernel, dim3((unsigned)((a.d * a.d / 4 + 255) / 256), (unsigned)(B * a.H)), dim3(256), 0, s, args);
+    hipLaunchKernelGGL((decay_chunk_kernel<T, DK, VT, NV, DC_SUMS>), grid, block, 0, s, args);
+    hipLaunchKernelGGL(decay_scan_kernel, dim3((unsigned)((a.d * a.d / 4 + 63) / 64), (unsigned)(B * a.H)), dim3(64), 0, s, args);
+    hipLaunchKernelGGL((decay_chunk_kernel<T, DK, VT, NV, DC_OUT>), grid, block, 0, s, args);
+  } else {
+    hipLaunchKernelGGL((decay_chunk_kernel<T, DK, VT, NV, DC_WHOLE>), grid, block, 0, s, args);
   }
-  hipLaunchKernelGGL((decay_chunk_kernel<T, DK, NW, true>), grid, block, 0, s, args);
   return hipGetLastError() == hipSuccess ? SANA_OK : SANA_ERR_LAUNCH;
 }
 
@@ -468,10 +482,10 @@ int launch_step(const DecayArgs& a, int B, hipStream_t s) {
 template <typename T>
 int decay_attention(const DecayArgs& a, int B, hipStream_t s) {
   if (a.N == 1) return launch_step<T>(a, B, s);
-  if (a.d <= 32) return launch_chunks<T, 1, 1>(a, B, s);
-  if (a.d <= 64) return launch_chunks<T, 2, 2>(a, B, s);
-  if (a.d <= 96) return launch_chunks<T, 3, 4>(a, B, s);
-  return launch_chunks<T, 4, 4>(a, B, s);
+  if (a.d <= 32) return launch_chunks<T, 1, 1, 2>(a, B, s);
+  if (a.d <= 64) return launch_chunks<T, 2, 1, 4>(a, B, s);
+  if (a.d <= 96) return launch_chunks<T, 3, 2, 4>(a, B, s);
+  return launch_chunks<T, 4, 2, 4>(a, B, s);
 }
 
 }  // namespace
