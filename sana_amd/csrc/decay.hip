@@ -41,6 +41,9 @@ __device__ __forceinline__ u32x2_t dc_read_tr(uint32_t lds) {  // 4 tokens x 16 
 __device__ __forceinline__ u32x4_t dc_read(uint32_t lds) {
   return *(__attribute__((address_space(3))) const u32x4_t*)(size_t)lds;
 }
+__device__ __forceinline__ u32x2_t dc_read8(uint32_t lds) {
+  return *(__attribute__((address_space(3))) const u32x2_t*)(size_t)lds;
+}
 // What this wave wrote to LDS is there and what it reads from there has come; loads from memory stay in flight.
 __device__ __forceinline__ void dc_barrier() {
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -63,13 +66,13 @@ __device__ __forceinline__ float dc_fit(float most) {
 // What a launch of the chunks gives: the sums of a segment alone, the outputs of segments whose states are known, or both for whole streams.
 enum { DC_SUMS, DC_OUT, DC_WHOLE };
 
-// One workgroup of four waves takes a (batch, head, segment) through its chunks.  NV of its waves share the channels of v, 16 VT
-// each, whose columns of the state stay in their registers (fp32) from chunk to chunk; where the head has fewer channels, 4 / NV waves
+// One workgroup of NW waves takes a (batch, head, segment) through its chunks.  NV of its waves share the channels of v, 16 VT
+// each, whose columns of the state stay in their registers (fp32) from chunk to chunk; where the head has fewer channels, NW / NV waves
 // with the same ones share the queries.  Each wave scores 16 queries for all, through LDS.
 // The operands of the MFMAs (16 x 16 x 32):
 //   scores^T = K Q^T   both from LDS as they lie;
 //   out^T    = S Q^T   S as its own accumulators hold it (row v of the product: lane; a lane's 8 values of k: the accumulators of two
-//                      tiles, whose rows are channels 32 s + 8 g + {0..3} and + {4..7}, by the addresses of the transposing read below);
+//                      tiles, channels 32 s + 4 g + {0..3} and + 16), Q in that order of k: two 8-byte reads;
 //   out^T   += V^T P^T V by transposing reads, P^T from LDS in the key order that these give;
 //   S       += K^T V   both by transposing reads.
 // Roundings.  Each product of the output has one operand of 16 bits that is rounded, P or S, as attention kernels round P: with the rounding of
@@ -77,18 +80,20 @@ enum { DC_SUMS, DC_OUT, DC_WHOLE };
 // 16-bit values: three of bf16 where the state is given back (fp32's accuracy; with two it is 1.3e-6 off after 32760
 // tokens), two of bf16 where it only goes on to outputs, two of f16 (22 bits), the second times 2^11, so that it stays a normal number.
 // f16 ends at 65504: S goes in scaled by a power of two for each wave, P for each query.
-template <typename T, int DK, int VT, int NV, int MODE>
-__global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) {
+template <typename T, int DK, int KT, int VT, int NV, int NW, int MODE>
+__global__ __launch_bounds__(64 * NW, NW / 2) void decay_chunk_kernel(const DecayArgs a) {
   constexpr bool OUT = MODE != DC_SUMS, F = is_f16<T>;
-  constexpr int PITCH = DK * 64, TILE = DC * PITCH, KT = 2 * DK;  // LDS row / tensor in bytes; 16-row tiles of k
-  constexpr int NT = 256, PIECES = DC * DK * 4 / NT, TERMS = F || MODE == DC_OUT ? 2 : 3;
-  constexpr int NQ = 4 / NV, QN = 4 / NQ;  // shares of the queries, query tiles of a share
-  __shared__ __attribute__((aligned(16))) unsigned char smem[(OUT ? 3 : 2) * TILE + (OUT ? DC * 128 + DC * 4 : 0)];
+  constexpr int PITCH = DK * 64, TILE = DC * PITCH;  // LDS row / tensor in bytes
+  constexpr int NT = 64 * NW, PIECES = DC * DK * 4 / NT, TERMS = F || MODE == DC_OUT ? 2 : 3;
+  constexpr int NQ = NW / NV, QN = 4 / NQ;   // shares of the queries, query tiles of a share
+  constexpr int HALVES = NW / 4, KS = 4 / HALVES;  // a wave scores 16 queries, eight waves against half of the keys each
+  static_assert(KT <= 2 * DK && DC * DK * 4 % NT == 0 && NW % NV == 0 && (NW == 4 || NW == 8) && 4 % NQ == 0, "");
+  __shared__ __attribute__((aligned(16))) unsigned char smem[(OUT ? 3 : 2) * TILE + (OUT ? DC * 128 + DC * 4 * HALVES : 0)];
   const uint32_t sk = (uint32_t)(size_t)(__attribute__((address_space(3))) unsigned char*)smem;
   const uint32_t sv = sk + TILE, sq = sk + 2 * TILE, sp = sk + 3 * TILE;
-  float* fit = reinterpret_cast<float*>(smem + 3 * TILE + DC * 128);  // f16: the scale of a query's P
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, fr = lane & 15, fg = lane >> 4;
-  const int v0 = 16 * VT * (wave % NV), qt0 = QN * (wave / NV);
+  float* fit = reinterpret_cast<float*>(smem + 3 * TILE + DC * 128);  // f16: the scales of a query's P
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), fr = tid & 15, fg = (tid >> 4) & 3;
+  const int v0 = 16 * VT * (wave % NV), qt0 = QN * (wave / NV), sqt = wave & 3, half = HALVES == 2 ? wave >> 2 : 0;
 
   // neighbouring heads, whose rows share cache lines, on one XCD
   const int per = (a.items + 7) >> 3, item = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
@@ -99,14 +104,14 @@ __global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) 
   if (MODE != DC_WHOLE && first >= n) return;
   const float g2 = dc_log2(a.log_decay[h]);
 
-  // ---- the state: st[vt][kt][r] = row v = v0 + 16 vt + fr, column k = 32 (kt / 2) + 8 fg + 4 (kt & 1) + r
+  // ---- the state: st[vt][kt][r] = row v = v0 + 16 vt + fr, column k = 16 kt + 4 fg + r
   f32x4_t st[VT][KT];
   const float* s0 = MODE == DC_SUMS ? nullptr : MODE == DC_OUT ? a.segments + ((int64_t)bh * a.nseg + seg) * d * d : a.state_in ? a.state_in + (int64_t)bh * d * d : nullptr;
 #pragma unroll
   for (int vt = 0; vt < VT; ++vt)
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
-      const int v = v0 + 16 * vt + fr, k = 32 * (kt >> 1) + 8 * fg + 4 * (kt & 1);
+      const int v = v0 + 16 * vt + fr, k = 16 * kt + 4 * fg;
       st[vt][kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
       if (s0 && v < d && k < d) st[vt][kt] = *reinterpret_cast<const f32x4_t*>(s0 + v * d + k);
     }
@@ -139,25 +144,43 @@ __global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) 
   };
   counted(DC);
 
-  // ---- a chunk's rows: requested into registers a chunk ahead, then to LDS
+  // ---- a chunk's rows: requested into registers a chunk ahead, then to LDS.  K, Q and V each at a time of its own: a wave that issues
+  // more loads than the memory pipeline holds waits there, and the LDS tile of V is not needed before the scores are done.
   u32x4_t rk[PIECES], rv[PIECES], rq[OUT ? PIECES : 1];
   const uint32_t k2 = 2 * (uint32_t)a.k_n, v2 = 2 * (uint32_t)a.v_n, q2 = 2 * (uint32_t)a.q_n;
-  auto request = [&](int at) {
+  auto request = [&](const uint16_t* tokens, int64_t stride, uint32_t ld2, int at, u32x4_t* r) {
     const int count = min(last - at, DC), empty = DC - count;
-    auto rows = [&](const uint16_t* base, uint32_t ld2, u32x4_t* r) {
-      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base), 0, (int)((uint32_t)(count - 1) * ld2 + 2 * d), 0x00020000);
+    const __amdgpu_buffer_rsrc_t rs =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(tokens + (int64_t)at * stride), 0, (int)((uint32_t)(count - 1) * ld2 + 2 * d), 0x00020000);
+    // (outside, as rows below 0 are: zeros.  63 rows are less than 2^31 bytes, so nothing comes back in)
+    if constexpr (NT % (DK * 4) == 0) {
+      const int row = tid / (DK * 4), c = tid - row * (DK * 4);
+      const uint32_t off = (8 * c < d ? (uint32_t)row * ld2 + 16 * c : 0x80000000u) - empty * ld2;
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i)
+        r[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rs, (int)(off + i * (NT / (DK * 4)) * ld2), 0, 0));
+    } else {
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
         const int idx = tid + NT * i, row = idx / (DK * 4), c = idx - row * (DK * 4);
-        const uint32_t off = 8 * c < d ? (uint32_t)(row - empty) * ld2 + 16 * c : 0x80000000u;  // (outside, as rows below 0 are: zeros)
+        const uint32_t off = 8 * c < d ? (uint32_t)(row - empty) * ld2 + 16 * c : 0x80000000u;
         r[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rs, (int)off, 0, 0));
       }
-    };
-    rows(a.k + b * a.k_b + (int64_t)at * a.k_n + h * d, k2, rk);
-    if constexpr (OUT) rows(a.q + b * a.q_b + (int64_t)at * a.q_n + h * d, q2, rq);
-    rows(a.v + b * a.v_b + (int64_t)at * a.v_n + h * d, v2, rv);
+    }
   };
-  if (first < last) request(first);
+  auto stage = [&](const u32x4_t* r, int tile) {
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const int idx = tid + NT * i, row = idx / (DK * 4), c = idx - row * (DK * 4);
+      *reinterpret_cast<u32x4_t*>(smem + tile * TILE + row * PITCH + ((c ^ dc_key<DK>(row)) << 4)) = r[i];
+    }
+  };
+  const uint16_t *kp = a.k + b * a.k_b + h * d, *vp = a.v + b * a.v_b + h * d, *qp = a.q + b * a.q_b + h * d;
+  if (first < last) {
+    request(kp, a.k_n, k2, first, rk);
+    if constexpr (OUT) request(qp, a.q_n, q2, first, rq);
+    request(vp, a.v_n, v2, first, rv);
+  }
 
   // ---- this lane's places in LDS
   const int key = dc_key<DK>(fr);
@@ -165,69 +188,68 @@ __global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) 
 #pragma unroll
   for (int s = 0; s < DK; ++s) row16[s] = fr * PITCH + (((4 * s + fg) ^ key) << 4);
   const int trow = 4 * fg + (fr >> 2), tkey = dc_key<DK>(trow), piece = fr & 3;  // of a transposing read
-  uint32_t vt_at[VT], kt_at[DK];
+  uint32_t vt_at[VT];
 #pragma unroll
   for (int vt = 0; vt < VT; ++vt) vt_at[vt] = sv + trow * PITCH + (((v0 / 8 + 2 * vt + (piece >> 1)) ^ tkey) << 4) + 8 * (piece & 1);
-#pragma unroll
-  for (int s = 0; s < DK; ++s) kt_at[s] = sk + trow * PITCH + (((4 * s + piece) ^ tkey) << 4);
+  auto kt_at = [&](int kt) { return sk + trow * PITCH + (((2 * kt + (piece >> 1)) ^ tkey) << 4) + 8 * (piece & 1); };
+  auto row8 = [&](int kt) { return (uint32_t)(fr * PITCH + (((2 * kt + (fg >> 1)) ^ key) << 4) + 8 * (fg & 1)); };  // row fr, k = 16 kt + 4 fg
   const bool own = v0 < 32 * DK;  // (DK = 3: the fourth wave has no channels of v, and its reads would leave the rows)
 
 #pragma unroll 1
   for (int at = first; at < last; at += DC) {
-    const int count = min(last - at, DC);
-#pragma unroll
-    for (int i = 0; i < PIECES; ++i) {
-      const int idx = tid + NT * i, row = idx / (DK * 4), c = idx - row * (DK * 4);
-      const uint32_t to = row * PITCH + ((c ^ dc_key<DK>(row)) << 4);
-      *reinterpret_cast<u32x4_t*>(smem + to) = rk[i];
-      if constexpr (OUT) *reinterpret_cast<u32x4_t*>(smem + 2 * TILE + to) = rq[i];
-      *reinterpret_cast<u32x4_t*>(smem + TILE + to) = rv[i];
-    }
+    const int count = min(last - at, DC), next = at + DC;
+    const bool more = next < last;
+    stage(rk, 0);
+    if constexpr (OUT) stage(rq, 2);
+    else stage(rv, 1);
     dc_barrier();
-    if (at + DC < last) request(at + DC);
+    if (more) request(kp, a.k_n, k2, next, rk);
+    __builtin_amdgcn_sched_barrier(0);
     if (count < DC) counted(count);
     f32x4_t oc[VT][QN];  // out^T: channel v0 + 16 vt + 4 fg + r, query 16 (qt0 + q) + fr
     u32x4_t vf[2][VT];   // values of two ranges of 32 tokens
     if constexpr (OUT) {
       // ---- scores, decayed, to LDS: row = query, 16-byte slot 4 s + g = keys 32 s + 4 g + {0..3}, + 16
-      f32x4_t sc[4];
+      f32x4_t sc[KS];
 #pragma unroll
-      for (int kt = 0; kt < 4; ++kt) sc[kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      for (int kt = 0; kt < KS; ++kt) sc[kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int s = 0; s < DK; ++s) {
-        const u32x4_t qf = dc_read(sq + 16 * wave * PITCH + row16[s]);
+        const u32x4_t qf = dc_read(sq + 16 * sqt * PITCH + row16[s]);
 #pragma unroll
-        for (int kt = 0; kt < 4; ++kt)
-          if (kt <= wave) sc[kt] = mfma_16x16x32<T>(dc_read(sk + 16 * kt * PITCH + row16[s]), qf, sc[kt]);
+        for (int kt = 0; kt < KS; ++kt)
+          if (KS * half + kt <= sqt) sc[kt] = mfma_16x16x32<T>(dc_read(sk + 16 * (KS * half + kt) * PITCH + row16[s]), qf, sc[kt]);
       }
       float most = 0.f, f = 1.f;
-      float ahead = before;  // of tile kt: a^(16 (wave - 1 - kt)), from the last in front of the diagonal on
+      float ahead = before;  // of tile kt: a^(16 (tiles between it and the diagonal)), from the last in front of the diagonal on
+      if (HALVES == 2 && half == 0 && sqt > 2) ahead *= step16;
 #pragma unroll
-      for (int kt = 3; kt >= 0; --kt) {
+      for (int kt = KS - 1; kt >= 0; --kt) {
+        const int tile = KS * half + kt;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          if (kt < wave) sc[kt][r] *= ahead * row4[r];
-          else sc[kt][r] = kt == wave && fr >= 4 * fg + r ? sc[kt][r] * diagonal[r] : 0.f;
+          if (tile < sqt) sc[kt][r] *= ahead * row4[r];
+          else sc[kt][r] = tile == sqt && fr >= 4 * fg + r ? sc[kt][r] * diagonal[r] : 0.f;
           if constexpr (F) most = fmaxf(most, fabsf(sc[kt][r]));
         }
-        if (kt < wave) ahead *= step16;
+        if (tile < sqt) ahead *= step16;
       }
       if constexpr (F) {
         most = fmaxf(most, __shfl_xor(most, 16));
         most = fmaxf(most, __shfl_xor(most, 32));
         f = dc_fit(most);
-        if (fg == 0) fit[16 * wave + fr] = f;
+        if (fg == 0) fit[DC * half + 16 * sqt + fr] = f;
       }
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const int q = 16 * wave + fr;
+      for (int s = 0; s < KS / 2; ++s) {
+        const int q = 16 * sqt + fr, at16 = 4 * ((KS / 2) * half + s) + fg;
         u32x4_t p;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const f32x4_t x = sc[2 * s + (e >> 1)];
           p[e] = F ? pk16<T>(x[2 * (e & 1)] * f, x[2 * (e & 1) + 1] * f) : pk16<T>(x[2 * (e & 1)], x[2 * (e & 1) + 1]);
         }
-        *reinterpret_cast<u32x4_t*>(smem + 3 * TILE + q * 128 + (((4 * s + fg) ^ ((q >> 1) & 7)) << 4)) = p;
+        *reinterpret_cast<u32x4_t*>(smem + 3 * TILE + q * 128 + ((at16 ^ ((q >> 1) & 7)) << 4)) = p;
       }
       __builtin_amdgcn_sched_barrier(0);
       // ---- the state in front of the chunk
@@ -255,17 +277,27 @@ __global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) 
         for (int vt = 0; vt < VT; ++vt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
+            if (2 * s + (e >> 1) >= KT) {
+              sf[vt][e] = 0u;
+              continue;
+            }
             const f32x4_t x = st[vt][2 * s + (e >> 1)];
             sf[vt][e] = F ? pk16<T>(x[2 * (e & 1)] * sfit, x[2 * (e & 1) + 1] * sfit) : pk16<T>(x[2 * (e & 1)], x[2 * (e & 1) + 1]);
           }
 #pragma unroll
         for (int q = 0; q < QN; ++q) {
-          const u32x4_t qf = dc_read(sq + 16 * (qt0 + q) * PITCH + row16[s]);
+          const uint32_t from = sq + 16 * (qt0 + q) * PITCH;
+          const u32x2_t lo = dc_read8(from + row8(2 * s)), hi = dc_read8(from + row8(2 * s + 1));
+          const u32x4_t qf = {lo.x, lo.y, hi.x, hi.y};
 #pragma unroll
           for (int vt = 0; vt < VT; ++vt) oc[vt][q] = mfma_16x16x32<T>(sf[vt], qf, oc[vt][q]);
         }
       }
+      stage(rv, 1);
+      if (more) request(qp, a.q_n, q2, next, rq);
       dc_barrier();
+      if (more) request(vp, a.v_n, v2, next, rv);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int q = 0; q < QN; ++q) {
         const float m = F ? since[q] * fit[16 * (qt0 + q) + fr] / sfit : since[q];
@@ -294,26 +326,39 @@ __global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) 
         for (int q = 0; q < QN; ++q) {
           if (NQ == 1 && 2 * s > q) continue;  // (queries of the first 32 see none of the second 32 tokens)
           const int row = 16 * (qt0 + q) + fr;
+          if (F && HALVES == 2 && s == 1) {
+            const float m = fit[DC + row] / fit[row];
+#pragma unroll
+            for (int vt = 0; vt < VT; ++vt)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) oc[vt][q][r] *= m;
+          }
           const u32x4_t pf = dc_read(sp + row * 128 + (((4 * s + fg) ^ ((row >> 1) & 7)) << 4));
 #pragma unroll
           for (int vt = 0; vt < VT; ++vt) oc[vt][q] = mfma_16x16x32<T>(vf[s][vt], pf, oc[vt][q]);
         }
-      uint16_t* o = a.out + b * a.o_b + (int64_t)at * a.o_n + h * d;
+      // (rows below 0 and channels past d lie outside the resource: not stored)
+      const uint32_t o2 = 2 * (uint32_t)a.o_n;
+      const __amdgpu_buffer_rsrc_t ro =
+          __builtin_amdgcn_make_buffer_rsrc(a.out + b * a.o_b + (int64_t)at * a.o_n + h * d, 0, (int)((uint32_t)(count - 1) * o2 + 2 * d), 0x00020000);
 #pragma unroll
       for (int q = 0; q < QN; ++q) {
         const int row = 16 * (qt0 + q) + fr;
-        const float m = F ? 1.0f / fit[row] : 1.f;
+        const float m = F ? 1.0f / fit[row + (HALVES == 2 && (NQ > 1 || q >= 2) ? DC : 0)] : 1.f;  // (of the half that came last)
 #pragma unroll
         for (int vt = 0; vt < VT; ++vt) {
           const int c = v0 + 16 * vt + 4 * fg;
+          const uint32_t off = (c < d ? (uint32_t)(16 * qt0 + fr) * o2 + 2 * c : 0x80000000u) - (DC - count) * o2 + 16 * q * o2;
           const f32x4_t x = oc[vt][q];
-          if (row >= DC - count && c < d)
-            *reinterpret_cast<u32x2_t*>(o + (int64_t)(row - (DC - count)) * a.o_n + c) =
-                F ? u32x2_t{pk16<T>(x[0] * m, x[1] * m), pk16<T>(x[2] * m, x[3] * m)} : u32x2_t{pk16<T>(x[0], x[1]), pk16<T>(x[2], x[3])};
+          const u32x2_t y = F ? u32x2_t{pk16<T>(x[0] * m, x[1] * m), pk16<T>(x[2] * m, x[3] * m)} : u32x2_t{pk16<T>(x[0], x[1]), pk16<T>(x[2], x[3])};
+          __builtin_amdgcn_raw_buffer_store_b64(y, ro, (int)off, 0, 0);
         }
       }
     }
-    // ---- the state behind the chunk
+    // ---- the state behind the chunk.  bf16 sums are weighted up to the segment's end at once and need no decay (f16 would run out of range)
+    constexpr bool FAR = MODE == DC_SUMS && !F;
+    if (!OUT && more) request(vp, a.v_n, v2, next, rv);
+    const float lane = FAR ? lane12 * dc_pow(g2, last - at - count) : lane12;
     __builtin_amdgcn_sched_barrier(0);
     if (own) {
 #pragma unroll
@@ -324,7 +369,7 @@ __global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) 
         for (int vt = 0; vt < VT; ++vt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            float x0 = lo16<T>(vf[s][vt][e]) * (lane12 * to_end[s][2 * e]), x1 = hi16<T>(vf[s][vt][e]) * (lane12 * to_end[s][2 * e + 1]);
+            float x0 = lo16<T>(vf[s][vt][e]) * (lane * to_end[s][2 * e]), x1 = hi16<T>(vf[s][vt][e]) * (lane * to_end[s][2 * e + 1]);
 #pragma unroll
             for (int i = 0; i < TERMS; ++i) {
               w[i][vt][e] = pk16<T>(x0, x1);
@@ -334,13 +379,13 @@ __global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) 
           }
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) {
-          const uint32_t from = kt_at[kt >> 1] + 8 * (kt & 1) + 32 * s * PITCH;
+          const uint32_t from = kt_at(kt) + 32 * s * PITCH;
           const u32x2_t lo = dc_read_tr(from), hi = dc_read_tr(from + 16 * PITCH);
           const u32x4_t kf = {lo.x, lo.y, hi.x, hi.y};
 #pragma unroll
           for (int vt = 0; vt < VT; ++vt) {
             f32x4_t x = st[vt][kt];
-            if (s == 0)
+            if (s == 0 && !FAR)
 #pragma unroll
               for (int r = 0; r < 4; ++r) x[r] *= over;
             if constexpr (F) {
@@ -366,7 +411,7 @@ __global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) 
     for (int vt = 0; vt < VT; ++vt)
 #pragma unroll
       for (int kt = 0; kt < KT; ++kt) {
-        const int v = v0 + 16 * vt + fr, k = 32 * (kt >> 1) + 8 * fg + 4 * (kt & 1);
+        const int v = v0 + 16 * vt + fr, k = 16 * kt + 4 * fg;
         if (v < d && k < d) *reinterpret_cast<f32x4_t*>(to + v * d + k) = st[vt][kt];
       }
   }
@@ -453,19 +498,19 @@ int segment_count(int B, int N, int H, int* tokens) {
   return (chunks + per - 1) / per;
 }
 
-template <typename T, int DK, int VT, int NV>
+template <typename T, int DK, int KT, int VT, int NV, int NW>
 int launch_chunks(const DecayArgs& a, int B, hipStream_t s) {
   const int64_t items = (int64_t)B * a.H * a.nseg;
   if (items > 0x7ffffff0) return SANA_ERR_SHAPE;
   DecayArgs args = a;
   args.items = (int)items;
-  const dim3 grid((unsigned)((items + 7) / 8 * 8)), block(256);
+  const dim3 grid((unsigned)((items + 7) / 8 * 8)), block(64 * NW);
   if (a.nseg > 1) {
-    hipLaunchKernelGGL((decay_chunk_kernel<T, DK, VT, NV, DC_SUMS>), grid, block, 0, s, args);
+    hipLaunchKernelGGL((decay_chunk_kernel<T, DK, KT, VT, NV, NW, DC_SUMS>), grid, block, 0, s, args);
     hipLaunchKernelGGL(decay_scan_kernel, dim3((unsigned)((a.d * a.d / 4 + 63) / 64), (unsigned)(B * a.H)), dim3(64), 0, s, args);
-    hipLaunchKernelGGL((decay_chunk_kernel<T, DK, VT, NV, DC_OUT>), grid, block, 0, s, args);
+    hipLaunchKernelGGL((decay_chunk_kernel<T, DK, KT, VT, NV, NW, DC_OUT>), grid, block, 0, s, args);
   } else {
-    hipLaunchKernelGGL((decay_chunk_kernel<T, DK, VT, NV, DC_WHOLE>), grid, block, 0, s, args);
+    hipLaunchKernelGGL((decay_chunk_kernel<T, DK, KT, VT, NV, NW, DC_WHOLE>), grid, block, 0, s, args);
   }
   return hipGetLastError() == hipSuccess ? SANA_OK : SANA_ERR_LAUNCH;
 }
@@ -482,10 +527,11 @@ int launch_step(const DecayArgs& a, int B, hipStream_t s) {
 template <typename T>
 int decay_attention(const DecayArgs& a, int B, hipStream_t s) {
   if (a.N == 1) return launch_step<T>(a, B, s);
-  if (a.d <= 32) return launch_chunks<T, 1, 1, 2>(a, B, s);
-  if (a.d <= 64) return launch_chunks<T, 2, 1, 4>(a, B, s);
-  if (a.d <= 96) return launch_chunks<T, 3, 2, 4>(a, B, s);
-  return launch_chunks<T, 4, 2, 4>(a, B, s);
+  if (a.d <= 32) return launch_chunks<T, 1, 2, 1, 2, 4>(a, B, s);
+  if (a.d <= 64) return launch_chunks<T, 2, 4, 1, 4, 4>(a, B, s);
+  if (a.d <= 96) return launch_chunks<T, 3, 6, 2, 4, 4>(a, B, s);
+  if (a.d <= 112) return launch_chunks<T, 4, 7, 2, 4, 4>(a, B, s);
+  return launch_chunks<T, 4, 8, 2, 4, 4>(a, B, s);
 }
 
 }  // namespace
