@@ -8,6 +8,7 @@
 // What a stream keeps of its past is a cache of sinks + window rows: row p for a position p below the sinks, then a ring.
 // The order of the keys does not matter to the sum, so a token's attention reads the rows as they lie.
 #include <initializer_list>
+#include <type_traits>
 
 #include "common.h"
 
@@ -33,13 +34,12 @@ template <int DK>
 __device__ __forceinline__ int wa_key(int row) {
   return DK == 4 ? (row & 15) : DK == 2 ? ((row >> 1) & 7) : ((row >> 2) & 3);
 }
-__device__ __forceinline__ u32x2_t wa_read_tr(uint32_t lds) {  // 4 keys x 16 channels -> this lane's channel, 4 keys
+typedef __attribute__((address_space(3))) unsigned char wa_lds;  // (pointers, not integers: the compiler sees which array is read)
+__device__ __forceinline__ u32x2_t wa_read_tr(wa_lds* at) {  // 4 keys x 16 channels -> this lane's channel, 4 keys
   typedef short s16x4_t __attribute__((ext_vector_type(4)));
-  return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(size_t)lds));
+  return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)at));
 }
-__device__ __forceinline__ u32x4_t wa_read(uint32_t lds) {
-  return *(__attribute__((address_space(3))) const u32x4_t*)(size_t)lds;
-}
+__device__ __forceinline__ u32x4_t wa_read(const wa_lds* at) { return *(__attribute__((address_space(3))) const u32x4_t*)at; }
 // What this wave wrote to LDS is there and what it reads from there has come; loads from memory stay in flight.
 __device__ __forceinline__ void wa_barrier() {
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -64,10 +64,9 @@ __device__ __forceinline__ float wa_sum_groups(float x) {
 // subnormal numbers.
 template <typename T, int DK, int DT, int QT, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void window_attn_kernel(const WindowArgs a) {
-  constexpr int PITCH = DK * 64, TILE = WK * PITCH, NT = 64 * NW, PIECES = WK * DK * 4 / NT, QB = NW * 16 * QT;
-  static_assert(WK * DK * 4 % NT == 0 && DT <= 2 * DK, "");
-  __shared__ __attribute__((aligned(16))) unsigned char smem[4 * TILE];  // two buffers of K, V
-  const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) unsigned char*)smem;
+  constexpr int PITCH = DK * 64, TILE = WK * PITCH, LOADS = TILE / 1024 / NW, QB = NW * 16 * QT;
+  static_assert(TILE % (1024 * NW) == 0 && DT <= 2 * DK, "");
+  __shared__ __attribute__((aligned(1024))) unsigned char k_even[TILE], k_odd[TILE], v_even[TILE], v_odd[TILE];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, fr = lane & 15, fg = lane >> 4;
 
   // the blocks of one head, which read the same keys, on one XCD
@@ -100,31 +99,34 @@ __global__ __launch_bounds__(64 * NW, 2) void window_attn_kernel(const WindowArg
   }
   const int wp0 = past + w0, wp1 = min(wp0 + 16 * QT - 1, p1);
 
-  u32x4_t rk[PIECES], rv[PIECES];
-  const uint16_t* kb = a.k + b * a.k_b + hk * d;
-  const uint16_t* vb = a.v + b * a.v_b + hk * d;
+  // K and V of a tile by direct loads to LDS, 1 KB each: a lane's 16 bytes are at the place that its number gives, so it fetches
+  // the piece that the row's exchange puts there.  Outside of the rows: zeros.  (63 rows are less than 2^31 bytes: nothing comes back in.)
+  const uint16_t *kp = a.k + b * a.k_b + hk * d, *vp = a.v + b * a.v_b + hk * d;
   const uint32_t k2 = 2 * (uint32_t)a.k_n, v2 = 2 * (uint32_t)a.v_n;
   auto tile_of = [&](int t) { return t < sink_tiles ? t : band_tile + (t - sink_tiles); };
-  auto request = [&](int t) {
+  auto request = [&](const uint16_t* rows, int64_t stride, uint32_t ld2, int t, unsigned char* to) {
     const int j0 = tile_of(t) * WK, count = min(keys - j0, WK);
-    auto rows = [&](const uint16_t* base, uint32_t ld2, u32x4_t* r) {
-      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base), 0, (int)((uint32_t)(count - 1) * ld2 + 2 * d), 0x00020000);
+    const __amdgpu_buffer_rsrc_t rs =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(rows + (int64_t)j0 * stride), 0, (int)((uint32_t)(count - 1) * ld2 + 2 * d), 0x00020000);
 #pragma unroll
-      for (int i = 0; i < PIECES; ++i) {
-        const int idx = tid + NT * i, row = idx / (DK * 4), c = idx - row * (DK * 4);
-        const uint32_t off = 8 * c < d ? (uint32_t)row * ld2 + 16 * c : 0x80000000u;  // (outside: zeros)
-        r[i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rs, (int)off, 0, 0));
-      }
-    };
-    rows(kb + (int64_t)j0 * a.k_n, k2, rk);
-    rows(vb + (int64_t)j0 * a.v_n, v2, rv);
+    for (int i = 0; i < LOADS; ++i) {
+      const int at = 64 * (NW * i + wave) + lane, row = at / (4 * DK), c = (at - row * (4 * DK)) ^ wa_key<DK>(row);
+      const uint32_t off = 8 * c < d ? (uint32_t)row * ld2 + 16 * c : 0x80000000u;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (wa_lds*)(to + 1024 * (NW * i + wave)), 16, (int)off, 0, 0, 0);
+    }
+  };
+  auto landed = [&]() {  // this wave's loads have, and everyone's behind the barrier
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0), as a builtin: the compiler counts on it and waits for no tile a second time
+    wa_barrier();
   };
 
   const int key = wa_key<DK>(fr), trow = 4 * fg + (fr >> 2), tkey = wa_key<DK>(trow), piece = fr & 3;
   uint32_t k_at[DK];
 #pragma unroll
   for (int s = 0; s < DK; ++s) k_at[s] = fr * PITCH + (((4 * s + fg) ^ key) << 4);
-  auto v_at = [&](int dt) { return (uint32_t)(TILE + trow * PITCH + (((2 * dt + (piece >> 1)) ^ tkey) << 4) + 8 * (piece & 1)); };
+  uint32_t v_slot = ((piece >> 1) ^ tkey) << 4;
+  const uint32_t v_row = trow * PITCH + 8 * (piece & 1);
+  auto v_at = [&](int dt) { return v_row + (v_slot ^ (dt << 5)); };  // slot (2 dt + (piece >> 1)) ^ tkey
 
   f32x4_t oc[QT][DT];  // out^T: channel 16 dt + 4 fg + r, query fr
   float mx[QT], sub[QT], sum[QT];
@@ -134,59 +136,54 @@ __global__ __launch_bounds__(64 * NW, 2) void window_attn_kernel(const WindowArg
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) oc[t][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
-
-  if (t0 < t1) request(t0);
-#pragma unroll 1
-  for (int t = t0; t < t1; ++t) {
-    const uint32_t buf = (t - t0) & 1 ? 2 * TILE : 0;
-#pragma unroll
-    for (int i = 0; i < PIECES; ++i) {
-      const int idx = tid + NT * i, row = idx / (DK * 4), c = idx - row * (DK * 4);
-      const uint32_t to = buf + row * PITCH + ((c ^ wa_key<DK>(row)) << 4);
-      *reinterpret_cast<u32x4_t*>(smem + to) = rk[i];
-      *reinterpret_cast<u32x4_t*>(smem + to + TILE) = rv[i];
-    }
-    wa_barrier();  // (also: everyone is done with the tile before the last, whose buffer is written next)
-    if (t + 1 < t1) request(t + 1);
+  auto whole = [&](int t) {  // whether this wave's queries see all keys of a tile (uniform)
     const int j0 = tile_of(t) * WK, j1 = j0 + WK - 1;
-    if (w0 >= queries || j0 > wp1 || (wp0 - j1 >= a.window && j0 >= a.sinks)) continue;  // (uniform; no barrier below)
-    const bool whole = j1 <= wp0 && (j1 < a.sinks || wp1 - j0 < a.window);
-    // ---- scores
-    f32x4_t sc[QT][4];
+    return j1 <= wp0 && (j1 < a.sinks || wp1 - j0 < a.window);
+  };
+  auto load_keys = [&](const unsigned char* from, int kt, u32x4_t (&kf)[DK]) {
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
+    for (int s = 0; s < DK; ++s) kf[s] = wa_read((const wa_lds*)from + 16 * kt * PITCH + k_at[s]);
+  };
+  auto multiply_keys = [&](int kt, const u32x4_t (&kf)[DK], f32x4_t (&sc)[QT][4]) {
 #pragma unroll
-      for (int q = 0; q < QT; ++q) sc[q][kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int q = 0; q < QT; ++q) sc[q][kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int s = 0; s < DK; ++s) {
-        const u32x4_t kf = wa_read(lds0 + buf + 16 * kt * PITCH + k_at[s]);
+    for (int s = 0; s < DK; ++s)
 #pragma unroll
-        for (int q = 0; q < QT; ++q) sc[q][kt] = mfma_16x16x32<T>(kf, qf[q][s], sc[q][kt]);
-      }
-    }
-    // ---- softmax
-    u32x2_t pk[QT][4];
+      for (int q = 0; q < QT; ++q) sc[q][kt] = mfma_16x16x32<T>(kf[s], qf[q][s], sc[q][kt]);
+  };
+  auto mask = [&](int t, f32x4_t (&sc)[QT][4]) {
+    const int lane_key = tile_of(t) * WK + 4 * fg, to_sinks = a.sinks - lane_key;  // c = 16 kt + r is key lane_key + c
 #pragma unroll
     for (int q = 0; q < QT; ++q) {
-      if (!whole) {
-        const int p = past + w0 + 16 * q + fr;
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int j = j0 + 16 * kt + 4 * fg + r;
-            if (!(j <= p && (p - j < a.window || j < a.sinks))) sc[q][kt][r] = -INFINITY;
-          }
-      }
-      // (the scale is positive: the maximum of the scaled scores is the scaled maximum)
-      float most = -INFINITY;
+      const int to_query = past + w0 + 16 * q + fr - lane_key, to_window = to_query - a.window;
 #pragma unroll
       for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) most = fmaxf(most, sc[q][kt][r]);
-      most *= a.scale_log2e;
-      if (__any(most > mx[q] + 8.f)) {
-        const float now = fmaxf(mx[q], wa_max_groups(most));
+        for (int r = 0; r < 4; ++r) {
+          const int c = 16 * kt + r;
+          if ((c > to_query) | ((c <= to_window) & (c >= to_sinks))) sc[q][kt][r] = -INFINITY;
+        }
+    }
+  };
+  auto maxima = [&](const f32x4_t (&sc)[QT][4]) {
+    // (the scale is positive: the maximum of the scaled scores is the scaled maximum)
+    float most[QT];
+    bool above = false;
+#pragma unroll
+    for (int q = 0; q < QT; ++q) {
+      most[q] = -INFINITY;
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) most[q] = fmaxf(most[q], sc[q][kt][r]);
+      most[q] *= a.scale_log2e;
+      above |= most[q] > mx[q] + 8.f;
+    }
+    if (__any(above)) {
+#pragma unroll
+      for (int q = 0; q < QT; ++q) {
+        const float now = fmaxf(mx[q], wa_max_groups(most[q]));
         const float f = __builtin_amdgcn_exp2f(mx[q] - (now == -INFINITY ? 0.f : now));  // (nothing yet: 0)
         mx[q] = now, sub[q] = now == -INFINITY ? 0.f : now - kShift<T>;
         sum[q] *= f;
@@ -195,29 +192,75 @@ __global__ __launch_bounds__(64 * NW, 2) void window_attn_kernel(const WindowArg
 #pragma unroll
           for (int r = 0; r < 4; ++r) oc[q][dt][r] *= f;
       }
-#pragma unroll
-      for (int kt = 0; kt < 4; ++kt) {
-        float p[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          p[r] = __builtin_amdgcn_exp2f(fmaf(sc[q][kt][r], a.scale_log2e, -sub[q]));
-          sum[q] += p[r];
-        }
-        pk[q][kt] = u32x2_t{pk16<T>(p[0], p[1]), pk16<T>(p[2], p[3])};
-      }
     }
-    // ---- values
+  };
+  auto powers = [&](int q, int kt, const f32x4_t (&sc)[QT][4], u32x2_t (&pk)[QT][4]) {
+    float p[4];
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+    for (int r = 0; r < 4; ++r) {
+      p[r] = __builtin_amdgcn_exp2f(fmaf(sc[q][kt][r], a.scale_log2e, -sub[q]));
+      sum[q] += p[r];
+    }
+    pk[q][kt] = u32x2_t{pk16<T>(p[0], p[1]), pk16<T>(p[2], p[3])};
+  };
+  auto values = [&](unsigned char* from, int s, const u32x2_t (&pk)[QT][4]) {
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        const uint32_t from = lds0 + buf + v_at(dt) + 32 * s * PITCH;
-        const u32x2_t x = wa_read_tr(from), y = wa_read_tr(from + 16 * PITCH);
-        const u32x4_t vf = {x.x, x.y, y.x, y.y};
+    for (int dt = 0; dt < DT; ++dt) {
+      wa_lds* at = (wa_lds*)from + v_at(dt) + 32 * s * PITCH;
+      const u32x2_t x = wa_read_tr(at), y = wa_read_tr(at + 16 * PITCH);
+      const u32x4_t vf = {x.x, x.y, y.x, y.y};
 #pragma unroll
-        for (int q = 0; q < QT; ++q)
-          oc[q][dt] = mfma_16x16x32<T>(vf, u32x4_t{pk[q][2 * s].x, pk[q][2 * s].y, pk[q][2 * s + 1].x, pk[q][2 * s + 1].y}, oc[q][dt]);
-      }
+      for (int q = 0; q < QT; ++q)
+        oc[q][dt] = mfma_16x16x32<T>(vf, u32x4_t{pk[q][2 * s].x, pk[q][2 * s].y, pk[q][2 * s + 1].x, pk[q][2 * s + 1].y}, oc[q][dt]);
+    }
+  };
+  // Tile t: its softmax and its product with V, and the scores of the tile behind it, whose MFMAs the vector work need not wait for.
+  // A buffer is written again two barriers after its last read.  No branch decides whether a tile is worked on: what a wave does not see is
+  // masked (one tile or two a block), and behind the last tile the scores of whatever lies there are not used.
+  auto step = [&](int t, f32x4_t (&sc)[QT][4], f32x4_t (&next)[QT][4], unsigned char* k_here, unsigned char* k_next, unsigned char* v_here,
+                  unsigned char* v_next) {
+    landed();  // K of t + 1, V of t
+    if (t + 2 < t1) request(kp, a.k_n, k2, t + 2, k_here);
+    if (t + 1 < t1) request(vp, a.v_n, v2, t + 1, v_next);
+    if (!whole(t)) mask(t, sc);
+    maxima(sc);
+    asm volatile("" : "+v"(v_slot));  // (addresses are worked out here again: kept, they would take the registers of the tiles)
+    // 16 keys of the next tile at a time, and a half of the queries' powers between their MFMAs
+    u32x2_t pk[QT][4];
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt) {
+      __builtin_amdgcn_sched_barrier(0);
+      u32x4_t kf[DK];
+      load_keys(k_next, kt, kf);
+      multiply_keys(kt, kf, next);
+      if constexpr (QT == 2) powers(kt & 1, kt >> 1, sc, pk);
+      else if (kt < 2) powers(0, kt, sc, pk);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    values(v_here, 0, pk);
+#pragma unroll
+    for (int q = 0; q < QT; ++q) powers(q, 2, sc, pk), powers(q, 3, sc, pk);
+    __builtin_amdgcn_sched_barrier(0);
+    values(v_here, 1, pk);
+  };
+  if (t0 < t1) {
+    f32x4_t even[QT][4], odd[QT][4];
+    request(kp, a.k_n, k2, t0, k_even);
+    request(vp, a.v_n, v2, t0, v_even);
+    if (t0 + 1 < t1) request(kp, a.k_n, k2, t0 + 1, k_odd);
+    landed();
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt) {
+      u32x4_t kf[DK];
+      load_keys(k_even, kt, kf);
+      multiply_keys(kt, kf, even);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll 1
+    for (int t = t0; t < t1; t += 2) {
+      step(t, even, odd, k_even, k_odd, v_even, v_odd);
+      if (t + 1 < t1) step(t + 1, odd, even, k_odd, k_even, v_odd, v_even);
+    }
   }
   // ---- out, or this part's
 #pragma unroll
@@ -288,7 +331,6 @@ __global__ __launch_bounds__(256) void window_step_kernel(const WindowArgs a) {
   constexpr int OWN = sizeof(smem) / 4;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, fr = lane & 15, fg = lane >> 4;
   unsigned char* mine = smem + wave * OWN;
-  const uint32_t lds = (uint32_t)(size_t)(__attribute__((address_space(3))) unsigned char*)mine;
   const int G = a.H / a.Hkv, blocks = (G + 15) / 16, d = a.d;
   const int split = blockIdx.y, gb = blockIdx.x % blocks, bk = blockIdx.x / blocks, b = bk / a.Hkv, hk = bk - b * a.Hkv;
   const int pos = a.positions[b];
@@ -391,7 +433,7 @@ __global__ __launch_bounds__(256) void window_step_kernel(const WindowArgs a) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the wave's own V is there)
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
-      const uint32_t from = lds + trow * PITCH + (((2 * dt + (piece >> 1)) ^ tkey) << 4) + 8 * (piece & 1);
+      wa_lds* from = (wa_lds*)mine + trow * PITCH + (((2 * dt + (piece >> 1)) ^ tkey) << 4) + 8 * (piece & 1);
       const u32x2_t x = wa_read_tr(from), y = wa_read_tr(from + 16 * PITCH);
       oc[dt] = mfma_16x16x32<T>(u32x4_t{x.x, x.y, y.x, y.y}, pf, oc[dt]);
     }
