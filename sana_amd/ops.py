@@ -874,28 +874,33 @@ def gate_residual(y: torch.Tensor, gate: torch.Tensor, residual: torch.Tensor) -
 
 # --------------------------------------------------------------------------- streams whose memory does not grow
 
-def _here(first: torch.Tensor, others, what: str) -> int:
-    """The device index of ``first``, on which all tensors of the call have to be (None entries aside)."""
-    _need_cuda(first, *others)
-    dev = first.get_device()
-    for t in others:
-        if t is not None and t.get_device() != dev:
+def _here(ts, what: str) -> int:
+    """The device index on which all tensors of the call have to be (None entries aside); no gradients are asked for."""
+    dev = ts[0].get_device()
+    for t in ts:
+        if t is not None and t.get_device() != dev or dev < 0:
+            _need_cuda(*ts)
             raise SanaHipError(f"{what}: all tensors must be on one device")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (first, *others)):
-        raise SanaHipError(f"{what} is forward only: call it under torch.no_grad() or on detached tensors")
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                raise SanaHipError(f"{what} is forward only: call it under torch.no_grad() or on detached tensors")
     return dev
 
 
 def _token_rows(t: torch.Tensor, what: str) -> Tuple[int, int]:
-    """:func:`_token_major_view` of [B, N, C] whose strides along axes of length 1 say nothing."""
-    sb, sn = _token_major_view(t, what) if t.shape[2] != 1 else (t.stride(0), t.stride(1))
-    return (sb if t.shape[0] > 1 else 0), (sn if t.shape[1] > 1 else t.shape[2])
+    """:func:`_token_major_view` of [B, N, C], where strides along axes of length 1 say nothing."""
+    B, N, C = t.shape
+    b, n, c = t.stride()
+    if c != 1 and C != 1:
+        _token_major_view(t, what)
+    return b if B > 1 else 0, n if N > 1 else C
 
 
 def _lengths_arg(t: Optional[torch.Tensor], B: int, what: str = "lengths") -> Optional[int]:
     if t is None:
         return None
-    if t.dtype != torch.int32 or tuple(t.shape) != (B,) or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.shape != (B,) or not t.is_contiguous():
         raise SanaHipError(f"{what} must be contiguous int32 [{B}], got {t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
 
@@ -922,28 +927,29 @@ def decay_linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lo
     it is a new tensor.  ``lengths``: int32 [B] on the device, the tokens that each batch entry really has (clamped to 0 .. N);
     rows behind them are not read, and stay in ``out`` as they were (zeros in a new one); an entry without tokens
     keeps its state.  ``out`` must not overlap the inputs.  Forward only."""
-    dev = _here(q, (k, v, log_decay, state, lengths, out, state_out), "decay_linear_attention")
+    dev = _here((q, k, v, log_decay, state, lengths, out, state_out), "decay_linear_attention")
     if dev != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
             return decay_linear_attention(q, k, v, log_decay, scale, state, lengths, out, state_out)
-    if q.dim() != 3 or q.dtype not in IO16 or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise SanaHipError(f"decay_linear_attention needs bf16 or fp16 q, k and v [B, N, C] of one dtype, got {q.dtype}, {k.dtype}, {v.dtype}")
-    if k.shape != q.shape or v.shape != q.shape:
-        raise SanaHipError(f"q, k and v must share their shape: {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    B, N, C = q.shape
+    dt, shape = q.dtype, q.shape
+    if len(shape) != 3 or dt not in IO16 or k.dtype is not dt or v.dtype is not dt:
+        raise SanaHipError(f"decay_linear_attention needs bf16 or fp16 q, k and v [B, N, C] of one dtype, got {dt}, {k.dtype}, {v.dtype}")
+    if k.shape != shape or v.shape != shape:
+        raise SanaHipError(f"q, k and v must share their shape: {tuple(shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    B, N, C = shape
     H = log_decay.numel()
-    if log_decay.dtype != torch.float32 or log_decay.dim() != 1 or not log_decay.is_contiguous() or H == 0 or C % H:
+    if log_decay.dtype is not torch.float32 or log_decay.dim() != 1 or not log_decay.is_contiguous() or H == 0 or C % H:
         raise SanaHipError(f"log_decay must be contiguous fp32 [H] with H dividing C={C}, got {log_decay.dtype} {tuple(log_decay.shape)}")
     d = C // H
     if d % 8 or not 0 < d <= 128:
         raise SanaHipError(f"head_dim {d} has no kernel (multiples of 8 up to 128)")
-    for name, t in (("state", state), ("state_out", state_out)):
-        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (B, H, d, d) or not t.is_contiguous()):
-            raise SanaHipError(f"{name} must be contiguous fp32 {(B, H, d, d)}, got {t.dtype} {tuple(t.shape)}")
+    for t in (state, state_out):
+        if t is not None and (t.dtype is not torch.float32 or t.shape != (B, H, d, d) or not t.is_contiguous()):
+            raise SanaHipError(f"state and state_out must be contiguous fp32 {(B, H, d, d)}, got {t.dtype} {tuple(t.shape)}")
     length_ptr = _lengths_arg(lengths, B)
     if out is None:
-        out = (torch.empty if lengths is None else torch.zeros)((B, N, C), dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype:
+        out = (torch.empty if lengths is None else torch.zeros)(shape, dtype=dt, device=q.device)
+    elif out.shape != shape or out.dtype is not dt:
         raise SanaHipError("out has the wrong shape or dtype")
     if state_out is None:
         state_out = torch.empty((B, H, d, d), dtype=torch.float32, device=q.device)
@@ -953,14 +959,13 @@ def decay_linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lo
         elif state_out is not state:
             state_out.copy_(state)
         return out, state_out
-    strides = [s for t, name in ((q, "q"), (k, "k"), (v, "v"), (out, "out")) for s in _token_rows(t, name)]
     lib = _lib.load()
     nbytes = lib.sana_hip_decay_attention_workspace_bytes(B, N, H, d) if N > 1 else 0
-    ws = _call_scratch(q.device, nbytes)
+    ws = _call_scratch(q.device, nbytes) if nbytes else None
     code = lib.sana_hip_decay_attention(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), None if state is None else state.data_ptr(),
-        state_out.data_ptr(), out.data_ptr(), length_ptr, None if ws is None else ws.data_ptr(), nbytes, B, N, H, d, *strides,
-        float(scale), _DT[q.dtype], _stream())
+        state_out.data_ptr(), out.data_ptr(), length_ptr, None if ws is None else ws.data_ptr(), nbytes, B, N, H, d,
+        *_token_rows(q, "q"), *_token_rows(k, "k"), *_token_rows(v, "v"), *_token_rows(out, "out"), scale, _DT[dt], _stream())
     if code:
         _lib.check(code, "sana_hip_decay_attention")
     return out, state_out
@@ -968,22 +973,23 @@ def decay_linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lo
 
 def _window_shapes(q, k, v, num_heads: int, window: int, sinks: int, scale: Optional[float], what: str) -> Tuple[int, int, float]:
     """-> (head_dim, key heads, scale) of [B, N, H*d] queries and [B, Nk, Hkv*d] keys and values."""
-    if q.dim() != 3 or k.dim() != 3 or q.dtype not in IO16 or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise SanaHipError(f"{what} needs bf16 or fp16 q [B, N, H*d], k and v [B, Nk, Hkv*d] of one dtype, got {q.dtype}, {k.dtype}, {v.dtype}")
-    C = q.shape[2]
+    dt, qs, ks = q.dtype, q.shape, k.shape
+    if len(qs) != 3 or len(ks) != 3 or dt not in IO16 or k.dtype is not dt or v.dtype is not dt:
+        raise SanaHipError(f"{what} needs bf16 or fp16 q [B, N, H*d], k and v [B, Nk, Hkv*d] of one dtype, got {dt}, {k.dtype}, {v.dtype}")
+    C, Ck = qs[2], ks[2]
     if num_heads < 1 or C % num_heads or C == 0:
         raise SanaHipError(f"{C} channels are not {num_heads} heads")
     d = C // num_heads
     if d % 8 or d > 128:
         raise SanaHipError(f"head_dim {d} has no kernel (multiples of 8 up to 128)")
-    if k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] == 0 or k.shape[2] % d or num_heads % (k.shape[2] // d):
-        raise SanaHipError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not match q {tuple(q.shape)} with {num_heads} heads of {d}")
+    if v.shape != ks or ks[0] != qs[0] or Ck == 0 or Ck % d or num_heads % (Ck // d):
+        raise SanaHipError(f"k {tuple(ks)} and v {tuple(v.shape)} do not match q {tuple(qs)} with {num_heads} heads of {d}")
     if not 1 <= window <= 1 << 30 or not 0 <= sinks <= 1 << 30:
         raise SanaHipError(f"window must be at least 1 and sinks at least 0, got {window} and {sinks}")
-    scale = float(d ** -0.5 if scale is None else scale)
+    scale = d ** -0.5 if scale is None else float(scale)
     if not scale > 0.0:
         raise SanaHipError(f"scale must be positive, got {scale}")
-    return d, k.shape[2] // d, scale
+    return d, Ck // d, scale
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, num_heads: int, window: int, sinks: int = 0,
@@ -996,7 +1002,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, num_head
     ``lengths``: int32 [B] on the device, the queries that each batch entry really has (clamped to 0 .. N; its keys end with its
     last query); rows behind them are not read, and stay in ``out`` as they were (zeros in a new one).
     Returns [B, N, H*d].  ``out`` must not overlap the inputs.  Forward only."""
-    dev = _here(q, (k, v, lengths, out), "window_attention")
+    dev = _here((q, k, v, lengths, out), "window_attention")
     if dev != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
             return window_attention(q, k, v, num_heads, window, sinks, scale, lengths, out)
@@ -1012,13 +1018,13 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, num_head
         raise SanaHipError("out has the wrong shape or dtype")
     if B * N == 0:
         return out
-    strides = [s for t, name in ((q, "q"), (k, "k"), (v, "v"), (out, "out")) for s in _token_rows(t, name)]
     lib = _lib.load()
     nbytes = lib.sana_hip_window_attention_workspace_bytes(B, N, Nk, num_heads, d, window, sinks)
-    ws = _call_scratch(q.device, nbytes)
+    ws = _call_scratch(q.device, nbytes) if nbytes else None
     code = lib.sana_hip_window_attention(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), length_ptr, None if ws is None else ws.data_ptr(), nbytes,
-        B, N, Nk, num_heads, Hkv, d, window, sinks, *strides, scale, _DT[q.dtype], _stream())
+        B, N, Nk, num_heads, Hkv, d, window, sinks, *_token_rows(q, "q"), *_token_rows(k, "k"), *_token_rows(v, "v"),
+        *_token_rows(out, "out"), scale, _DT[q.dtype], _stream())
     if code:
         _lib.check(code, "sana_hip_window_attention")
     return out
@@ -1026,12 +1032,12 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, num_head
 
 def _cache_rows(cache_k: torch.Tensor, cache_v: torch.Tensor, k: torch.Tensor, sinks: int, what: str) -> int:
     """The window of a cache [B, sinks + window, C] for new tokens ``k`` [B, N, C]."""
-    if cache_k.dim() != 3 or cache_k.shape != cache_v.shape or cache_k.dtype != k.dtype or cache_v.dtype != k.dtype or \
-            cache_k.shape[0] != k.shape[0] or cache_k.shape[2] != k.shape[2]:
-        raise SanaHipError(f"{what}: the caches {tuple(cache_k.shape)}, {tuple(cache_v.shape)} do not match new tokens {tuple(k.shape)}")
-    if not 0 <= sinks < cache_k.shape[1]:
-        raise SanaHipError(f"{what}: a cache of {cache_k.shape[1]} rows holds {sinks} sinks and no window")
-    return cache_k.shape[1] - sinks
+    cs, ks, dt = cache_k.shape, k.shape, k.dtype
+    if len(cs) != 3 or cache_v.shape != cs or cache_k.dtype is not dt or cache_v.dtype is not dt or cs[0] != ks[0] or cs[2] != ks[2]:
+        raise SanaHipError(f"{what}: the caches {tuple(cs)}, {tuple(cache_v.shape)} do not match new tokens {tuple(ks)}")
+    if not 0 <= sinks < cs[1]:
+        raise SanaHipError(f"{what}: a cache of {cs[1]} rows holds {sinks} sinks and no window")
+    return cs[1] - sinks
 
 
 def window_cache_append_(cache_k: torch.Tensor, cache_v: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
@@ -1041,7 +1047,7 @@ def window_cache_append_(cache_k: torch.Tensor, cache_v: torch.Tensor, k: torch.
     [B] on the device, the tokens that each stream has seen before (negative: idle, nothing is written), which the
     caller advances; ``lengths``: int32 [B], the tokens that each stream really adds.  bf16 or fp16, C a multiple of 8.  The
     caches must not overlap k and v, and no two streams may share rows."""
-    dev = _here(cache_k, (cache_v, k, v, positions, lengths), "window_cache_append_")
+    dev = _here((cache_k, cache_v, k, v, positions, lengths), "window_cache_append_")
     if dev != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
             return window_cache_append_(cache_k, cache_v, k, v, positions, sinks, lengths)
@@ -1052,9 +1058,10 @@ def window_cache_append_(cache_k: torch.Tensor, cache_v: torch.Tensor, k: torch.
     position_ptr, length_ptr = _lengths_arg(positions, B, "positions"), _lengths_arg(lengths, B)
     if B * N * C == 0:
         return
-    strides = [s for t, name in ((cache_k, "cache_k"), (cache_v, "cache_v"), (k, "k"), (v, "v")) for s in _token_rows(t, name)]
-    code = _lib.load().sana_hip_window_cache_append(cache_k.data_ptr(), cache_v.data_ptr(), k.data_ptr(), v.data_ptr(), position_ptr,
-                                                    length_ptr, B, N, C, window, sinks, *strides, _DT[k.dtype], _stream())
+    code = _lib.load().sana_hip_window_cache_append(
+        cache_k.data_ptr(), cache_v.data_ptr(), k.data_ptr(), v.data_ptr(), position_ptr, length_ptr, B, N, C, window, sinks,
+        *_token_rows(cache_k, "cache_k"), *_token_rows(cache_v, "cache_v"), *_token_rows(k, "k"), *_token_rows(v, "v"),
+        _DT[k.dtype], _stream())
     if code:
         _lib.check(code, "sana_hip_window_cache_append")
 
@@ -1067,7 +1074,7 @@ def window_attention_step_(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ca
     which the caller advances once all layers are through), and the token attends to what the caches then hold: the last
     ``window`` tokens up to itself and the first ``sinks``.  A stream with a negative position is idle: its caches stay as they are, its
     output is zero.  Returns [B, 1, H*d].  Forward only."""
-    dev = _here(q, (k, v, cache_k, cache_v, positions, out), "window_attention_step_")
+    dev = _here((q, k, v, cache_k, cache_v, positions, out), "window_attention_step_")
     if dev != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
             return window_attention_step_(q, k, v, cache_k, cache_v, positions, num_heads, sinks, scale, out)
@@ -1083,14 +1090,14 @@ def window_attention_step_(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ca
         raise SanaHipError("out has the wrong shape or dtype")
     if B == 0:
         return out
-    (qb, _), (kb, _), (vb, _), (ob, _) = (_token_rows(t, name) for t, name in ((q, "q"), (k, "k"), (v, "v"), (out, "out")))
-    (ckb, ckn), (cvb, cvn) = _token_rows(cache_k, "cache_k"), _token_rows(cache_v, "cache_v")
     lib = _lib.load()
     nbytes = lib.sana_hip_window_step_workspace_bytes(B, num_heads, Hkv, d, window, sinks)
-    ws = _call_scratch(q.device, nbytes)
-    code = lib.sana_hip_window_step(q.data_ptr(), k.data_ptr(), v.data_ptr(), cache_k.data_ptr(), cache_v.data_ptr(), position_ptr,
-                                    out.data_ptr(), None if ws is None else ws.data_ptr(), nbytes, B, num_heads, Hkv, d, window,
-                                    sinks, qb, kb, vb, ckb, ckn, cvb, cvn, ob, scale, _DT[q.dtype], _stream())
+    ws = _call_scratch(q.device, nbytes) if nbytes else None
+    code = lib.sana_hip_window_step(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), cache_k.data_ptr(), cache_v.data_ptr(), position_ptr, out.data_ptr(),
+        None if ws is None else ws.data_ptr(), nbytes, B, num_heads, Hkv, d, window, sinks, _token_rows(q, "q")[0],
+        _token_rows(k, "k")[0], _token_rows(v, "v")[0], *_token_rows(cache_k, "cache_k"), *_token_rows(cache_v, "cache_v"),
+        _token_rows(out, "out")[0], scale, _DT[q.dtype], _stream())
     if code:
         _lib.check(code, "sana_hip_window_step")
     return out
