@@ -288,28 +288,36 @@ __global__ __launch_bounds__(64 * NW, 2) void window_attn_kernel(const WindowArg
   }
 }
 
-// The parts of a query and head: weights 2^(m_s - m), sums and outputs added up in the order of the parts.  A wave a (query, head), four
-// channels a lane.
+// The parts of a query and head: weights 2^(m_s - m), sums and outputs added up in the order of the parts.  Half a wave a (query, head):
+// a lane reads the maximum and the sum of one part, then four channels of all.
 template <typename T>
 __global__ __launch_bounds__(256) void window_join_kernel(const WindowArgs a) {
+  static_assert(WA_MAX_SPLITS <= 32, "");
   const int64_t rows = (int64_t)a.B * a.N * a.H, row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (row >= rows) return;
-  const int c = 4 * (threadIdx.x & 31);
+  const int lane = threadIdx.x & 31, c = 4 * lane;
   const int64_t bn = row / a.H;
   const int h = (int)(row - bn * a.H), b = (int)(bn / a.N), i = (int)(bn - (int64_t)b * a.N);
   if ((a.lengths && i >= a.lengths[b]) || (a.positions && a.positions[b] < 0)) return;
-  float m = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[2 * (s * rows + row)]);
+  f32x2_t ml = {-INFINITY, 0.f};
+  if (lane < a.splits) ml = *reinterpret_cast<const f32x2_t*>(a.part_ml + 2 * (lane * rows + row));
+  float m = ml[0];
+#pragma unroll
+  for (int x = 1; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor(m, x, 32));
+  const float mine = lane < a.splits ? __builtin_amdgcn_exp2f(ml[0] - m) : 0.f;
+  const float* from = a.part_o + row * a.d + (c < a.d ? c : 0);
   float l = 0.f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < a.splits; ++s) {
-    const int64_t at = s * rows + row;
-    const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * at] - m);
-    l = fmaf(f, a.part_ml[2 * at + 1], l);
-    if (c < a.d) {
-      const f32x4_t x = *reinterpret_cast<const f32x4_t*>(a.part_o + at * a.d + c);
+  for (int s0 = 0; s0 < a.splits; s0 += 8) {
+    f32x4_t x[8];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) o[r] = fmaf(f, x[r], o[r]);
+    for (int s = 0; s < 8; ++s) x[s] = *reinterpret_cast<const f32x4_t*>(from + min(s0 + s, a.splits - 1) * rows * a.d);
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      const float f = __shfl(mine, s0 + s, 32);  // (0 behind the last part)
+      l = fmaf(f, __shfl(ml[1], s0 + s, 32), l);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[r] = fmaf(f, x[s][r], o[r]);
     }
   }
   const float inv = 1.0f / l;
@@ -320,15 +328,15 @@ __global__ __launch_bounds__(256) void window_join_kernel(const WindowArgs a) {
 
 __device__ __forceinline__ int wa_slot(int64_t p, int sinks, int window) { return (int)(p < sinks ? p : sinks + (p - sinks) % window); }
 
-// One token of each stream over its cache.  A workgroup takes a part of the rows of one (stream, key head), its waves every fourth
+// One token of each stream over its cache.  A workgroup takes a part of the rows of one (stream, key head), its NW waves in turn a
 // tile of 32 rows; the query heads that share the key head are the 16 columns of the products (more than 16 in further workgroups).  K comes
 // from memory as the operand it is, V through the wave's own LDS to be transposed.  The new token's row is taken from k and v, wherever its
 // slot is met, and written to the cache by the workgroup whose part holds the slot: nobody reads that row of the cache.
-template <typename T, int DK, int DT>
-__global__ __launch_bounds__(256) void window_step_kernel(const WindowArgs a) {
+template <typename T, int DK, int DT, int NW>
+__global__ __launch_bounds__(64 * NW) void window_step_kernel(const WindowArgs a) {
   constexpr int PITCH = DK * 64, TILE = 32 * PITCH, PV = DK * 2;  // PV: 16-byte pieces of V a lane
-  __shared__ __attribute__((aligned(16))) unsigned char smem[4 * (TILE > 16 * 16 * DT * 4 + 128 ? TILE : 16 * 16 * DT * 4 + 128)];
-  constexpr int OWN = sizeof(smem) / 4;
+  __shared__ __attribute__((aligned(16))) unsigned char smem[NW * (TILE > 16 * 16 * DT * 4 + 128 ? TILE : 16 * 16 * DT * 4 + 128)];
+  constexpr int OWN = sizeof(smem) / NW;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, fr = lane & 15, fg = lane >> 4;
   unsigned char* mine = smem + wave * OWN;
   const int G = a.H / a.Hkv, blocks = (G + 15) / 16, d = a.d;
@@ -336,7 +344,7 @@ __global__ __launch_bounds__(256) void window_step_kernel(const WindowArgs a) {
   const int pos = a.positions[b];
   if (pos < 0) {  // an idle stream: zeros
     if (split == 0 && gb == 0)
-      for (int c = tid; c < G * d; c += 256) a.out[b * a.o_b + hk * G * d + c] = 0;
+      for (int c = tid; c < G * d; c += 64 * NW) a.out[b * a.o_b + hk * G * d + c] = 0;
     return;
   }
   const int rows = a.window + a.sinks, count = pos < rows ? pos + 1 : rows, slot = wa_slot(pos, a.sinks, a.window);
@@ -383,7 +391,7 @@ __global__ __launch_bounds__(256) void window_step_kernel(const WindowArgs a) {
   const int trow = 4 * fg + (fr >> 2), tkey = wa_key<DK>(trow), piece = fr & 3;
   if (t0 + wave < t1) request(t0 + wave);
 #pragma unroll 1
-  for (int t = t0 + wave; t < t1; t += 4) {
+  for (int t = t0 + wave; t < t1; t += NW) {
     f32x4_t sc[2];
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
@@ -400,7 +408,7 @@ __global__ __launch_bounds__(256) void window_step_kernel(const WindowArgs a) {
       const int idx = lane + 64 * i, r = idx / (DK * 4), c = idx - r * (DK * 4);
       *reinterpret_cast<u32x4_t*>(mine + r * PITCH + ((c ^ wa_key<DK>(r)) << 4)) = rv[i];
     }
-    if (t + 4 < t1) request(t + 4);
+    if (t + NW < t1) request(t + NW);
     float most = -INFINITY;
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
@@ -452,21 +460,21 @@ __global__ __launch_bounds__(256) void window_step_kernel(const WindowArgs a) {
   const int col = tid & 15, g = 16 * gb + col;
   float m = -INFINITY;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) m = fmaxf(m, part(w)[16 * 16 * DT + col]);
+  for (int w = 0; w < NW; ++w) m = fmaxf(m, part(w)[16 * 16 * DT + col]);
   const float base = m == -INFINITY ? 0.f : m;
-  float f[4], l = 0.f;
+  float f[NW], l = 0.f;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
+  for (int w = 0; w < NW; ++w) {
     f[w] = __builtin_amdgcn_exp2f(part(w)[16 * 16 * DT + col] - base);
     l = fmaf(f[w], part(w)[16 * 16 * DT + 16 + col], l);
   }
   if (g >= G) return;
   const int64_t at = ((int64_t)split * a.B + b) * a.H + hk * G + g;
   const float inv = 1.0f / l;
-  for (int c = tid >> 4; c < d; c += 16) {
+  for (int c = tid >> 4; c < d; c += 4 * NW) {
     float o = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) o = fmaf(f[w], part(w)[c * 16 + col], o);
+    for (int w = 0; w < NW; ++w) o = fmaf(f[w], part(w)[c * 16 + col], o);
     if (a.splits == 1) a.out[b * a.o_b + (hk * G + g) * d + c] = (uint16_t)pk16<T>(o * inv, 0.f);
     else a.part_o[at * d + c] = o;
   }
@@ -502,10 +510,16 @@ int prompt_splits(int B, int N, int Nk, int H, int window, int sinks) {
   want = want > tiles / 4 ? tiles / 4 : want;
   return (int)(want < 1 ? 1 : want > WA_MAX_SPLITS ? WA_MAX_SPLITS : want);
 }
-// Parts of a cache's rows for one token: four tiles of 32 rows a workgroup at least.
+// One token: the workgroups of a whole cache, one a (stream, key head, 16 query heads).
+int64_t step_groups(int B, int H, int Hkv) { return (int64_t)B * Hkv * ((H / Hkv + 15) / 16); }
+// Eight waves take a short cache whole, where its workgroups are few: the second launch that joins parts takes longer than the tiles of a
+// wave one after the other.
+bool step_in_one(int64_t groups, int rows) { return groups <= 256 && (rows + 31) / 32 <= 48; }
+// Parts of a cache's rows: four tiles of 32 rows a workgroup at least.
 int step_splits(int B, int H, int Hkv, int rows) {
-  const int64_t groups = (int64_t)B * Hkv * ((H / Hkv + 15) / 16);
+  const int64_t groups = step_groups(B, H, Hkv);
   const int tiles = (rows + 31) / 32;
+  if (step_in_one(groups, rows)) return 1;
   int64_t want = (1024 + groups - 1) / groups;
   want = want > tiles / 4 ? tiles / 4 : want;
   return (int)(want < 1 ? 1 : want > WA_MAX_SPLITS ? WA_MAX_SPLITS : want);
@@ -536,9 +550,12 @@ int launch_prompt(WindowArgs a, hipStream_t s) {
 
 template <typename T, int DK, int DT>
 int launch_step(const WindowArgs& a, hipStream_t s) {
-  const int64_t groups = (int64_t)a.B * a.Hkv * ((a.H / a.Hkv + 15) / 16);
+  const int64_t groups = step_groups(a.B, a.H, a.Hkv);
   if (groups > 0x7fffffff) return SANA_ERR_SHAPE;
-  hipLaunchKernelGGL((window_step_kernel<T, DK, DT>), dim3((unsigned)groups, (unsigned)a.splits), dim3(256), 0, s, a);
+  if (step_in_one(groups, a.window + a.sinks))
+    hipLaunchKernelGGL((window_step_kernel<T, DK, DT, 8>), dim3((unsigned)groups), dim3(512), 0, s, a);
+  else
+    hipLaunchKernelGGL((window_step_kernel<T, DK, DT, 4>), dim3((unsigned)groups, (unsigned)a.splits), dim3(256), 0, s, a);
   if (a.splits > 1) {
     const int rc = launch_join<T>(a, s);
     if (rc != SANA_OK) return rc;
