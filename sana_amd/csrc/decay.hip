@@ -66,8 +66,8 @@ __device__ __forceinline__ float dc_fit(float most) {
 // What a launch of the chunks gives: the sums of a segment alone, the outputs of segments whose states are known, or both for whole streams.
 enum { DC_SUMS, DC_OUT, DC_WHOLE };
 
-// One workgroup of NW waves takes a (batch, head, segment) through its chunks.  NV of its waves share the channels of v, 16 VT
-// each, whose columns of the state stay in their registers (fp32) from chunk to chunk; where the head has fewer channels, NW / NV waves
+// One workgroup of four waves takes a (batch, head, segment) through its chunks.  NV of its waves share the channels of v, 16 VT
+// each, whose columns of the state stay in their registers (fp32) from chunk to chunk; where the head has fewer channels, 4 / NV waves
 // with the same ones share the queries.  Each wave scores 16 queries for all, through LDS.
 // The operands of the MFMAs (16 x 16 x 32):
 //   scores^T = K Q^T   both from LDS as they lie;
@@ -80,20 +80,19 @@ enum { DC_SUMS, DC_OUT, DC_WHOLE };
 // 16-bit values: three of bf16 where the state is given back (fp32's accuracy; with two it is 1.3e-6 off after 32760
 // tokens), two of bf16 where it only goes on to outputs, two of f16 (22 bits), the second times 2^11, so that it stays a normal number.
 // f16 ends at 65504: S goes in scaled by a power of two for each wave, P for each query.
-template <typename T, int DK, int KT, int VT, int NV, int NW, int MODE>
-__global__ __launch_bounds__(64 * NW, NW / 2) void decay_chunk_kernel(const DecayArgs a) {
+template <typename T, int DK, int KT, int VT, int NV, int MODE>
+__global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) {
   constexpr bool OUT = MODE != DC_SUMS, F = is_f16<T>;
   constexpr int PITCH = DK * 64, TILE = DC * PITCH;  // LDS row / tensor in bytes
-  constexpr int NT = 64 * NW, PIECES = DC * DK * 4 / NT, TERMS = F || MODE == DC_OUT ? 2 : 3;
-  constexpr int NQ = NW / NV, QN = 4 / NQ;   // shares of the queries, query tiles of a share
-  constexpr int HALVES = NW / 4, KS = 4 / HALVES;  // a wave scores 16 queries, eight waves against half of the keys each
-  static_assert(KT <= 2 * DK && DC * DK * 4 % NT == 0 && NW % NV == 0 && (NW == 4 || NW == 8) && 4 % NQ == 0, "");
-  __shared__ __attribute__((aligned(16))) unsigned char smem[(OUT ? 3 : 2) * TILE + (OUT ? DC * 128 + DC * 4 * HALVES : 0)];
+  constexpr int NT = 256, PIECES = DC * DK * 4 / NT, TERMS = F || MODE == DC_OUT ? 2 : 3;
+  constexpr int NQ = 4 / NV, QN = 4 / NQ;  // shares of the queries, query tiles of a share
+  static_assert(KT <= 2 * DK && DC * DK * 4 % NT == 0 && 4 % NV == 0, "");
+  __shared__ __attribute__((aligned(16))) unsigned char smem[(OUT ? 3 : 2) * TILE + (OUT ? DC * 128 + DC * 4 : 0)];
   const uint32_t sk = (uint32_t)(size_t)(__attribute__((address_space(3))) unsigned char*)smem;
   const uint32_t sv = sk + TILE, sq = sk + 2 * TILE, sp = sk + 3 * TILE;
-  float* fit = reinterpret_cast<float*>(smem + 3 * TILE + DC * 128);  // f16: the scales of a query's P
+  float* fit = reinterpret_cast<float*>(smem + 3 * TILE + DC * 128);  // f16: the scale of a query's P
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), fr = tid & 15, fg = (tid >> 4) & 3;
-  const int v0 = 16 * VT * (wave % NV), qt0 = QN * (wave / NV), sqt = wave & 3, half = HALVES == 2 ? wave >> 2 : 0;
+  const int v0 = 16 * VT * (wave % NV), qt0 = QN * (wave / NV);
 
   // neighbouring heads, whose rows share cache lines, on one XCD
   const int per = (a.items + 7) >> 3, item = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
@@ -210,46 +209,46 @@ __global__ __launch_bounds__(64 * NW, NW / 2) void decay_chunk_kernel(const Deca
     u32x4_t vf[2][VT];   // values of two ranges of 32 tokens
     if constexpr (OUT) {
       // ---- scores, decayed, to LDS: row = query, 16-byte slot 4 s + g = keys 32 s + 4 g + {0..3}, + 16
-      f32x4_t sc[KS];
+      f32x4_t sc[4];
 #pragma unroll
-      for (int kt = 0; kt < KS; ++kt) sc[kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      for (int kt = 0; kt < 4; ++kt) sc[kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int s = 0; s < DK; ++s) {
-        const u32x4_t qf = dc_read(sq + 16 * sqt * PITCH + row16[s]);
+        const u32x4_t qf = dc_read(sq + 16 * wave * PITCH + row16[s]);
 #pragma unroll
-        for (int kt = 0; kt < KS; ++kt)
-          if (KS * half + kt <= sqt) sc[kt] = mfma_16x16x32<T>(dc_read(sk + 16 * (KS * half + kt) * PITCH + row16[s]), qf, sc[kt]);
+        for (int kt = 0; kt < 4; ++kt)
+          if (kt <= wave) sc[kt] = mfma_16x16x32<T>(dc_read(sk + 16 * kt * PITCH + row16[s]), qf, sc[kt]);
       }
       float most = 0.f, f = 1.f;
       float ahead = before;  // of tile kt: a^(16 (tiles between it and the diagonal)), from the last in front of the diagonal on
-      if (HALVES == 2 && half == 0 && sqt > 2) ahead *= step16;
+      // (selects, no branches: a tile's place is uniform, and each of these as a branch of its own takes longer than the arithmetic)
 #pragma unroll
-      for (int kt = KS - 1; kt >= 0; --kt) {
-        const int tile = KS * half + kt;
+      for (int kt = 3; kt >= 0; --kt) {
+        const bool in_front = kt < wave, at_diagonal = kt == wave;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          if (tile < sqt) sc[kt][r] *= ahead * row4[r];
-          else sc[kt][r] = tile == sqt && fr >= 4 * fg + r ? sc[kt][r] * diagonal[r] : 0.f;
+          const float x = sc[kt][r] * (in_front ? ahead * row4[r] : diagonal[r]);
+          sc[kt][r] = in_front | (at_diagonal & (fr >= 4 * fg + r)) ? x : 0.f;
           if constexpr (F) most = fmaxf(most, fabsf(sc[kt][r]));
         }
-        if (tile < sqt) ahead *= step16;
+        ahead *= in_front ? step16 : 1.f;
       }
       if constexpr (F) {
         most = fmaxf(most, __shfl_xor(most, 16));
         most = fmaxf(most, __shfl_xor(most, 32));
         f = dc_fit(most);
-        if (fg == 0) fit[DC * half + 16 * sqt + fr] = f;
+        if (fg == 0) fit[16 * wave + fr] = f;
       }
 #pragma unroll
-      for (int s = 0; s < KS / 2; ++s) {
-        const int q = 16 * sqt + fr, at16 = 4 * ((KS / 2) * half + s) + fg;
+      for (int s = 0; s < 2; ++s) {
+        const int q = 16 * wave + fr;
         u32x4_t p;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const f32x4_t x = sc[2 * s + (e >> 1)];
           p[e] = F ? pk16<T>(x[2 * (e & 1)] * f, x[2 * (e & 1) + 1] * f) : pk16<T>(x[2 * (e & 1)], x[2 * (e & 1) + 1]);
         }
-        *reinterpret_cast<u32x4_t*>(smem + 3 * TILE + q * 128 + ((at16 ^ ((q >> 1) & 7)) << 4)) = p;
+        *reinterpret_cast<u32x4_t*>(smem + 3 * TILE + q * 128 + (((4 * s + fg) ^ ((q >> 1) & 7)) << 4)) = p;
       }
       __builtin_amdgcn_sched_barrier(0);
       // ---- the state in front of the chunk
@@ -326,13 +325,6 @@ __global__ __launch_bounds__(64 * NW, NW / 2) void decay_chunk_kernel(const Deca
         for (int q = 0; q < QN; ++q) {
           if (NQ == 1 && 2 * s > q) continue;  // (queries of the first 32 see none of the second 32 tokens)
           const int row = 16 * (qt0 + q) + fr;
-          if (F && HALVES == 2 && s == 1) {
-            const float m = fit[DC + row] / fit[row];
-#pragma unroll
-            for (int vt = 0; vt < VT; ++vt)
-#pragma unroll
-              for (int r = 0; r < 4; ++r) oc[vt][q][r] *= m;
-          }
           const u32x4_t pf = dc_read(sp + row * 128 + (((4 * s + fg) ^ ((row >> 1) & 7)) << 4));
 #pragma unroll
           for (int vt = 0; vt < VT; ++vt) oc[vt][q] = mfma_16x16x32<T>(vf[s][vt], pf, oc[vt][q]);
@@ -344,7 +336,7 @@ __global__ __launch_bounds__(64 * NW, NW / 2) void decay_chunk_kernel(const Deca
 #pragma unroll
       for (int q = 0; q < QN; ++q) {
         const int row = 16 * (qt0 + q) + fr;
-        const float m = F ? 1.0f / fit[row + (HALVES == 2 && (NQ > 1 || q >= 2) ? DC : 0)] : 1.f;  // (of the half that came last)
+        const float m = F ? 1.0f / fit[row] : 1.f;
 #pragma unroll
         for (int vt = 0; vt < VT; ++vt) {
           const int c = v0 + 16 * vt + 4 * fg;
@@ -498,19 +490,19 @@ int segment_count(int B, int N, int H, int* tokens) {
   return (chunks + per - 1) / per;
 }
 
-template <typename T, int DK, int KT, int VT, int NV, int NW>
+template <typename T, int DK, int KT, int VT, int NV>
 int launch_chunks(const DecayArgs& a, int B, hipStream_t s) {
   const int64_t items = (int64_t)B * a.H * a.nseg;
   if (items > 0x7ffffff0) return SANA_ERR_SHAPE;
   DecayArgs args = a;
   args.items = (int)items;
-  const dim3 grid((unsigned)((items + 7) / 8 * 8)), block(64 * NW);
+  const dim3 grid((unsigned)((items + 7) / 8 * 8)), block(256);
   if (a.nseg > 1) {
-    hipLaunchKernelGGL((decay_chunk_kernel<T, DK, KT, VT, NV, NW, DC_SUMS>), grid, block, 0, s, args);
+    hipLaunchKernelGGL((decay_chunk_kernel<T, DK, KT, VT, NV, DC_SUMS>), grid, block, 0, s, args);
     hipLaunchKernelGGL(decay_scan_kernel, dim3((unsigned)((a.d * a.d / 4 + 63) / 64), (unsigned)(B * a.H)), dim3(64), 0, s, args);
-    hipLaunchKernelGGL((decay_chunk_kernel<T, DK, KT, VT, NV, NW, DC_OUT>), grid, block, 0, s, args);
+    hipLaunchKernelGGL((decay_chunk_kernel<T, DK, KT, VT, NV, DC_OUT>), grid, block, 0, s, args);
   } else {
-    hipLaunchKernelGGL((decay_chunk_kernel<T, DK, KT, VT, NV, NW, DC_WHOLE>), grid, block, 0, s, args);
+    hipLaunchKernelGGL((decay_chunk_kernel<T, DK, KT, VT, NV, DC_WHOLE>), grid, block, 0, s, args);
   }
   return hipGetLastError() == hipSuccess ? SANA_OK : SANA_ERR_LAUNCH;
 }
@@ -527,11 +519,11 @@ int launch_step(const DecayArgs& a, int B, hipStream_t s) {
 template <typename T>
 int decay_attention(const DecayArgs& a, int B, hipStream_t s) {
   if (a.N == 1) return launch_step<T>(a, B, s);
-  if (a.d <= 32) return launch_chunks<T, 1, 2, 1, 2, 4>(a, B, s);
-  if (a.d <= 64) return launch_chunks<T, 2, 4, 1, 4, 4>(a, B, s);
-  if (a.d <= 96) return launch_chunks<T, 3, 6, 2, 4, 4>(a, B, s);
-  if (a.d <= 112) return launch_chunks<T, 4, 7, 2, 4, 4>(a, B, s);
-  return launch_chunks<T, 4, 8, 2, 4, 4>(a, B, s);
+  if (a.d <= 32) return launch_chunks<T, 1, 2, 1, 2>(a, B, s);
+  if (a.d <= 64) return launch_chunks<T, 2, 4, 1, 4>(a, B, s);
+  if (a.d <= 96) return launch_chunks<T, 3, 6, 2, 4>(a, B, s);
+  if (a.d <= 112) return launch_chunks<T, 4, 7, 2, 4>(a, B, s);
+  return launch_chunks<T, 4, 8, 2, 4>(a, B, s);
 }
 
 }  // namespace
