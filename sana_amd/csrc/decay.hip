@@ -175,10 +175,15 @@ __global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) 
     }
   };
   const uint16_t *kp = a.k + b * a.k_b + h * d, *vp = a.v + b * a.v_b + h * d, *qp = a.q + b * a.q_b + h * d;
+  // bf16 sums are weighted up to the segment's end at once: they need no decay from chunk to chunk (f16 would run out of range) and no
+  // order, and go backwards, so that the rows with which the outputs begin are the ones that the memory-side cache has seen last.
+  constexpr bool FAR = MODE == DC_SUMS && !F;
+  const int chunks = (last - first + DC - 1) / DC;
+  auto token_of = [&](int i) { return first + DC * (FAR ? chunks - 1 - i : i); };
   if (first < last) {
-    request(kp, a.k_n, k2, first, rk);
-    if constexpr (OUT) request(qp, a.q_n, q2, first, rq);
-    request(vp, a.v_n, v2, first, rv);
+    request(kp, a.k_n, k2, token_of(0), rk);
+    if constexpr (OUT) request(qp, a.q_n, q2, token_of(0), rq);
+    request(vp, a.v_n, v2, token_of(0), rv);
   }
 
   // ---- this lane's places in LDS
@@ -195,9 +200,9 @@ __global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) 
   const bool own = v0 < 32 * DK;  // (DK = 3: the fourth wave has no channels of v, and its reads would leave the rows)
 
 #pragma unroll 1
-  for (int at = first; at < last; at += DC) {
-    const int count = min(last - at, DC), next = at + DC;
-    const bool more = next < last;
+  for (int i = 0; i < chunks; ++i) {
+    const int at = token_of(i), count = min(last - at, DC), next = token_of(i + 1);
+    const bool more = i + 1 < chunks;
     stage(rk, 0);
     if constexpr (OUT) stage(rq, 2);
     else stage(rv, 1);
@@ -347,8 +352,7 @@ __global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) 
         }
       }
     }
-    // ---- the state behind the chunk.  bf16 sums are weighted up to the segment's end at once and need no decay (f16 would run out of range)
-    constexpr bool FAR = MODE == DC_SUMS && !F;
+    // ---- the state behind the chunk
     if (!OUT && more) request(vp, a.v_n, v2, next, rv);
     const float lane = FAR ? lane12 * dc_pow(g2, last - at - count) : lane12;
     __builtin_amdgcn_sched_barrier(0);
