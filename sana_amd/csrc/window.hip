@@ -63,7 +63,7 @@ __device__ __forceinline__ float wa_sum_groups(float x) {
 // nothing is rescaled (the 16-bit p keeps its relative step, l and o are fp32).  f16: p times 2^6, the small ones away from its
 // subnormal numbers.
 template <typename T, int DK, int DT, int QT, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void window_attn_kernel(const WindowArgs a) {
+__global__ __launch_bounds__(64 * NW, QT == 1 && DK < 4 ? 3 : 2) void window_attn_kernel(const WindowArgs a) {
   constexpr int PITCH = DK * 64, TILE = WK * PITCH, LOADS = TILE / 1024 / NW, QB = NW * 16 * QT;
   static_assert(TILE % (1024 * NW) == 0 && DT <= 2 * DK, "");
   __shared__ __attribute__((aligned(1024))) unsigned char k_even[TILE], k_odd[TILE], v_even[TILE], v_odd[TILE];
@@ -498,14 +498,20 @@ __global__ __launch_bounds__(256) void window_append_kernel(const WindowArgs a) 
       *reinterpret_cast<const u32x4_t*>(a.v + b * a.v_b + (int64_t)t * a.v_n + c);
 }
 
-constexpr int WA_QT = 2, WA_NW = 4, WA_QB = WA_NW * 16 * WA_QT;
-
-// Parts of a prompt's keys: where the blocks of queries leave compute units idle and have keys enough.
-int prompt_splits(int B, int N, int Nk, int H, int window, int sinks) {
-  const int64_t blocks = (int64_t)B * H * ((N + WA_QB - 1) / WA_QB);
-  const int64_t seen = (int64_t)window + WA_QB + sinks;
+constexpr int WA_NW = 4;
+// 16-query tiles of a wave, 64 or 128 queries a workgroup.  Two feed twice the MFMAs with a read of K or V; one gives more and shorter
+// workgroups, which is what counts while two leave compute units idle, and more waves a unit for narrow heads.  us, two / one: 16 heads of 72
+// 300 tokens 10.5 / 8.8, 1000 25.2 / 19.2, 2000 41.9 / 38.5, in a window of 256 2000 16.7 / 13.4, 4000 24.0 / 26.4; 20 heads of 112 600 tokens
+// 22.7 / 18.0, 1500 41.6 / 41.4, 3000 81 / 123; 36 heads of 32 300 7.8 / 6.4, 3000 75 / 59.
+int query_tiles(int B, int N, int H, int d) { return d <= 32 || (int64_t)B * H * ((N + 127) / 128) <= 256 ? 1 : 2; }
+// Parts of a prompt's keys: where the blocks of queries leave compute units idle and have tiles of keys enough to pay for a second launch
+// (600 tokens, 20 heads of 112, ten tiles: whole 18.0 us, in two parts 22.6).
+int prompt_splits(int B, int N, int Nk, int H, int d, int window, int sinks) {
+  const int qb = WA_NW * 16 * query_tiles(B, N, H, d);
+  const int64_t blocks = (int64_t)B * H * ((N + qb - 1) / qb);
+  const int64_t seen = (int64_t)window + qb + sinks;
   const int tiles = (int)((seen < Nk ? seen : Nk) / WK);
-  if (blocks >= 256 || tiles < 8) return 1;
+  if (blocks >= 256 || tiles < 16) return 1;
   int64_t want = 512 / blocks;
   want = want > tiles / 4 ? tiles / 4 : want;
   return (int)(want < 1 ? 1 : want > WA_MAX_SPLITS ? WA_MAX_SPLITS : want);
@@ -536,11 +542,15 @@ int launch_join(const WindowArgs& a, hipStream_t s) {
 
 template <typename T, int DK, int DT>
 int launch_prompt(WindowArgs a, hipStream_t s) {
-  a.qblocks = (a.N + WA_QB - 1) / WA_QB;
+  const bool one = DK == 1 || query_tiles(a.B, a.N, a.H, a.d) == 1;
+  const int qb = WA_NW * 16 * (one ? 1 : 2);
+  a.qblocks = (a.N + qb - 1) / qb;
   const int64_t items = (int64_t)a.B * a.H * a.qblocks * a.splits;
   if (items > 0x7ffffff0) return SANA_ERR_SHAPE;
   a.items = (int)items;
-  hipLaunchKernelGGL((window_attn_kernel<T, DK, DT, WA_QT, WA_NW>), dim3((unsigned)((items + 7) / 8 * 8)), dim3(64 * WA_NW), 0, s, a);
+  const dim3 grid((unsigned)((items + 7) / 8 * 8)), block(64 * WA_NW);
+  if (one) hipLaunchKernelGGL((window_attn_kernel<T, DK, DT, 1, WA_NW>), grid, block, 0, s, a);
+  else if constexpr (DK > 1) hipLaunchKernelGGL((window_attn_kernel<T, DK, DT, 2, WA_NW>), grid, block, 0, s, a);
   if (a.splits > 1) {
     const int rc = launch_join<T>(a, s);
     if (rc != SANA_OK) return rc;
@@ -602,7 +612,7 @@ using namespace sana;
 
 SANA_API size_t sana_hip_window_attention_workspace_bytes(int B, int N, int Nk, int H, int d, int window, int sinks) {
   if (B <= 0 || N <= 0 || Nk < N || H <= 0 || d <= 0 || window <= 0 || sinks < 0) return 0;
-  return part_bytes(prompt_splits(B, N, Nk, H, window, sinks), (int64_t)B * N * H, d);
+  return part_bytes(prompt_splits(B, N, Nk, H, d, window, sinks), (int64_t)B * N * H, d);
 }
 
 SANA_API int sana_hip_window_attention(const void* q, const void* k, const void* v, void* out, const int32_t* lengths, void* workspace,
@@ -628,7 +638,7 @@ SANA_API int sana_hip_window_attention(const void* q, const void* k, const void*
   a.B = B, a.N = N, a.Nk = Nk, a.H = H, a.Hkv = Hkv, a.d = d, a.window = window, a.sinks = sinks;
   a.q_b = q_stride_b, a.q_n = q_stride_n, a.k_b = k_stride_b, a.k_n = k_stride_n, a.v_b = v_stride_b, a.v_n = v_stride_n;
   a.o_b = o_stride_b, a.o_n = o_stride_n, a.scale_log2e = scale * 1.44269504088896341f;
-  a.splits = prompt_splits(B, N, Nk, H, window, sinks);
+  a.splits = prompt_splits(B, N, Nk, H, d, window, sinks);
   const int64_t rows = (int64_t)B * N * H;
   if (a.splits > 1) {
     if (!workspace || workspace_bytes < part_bytes(a.splits, rows, d)) return SANA_ERR_WORKSPACE;

@@ -948,7 +948,7 @@ def decay_linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lo
             raise SanaHipError(f"state and state_out must be contiguous fp32 {(B, H, d, d)}, got {t.dtype} {tuple(t.shape)}")
     length_ptr = _lengths_arg(lengths, B)
     if out is None:
-        out = (torch.empty if lengths is None else torch.zeros)(shape, dtype=dt, device=q.device)
+        out = q.new_empty(shape) if lengths is None else q.new_zeros(shape)
     elif out.shape != shape or out.dtype is not dt:
         raise SanaHipError("out has the wrong shape or dtype")
     if state_out is None:
@@ -1013,7 +1013,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, num_head
         raise SanaHipError(f"the {N} queries are the last of the keys, of which there are {Nk}")
     length_ptr = _lengths_arg(lengths, B)
     if out is None:
-        out = (torch.empty if lengths is None else torch.zeros)((B, N, C), dtype=q.dtype, device=q.device)
+        out = q.new_empty(q.shape) if lengths is None else q.new_zeros(q.shape)
     elif out.shape != q.shape or out.dtype != q.dtype:
         raise SanaHipError("out has the wrong shape or dtype")
     if B * N == 0:
@@ -1085,7 +1085,7 @@ def window_attention_step_(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ca
     B, _, C = q.shape
     position_ptr = _lengths_arg(positions, B, "positions")
     if out is None:
-        out = torch.empty((B, 1, C), dtype=q.dtype, device=q.device)
+        out = q.new_empty(q.shape)
     elif out.shape != q.shape or out.dtype != q.dtype:
         raise SanaHipError("out has the wrong shape or dtype")
     if B == 0:
