@@ -23,7 +23,7 @@ struct DecayArgs {
   const float *log_decay, *state_in;
   float *state_out, *segments;  // segments: [B * H][nseg][d * d], the states in front of each segment
   const int* lengths;
-  int N, H, d, nseg, seg_tokens, items;
+  int N, H, d, nseg, seg_tokens, units;
   int64_t q_b, q_n, k_b, k_n, v_b, v_n, o_b, o_n;
   float scale;
 };
@@ -94,10 +94,12 @@ __global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) 
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), fr = tid & 15, fg = (tid >> 4) & 3;
   const int v0 = 16 * VT * (wave % NV), qt0 = QN * (wave / NV);
 
-  // neighbouring heads, whose rows share cache lines, on one XCD
-  const int per = (a.items + 7) >> 3, item = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  if (item >= a.items) return;
-  const int h = item % a.H, rest = item / a.H, seg = rest % a.nseg, b = rest / a.nseg, d = a.d, bh = b * a.H + h;
+  // Four neighbouring heads, whose rows share cache lines, go to one XCD, the next four to the next: streams of unlike length, whose last
+  // segments are not there, leave no XCD idle.
+  const int slot = blockIdx.x >> 3, unit = (slot >> 2) * 8 + (blockIdx.x & 7), parts = (a.H + 3) >> 2;
+  if (unit >= a.units) return;
+  const int h = 4 * (unit % parts) + (slot & 3), rest = unit / parts, seg = rest % a.nseg, b = rest / a.nseg, d = a.d, bh = b * a.H + h;
+  if (h >= a.H) return;
   const int n = a.lengths ? min(max(a.lengths[b], 0), a.N) : a.N;
   const int first = seg * a.seg_tokens, last = min(n, first + a.seg_tokens);  // (host: seg * seg_tokens < N)
   if (MODE != DC_WHOLE && first >= n) return;
@@ -496,11 +498,11 @@ int segment_count(int B, int N, int H, int* tokens) {
 
 template <typename T, int DK, int KT, int VT, int NV>
 int launch_chunks(const DecayArgs& a, int B, hipStream_t s) {
-  const int64_t items = (int64_t)B * a.H * a.nseg;
-  if (items > 0x7ffffff0) return SANA_ERR_SHAPE;
+  const int64_t units = (int64_t)B * a.nseg * ((a.H + 3) / 4);
+  if (units > (1 << 28)) return SANA_ERR_SHAPE;
   DecayArgs args = a;
-  args.items = (int)items;
-  const dim3 grid((unsigned)((items + 7) / 8 * 8)), block(256);
+  args.units = (int)units;
+  const dim3 grid((unsigned)((units + 7) / 8 * 32)), block(256);
   if (a.nseg > 1) {
     hipLaunchKernelGGL((decay_chunk_kernel<T, DK, KT, VT, NV, DC_SUMS>), grid, block, 0, s, args);
     hipLaunchKernelGGL(decay_scan_kernel, dim3((unsigned)((a.d * a.d / 4 + 63) / 64), (unsigned)(B * a.H)), dim3(64), 0, s, args);
@@ -569,7 +571,7 @@ SANA_API int sana_hip_decay_attention(const void* q, const void* k, const void* 
   a.q = static_cast<const uint16_t*>(q), a.k = static_cast<const uint16_t*>(k), a.v = static_cast<const uint16_t*>(v);
   a.out = static_cast<uint16_t*>(out);
   a.log_decay = log_decay, a.state_in = state_in, a.state_out = state_out, a.segments = nullptr, a.lengths = lengths;
-  a.N = N, a.H = H, a.d = d, a.nseg = 1, a.seg_tokens = N, a.items = 0;
+  a.N = N, a.H = H, a.d = d, a.nseg = 1, a.seg_tokens = N, a.units = 0;
   a.q_b = q_stride_b, a.q_n = q_stride_n, a.k_b = k_stride_b, a.k_n = k_stride_n, a.v_b = v_stride_b, a.v_n = v_stride_n;
   a.o_b = o_stride_b, a.o_n = o_stride_n, a.scale = scale;
   if (N > 1) a.nseg = segment_count(B, N, H, &a.seg_tokens);

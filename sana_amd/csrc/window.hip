@@ -69,11 +69,11 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DK < 4 ? 3 : 2) void window_att
   __shared__ __attribute__((aligned(1024))) unsigned char k_even[TILE], k_odd[TILE], v_even[TILE], v_odd[TILE];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, fr = lane & 15, fg = lane >> 4;
 
-  // the blocks of one head, which read the same keys, on one XCD
+  // The blocks of a head and of those that share its keys on one XCD; the streams, which may be of unlike length, one after the other.
   const int per = (a.items + 7) >> 3, item = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
   if ((int)(blockIdx.x >> 3) >= per || item >= a.items) return;
-  const int split = item % a.splits, r1 = item / a.splits, qb = a.qblocks - 1 - r1 % a.qblocks, bh = r1 / a.qblocks;
-  const int b = bh / a.H, h = bh - b * a.H, hk = h / (a.H / a.Hkv), d = a.d;
+  const int share = a.H / a.Hkv, split = item % a.splits, r1 = item / a.splits, qb = a.qblocks - 1 - r1 % a.qblocks, r2 = r1 / a.qblocks;
+  const int r3 = r2 / share, hk = r3 / a.B, b = r3 - hk * a.B, h = hk * share + (r2 - r3 * share), d = a.d;
   const int queries = a.lengths ? min(max(a.lengths[b], 0), a.N) : a.N;  // that there are
   const int q0 = qb * QB;
   if (q0 >= queries) return;
@@ -233,8 +233,8 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DK < 4 ? 3 : 2) void window_att
       u32x4_t kf[DK];
       load_keys(k_next, kt, kf);
       multiply_keys(kt, kf, next);
-      if constexpr (QT == 2) powers(kt & 1, kt >> 1, sc, pk);
-      else if (kt < 2) powers(0, kt, sc, pk);
+#pragma unroll
+      for (int u = kt * QT / 2; u < (kt + 1) * QT / 2; ++u) powers(u % QT, u / QT, sc, pk);
     }
     __builtin_amdgcn_sched_barrier(0);
     values(v_here, 0, pk);
