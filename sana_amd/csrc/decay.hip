@@ -375,27 +375,43 @@ __global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) 
               if constexpr (F) x0 *= 2048.f, x1 *= 2048.f;
             }
           }
+        // (two tiles of k at a time, term by term: an MFMA that adds to what the one before it has just summed waits for twice its own time)
 #pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-          const uint32_t from = kt_at(kt) + 32 * s * PITCH;
-          const u32x2_t lo = dc_read_tr(from), hi = dc_read_tr(from + 16 * PITCH);
-          const u32x4_t kf = {lo.x, lo.y, hi.x, hi.y};
+        for (int k0 = 0; k0 < KT; k0 += 2) {
+          u32x4_t kf[2];
+          f32x4_t y[2][VT];
 #pragma unroll
-          for (int vt = 0; vt < VT; ++vt) {
-            f32x4_t x = st[vt][kt];
-            if (s == 0 && !FAR)
+          for (int j = 0; j < 2; ++j) {
+            if (k0 + j >= KT) continue;
+            const uint32_t from = kt_at(k0 + j) + 32 * s * PITCH;
+            const u32x2_t lo = dc_read_tr(from), hi = dc_read_tr(from + 16 * PITCH);
+            kf[j] = u32x4_t{lo.x, lo.y, hi.x, hi.y};
 #pragma unroll
-              for (int r = 0; r < 4; ++r) x[r] *= over;
-            if constexpr (F) {
-              const f32x4_t y = mfma_16x16x32<T>(kf, w[1][vt], f32x4_t{0.f, 0.f, 0.f, 0.f});
-              x = mfma_16x16x32<T>(kf, w[0][vt], x);
+            for (int vt = 0; vt < VT; ++vt) {
+              if (s == 0 && !FAR)
 #pragma unroll
-              for (int r = 0; r < 4; ++r) x[r] = fmaf(y[r], 1.0f / 2048.f, x[r]);
-            } else {
-#pragma unroll
-              for (int i = 0; i < TERMS; ++i) x = mfma_16x16x32<T>(kf, w[i][vt], x);
+                for (int r = 0; r < 4; ++r) st[vt][k0 + j][r] *= over;
+              y[j][vt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
             }
-            st[vt][kt] = x;
+          }
+#pragma unroll
+          for (int i = 0; i < TERMS; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int vt = 0; vt < VT; ++vt) {
+                if (k0 + j >= KT) continue;
+                f32x4_t& x = F && i == 1 ? y[j][vt] : st[vt][k0 + j];
+                x = mfma_16x16x32<T>(kf[j], w[i][vt], x);
+              }
+          if constexpr (F) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int vt = 0; vt < VT; ++vt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                  if (k0 + j < KT) st[vt][k0 + j][r] = fmaf(y[j][vt][r], 1.0f / 2048.f, st[vt][k0 + j][r]);
           }
         }
       }
