@@ -140,17 +140,25 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DK < 4 ? 3 : 2) void window_att
     const int j0 = tile_of(t) * WK, j1 = j0 + WK - 1;
     return j1 <= wp0 && (j1 < a.sinks || wp1 - j0 < a.window);
   };
-  auto load_keys = [&](const unsigned char* from, int kt, u32x4_t (&kf)[DK]) {
+  // Scores of KP tiles of 16 keys at a time: one where two query tiles take turns, two otherwise (an MFMA that adds to what the one before
+  // it has just summed waits for twice its own time).
+  constexpr int KP = QT == 1 ? 2 : 1;
+  auto score = [&](const unsigned char* from, int k0, f32x4_t (&sc)[QT][4]) {
+    u32x4_t kf[KP][DK];
 #pragma unroll
-    for (int s = 0; s < DK; ++s) kf[s] = wa_read((const wa_lds*)from + 16 * kt * PITCH + k_at[s]);
-  };
-  auto multiply_keys = [&](int kt, const u32x4_t (&kf)[DK], f32x4_t (&sc)[QT][4]) {
+    for (int j = 0; j < KP; ++j)
 #pragma unroll
-    for (int q = 0; q < QT; ++q) sc[q][kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      for (int s = 0; s < DK; ++s) kf[j][s] = wa_read((const wa_lds*)from + 16 * (k0 + j) * PITCH + k_at[s]);
+#pragma unroll
+    for (int j = 0; j < KP; ++j)
+#pragma unroll
+      for (int q = 0; q < QT; ++q) sc[q][k0 + j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int s = 0; s < DK; ++s)
 #pragma unroll
-      for (int q = 0; q < QT; ++q) sc[q][kt] = mfma_16x16x32<T>(kf[s], qf[q][s], sc[q][kt]);
+      for (int j = 0; j < KP; ++j)
+#pragma unroll
+        for (int q = 0; q < QT; ++q) sc[q][k0 + j] = mfma_16x16x32<T>(kf[j][s], qf[q][s], sc[q][k0 + j]);
   };
   auto mask = [&](int t, f32x4_t (&sc)[QT][4]) {
     const int lane_key = tile_of(t) * WK + 4 * fg, to_sinks = a.sinks - lane_key;  // c = 16 kt + r is key lane_key + c
@@ -225,16 +233,14 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DK < 4 ? 3 : 2) void window_att
     if (!whole(t)) mask(t, sc);
     maxima(sc);
     asm volatile("" : "+v"(v_slot));  // (addresses are worked out here again: kept, they would take the registers of the tiles)
-    // 16 keys of the next tile at a time, and a half of the queries' powers between their MFMAs
+    // 16 or 32 keys of the next tile at a time, and the powers of half of the keys between their MFMAs
     u32x2_t pk[QT][4];
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
+    for (int kt = 0; kt < 4; kt += KP) {
       __builtin_amdgcn_sched_barrier(0);
-      u32x4_t kf[DK];
-      load_keys(k_next, kt, kf);
-      multiply_keys(kt, kf, next);
+      score(k_next, kt, next);
 #pragma unroll
-      for (int u = kt * QT / 2; u < (kt + 1) * QT / 2; ++u) powers(u % QT, u / QT, sc, pk);
+      for (int u = kt * QT / 2; u < (kt + KP) * QT / 2; ++u) powers(u % QT, u / QT, sc, pk);
     }
     __builtin_amdgcn_sched_barrier(0);
     values(v_here, 0, pk);
@@ -250,10 +256,8 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DK < 4 ? 3 : 2) void window_att
     if (t0 + 1 < t1) request(kp, a.k_n, k2, t0 + 1, k_odd);
     landed();
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
-      u32x4_t kf[DK];
-      load_keys(k_even, kt, kf);
-      multiply_keys(kt, kf, even);
+    for (int kt = 0; kt < 4; kt += KP) {
+      score(k_even, kt, even);
       __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll 1
@@ -392,17 +396,15 @@ __global__ __launch_bounds__(64 * NW) void window_step_kernel(const WindowArgs a
   if (t0 + wave < t1) request(t0 + wave);
 #pragma unroll 1
   for (int t = t0 + wave; t < t1; t += NW) {
-    f32x4_t sc[2];
+    f32x4_t sc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-      sc[kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < DK; ++s)  // (channels past d: K repeats others there, q is zero; an inf there must not count)
 #pragma unroll
-      for (int s = 0; s < DK; ++s) {  // (channels past d: K repeats others there, q is zero; an inf there must not count)
+      for (int kt = 0; kt < 2; ++kt) {
         u32x4_t kf = rk[kt][s];
         if (32 * s + 8 * fg >= d) kf = u32x4_t{0u, 0u, 0u, 0u};
         sc[kt] = mfma_16x16x32<T>(kf, qf[s], sc[kt]);
       }
-    }
 #pragma unroll
     for (int i = 0; i < PV; ++i) {
       const int idx = lane + 64 * i, r = idx / (DK * 4), c = idx - r * (DK * 4);
