@@ -501,13 +501,14 @@ __global__ __launch_bounds__(256) void window_append_kernel(const WindowArgs a) 
 }
 
 constexpr int WA_NW = 4;
-// 16-query tiles of a wave, 64 or 128 queries a workgroup.  Two feed twice the MFMAs with a read of K or V; one gives more and shorter
-// workgroups, which is what counts while two leave compute units idle, and more waves a unit for narrow heads.  us, two / one: 16 heads of 72
-// 300 tokens 10.5 / 8.8, 1000 25.2 / 19.2, 2000 41.9 / 38.5, in a window of 256 2000 16.7 / 13.4, 4000 24.0 / 26.4; 20 heads of 112 600 tokens
-// 22.7 / 18.0, 1500 41.6 / 41.4, 3000 81 / 123; 36 heads of 32 300 7.8 / 6.4, 3000 75 / 59.
-int query_tiles(int B, int N, int H, int d) { return d <= 32 || (int64_t)B * H * ((N + 127) / 128) <= 256 ? 1 : 2; }
+// 16-query tiles of a wave, 64 or 128 queries a workgroup.  Two feed twice the MFMAs with a read of K or V and pay where heads are wide
+// and the blocks many; one gives more and shorter workgroups, and up to 96 channels three and more waves a SIMD.  us, two / one, window 4096:
+// 20 heads of 112 1500 tokens 39 / 32, 2000 63 / 49, 3000 77 / 93, 8000 304 / 357; 16 of 128 3000 82 / 62, 4680 139 / 129, 8000 253 / 272;
+// 16 of 72 1500 34.4 / 26.5, 4680 109 / 100, 8000 193 / 204, 12 of 96 8000 193 / 187, 35 of 64 8000 325 / 316; window 256: 35 of 64
+// 8000 72 / 56, 12 of 96 8000 38 / 31, 20 of 112 16384 133 / 145.
+int query_tiles(int B, int N, int H, int d) { return d <= 96 || (int64_t)B * H * ((N + 127) / 128) <= 400 ? 1 : 2; }
 // Parts of a prompt's keys: where the blocks of queries leave compute units idle and have tiles of keys enough to pay for a second launch
-// (600 tokens, 20 heads of 112, ten tiles: whole 18.0 us, in two parts 22.6).
+// (600 tokens, 20 heads of 112, ten tiles: whole 13.9 us, in two parts over 20).
 int prompt_splits(int B, int N, int Nk, int H, int d, int window, int sinks) {
   const int qb = WA_NW * 16 * query_tiles(B, N, H, d);
   const int64_t blocks = (int64_t)B * H * ((N + qb - 1) / qb);
@@ -544,7 +545,7 @@ int launch_join(const WindowArgs& a, hipStream_t s) {
 
 template <typename T, int DK, int DT>
 int launch_prompt(WindowArgs a, hipStream_t s) {
-  const bool one = DK == 1 || query_tiles(a.B, a.N, a.H, a.d) == 1;
+  const bool one = DK < 4 || query_tiles(a.B, a.N, a.H, a.d) == 1;
   const int qb = WA_NW * 16 * (one ? 1 : 2);
   a.qblocks = (a.N + qb - 1) / qb;
   const int64_t items = (int64_t)a.B * a.H * a.qblocks * a.splits;
@@ -552,7 +553,7 @@ int launch_prompt(WindowArgs a, hipStream_t s) {
   a.items = (int)items;
   const dim3 grid((unsigned)((items + 7) / 8 * 8)), block(64 * WA_NW);
   if (one) hipLaunchKernelGGL((window_attn_kernel<T, DK, DT, 1, WA_NW>), grid, block, 0, s, a);
-  else if constexpr (DK > 1) hipLaunchKernelGGL((window_attn_kernel<T, DK, DT, 2, WA_NW>), grid, block, 0, s, a);
+  else if constexpr (DK == 4) hipLaunchKernelGGL((window_attn_kernel<T, DK, DT, 2, WA_NW>), grid, block, 0, s, a);
   if (a.splits > 1) {
     const int rc = launch_join<T>(a, s);
     if (rc != SANA_OK) return rc;
