@@ -57,11 +57,14 @@ __device__ __forceinline__ float wa_sum_groups(float x) {
 }
 
 // A prompt or a chunk: the queries are the last N of Nk keys.  A workgroup takes NW * 16 * QT queries of one head through its
-// tiles of 64 keys, the tiles of the sinks first; K and V go to LDS through registers, a tile ahead.  scores^T = K Q^T: a lane
-// owns a query (its column) and four keys of every 16; the probabilities are fed back from the accumulators, V by transposing reads in the
-// order of keys that this gives.  The running maximum moves only when some score is 2^8 above it: until then p <= 2^8 and
-// nothing is rescaled (the 16-bit p keeps its relative step, l and o are fp32).  f16: p times 2^6, the small ones away from its
-// subnormal numbers.
+// tiles of 64 keys, the tiles of the sinks first; K and V go to LDS by direct loads, V a tile behind K, one barrier a tile.  scores^T = K Q^T: a
+// lane owns a query (its column) and four keys of every 16; the probabilities are fed back from the accumulators, V by transposing reads in
+// the order of keys that this gives.  The running maximum moves only when some score is 2^8 above it: until then p <= 2^8 and nothing is
+// rescaled (the 16-bit p keeps its relative step, l and o are fp32).  f16: p times 2^6, the small ones away from its subnormal numbers.
+// Of a tile of 64 keys x 32 queries x 112 channels the matrix pipe takes 960 cycles, the vector unit some 1000 (half of them powers) and
+// the LDS 350 for each of four waves: with two waves a SIMD 16384 tokens x 20 heads over a window of 4096 run at 0.82 - 0.86 PFLOP/s
+// (615 - 645 us).  Through registers instead of direct loads 705 us; each tile's scores in front of its own powers instead of those of
+// the tile before: 630 - 690, by how the compiler mixes them; three or four query tiles a wave: the registers do not hold them.
 template <typename T, int DK, int DT, int QT, int NW>
 __global__ __launch_bounds__(64 * NW, QT == 1 && DK < 4 ? 3 : 2) void window_attn_kernel(const WindowArgs a) {
   constexpr int PITCH = DK * 64, TILE = WK * PITCH, LOADS = TILE / 1024 / NW, QB = NW * 16 * QT;
@@ -99,7 +102,7 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DK < 4 ? 3 : 2) void window_att
   }
   const int wp0 = past + w0, wp1 = min(wp0 + 16 * QT - 1, p1);
 
-  // K and V of a tile by direct loads to LDS, 1 KB each: a lane's 16 bytes are at the place that its number gives, so it fetches
+  // K and V of a tile by direct loads to LDS, 1 KB each, arrays of their own, by which the compiler sees that no read waits for another tile: a lane's 16 bytes are at the place that its number gives, so it fetches
   // the piece that the row's exchange puts there.  Outside of the rows: zeros.  (63 rows are less than 2^31 bytes: nothing comes back in.)
   const uint16_t *kp = a.k + b * a.k_b + hk * d, *vp = a.v + b * a.v_b + hk * d;
   const uint32_t k2 = 2 * (uint32_t)a.k_n, v2 = 2 * (uint32_t)a.v_n;
