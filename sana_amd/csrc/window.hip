@@ -626,7 +626,7 @@ SANA_API int sana_hip_window_attention(const void* q, const void* k, const void*
                                        int64_t q_stride_b, int64_t q_stride_n, int64_t k_stride_b, int64_t k_stride_n,
                                        int64_t v_stride_b, int64_t v_stride_n, int64_t o_stride_b, int64_t o_stride_n, float scale,
                                        int io_dtype, void* stream) {
-  if (!q || !k || !v || !out || Nk < N || !(scale > 0.f)) return SANA_ERR_ARG;
+  if (!q || !k || !v || !out || Nk < N || !(scale > 0.f && scale < INFINITY)) return SANA_ERR_ARG;
   const int rc = check_sizes(B, N, H, Hkv, d, window, sinks, io_dtype);
   if (rc != SANA_OK) return rc;
   if (Nk > (1 << 30)) return SANA_ERR_SHAPE;
@@ -634,6 +634,7 @@ SANA_API int sana_hip_window_attention(const void* q, const void* k, const void*
     return SANA_ERR_ARG;
   for (const int64_t sb : {q_stride_b, k_stride_b, v_stride_b, o_stride_b})
     if (sb < 0) return SANA_ERR_ARG;
+  if (B > 1 && o_stride_b == 0) return SANA_ERR_ARG;  // (entries that would write the same rows)
   if (k_stride_n >= (1 << 23) || v_stride_n >= (1 << 23)) return SANA_ERR_SHAPE;  // 32-bit byte offsets within a tile
   if (misaligned({q, k, v}, {q_stride_b, q_stride_n, k_stride_b, k_stride_n, v_stride_b, v_stride_n}) ||
       (reinterpret_cast<uintptr_t>(out) & 7u) || o_stride_b % 4 || o_stride_n % 4 || off4(lengths))
@@ -668,6 +669,8 @@ SANA_API int sana_hip_window_cache_append(void* cache_k, void* cache_v, const vo
   if (ck_stride_n < C || cv_stride_n < C || k_stride_n < C || v_stride_n < C) return SANA_ERR_ARG;
   for (const int64_t sb : {ck_stride_b, cv_stride_b, k_stride_b, v_stride_b})
     if (sb < 0) return SANA_ERR_ARG;
+  if (B > 1 && (ck_stride_b == 0 || cv_stride_b == 0)) return SANA_ERR_ARG;  // (streams that would write the same rows)
+  if ((int64_t)window + sinks > (1 << 30)) return SANA_ERR_SHAPE;
   if (C % 8 || groups > 0x7fffffff || B > 65535) return SANA_ERR_SHAPE;
   if (misaligned({cache_k, cache_v, k, v}, {ck_stride_b, ck_stride_n, cv_stride_b, cv_stride_n, k_stride_b, k_stride_n, v_stride_b, v_stride_n}) ||
       off4(positions) || off4(lengths))
@@ -683,7 +686,7 @@ SANA_API int sana_hip_window_cache_append(void* cache_k, void* cache_v, const vo
 }
 
 SANA_API size_t sana_hip_window_step_workspace_bytes(int B, int H, int Hkv, int d, int window, int sinks) {
-  if (B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || d <= 0 || window <= 0 || window > (1 << 30) || sinks < 0 || sinks > (1 << 30)) return 0;
+  if (B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || d <= 0 || window <= 0 || sinks < 0 || (int64_t)window + sinks > (1 << 30)) return 0;
   return part_bytes(step_splits(B, H, Hkv, window + sinks), (int64_t)B * H, d);
 }
 
@@ -692,13 +695,15 @@ SANA_API int sana_hip_window_step(const void* q, const void* k, const void* v, v
                                   int sinks, int64_t q_stride_b, int64_t k_stride_b, int64_t v_stride_b, int64_t ck_stride_b,
                                   int64_t ck_stride_n, int64_t cv_stride_b, int64_t cv_stride_n, int64_t o_stride_b, float scale,
                                   int io_dtype, void* stream) {
-  if (!q || !k || !v || !cache_k || !cache_v || !positions || !out || !(scale > 0.f)) return SANA_ERR_ARG;
+  if (!q || !k || !v || !cache_k || !cache_v || !positions || !out || !(scale > 0.f && scale < INFINITY)) return SANA_ERR_ARG;
   const int rc = check_sizes(B, 1, H, Hkv, d, window, sinks, io_dtype);
   if (rc != SANA_OK) return rc;
   const int64_t C = (int64_t)Hkv * d;
   if (ck_stride_n < C || cv_stride_n < C) return SANA_ERR_ARG;
   for (const int64_t sb : {q_stride_b, k_stride_b, v_stride_b, ck_stride_b, cv_stride_b, o_stride_b})
     if (sb < 0) return SANA_ERR_ARG;
+  if (B > 1 && (o_stride_b == 0 || ck_stride_b == 0 || cv_stride_b == 0)) return SANA_ERR_ARG;  // (streams that would write the same rows)
+  if ((int64_t)window + sinks > (1 << 30)) return SANA_ERR_SHAPE;
   if (misaligned({q, k, v, cache_k, cache_v}, {q_stride_b, k_stride_b, v_stride_b, ck_stride_b, ck_stride_n, cv_stride_b, cv_stride_n}) ||
       (reinterpret_cast<uintptr_t>(out) & 7u) || o_stride_b % 4 || off4(positions))
     return SANA_ERR_ALIGN;

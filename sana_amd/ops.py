@@ -987,7 +987,7 @@ def _window_shapes(q, k, v, num_heads: int, window: int, sinks: int, scale: Opti
     if not 1 <= window <= 1 << 30 or not 0 <= sinks <= 1 << 30:
         raise SanaHipError(f"window must be at least 1 and sinks at least 0, got {window} and {sinks}")
     scale = d ** -0.5 if scale is None else float(scale)
-    if not scale > 0.0:
+    if not 0.0 < scale < float("inf"):
         raise SanaHipError(f"scale must be positive, got {scale}")
     return d, Ck // d, scale
 
@@ -1073,7 +1073,8 @@ def window_attention_step_(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ca
     [B, sinks + window, Hkv*d] (:func:`window_cache_append_`) at ``positions`` [B] (int32, on the device: the tokens seen before,
     which the caller advances once all layers are through), and the token attends to what the caches then hold: the last
     ``window`` tokens up to itself and the first ``sinks``.  A stream with a negative position is idle: its caches stay as they are, its
-    output is zero.  Returns [B, 1, H*d].  Forward only."""
+    output is zero.  The caches must not overlap q, k, v or ``out``, and no two streams may share rows.  Returns [B, 1, H*d].
+    Forward only."""
     dev = _here((q, k, v, cache_k, cache_v, positions, out), "window_attention_step_")
     if dev != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):

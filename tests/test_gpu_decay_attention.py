@@ -254,6 +254,7 @@ def test_refusals(cuda):
            lambda: call(q[..., :84], k[..., :84], v[..., :84], g), lambda: call(*[t[:, :, ::2] for t in (q, k, v)], g),
            lambda: call(*[t[:1].expand(2, 8, 96)[:, :1].expand(2, 8, 96) for t in (q, k, v)], g),
            lambda: call(*[torch.zeros(2 * 8 * 96 + 1, dtype=BF16, device="cuda")[1:].view(2, 8, 96)] * 3, g),
+           lambda: call(q, k, v, g, out=torch.empty_like(q[:1]).expand(2, 8, 96)),
            lambda: call(q, k, v.clone().requires_grad_(), g)]
     for i, f in enumerate(bad):
         with pytest.raises(sana_amd.SanaHipError):
@@ -277,6 +278,7 @@ def test_c_entry_refuses_before_any_launch():
     for i in (15, 17, 19, 21):
         assert call((i, 88)) == -1 and call((i, 1 << 23)) == -2
         assert call((i, 98)) == -3 and call((i - 1, -8)) == -1
+    assert call((20, 0)) == -1 and call((20, 0), (10, 0)) == -1   # two entries of one output
     for i in (0, 1, 2, 4, 5):
         assert call((i, P + 8)) == -3
     assert call((6, P + 4)) == -3 and call((3, P + 2)) == -3 and call((7, P + 2)) == -3

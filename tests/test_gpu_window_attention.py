@@ -303,6 +303,8 @@ def test_refusals(cuda):
            lambda: w(q[..., :112], k[..., :56], v[..., :56], 4, 5), lambda: w(odd, k, v, 4, 5), lambda: w(q, k, v, 4, 5, out=q[:, :4]),
            lambda: w(q, k, v, 4, 5, lengths=pos.long()), lambda: w(q, k, v, 4, 5, lengths=pos[:1]), lambda: w(q, k, v, 4, 5, lengths=pos.cpu()),
            lambda: w(q.clone().requires_grad_(), k, v, 4, 5), lambda: w(q, k[:1].expand(2, 8, 64)[:, :1].expand(2, 8, 64), v, 4, 5),
+           lambda: w(q, k, v, 4, 5, scale=float("inf")), lambda: w(q, k, v, 4, 5, out=torch.empty_like(q[:1]).expand(2, 8, 128)),
+           lambda: s(q1, k1, v1, ck[:1].expand(2, 20, 64), cv, pos, 4), lambda: a(ck, cv[:1].expand(2, 20, 64), k, v, pos),
            lambda: s(q, k, v, ck, cv, pos, 4), lambda: s(q1, k1, v1, ck[:1], cv[:1], pos, 4), lambda: s(q1, k1, v1, ck, cv[:, :9], pos, 4),
            lambda: s(q1, k1, v1, ck.half(), cv.half(), pos, 4), lambda: s(q1, k1, v1, ck, cv, pos, 4, 20), lambda: s(q1, k1, v1, ck, cv, pos, 4, -1),
            lambda: s(q1, k1, v1, ck, cv, pos.long(), 4), lambda: s(q1, k1, v1, ck, cv, None, 4), lambda: s(q1, k1, v1, ck, cv, pos, 5),
@@ -346,6 +348,9 @@ def test_c_entries_refuse_before_any_launch():
         assert step((i, None)) == -1
     for i in (9, 10, 11, 12, 13):
         assert step((i, 0)) == -1
+    many = ((9, 2),)
+    assert step(*many, (18, 0)) == -1 and step(*many, (20, 0)) == -1 and step(*many, (22, 0)) == -1 and step((13, 1 << 30)) == -2
+    assert step((23, float("inf"))) == -1
     assert step((14, -1)) == -1 and step((11, 7)) == -1 and step((23, -1.0)) == -1 and step((24, 0)) == -6 and step((12, 132)) == -2
     assert step((19, 1024)) == -1 and step((21, 1024)) == -1 and step((18, -8)) == -1 and step((15, 4100)) == -3 and step((5, P + 2)) == -3
     need = lib.sana_hip_window_step_workspace_bytes(1, 4, 2, 64, 4000, 4)
@@ -358,6 +363,7 @@ def test_c_entries_refuse_before_any_launch():
         assert put((i, None)) == -1
     for i in (6, 7, 8, 9):
         assert put((i, 0)) == -1
+    assert put((11, 0)) == -1 and put((13, 0)) == -1 and put((9, 1 << 30)) == -2
     assert put((10, -1)) == -1 and put((8, 252)) == -2 and put((6, 70000)) == -2 and put((19, 0)) == -6 and put((12, 128)) == -1
     assert put((0, P + 2)) == -3 and put((15, 2564)) == -3 and put((17, -8)) == -1
 
