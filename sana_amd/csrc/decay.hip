@@ -8,9 +8,7 @@
 //   o_t = scale * (a^(t+1) S0 q_t + sum_{j <= t} a^(t-j) (q_t . k_j) v_j),     S = a^C S0 + sum_j a^(C-1-j) v_j k_j^T:
 //
 // four products of 64 rows on the matrix pipes, 4 C d + 4 d^2 operations a token and head against 8 d bytes of memory.
-#include <type_traits>
-
-#include "common.h"
+#include "stream_common.h"
 
 namespace sana {
 namespace {
@@ -28,28 +26,10 @@ struct DecayArgs {
   float scale;
 };
 
-// 16-byte slots of an LDS row of DK * 64 bytes are exchanged by a key of the row: 16 consecutive rows of one slot, and the 16 rows of a
-// transposing read, cover all banks.  The key of row 16 i + r is that of r.
-template <int DK>
-__device__ __forceinline__ int dc_key(int row) {
-  return DK == 4 ? (row & 15) : DK == 2 ? ((row >> 1) & 7) : ((row >> 2) & 3);
-}
-__device__ __forceinline__ u32x2_t dc_read_tr(uint32_t lds) {  // 4 tokens x 16 channels -> this lane's channel, 4 tokens
-  typedef short s16x4_t __attribute__((ext_vector_type(4)));
-  return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(size_t)lds));
-}
-__device__ __forceinline__ u32x4_t dc_read(uint32_t lds) {
-  return *(__attribute__((address_space(3))) const u32x4_t*)(size_t)lds;
-}
-__device__ __forceinline__ u32x2_t dc_read8(uint32_t lds) {
-  return *(__attribute__((address_space(3))) const u32x2_t*)(size_t)lds;
-}
-// What this wave wrote to LDS is there and what it reads from there has come; loads from memory stay in flight.
-__device__ __forceinline__ void dc_barrier() {
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-}
+// (addresses as integers: through pointers the compiler reads further ahead than the registers hold)
+__device__ __forceinline__ u32x2_t dc_read_tr(uint32_t at) { return lds_read_tr((lds_t*)(size_t)at); }
+__device__ __forceinline__ u32x4_t dc_read(uint32_t at) { return lds_read((const lds_t*)(size_t)at); }
+__device__ __forceinline__ u32x2_t dc_read8(uint32_t at) { return lds_read8((const lds_t*)(size_t)at); }
 // exp(g) as a power of two; below 2^-256 a decay is 0 in every power but the 0th, and -inf * 0 must not be NaN
 __device__ __forceinline__ float dc_log2(float g) {
   const float g2 = g * 1.44269504088896341f;
@@ -88,7 +68,7 @@ __global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) 
   constexpr int NQ = 4 / NV, QN = 4 / NQ;  // shares of the queries, query tiles of a share
   static_assert(KT <= 2 * DK && DC * DK * 4 % NT == 0 && 4 % NV == 0, "");
   __shared__ __attribute__((aligned(16))) unsigned char smem[(OUT ? 3 : 2) * TILE + (OUT ? DC * 128 + DC * 4 : 0)];
-  const uint32_t sk = (uint32_t)(size_t)(__attribute__((address_space(3))) unsigned char*)smem;
+  const uint32_t sk = (uint32_t)(size_t)(lds_t*)smem;
   const uint32_t sv = sk + TILE, sq = sk + 2 * TILE, sp = sk + 3 * TILE;
   float* fit = reinterpret_cast<float*>(smem + 3 * TILE + DC * 128);  // f16: the scale of a query's P
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), fr = tid & 15, fg = (tid >> 4) & 3;
@@ -173,7 +153,7 @@ __global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) 
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
       const int idx = tid + NT * i, row = idx / (DK * 4), c = idx - row * (DK * 4);
-      *reinterpret_cast<u32x4_t*>(smem + tile * TILE + row * PITCH + ((c ^ dc_key<DK>(row)) << 4)) = r[i];
+      *reinterpret_cast<u32x4_t*>(smem + tile * TILE + row * PITCH + ((c ^ row_key<DK>(row)) << 4)) = r[i];
     }
   };
   const uint16_t *kp = a.k + b * a.k_b + h * d, *vp = a.v + b * a.v_b + h * d, *qp = a.q + b * a.q_b + h * d;
@@ -189,11 +169,11 @@ __global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) 
   }
 
   // ---- this lane's places in LDS
-  const int key = dc_key<DK>(fr);
+  const int key = row_key<DK>(fr);
   uint32_t row16[DK];  // row fr, k = 32 s + 8 fg
 #pragma unroll
   for (int s = 0; s < DK; ++s) row16[s] = fr * PITCH + (((4 * s + fg) ^ key) << 4);
-  const int trow = 4 * fg + (fr >> 2), tkey = dc_key<DK>(trow), piece = fr & 3;  // of a transposing read
+  const int trow = 4 * fg + (fr >> 2), tkey = row_key<DK>(trow), piece = fr & 3;  // of a transposing read
   uint32_t vt_at[VT];
 #pragma unroll
   for (int vt = 0; vt < VT; ++vt) vt_at[vt] = sv + trow * PITCH + (((v0 / 8 + 2 * vt + (piece >> 1)) ^ tkey) << 4) + 8 * (piece & 1);
@@ -208,7 +188,7 @@ __global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) 
     stage(rk, 0);
     if constexpr (OUT) stage(rq, 2);
     else stage(rv, 1);
-    dc_barrier();
+    lds_barrier();
     if (more) request(kp, a.k_n, k2, next, rk);
     __builtin_amdgcn_sched_barrier(0);
     if (count < DC) counted(count);
@@ -241,9 +221,7 @@ __global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) 
         ahead *= in_front ? step16 : 1.f;
       }
       if constexpr (F) {
-        most = fmaxf(most, __shfl_xor(most, 16));
-        most = fmaxf(most, __shfl_xor(most, 32));
-        f = dc_fit(most);
+        f = dc_fit(max_groups(most));
         if (fg == 0) fit[16 * wave + fr] = f;
       }
 #pragma unroll
@@ -268,9 +246,7 @@ __global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) 
           for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
             for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(st[vt][kt][r]));
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) most = fmaxf(most, __shfl_xor(most, m));
-        sfit = dc_fit(most);
+        sfit = dc_fit(max_wave(most));
       }
 #pragma unroll
       for (int vt = 0; vt < VT; ++vt)
@@ -301,7 +277,7 @@ __global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) 
       }
       stage(rv, 1);
       if (more) request(qp, a.q_n, q2, next, rq);
-      dc_barrier();
+      lds_barrier();
       if (more) request(vp, a.v_n, v2, next, rv);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -416,7 +392,7 @@ __global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) 
         }
       }
     }
-    dc_barrier();
+    lds_barrier();
   }
   // ---- the state behind the last token, or the segment's sum
   if (MODE != DC_OUT && qt0 == 0) {

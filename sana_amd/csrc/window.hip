@@ -8,9 +8,8 @@
 // What a stream keeps of its past is a cache of sinks + window rows: row p for a position p below the sinks, then a ring.
 // The order of the keys does not matter to the sum, so a token's attention reads the rows as they lie.
 #include <initializer_list>
-#include <type_traits>
 
-#include "common.h"
+#include "stream_common.h"
 
 namespace sana {
 namespace {
@@ -28,33 +27,7 @@ struct WindowArgs {
   float scale_log2e;
 };
 
-// 16-byte slots of an LDS row of DK * 64 bytes are exchanged by a key of the row: 16 consecutive rows of one slot, and the 16 rows of a
-// transposing read, cover all banks.  The key of row 16 i + r is that of r.
-template <int DK>
-__device__ __forceinline__ int wa_key(int row) {
-  return DK == 4 ? (row & 15) : DK == 2 ? ((row >> 1) & 7) : ((row >> 2) & 3);
-}
-typedef __attribute__((address_space(3))) unsigned char wa_lds;  // (pointers, not integers: the compiler sees which array is read)
-__device__ __forceinline__ u32x2_t wa_read_tr(wa_lds* at) {  // 4 keys x 16 channels -> this lane's channel, 4 keys
-  typedef short s16x4_t __attribute__((ext_vector_type(4)));
-  return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)at));
-}
-__device__ __forceinline__ u32x4_t wa_read(const wa_lds* at) { return *(__attribute__((address_space(3))) const u32x4_t*)at; }
-// What this wave wrote to LDS is there and what it reads from there has come; loads from memory stay in flight.
-__device__ __forceinline__ void wa_barrier() {
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-}
 template <typename T> inline constexpr float kShift = is_f16<T> ? 6.f : 0.f;
-__device__ __forceinline__ float wa_max_groups(float x) {  // over the four lane groups that share a query
-  x = fmaxf(x, __shfl_xor(x, 16));
-  return fmaxf(x, __shfl_xor(x, 32));
-}
-__device__ __forceinline__ float wa_sum_groups(float x) {
-  x += __shfl_xor(x, 16);
-  return x + __shfl_xor(x, 32);
-}
 
 // A prompt or a chunk: the queries are the last N of Nk keys.  A workgroup takes NW * 16 * QT queries of one head through its
 // tiles of 64 keys, the tiles of the sinks first; K and V go to LDS by direct loads, V a tile behind K, one barrier a tile.  scores^T = K Q^T: a
@@ -113,17 +86,17 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DK < 4 ? 3 : 2) void window_att
         __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(rows + (int64_t)j0 * stride), 0, (int)((uint32_t)(count - 1) * ld2 + 2 * d), 0x00020000);
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int at = 64 * (NW * i + wave) + lane, row = at / (4 * DK), c = (at - row * (4 * DK)) ^ wa_key<DK>(row);
+      const int at = 64 * (NW * i + wave) + lane, row = at / (4 * DK), c = (at - row * (4 * DK)) ^ row_key<DK>(row);
       const uint32_t off = 8 * c < d ? (uint32_t)row * ld2 + 16 * c : 0x80000000u;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (wa_lds*)(to + 1024 * (NW * i + wave)), 16, (int)off, 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_t*)(to + 1024 * (NW * i + wave)), 16, (int)off, 0, 0, 0);
     }
   };
   auto landed = [&]() {  // this wave's loads have, and everyone's behind the barrier
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0), as a builtin: the compiler counts on it and waits for no tile a second time
-    wa_barrier();
+    lds_barrier();
   };
 
-  const int key = wa_key<DK>(fr), trow = 4 * fg + (fr >> 2), tkey = wa_key<DK>(trow), piece = fr & 3;
+  const int key = row_key<DK>(fr), trow = 4 * fg + (fr >> 2), tkey = row_key<DK>(trow), piece = fr & 3;
   uint32_t k_at[DK];
 #pragma unroll
   for (int s = 0; s < DK; ++s) k_at[s] = fr * PITCH + (((4 * s + fg) ^ key) << 4);
@@ -151,7 +124,7 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DK < 4 ? 3 : 2) void window_att
 #pragma unroll
     for (int j = 0; j < KP; ++j)
 #pragma unroll
-      for (int s = 0; s < DK; ++s) kf[j][s] = wa_read((const wa_lds*)from + 16 * (k0 + j) * PITCH + k_at[s]);
+      for (int s = 0; s < DK; ++s) kf[j][s] = lds_read((const lds_t*)from + 16 * (k0 + j) * PITCH + k_at[s]);
 #pragma unroll
     for (int j = 0; j < KP; ++j)
 #pragma unroll
@@ -194,7 +167,7 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DK < 4 ? 3 : 2) void window_att
     if (__any(above)) {
 #pragma unroll
       for (int q = 0; q < QT; ++q) {
-        const float now = fmaxf(mx[q], wa_max_groups(most[q]));
+        const float now = fmaxf(mx[q], max_groups(most[q]));
         const float f = __builtin_amdgcn_exp2f(mx[q] - (now == -INFINITY ? 0.f : now));  // (nothing yet: 0)
         mx[q] = now, sub[q] = now == -INFINITY ? 0.f : now - kShift<T>;
         sum[q] *= f;
@@ -217,8 +190,8 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DK < 4 ? 3 : 2) void window_att
   auto values = [&](unsigned char* from, int s, const u32x2_t (&pk)[QT][4]) {
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
-      wa_lds* at = (wa_lds*)from + v_at(dt) + 32 * s * PITCH;
-      const u32x2_t x = wa_read_tr(at), y = wa_read_tr(at + 16 * PITCH);
+      lds_t* at = (lds_t*)from + v_at(dt) + 32 * s * PITCH;
+      const u32x2_t x = lds_read_tr(at), y = lds_read_tr(at + 16 * PITCH);
       const u32x4_t vf = {x.x, x.y, y.x, y.y};
 #pragma unroll
       for (int q = 0; q < QT; ++q)
@@ -273,7 +246,7 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DK < 4 ? 3 : 2) void window_att
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
     const int qi = w0 + 16 * t + fr;
-    const float l = wa_sum_groups(sum[t]);
+    const float l = sum_groups(sum[t]);
     if (qi >= queries) continue;
     if (a.splits == 1) {
       const float inv = 1.0f / l;
@@ -395,7 +368,7 @@ __global__ __launch_bounds__(64 * NW) void window_step_kernel(const WindowArgs a
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) oc[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   float mx = -INFINITY, sub = 0.f, sum = 0.f;
-  const int trow = 4 * fg + (fr >> 2), tkey = wa_key<DK>(trow), piece = fr & 3;
+  const int trow = 4 * fg + (fr >> 2), tkey = row_key<DK>(trow), piece = fr & 3;
   if (t0 + wave < t1) request(t0 + wave);
 #pragma unroll 1
   for (int t = t0 + wave; t < t1; t += NW) {
@@ -411,7 +384,7 @@ __global__ __launch_bounds__(64 * NW) void window_step_kernel(const WindowArgs a
 #pragma unroll
     for (int i = 0; i < PV; ++i) {
       const int idx = lane + 64 * i, r = idx / (DK * 4), c = idx - r * (DK * 4);
-      *reinterpret_cast<u32x4_t*>(mine + r * PITCH + ((c ^ wa_key<DK>(r)) << 4)) = rv[i];
+      *reinterpret_cast<u32x4_t*>(mine + r * PITCH + ((c ^ row_key<DK>(r)) << 4)) = rv[i];
     }
     if (t + NW < t1) request(t + NW);
     float most = -INFINITY;
@@ -423,7 +396,7 @@ __global__ __launch_bounds__(64 * NW) void window_step_kernel(const WindowArgs a
         most = fmaxf(most, sc[kt][r]);
       }
     if (__any(most > mx + 8.f)) {
-      const float now = fmaxf(mx, wa_max_groups(most));
+      const float now = fmaxf(mx, max_groups(most));
       const float f = __builtin_amdgcn_exp2f(mx - (now == -INFINITY ? 0.f : now));
       mx = now, sub = now == -INFINITY ? 0.f : now - kShift<T>;
       sum *= f;
@@ -446,21 +419,21 @@ __global__ __launch_bounds__(64 * NW) void window_step_kernel(const WindowArgs a
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the wave's own V is there)
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
-      wa_lds* from = (wa_lds*)mine + trow * PITCH + (((2 * dt + (piece >> 1)) ^ tkey) << 4) + 8 * (piece & 1);
-      const u32x2_t x = wa_read_tr(from), y = wa_read_tr(from + 16 * PITCH);
+      lds_t* from = (lds_t*)mine + trow * PITCH + (((2 * dt + (piece >> 1)) ^ tkey) << 4) + 8 * (piece & 1);
+      const u32x2_t x = lds_read_tr(from), y = lds_read_tr(from + 16 * PITCH);
       oc[dt] = mfma_16x16x32<T>(u32x4_t{x.x, x.y, y.x, y.y}, pf, oc[dt]);
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
   // ---- the waves' parts, through LDS: [channel][head], then the maxima and sums
-  sum = wa_sum_groups(sum);
+  sum = sum_groups(sum);
   float* po = reinterpret_cast<float*>(mine);
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int r = 0; r < 4; ++r) po[(16 * dt + 4 * fg + r) * 16 + fr] = oc[dt][r];
   if (fg == 0) po[16 * 16 * DT + fr] = mx, po[16 * 16 * DT + 16 + fr] = sum;
-  wa_barrier();
+  lds_barrier();
   auto part = [&](int w) { return reinterpret_cast<const float*>(smem + w * OWN); };
   const int col = tid & 15, g = 16 * gb + col;
   float m = -INFINITY;
