@@ -60,6 +60,8 @@ enum { DC_SUMS, DC_OUT, DC_WHOLE };
 // 16-bit values: three of bf16 where the state is given back (fp32's accuracy; with two it is 1.3e-6 off after 32760
 // tokens), two of bf16 where it only goes on to outputs, two of f16 (22 bits), the second times 2^11, so that it stays a normal number.
 // f16 ends at 65504: S goes in scaled by a power of two for each wave, P for each query.
+// A value that is not finite must not reach the queries in front of it (0 * inf): it is staged as 0, and its channel is set to NaN from its
+// token on.
 template <typename T, int DK, int KT, int VT, int NV, int MODE>
 __global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) {
   constexpr bool OUT = MODE != DC_SUMS, F = is_f16<T>;
@@ -67,10 +69,11 @@ __global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) 
   constexpr int NT = 256, PIECES = DC * DK * 4 / NT, TERMS = F || MODE == DC_OUT ? 2 : 3;
   constexpr int NQ = 4 / NV, QN = 4 / NQ;  // shares of the queries, query tiles of a share
   static_assert(KT <= 2 * DK && DC * DK * 4 % NT == 0 && 4 % NV == 0, "");
-  __shared__ __attribute__((aligned(16))) unsigned char smem[(OUT ? 3 : 2) * TILE + (OUT ? DC * 128 + DC * 4 : 0)];
+  __shared__ __attribute__((aligned(16))) unsigned char smem[(OUT ? 3 : 2) * TILE + (OUT ? DC * 128 + DC * 4 + DK * 128 + 16 : 0)];
   const uint32_t sk = (uint32_t)(size_t)(lds_t*)smem;
   const uint32_t sv = sk + TILE, sq = sk + 2 * TILE, sp = sk + 3 * TILE;
   float* fit = reinterpret_cast<float*>(smem + 3 * TILE + DC * 128);  // f16: the scale of a query's P
+  int* odd = reinterpret_cast<int*>(fit + DC);  // each channel's first row that is not finite; behind them: the last chunk that holds one
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), fr = tid & 15, fg = (tid >> 4) & 3;
   const int v0 = 16 * VT * (wave % NV), qt0 = QN * (wave / NV);
 
@@ -156,6 +159,25 @@ __global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) 
       *reinterpret_cast<u32x4_t*>(smem + tile * TILE + row * PITCH + ((c ^ row_key<DK>(row)) << 4)) = r[i];
     }
   };
+  auto clean = [&](const u32x4_t* r, int chunk) {  // V as it is staged
+    u16x2_t most = {0, 0};
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) most = max_magnitude(most, r[i]);
+    if (__builtin_expect(most.x >= kInf16<T> || most.y >= kInf16<T>, 0)) {
+      int me = tid;
+      asm volatile("" : "+v"(me));  // (here and where `odd` is read: no address of this is worked out ahead and kept)
+#pragma unroll 1
+      for (int at = 0; at < 8 * PIECES; ++at) {  // this thread's own pieces, in LDS
+        const int idx = me + NT * (at >> 3), row = idx / (DK * 4), c = idx - row * (DK * 4);
+        uint16_t* x = reinterpret_cast<uint16_t*>(smem + TILE + row * PITCH + ((c ^ row_key<DK>(row)) << 4)) + (at & 7);
+        if ((*x & 0x7fffu) < kInf16<T>) continue;
+        *x = 0;
+        __hip_atomic_fetch_min(odd + 8 * c + (at & 7), row, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+      }
+      odd[32 * DK] = chunk;
+    }
+  };
+  if (OUT && tid <= 32 * DK) odd[tid] = tid < 32 * DK ? DC : -1;
   const uint16_t *kp = a.k + b * a.k_b + h * d, *vp = a.v + b * a.v_b + h * d, *qp = a.q + b * a.q_b + h * d;
   // bf16 sums are weighted up to the segment's end at once: they need no decay from chunk to chunk (f16 would run out of range) and no
   // order, and go backwards, so that the rows with which the outputs begin are the ones that the memory-side cache has seen last.
@@ -194,6 +216,7 @@ __global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) 
     if (count < DC) counted(count);
     f32x4_t oc[VT][QN];  // out^T: channel v0 + 16 vt + 4 fg + r, query 16 (qt0 + q) + fr
     u32x4_t vf[2][VT];   // values of two ranges of 32 tokens
+    bool some_odd = false;
     if constexpr (OUT) {
       // ---- scores, decayed, to LDS: row = query, 16-byte slot 4 s + g = keys 32 s + 4 g + {0..3}, + 16
       f32x4_t sc[4];
@@ -276,8 +299,10 @@ __global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) 
         }
       }
       stage(rv, 1);
+      clean(rv, i);
       if (more) request(qp, a.q_n, q2, next, rq);
       lds_barrier();
+      some_odd = __builtin_amdgcn_readfirstlane(odd[32 * DK]) == i;
       if (more) request(vp, a.v_n, v2, next, rv);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -312,6 +337,19 @@ __global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) 
 #pragma unroll
           for (int vt = 0; vt < VT; ++vt) oc[vt][q] = mfma_16x16x32<T>(vf[s][vt], pf, oc[vt][q]);
         }
+      if (__builtin_expect(some_odd && own, 0)) {
+        int at = tid;
+        asm volatile("" : "+v"(at));
+        const int first_row = 16 * qt0 + (at & 15), c = v0 + 4 * ((at >> 4) & 3);
+#pragma unroll
+        for (int vt = 0; vt < VT; ++vt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int from = odd[c + 16 * vt + r] - first_row;
+#pragma unroll
+            for (int q = 0; q < QN; ++q) oc[vt][q][r] = 16 * q >= from ? NAN : oc[vt][q][r];
+          }
+      }
       // (rows below 0 and channels past d lie outside the resource: not stored)
       const uint32_t o2 = 2 * (uint32_t)a.o_n;
       const __amdgpu_buffer_rsrc_t ro =
@@ -389,6 +427,20 @@ __global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) 
                 for (int r = 0; r < 4; ++r)
                   if (k0 + j < KT) st[vt][k0 + j][r] = fmaf(y[j][vt][r], 1.0f / 2048.f, st[vt][k0 + j][r]);
           }
+        }
+      }
+    }
+    if constexpr (OUT) {
+      if (__builtin_expect(some_odd && own, 0)) {
+        int at = tid;
+        asm volatile("" : "+v"(at));
+#pragma unroll
+        for (int vt = 0; vt < VT; ++vt) {
+          const float x = odd[v0 + 16 * vt + (at & 15)] < DC ? NAN : 0.f;
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) st[vt][kt][r] += x;
         }
       }
     }
@@ -491,7 +543,7 @@ int segment_count(int B, int N, int H, int* tokens) {
 template <typename T, int DK, int KT, int VT, int NV>
 int launch_chunks(const DecayArgs& a, int B, hipStream_t s) {
   const int64_t units = (int64_t)B * a.nseg * ((a.H + 3) / 4);
-  if (units > (1 << 28)) return SANA_ERR_SHAPE;
+  if (units > (1 << 22) - 8) return SANA_ERR_SHAPE;  // 4 blocks of 256 threads a unit: fewer than 2^32 threads
   DecayArgs args = a;
   args.units = (int)units;
   const dim3 grid((unsigned)((units + 7) / 8 * 32)), block(256);
@@ -532,7 +584,7 @@ using namespace sana;
 #define SANA_API extern "C" __attribute__((visibility("default")))
 
 SANA_API size_t sana_hip_decay_attention_workspace_bytes(int B, int N, int H, int d) {
-  if (B <= 0 || N <= 1 || H <= 0 || d <= 0 || d > 128 || (int64_t)B * H > (1 << 24)) return 0;
+  if (B <= 0 || N <= 1 || H <= 0 || d <= 0 || d > 128 || (int64_t)B * H >= (1 << 24)) return 0;
   int tokens;
   const int nseg = segment_count(B, N, H, &tokens);
   return nseg > 1 ? (size_t)B * H * nseg * d * d * sizeof(float) : 0;
@@ -545,7 +597,7 @@ SANA_API int sana_hip_decay_attention(const void* q, const void* k, const void* 
                                       int64_t o_stride_n, float scale, int io_dtype, void* stream) {
   if (!q || !k || !v || !log_decay || !state_out || !out || B <= 0 || N <= 0 || H <= 0 || d <= 0) return SANA_ERR_ARG;
   if (io_dtype != SANA_DT_BF16 && io_dtype != SANA_DT_F16) return SANA_ERR_DTYPE;
-  if (d % 8 || d > 128 || (int64_t)B * H > (1 << 24) || N > (1 << 30)) return SANA_ERR_SHAPE;
+  if (d % 8 || d > 128 || (int64_t)B * H >= (1 << 24) || N > (1 << 30)) return SANA_ERR_SHAPE;
   for (const int64_t ld : {q_stride_n, k_stride_n, v_stride_n, o_stride_n}) {
     if (ld < (int64_t)H * d) return SANA_ERR_ARG;
     if (ld >= (1 << 23)) return SANA_ERR_SHAPE;  // 32-bit byte offsets within a chunk

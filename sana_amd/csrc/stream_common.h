@@ -53,4 +53,15 @@ __device__ __forceinline__ float max_wave(float x) {  // over all 64 lanes: rota
   return max_groups(x);
 }
 
+// Values that are not finite.  What a query does not see has a probability of 0, but 0 * inf is NaN: through a product of a tile, one
+// such value would reach all of the tile's queries.
+template <typename T> inline constexpr uint32_t kInf16 = is_f16<T> ? 0x7c00u : 0x7f80u;
+template <typename T> inline constexpr uint32_t kOne16 = is_f16<T> ? 0x3c00u : 0x3f80u;
+typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ u16x2_t max_magnitude(u16x2_t most, u32x4_t x) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, x[e] & 0x7fff7fffu));
+  return most;
+}
+
 }  // namespace sana

@@ -242,6 +242,70 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DK < 4 ? 3 : 2) void window_att
       if (t + 1 < t1) step(t + 1, odd, even, k_odd, k_even, v_odd, v_even);
     }
   }
+  // ---- Values that are not finite: the products with V once more, so that they reach the queries that see them and no others.  32 keys at a
+  // time straight from memory, the finite values; the others counted, and their signs summed, over the keys that are seen.
+  bool odd = false;
+#pragma unroll
+  for (int q = 0; q < QT; ++q)
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) odd |= !(fabsf(oc[q][dt][r]) < INFINITY);
+  if (__builtin_expect(__any(odd), 0)) {
+#pragma unroll
+    for (int q = 0; q < QT; ++q)
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) oc[q][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int half = 2 * t0; half < 2 * t1; ++half) {
+      const int j0 = tile_of(half >> 1) * WK + 32 * (half & 1);
+      u32x4_t p[QT], seen[QT];
+#pragma unroll
+      for (int q = 0; q < QT; ++q) p[q] = seen[q] = u32x4_t{0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        f32x4_t sc[QT];
+#pragma unroll
+        for (int q = 0; q < QT; ++q) sc[q] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < DK; ++s) {
+          const int c = 32 * s + 8 * fg;
+          u32x4_t kf = *reinterpret_cast<const u32x4_t*>(kp + (int64_t)min(j0 + 16 * kt + fr, keys - 1) * a.k_n + (c < d ? c : 0));
+          if (c >= d) kf = u32x4_t{0u, 0u, 0u, 0u};
+#pragma unroll
+          for (int q = 0; q < QT; ++q) sc[q] = mfma_16x16x32<T>(kf, qf[q][s], sc[q]);
+        }
+#pragma unroll
+        for (int q = 0; q < QT; ++q)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int j = j0 + 16 * kt + 4 * fg + r, i = past + w0 + 16 * q + fr;
+            if (j > i || (i - j >= a.window && j >= a.sinks)) continue;
+            const float x = __builtin_amdgcn_exp2f(fmaf(sc[q][r], a.scale_log2e, -sub[q]));
+            p[q][2 * kt + (r >> 1)] |= (pk16<T>(x, 0.f) & 0xffffu) << (16 * (r & 1)), seen[q][2 * kt + (r >> 1)] |= kOne16<T> << (16 * (r & 1));
+          }
+      }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        u32x4_t finite = {0u, 0u, 0u, 0u}, other = finite, sign = finite;
+        const int c = 16 * dt + fr;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int j = j0 + 16 * (e >> 2) + 4 * fg + (e & 3), at = 16 * (e & 1);
+          const uint32_t x = c < d && j < keys ? vp[(int64_t)j * a.v_n + c] : 0u, m = x & 0x7fffu;
+          finite[e >> 1] |= (m < kInf16<T> ? x : 0u) << at, other[e >> 1] |= (m < kInf16<T> ? 0u : kOne16<T>) << at;
+          sign[e >> 1] |= (m == kInf16<T> ? kOne16<T> | (x & 0x8000u) : 0u) << at;
+        }
+#pragma unroll
+        for (int q = 0; q < QT; ++q) {
+          oc[q][dt] = mfma_16x16x32<T>(finite, p[q], oc[q][dt]);
+          const f32x4_t zero = {0.f, 0.f, 0.f, 0.f}, n = mfma_16x16x32<T>(other, seen[q], zero), to = mfma_16x16x32<T>(sign, seen[q], zero);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) oc[q][dt][r] += n[r] == 0.f ? 0.f : to[r] == n[r] ? INFINITY : to[r] == -n[r] ? -INFINITY : NAN;
+        }
+      }
+    }
+  }
   // ---- out, or this part's
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
@@ -294,10 +358,10 @@ __global__ __launch_bounds__(256) void window_join_kernel(const WindowArgs a) {
     for (int s = 0; s < 8; ++s) x[s] = *reinterpret_cast<const f32x4_t*>(from + min(s0 + s, a.splits - 1) * rows * a.d);
 #pragma unroll
     for (int s = 0; s < 8; ++s) {
-      const float f = __shfl(mine, s0 + s, 32);  // (0 behind the last part)
+      const float f = __shfl(mine, s0 + s, 32);  // (0 behind the last part, whose values are repeated there: they may be inf)
       l = fmaf(f, __shfl(ml[1], s0 + s, 32), l);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) o[r] = fmaf(f, x[s][r], o[r]);
+      for (int r = 0; r < 4; ++r) o[r] = fmaf(f, f == 0.f ? 0.f : x[s][r], o[r]);
     }
   }
   const float inv = 1.0f / l;
@@ -384,7 +448,7 @@ __global__ __launch_bounds__(64 * NW) void window_step_kernel(const WindowArgs a
 #pragma unroll
     for (int i = 0; i < PV; ++i) {
       const int idx = lane + 64 * i, r = idx / (DK * 4), c = idx - r * (DK * 4);
-      *reinterpret_cast<u32x4_t*>(mine + r * PITCH + ((c ^ row_key<DK>(r)) << 4)) = rv[i];
+      *reinterpret_cast<u32x4_t*>(mine + r * PITCH + ((c ^ row_key<DK>(r)) << 4)) = 32 * t + r < count ? rv[i] : u32x4_t{0u, 0u, 0u, 0u};
     }
     if (t + NW < t1) request(t + NW);
     float most = -INFINITY;
@@ -477,6 +541,7 @@ __global__ __launch_bounds__(256) void window_append_kernel(const WindowArgs a) 
 }
 
 constexpr int WA_NW = 4;
+constexpr int64_t WA_MAX_BLOCKS = 1 << 24;  // of 256 threads: a launch has fewer than 2^32 threads an axis
 // 16-query tiles of a wave, 64 or 128 queries a workgroup.  Two feed twice the MFMAs with a read of K or V and pay where heads are wide
 // and the blocks many; one gives more and shorter workgroups, and up to 96 channels three and more waves a SIMD.  us, two / one, window 4096:
 // 20 heads of 112 1500 tokens 39 / 32, 2000 63 / 49, 3000 77 / 93, 8000 304 / 357; 16 of 128 3000 82 / 62, 4680 139 / 129, 8000 253 / 272;
@@ -514,7 +579,7 @@ size_t part_bytes(int splits, int64_t rows, int d) { return splits > 1 ? (size_t
 template <typename T>
 int launch_join(const WindowArgs& a, hipStream_t s) {
   const int64_t groups = ((int64_t)a.B * a.N * a.H + 7) / 8;
-  if (groups > 0x7fffffff) return SANA_ERR_SHAPE;
+  if (groups >= WA_MAX_BLOCKS) return SANA_ERR_SHAPE;
   hipLaunchKernelGGL(window_join_kernel<T>, dim3((unsigned)groups), dim3(256), 0, s, a);
   return SANA_OK;
 }
@@ -525,7 +590,7 @@ int launch_prompt(WindowArgs a, hipStream_t s) {
   const int qb = WA_NW * 16 * (one ? 1 : 2);
   a.qblocks = (a.N + qb - 1) / qb;
   const int64_t items = (int64_t)a.B * a.H * a.qblocks * a.splits;
-  if (items > 0x7ffffff0) return SANA_ERR_SHAPE;
+  if (items > WA_MAX_BLOCKS - 8) return SANA_ERR_SHAPE;
   a.items = (int)items;
   const dim3 grid((unsigned)((items + 7) / 8 * 8)), block(64 * WA_NW);
   if (one) hipLaunchKernelGGL((window_attn_kernel<T, DK, DT, 1, WA_NW>), grid, block, 0, s, a);
@@ -540,7 +605,7 @@ int launch_prompt(WindowArgs a, hipStream_t s) {
 template <typename T, int DK, int DT>
 int launch_step(const WindowArgs& a, hipStream_t s) {
   const int64_t groups = step_groups(a.B, a.H, a.Hkv);
-  if (groups > 0x7fffffff) return SANA_ERR_SHAPE;
+  if (groups >= WA_MAX_BLOCKS) return SANA_ERR_SHAPE;
   if (step_in_one(groups, a.window + a.sinks))
     hipLaunchKernelGGL((window_step_kernel<T, DK, DT, 8>), dim3((unsigned)groups), dim3(512), 0, s, a);
   else
@@ -599,7 +664,7 @@ SANA_API int sana_hip_window_attention(const void* q, const void* k, const void*
                                        int64_t q_stride_b, int64_t q_stride_n, int64_t k_stride_b, int64_t k_stride_n,
                                        int64_t v_stride_b, int64_t v_stride_n, int64_t o_stride_b, int64_t o_stride_n, float scale,
                                        int io_dtype, void* stream) {
-  if (!q || !k || !v || !out || Nk < N || !(scale > 0.f && scale < INFINITY)) return SANA_ERR_ARG;
+  if (!q || !k || !v || !out || Nk < N || !(scale > 0.f && scale * 1.44269504088896341f < INFINITY)) return SANA_ERR_ARG;
   const int rc = check_sizes(B, N, H, Hkv, d, window, sinks, io_dtype);
   if (rc != SANA_OK) return rc;
   if (Nk > (1 << 30)) return SANA_ERR_SHAPE;
@@ -644,7 +709,7 @@ SANA_API int sana_hip_window_cache_append(void* cache_k, void* cache_v, const vo
     if (sb < 0) return SANA_ERR_ARG;
   if (B > 1 && (ck_stride_b == 0 || cv_stride_b == 0)) return SANA_ERR_ARG;  // (streams that would write the same rows)
   if ((int64_t)window + sinks > (1 << 30)) return SANA_ERR_SHAPE;
-  if (C % 8 || groups > 0x7fffffff || B > 65535) return SANA_ERR_SHAPE;
+  if (C % 8 || groups >= WA_MAX_BLOCKS || B > 65535) return SANA_ERR_SHAPE;
   if (misaligned({cache_k, cache_v, k, v}, {ck_stride_b, ck_stride_n, cv_stride_b, cv_stride_n, k_stride_b, k_stride_n, v_stride_b, v_stride_n}) ||
       off4(positions) || off4(lengths))
     return SANA_ERR_ALIGN;
@@ -668,7 +733,7 @@ SANA_API int sana_hip_window_step(const void* q, const void* k, const void* v, v
                                   int sinks, int64_t q_stride_b, int64_t k_stride_b, int64_t v_stride_b, int64_t ck_stride_b,
                                   int64_t ck_stride_n, int64_t cv_stride_b, int64_t cv_stride_n, int64_t o_stride_b, float scale,
                                   int io_dtype, void* stream) {
-  if (!q || !k || !v || !cache_k || !cache_v || !positions || !out || !(scale > 0.f && scale < INFINITY)) return SANA_ERR_ARG;
+  if (!q || !k || !v || !cache_k || !cache_v || !positions || !out || !(scale > 0.f && scale * 1.44269504088896341f < INFINITY)) return SANA_ERR_ARG;
   const int rc = check_sizes(B, 1, H, Hkv, d, window, sinks, io_dtype);
   if (rc != SANA_OK) return rc;
   const int64_t C = (int64_t)Hkv * d;

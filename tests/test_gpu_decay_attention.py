@@ -169,6 +169,29 @@ def test_half_precision_where_states_and_scores_leave_its_range(cuda, N):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("N,H,d", [(1, 3, 32), (100, 3, 32), (150, 3, 112), (90, 3, 96), (1300, 2, 64), (1500, 2, 112)])
+def test_what_is_not_finite_reaches_nothing_in_front_of_it(cuda, N, H, d, dtype):
+    """Values of inf and NaN: the outputs in front of them, the other channels' and the other heads' are what they are without; from the
+    token on their channel is not finite, nor are its rows of the state.  A key of NaN: the same for all channels of its head."""
+    q, k, v, log_decay, state = make(2, N, H, d, dtype, seed=N, carried=True, packed=False)
+    clean_k, clean_v = k.clone(), v.clone()
+    odd, odd_state = torch.zeros(2, N, H, d, dtype=torch.bool), torch.zeros(2, H, d, d, dtype=torch.bool)
+    for b, j, h, c, x in [(0, N // 2, 0, 3, float("inf")), (0, N // 2, 1, 7, -float("inf")), (1, N // 3, 1, 7, float("nan")), (1, N - 1, 0, 1, float("inf"))]:
+        v[b, j, h * d + c], clean_v[b, j, h * d + c] = x, 0
+        odd[b, j:, h, c], odd_state[b, h, c] = True, True
+    for b, j, h, c in [(1, 2 * N // 3, H - 1, 2)]:
+        k[b, j, h * d + c], clean_k[b, j, h * d + c] = float("nan"), 0
+        odd[b, j:, h], odd_state[b, h, :, c] = True, True
+    want = definition(q, clean_k, clean_v, log_decay, 0.3, state, None)
+    got, last = ops.decay_linear_attention(q.cuda(), k.cuda(), v.cuda(), log_decay.cuda(), 0.3, state.cuda())
+    odd = odd.reshape(2, N, H * d)
+    got, last = got.double().cpu(), last.double().cpu()
+    assert not torch.isfinite(got[odd]).any() and not torch.isfinite(last[odd_state]).any()
+    check((torch.where(odd, want[0], got), torch.where(odd_state, want[1], last)), want, q, N)
+
+
+@gpu
 def test_views_of_every_kind(cuda):
     """Rows further apart than their channels, batches in front of tokens, a stream cut out of a longer one, an out of other strides."""
     B, N, H, d = 2, 150, 3, 40
@@ -290,6 +313,13 @@ def test_c_entry_refuses_before_any_launch():
     assert lib.sana_hip_decay_attention_workspace_bytes(1, 1, 3, 32) == 0
     assert lib.sana_hip_decay_attention_workspace_bytes(0, 8, 3, 32) == 0
     assert lib.sana_hip_decay_attention_workspace_bytes(64, 32760, 64, 32) == 0
+
+
+def test_c_entry_refuses_launches_of_too_many_threads():
+    """Host checks of sizes whose grids no launch takes (2^32 threads)."""
+    lib, P = _lib.load(), 0x10000
+    call = lambda B, N, H: lib.sana_hip_decay_attention(P, P, P, P, None, P, P, None, None, 0, B, N, H, 32, *[8 * 96, 96] * 4, 1.0, _lib.DT_BF16, None)  # noqa: E731
+    assert call(1 << 22, 8, 3) == -2 and call(1 << 24, 1, 1) == -2
 
 
 def test_cpu_tensors_are_refused():

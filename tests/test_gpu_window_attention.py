@@ -116,6 +116,40 @@ def test_scores_of_every_size(cuda, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("N,past,window,sinks,d", [(300, 0, 70, 5, 112), (300, 20, 400, 0, 64), (5, 3333, 3000, 2, 112), (2500, 0, 100, 3, 128), (90, 7, 64, 0, 8)])
+def test_values_that_are_not_finite_reach_who_sees_them(cuda, N, past, window, sinks, d, dtype):
+    """A value of inf or NaN in front of a query's window, or behind the query: its output is what it is without; a query that sees it has
+    the definition's inf or NaN in that channel.  A key of NaN makes the outputs of its head NaN for who sees it."""
+    H, G, Nk = 20 if N > 1000 else 4, 2, N + past
+    q, k, v = make(1, N, Nk, H, G, d, dtype, seed=N, packed=False)
+    bad = [(1, 0, 3, math.inf), (Nk - N // 2, 0, 5, -math.inf), (Nk - N // 2 - 1, 1, 3, math.nan), (Nk - N // 2, 0, 6, math.inf),
+           (Nk - N // 2 + 1, 0, 6, -math.inf), (Nk - 1, 1, 7, math.inf), (Nk - 2, 0, 3, math.inf)]
+    i = torch.arange(Nk - N, Nk)
+    sees = lambda j: (j <= i) & ((i - j < window) | (j < sinks))  # noqa: E731
+    extra = torch.zeros(1, N, H, d, dtype=torch.float64)
+    clean = v.clone()
+    for j, g, c, x in bad:
+        v[0, j, g * d + c], clean[0, j, g * d + c] = x, 0
+        extra[0, sees(j), g * H // G:(g + 1) * H // G, c] += x
+    want = definition(q, k, clean, H, window, sinks, d ** -0.5)
+    extra = extra.reshape(1, N, H * d)
+
+    def hold(got, extra):
+        got = got.double().cpu()
+        odd = extra != 0
+        assert torch.equal(torch.nan_to_num(got[odd], nan=7.0, posinf=8.0, neginf=9.0), torch.nan_to_num(extra[odd], nan=7.0, posinf=8.0, neginf=9.0))
+        check(torch.where(odd, want[0], got), want, Nk, dtype)
+
+    hold(ops.window_attention(q.cuda(), k.cuda(), v.cuda(), H, window, sinks), extra)
+    j = Nk - N // 2 - 1
+    k[0, j, 2] = math.nan
+    extra = extra.reshape(1, N, H, d)
+    extra[0, sees(j), :H // G] = math.nan
+    hold(ops.window_attention(q.cuda(), k.cuda(), v.cuda(), H, window, sinks), extra.reshape(1, N, H * d))
+
+
+@gpu
 @pytest.mark.parametrize("past", [0, 40, 2500])
 def test_lengths_leave_rows_alone(cuda, past):
     N, H = 130, 2
@@ -264,6 +298,24 @@ def test_step_scores_of_thousands(cuda):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("rows", [5, 33, 700, 4000])
+def test_step_values_that_are_not_finite(cuda, rows, dtype):
+    """The newest token's value of inf, a row that the last tile of rows holds alone or with others that are not there yet: inf, not NaN."""
+    g = torch.Generator().manual_seed(rows)
+    q, k, v = (torch.randn(1, 1, 128, generator=g).to(dtype) for _ in range(3))
+    ck, cv = torch.randn(2, 1, rows + 90, 128, generator=g).to(dtype).unbind(0)
+    v[0, 0, 3], v[0, 0, 70] = math.inf, -math.inf
+    want_k, want_v, want = step_definition(q, k, v, ck, cv, [rows - 1], 2, 4, 0.125)
+    got = ops.window_attention_step_(q.cuda(), k.cuda(), v.cuda(), ck.cuda(), cv.cuda(), torch.tensor([rows - 1], dtype=torch.int32, device="cuda"), 2, 4)
+    assert got[0, 0, 3] == math.inf and got[0, 0, 70] == -math.inf
+    fine = torch.isfinite(want[0])
+    assert fine.sum() == 126
+    zero = torch.zeros(1, dtype=torch.float64)
+    check(torch.where(fine, got.double().cpu(), zero), (torch.where(fine, want[0], zero), torch.where(fine, want[1], zero), want[2]), rows, dtype)
+
+
+@gpu
 def test_a_cache_of_more_than_32_bits_of_bytes(cuda):
     """Streams whose rows lie further into a cache than 2^31 elements and 2^32 bytes."""
     B, rows, C = 3, 9000, 1 << 17
@@ -366,6 +418,18 @@ def test_c_entries_refuse_before_any_launch():
     assert put((11, 0)) == -1 and put((13, 0)) == -1 and put((9, 1 << 30)) == -2
     assert put((10, -1)) == -1 and put((8, 252)) == -2 and put((6, 70000)) == -2 and put((19, 0)) == -6 and put((12, 128)) == -1
     assert put((0, P + 2)) == -3 and put((15, 2564)) == -3 and put((17, -8)) == -1
+
+
+def test_c_entries_refuse_launches_of_too_many_threads():
+    """Host checks of sizes whose grids no launch takes (2^32 threads an axis), and of a scale that overflows in powers of two."""
+    lib, P, bf16 = _lib.load(), 0x10000, _lib.DT_BF16
+    rows = [200 * 4096, 4096, 200 * 2048, 2048, 200 * 2048, 2048, 200 * 4096, 4096]
+    prompt = lambda B, scale: lib.sana_hip_window_attention(P, P, P, P, None, None, 0, B, 200, 200, 64, 32, 64, 50, 4, *rows, scale, bf16, None)  # noqa: E731
+    assert prompt(1 << 16, 0.1) == -2 and prompt(1, 3e38) == -1
+    step = lambda B, scale: lib.sana_hip_window_step(P, P, P, P, P, P, P, None, 0, B, 64, 32, 64, 100, 4, 4096, 2048, 2048, 104 * 2048,  # noqa: E731
+                                                     2048, 104 * 2048, 2048, 4096, scale, bf16, None)
+    assert step(1 << 19, 0.1) == -2 and step(1, 3e38) == -1
+    assert lib.sana_hip_window_cache_append(P, P, P, P, P, None, 2, 1 << 27, 256, 50, 4, 54 * 256, 256, 54 * 256, 256, 2560, 256, 2560, 256, bf16, None) == -2
 
 
 def test_cpu_tensors_are_refused():
