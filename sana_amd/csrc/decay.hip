@@ -528,14 +528,25 @@ __global__ __launch_bounds__(256) void decay_step_kernel(const DecayArgs a) {
   }
 }
 
-// Segments of a stream: none for a state alone; otherwise whole chunks.
-int segment_count(int B, int N, int H, int* tokens) {
+// Segments of a stream, whole chunks each.  A head alone is a chain of chunks, some 2 us each (112 channels 4), on one compute unit;
+// segments run side by side, but read K and V twice, and each reads and writes a state three times.  us, whole / in segments:
+//   enough of them to fill the chip: 20 heads of 112 x 4096 tokens 274 / 51 (12 segments), 32768 tokens 2143 / 234 (25), 140 of 112 x 4680
+//   330 / 251 (3), 200 of 112 x 4096 296 / 313 (2): at least three, or none;
+//   one workgroup a compute unit where the segments are short (20 of 112 x 4096, 11 and 22 segments: 51 / 57; 48 of 128 x 2048, 5 and 11: 62 / 66),
+//   as many as it holds where they are long (20 of 112 x 16384, 12 and 24: 142 / 132) or the head narrow (70 of 32 x 2048, 4 and 11: 29 / 22);
+//   two chunks at least (20 of 112 x 1024, 8 and 16: 26 / 28) and 64 segments at most (the scan is a chain too: 8 of 64 x 32768, 64 and 128: 57 / 71);
+//   few chunks pay for two more launches where the heads are few: 8 of 64 x 384 15 / 13, 20 of 112 x 384 31 / 23, 80 of 112 x 640 48 / 40, but 64 of 64
+//   x 320 14 / 18, 128 of 64 x 640 24 / 27, 70 of 32 x 512 14 / 15.
+int segment_count(int B, int N, int H, int d, int* tokens) {
   const int chunks = (N + DC - 1) / DC;
   const int64_t heads = (int64_t)B * H;
-  int want = 1;
-  if (heads < 256 && chunks >= 16) want = (int)(512 / heads);
-  want = want > chunks / 4 ? (chunks / 4 > 1 ? chunks / 4 : 1) : want;
-  const int per = (chunks + want - 1) / want;
+  const int room = 256 * (d <= 32 ? 4 : d <= 64 ? 3 : 2);  // workgroups that the chip holds at a time
+  int64_t want = room / heads;
+  if (d > 64 && heads <= 256 && chunks < 12 * (256 / heads)) want = 256 / heads;
+  want = want > 64 ? 64 : want;
+  want = want > chunks / 2 ? chunks / 2 : want;
+  if (want < 3 || chunks < 4 + heads / (d > 64 ? 16 : 8)) want = 1;
+  const int per = (int)((chunks + want - 1) / want);
   *tokens = per * DC;
   return (chunks + per - 1) / per;
 }
@@ -559,7 +570,9 @@ int launch_chunks(const DecayArgs& a, int B, hipStream_t s) {
 
 template <typename T>
 int launch_step(const DecayArgs& a, int B, hipStream_t s) {
-  const dim3 grid((unsigned)(B * a.H), a.d > 64 ? 2 : 1), block(256);
+  // (workgroups of a head: 1 stream of 20 heads of 112 with 1, 2, 4 8.5, 5.6, 4.5 us, 64 streams 29, 27, 26; 35 of 64
+  // with 1, 2, 4 4.2, 3.5, 3.2, 16 streams 6.7, 6.0, 6.7; 16 streams of 70 of 32 with 1, 4 4.5, 5.4)
+  const dim3 grid((unsigned)(B * a.H), a.d > 64 ? 4 : a.d > 32 ? 2 : 1), block(256);
   if (a.d > 64) hipLaunchKernelGGL((decay_step_kernel<T, 32>), grid, block, 0, s, a);
   else if (a.d > 32) hipLaunchKernelGGL((decay_step_kernel<T, 16>), grid, block, 0, s, a);
   else hipLaunchKernelGGL((decay_step_kernel<T, 8>), grid, block, 0, s, a);
@@ -586,7 +599,7 @@ using namespace sana;
 SANA_API size_t sana_hip_decay_attention_workspace_bytes(int B, int N, int H, int d) {
   if (B <= 0 || N <= 1 || H <= 0 || d <= 0 || d > 128 || (int64_t)B * H >= (1 << 24)) return 0;
   int tokens;
-  const int nseg = segment_count(B, N, H, &tokens);
+  const int nseg = segment_count(B, N, H, d, &tokens);
   return nseg > 1 ? (size_t)B * H * nseg * d * d * sizeof(float) : 0;
 }
 
@@ -619,7 +632,7 @@ SANA_API int sana_hip_decay_attention(const void* q, const void* k, const void* 
   a.N = N, a.H = H, a.d = d, a.nseg = 1, a.seg_tokens = N, a.units = 0;
   a.q_b = q_stride_b, a.q_n = q_stride_n, a.k_b = k_stride_b, a.k_n = k_stride_n, a.v_b = v_stride_b, a.v_n = v_stride_n;
   a.o_b = o_stride_b, a.o_n = o_stride_n, a.scale = scale;
-  if (N > 1) a.nseg = segment_count(B, N, H, &a.seg_tokens);
+  if (N > 1) a.nseg = segment_count(B, N, H, d, &a.seg_tokens);
   if (a.nseg > 1) {
     if (!workspace || workspace_bytes < sana_hip_decay_attention_workspace_bytes(B, N, H, d)) return SANA_ERR_WORKSPACE;
     if (!aligned16(workspace)) return SANA_ERR_ALIGN;

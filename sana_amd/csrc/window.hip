@@ -549,7 +549,8 @@ constexpr int64_t WA_MAX_BLOCKS = 1 << 24;  // of 256 threads: a launch has fewe
 // 8000 72 / 56, 12 of 96 8000 38 / 31, 20 of 112 16384 133 / 145.
 int query_tiles(int B, int N, int H, int d) { return d <= 96 || (int64_t)B * H * ((N + 127) / 128) <= 400 ? 1 : 2; }
 // Parts of a prompt's keys: where the blocks of queries leave compute units idle and have tiles of keys enough to pay for a second launch
-// (600 tokens, 20 heads of 112, ten tiles: whole 13.9 us, in two parts over 20).
+// (600 tokens, 20 heads of 112, ten tiles: whole 13.9 us, in two parts over 20; 128 of 1128 keys 22.7 / 17.0 (four parts), 300 of 4300 67 / 32 (five), 1 of
+// 4096 62 / 16 (sixteen), 64 of 764, four streams of 16 heads of 128 17 / 17; two tiles a part are no faster than four).
 int prompt_splits(int B, int N, int Nk, int H, int d, int window, int sinks) {
   const int qb = WA_NW * 16 * query_tiles(B, N, H, d);
   const int64_t blocks = (int64_t)B * H * ((N + qb - 1) / qb);
@@ -562,17 +563,19 @@ int prompt_splits(int B, int N, int Nk, int H, int d, int window, int sinks) {
 }
 // One token: the workgroups of a whole cache, one a (stream, key head, 16 query heads).
 int64_t step_groups(int B, int H, int Hkv) { return (int64_t)B * Hkv * ((H / Hkv + 15) / 16); }
-// Eight waves take a short cache whole, where its workgroups are few: the second launch that joins parts takes longer than the tiles of a
-// wave one after the other.
-bool step_in_one(int64_t groups, int rows) { return groups <= 256 && (rows + 31) / 32 <= 48; }
-// Parts of a cache's rows: four tiles of 32 rows a workgroup at least.
-int step_splits(int B, int H, int Hkv, int rows) {
-  const int64_t groups = step_groups(B, H, Hkv);
-  const int tiles = (rows + 31) / 32;
-  if (step_in_one(groups, rows)) return 1;
-  int64_t want = (1024 + groups - 1) / groups;
-  want = want > tiles / 4 ? tiles / 4 : want;
-  return (int)(want < 1 ? 1 : want > WA_MAX_SPLITS ? WA_MAX_SPLITS : want);
+// Parts of a cache's rows.  A short cache is taken whole: a second launch that joins parts takes 3.4 us, and 3.6 of the host's where calls are issued
+// one by one.  us on the device, whole / best of 2 to 32 parts: 20 key heads of 112 x 260 rows 8.4 / 8.8, 516 11.6 / 10.1, 1028 16.3 / 12.3; 8 of 128
+// x 260 7.7 / 8.8, 1028 14 / 9.3; 80 of 112 x 516 12 / 14; 70 of 32 x 1028 8.0 / 10.8; where there are more, longer ones too: 160 of 112 x 1028
+// 27 / 29, 140 of 32 x 4100 27 / 29.  Otherwise the least number with which the last round of compute units is not mostly idle: 20 of 112 x
+// 4100 47 / 18 (10 parts), 120 of 112 x 4100 79 / 57 (2), 200 90 / 88, 260 167 / 112 (12; 4: 122), 512 of 128 x 8192 366 / 380 (2).
+// (Two tiles of a wave requested ahead in the place of one make a whole cache slower: 20 of 112 x 1028 16.3 / 19.9.)
+int step_splits(int B, int H, int Hkv, int rows, int d) {
+  const int64_t groups = step_groups(B, H, Hkv), bytes = (int64_t)rows * d * 4;
+  if (bytes <= (groups <= 128 ? 384 << 10 : 1 << 20)) return 1;
+  const int most = rows / 64 < WA_MAX_SPLITS ? rows / 64 : WA_MAX_SPLITS;
+  for (int s = 1; s < most; ++s)
+    if (groups * s * 32 >= (groups * s + 255) / 256 * 256 * 25) return s;
+  return most > 1 ? most : 1;
 }
 size_t part_bytes(int splits, int64_t rows, int d) { return splits > 1 ? (size_t)splits * rows * (d + 2) * sizeof(float) : 0; }
 
@@ -606,7 +609,8 @@ template <typename T, int DK, int DT>
 int launch_step(const WindowArgs& a, hipStream_t s) {
   const int64_t groups = step_groups(a.B, a.H, a.Hkv);
   if (groups >= WA_MAX_BLOCKS) return SANA_ERR_SHAPE;
-  if (step_in_one(groups, a.window + a.sinks))
+  // (eight waves where a cache is not split and the chip has room for them: 20 key heads of 112 x 772 rows 13.7 us, four 15.3; 320 x 516 29.8 / 28.3)
+  if (a.splits == 1 && groups <= 256)
     hipLaunchKernelGGL((window_step_kernel<T, DK, DT, 8>), dim3((unsigned)groups), dim3(512), 0, s, a);
   else
     hipLaunchKernelGGL((window_step_kernel<T, DK, DT, 4>), dim3((unsigned)groups, (unsigned)a.splits), dim3(256), 0, s, a);
@@ -725,7 +729,7 @@ SANA_API int sana_hip_window_cache_append(void* cache_k, void* cache_v, const vo
 
 SANA_API size_t sana_hip_window_step_workspace_bytes(int B, int H, int Hkv, int d, int window, int sinks) {
   if (B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || d <= 0 || window <= 0 || sinks < 0 || (int64_t)window + sinks > (1 << 30)) return 0;
-  return part_bytes(step_splits(B, H, Hkv, window + sinks), (int64_t)B * H, d);
+  return part_bytes(step_splits(B, H, Hkv, window + sinks, d), (int64_t)B * H, d);
 }
 
 SANA_API int sana_hip_window_step(const void* q, const void* k, const void* v, void* cache_k, void* cache_v, const int32_t* positions,
@@ -752,7 +756,7 @@ SANA_API int sana_hip_window_step(const void* q, const void* k, const void* v, v
   a.q_b = q_stride_b, a.k_b = k_stride_b, a.v_b = v_stride_b, a.o_b = o_stride_b;
   a.ck_b = ck_stride_b, a.ck_n = ck_stride_n, a.cv_b = cv_stride_b, a.cv_n = cv_stride_n;
   a.scale_log2e = scale * 1.44269504088896341f;
-  a.splits = step_splits(B, H, Hkv, window + sinks);
+  a.splits = step_splits(B, H, Hkv, window + sinks, d);
   const int64_t rows = (int64_t)B * H;
   if (a.splits > 1) {
     if (!workspace || workspace_bytes < part_bytes(a.splits, rows, d)) return SANA_ERR_WORKSPACE;
