@@ -949,11 +949,11 @@ def decay_linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lo
             raise SanaHipError(f"state and state_out must be contiguous fp32 {(B, H, d, d)}, got {t.dtype} {tuple(t.shape)}")
     length_ptr = _lengths_arg(lengths, B)
     if out is None:
-        out = q.new_empty(shape) if lengths is None else q.new_zeros(shape)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format) if lengths is None else q.new_zeros(shape)
     elif out.shape != shape or out.dtype is not dt:
         raise SanaHipError("out has the wrong shape or dtype")
     if state_out is None:
-        state_out = torch.empty((B, H, d, d), dtype=torch.float32, device=q.device)
+        state_out = torch.empty_like(state) if state is not None else log_decay.new_empty((B, H, d, d))
     if B * N == 0:
         if state is None:
             state_out.zero_()
@@ -1015,7 +1015,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, num_head
         raise SanaHipError(f"the {N} queries are the last of the keys, of which there are {Nk}")
     length_ptr = _lengths_arg(lengths, B)
     if out is None:
-        out = q.new_empty(q.shape) if lengths is None else q.new_zeros(q.shape)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format) if lengths is None else q.new_zeros(q.shape)
     elif out.shape != q.shape or out.dtype != q.dtype:
         raise SanaHipError("out has the wrong shape or dtype")
     if B * N == 0:
@@ -1088,7 +1088,7 @@ def window_attention_step_(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ca
     B, _, C = q.shape
     position_ptr = _lengths_arg(positions, B, "positions")
     if out is None:
-        out = q.new_empty(q.shape)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != q.dtype:
         raise SanaHipError("out has the wrong shape or dtype")
     if B == 0:
