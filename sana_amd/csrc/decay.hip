@@ -62,6 +62,10 @@ enum { DC_SUMS, DC_OUT, DC_WHOLE };
 // f16 ends at 65504: S goes in scaled by a power of two for each wave, P for each query.
 // A value that is not finite must not reach the queries in front of it (0 * inf): it is staged as 0, and its channel is set to NaN from its
 // token on.
+// What bounds it: where all compute units work, memory (32760 tokens x 20 heads of 112, 25 segments: sums 78 us = 318 MB at 4.1 TB/s, outputs 155 us =
+// 563 MB at 3.6 TB/s; rows of 224 bytes come at 3.8 - 4.1 TB/s to any kernel here); few chunks, the chain of a chunk's steps, some 2 us
+// (32 channels) to 4 us (112) each: three barriers, each with the LDS and MFMA latencies in front of it (300 tokens x 70 heads of 32: five
+// chunks, 12 us).  Two chunks requested ahead, three workgroups a compute unit and eight waves a workgroup were no faster.
 template <typename T, int DK, int KT, int VT, int NV, int MODE>
 __global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) {
   constexpr bool OUT = MODE != DC_SUMS, F = is_f16<T>;
@@ -460,7 +464,8 @@ __global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) 
 }
 
 // The segments' own sums -> the states in front of them, and the one behind the last: run = S0; run = a^(tokens) run + sum.  Four
-// values a thread, eight segments requested at a time.
+// values a thread, eight segments requested at a time, so that a chain of 25 waits for memory four times: 10 us for 25 MB read and written (with 20
+// heads of 112, one pass over the workspace; its threads are too few to do better).
 __global__ __launch_bounds__(64) void decay_scan_kernel(const DecayArgs a) {
   constexpr int AHEAD = 8;
   const int bh = blockIdx.y, b = bh / a.H, i = blockIdx.x * 64 + threadIdx.x, dd4 = a.d * a.d / 4;
@@ -487,7 +492,9 @@ __global__ __launch_bounds__(64) void decay_scan_kernel(const DecayArgs a) {
   reinterpret_cast<f32x4_t*>(a.state_out)[(int64_t)bh * dd4 + i] = run;
 }
 
-// One token of each stream.  A row of the state is d floats in LPR lanes of four; a wave holds 64 / LPR rows at a time.
+// One token of each stream.  A row of the state is d floats in LPR lanes of four; a wave holds 64 / LPR rows at a time.  Memory alone bounds it: 128
+// streams x 35 heads of 64, 147 MB of state in and out, 30.6 us = 4.8 TB/s, as a large copy; one stream is a launch and two loads (20 heads
+// of 112 4.5 us).
 template <typename T, int LPR>
 __global__ __launch_bounds__(256) void decay_step_kernel(const DecayArgs a) {
   constexpr int RW = 64 / LPR;  // rows of a wave
