@@ -35,9 +35,11 @@ template <typename T> inline constexpr float kShift = is_f16<T> ? 6.f : 0.f;
 // the order of keys that this gives.  The running maximum moves only when some score is 2^8 above it: until then p <= 2^8 and nothing is
 // rescaled (the 16-bit p keeps its relative step, l and o are fp32).  f16: p times 2^6, the small ones away from its subnormal numbers.
 // Of a tile of 64 keys x 32 queries x 112 channels the matrix pipe takes 960 cycles, the vector unit some 1000 (half of them powers) and
-// the LDS 350 for each of four waves: with two waves a SIMD 16384 tokens x 20 heads over a window of 4096 run at 0.82 - 0.86 PFLOP/s
-// (615 - 645 us).  Through registers instead of direct loads 705 us; each tile's scores in front of its own powers instead of those of
-// the tile before: 630 - 690, by how the compiler mixes them; three or four query tiles a wave: the registers do not hold them.
+// the LDS 350 for each of four waves: with two waves a SIMD 16384 tokens x 20 heads over a window of 4096 run at 0.84 PFLOP/s (633 us), f16 with
+// shared key heads at 0.86.  Through registers instead of direct loads 705 us; each tile's scores in front of its own powers instead of those of the tile
+// before: 630 - 690, by how the compiler mixes them; each operand read from LDS where it is used instead of an MFMA group ahead, and the
+// maxima in front of the powers instead of beside the values' MFMAs: 653; where in a tile the rest of the vector work stands, wave priorities
+// and reads further ahead change it by less than 0.5 %; three or four query tiles a wave: the registers do not hold them.
 template <typename T, int DK, int DT, int QT, int NW>
 __global__ __launch_bounds__(64 * NW, QT == 1 && DK < 4 ? 3 : 2) void window_attn_kernel(const WindowArgs a) {
   constexpr int PITCH = DK * 64, TILE = WK * PITCH, LOADS = TILE / 1024 / NW, QB = NW * 16 * QT;
@@ -117,14 +119,15 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DK < 4 ? 3 : 2) void window_att
     return j1 <= wp0 && (j1 < a.sinks || wp1 - j0 < a.window);
   };
   // Scores of KP tiles of 16 keys at a time: one where two query tiles take turns, two otherwise (an MFMA that adds to what the one before
-  // it has just summed waits for twice its own time).
-  constexpr int KP = QT == 1 ? 2 : 1;
-  auto score = [&](const unsigned char* from, int k0, f32x4_t (&sc)[QT][4]) {
-    u32x4_t kf[KP][DK];
+  // it has just summed waits for twice its own time).  Values are read AHEAD products in front of their own.
+  constexpr int KP = QT == 1 ? 2 : 1, AHEAD = 2;
+  auto keys_of = [&](const unsigned char* from, int k0, u32x4_t (&kf)[KP][DK]) {
 #pragma unroll
     for (int j = 0; j < KP; ++j)
 #pragma unroll
       for (int s = 0; s < DK; ++s) kf[j][s] = lds_read((const lds_t*)from + 16 * (k0 + j) * PITCH + k_at[s]);
+  };
+  auto score = [&](const u32x4_t (&kf)[KP][DK], int k0, f32x4_t (&sc)[QT][4]) {
 #pragma unroll
     for (int j = 0; j < KP; ++j)
 #pragma unroll
@@ -150,18 +153,18 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DK < 4 ? 3 : 2) void window_att
         }
     }
   };
-  auto maxima = [&](const f32x4_t (&sc)[QT][4]) {
+  float top[QT];  // of the tile whose scores are there, this lane's keys
+  auto highest = [&](int q, int kt, const f32x4_t (&sc)[QT][4]) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) top[q] = fmaxf(kt + r == 0 ? -INFINITY : top[q], sc[q][kt][r]);
+  };
+  auto maxima = [&]() {
     // (the scale is positive: the maximum of the scaled scores is the scaled maximum)
     float most[QT];
     bool above = false;
 #pragma unroll
     for (int q = 0; q < QT; ++q) {
-      most[q] = -INFINITY;
-#pragma unroll
-      for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) most[q] = fmaxf(most[q], sc[q][kt][r]);
-      most[q] *= a.scale_log2e;
+      most[q] = top[q] * a.scale_log2e;
       above |= most[q] > mx[q] + 8.f;
     }
     if (__any(above)) {
@@ -187,16 +190,10 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DK < 4 ? 3 : 2) void window_att
     }
     pk[q][kt] = u32x2_t{pk16<T>(p[0], p[1]), pk16<T>(p[2], p[3])};
   };
-  auto values = [&](unsigned char* from, int s, const u32x2_t (&pk)[QT][4]) {
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      lds_t* at = (lds_t*)from + v_at(dt) + 32 * s * PITCH;
-      const u32x2_t x = lds_read_tr(at), y = lds_read_tr(at + 16 * PITCH);
-      const u32x4_t vf = {x.x, x.y, y.x, y.y};
-#pragma unroll
-      for (int q = 0; q < QT; ++q)
-        oc[q][dt] = mfma_16x16x32<T>(vf, u32x4_t{pk[q][2 * s].x, pk[q][2 * s].y, pk[q][2 * s + 1].x, pk[q][2 * s + 1].y}, oc[q][dt]);
-    }
+  auto values_of = [&](unsigned char* from, int i) {  // 32 keys i / DT of 16 channels i % DT
+    lds_t* at = (lds_t*)from + v_at(i % DT) + 32 * (i / DT) * PITCH;
+    const u32x2_t x = lds_read_tr(at), y = lds_read_tr(at + 16 * PITCH);
+    return u32x4_t{x.x, x.y, y.x, y.y};
   };
   // Tile t: its softmax and its product with V, and the scores of the tile behind it, whose MFMAs the vector work need not wait for.
   // A buffer is written again two barriers after its last read.  No branch decides whether a tile is worked on: what a wave does not see is
@@ -206,24 +203,45 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DK < 4 ? 3 : 2) void window_att
     landed();  // K of t + 1, V of t
     if (t + 2 < t1) request(kp, a.k_n, k2, t + 2, k_here);
     if (t + 1 < t1) request(vp, a.v_n, v2, t + 1, v_next);
-    if (!whole(t)) mask(t, sc);
-    maxima(sc);
+    u32x4_t kf[2][KP][DK], vf[AHEAD + 1];
+    keys_of(k_next, 0, kf[0]);
+    __builtin_amdgcn_sched_barrier(0);
+    if (!whole(t)) {
+      mask(t, sc);
+#pragma unroll
+      for (int u = 0; u < 4 * QT; ++u) highest(u % QT, u / QT, sc);
+    }
+    maxima();
     asm volatile("" : "+v"(v_slot));  // (addresses are worked out here again: kept, they would take the registers of the tiles)
     // 16 or 32 keys of the next tile at a time, and the powers of half of the keys between their MFMAs
     u32x2_t pk[QT][4];
 #pragma unroll
     for (int kt = 0; kt < 4; kt += KP) {
       __builtin_amdgcn_sched_barrier(0);
-      score(k_next, kt, next);
+      if (kt + KP < 4) keys_of(k_next, kt + KP, kf[(kt / KP + 1) & 1]);
+      else
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) vf[i] = values_of(v_here, i);
+      __builtin_amdgcn_sched_barrier(0);
+      score(kf[(kt / KP) & 1], kt, next);
 #pragma unroll
       for (int u = kt * QT / 2; u < (kt + KP) * QT / 2; ++u) powers(u % QT, u / QT, sc, pk);
     }
-    __builtin_amdgcn_sched_barrier(0);
-    values(v_here, 0, pk);
 #pragma unroll
-    for (int q = 0; q < QT; ++q) powers(q, 2, sc, pk), powers(q, 3, sc, pk);
-    __builtin_amdgcn_sched_barrier(0);
-    values(v_here, 1, pk);
+    for (int i = 0; i < 2 * DT; ++i) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (i + AHEAD < 2 * DT) vf[(i + AHEAD) % (AHEAD + 1)] = values_of(v_here, i + AHEAD);
+      const int s = i / DT, dt = i % DT;
+#pragma unroll
+      for (int q = 0; q < QT; ++q)
+        oc[q][dt] = mfma_16x16x32<T>(vf[i % (AHEAD + 1)], u32x4_t{pk[q][2 * s].x, pk[q][2 * s].y, pk[q][2 * s + 1].x, pk[q][2 * s + 1].y}, oc[q][dt]);
+#pragma unroll
+      for (int u = 0; u < 2 * QT; ++u)
+        if (i == u * DT / (2 * QT)) powers(u % QT, 2 + u / QT, sc, pk);
+#pragma unroll
+      for (int u = 0; u < 4 * QT; ++u)
+        if (i == DT + u * DT / (4 * QT)) highest(u % QT, u / QT, next);
+    }
   };
   if (t0 < t1) {
     f32x4_t even[QT][4], odd[QT][4];
@@ -233,7 +251,11 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DK < 4 ? 3 : 2) void window_att
     landed();
 #pragma unroll
     for (int kt = 0; kt < 4; kt += KP) {
-      score(k_even, kt, even);
+      u32x4_t kf[KP][DK];
+      keys_of(k_even, kt, kf);
+      score(kf, kt, even);
+#pragma unroll
+      for (int u = kt * QT; u < (kt + KP) * QT; ++u) highest(u % QT, u / QT, even);
       __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll 1
