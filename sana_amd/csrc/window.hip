@@ -569,9 +569,9 @@ constexpr int WA_NW = 4;
 constexpr int64_t WA_MAX_BLOCKS = 1 << 24;  // of 256 threads: a launch has fewer than 2^32 threads an axis
 // 16-query tiles of a wave, 64 or 128 queries a workgroup.  Two feed twice the MFMAs with a read of K or V and pay where heads are wide
 // and the blocks many; one gives more and shorter workgroups, and up to 96 channels three and more waves a SIMD.  us, two / one, window 4096:
-// 20 heads of 112 1500 tokens 39 / 32, 2000 63 / 49, 3000 77 / 93, 8000 304 / 357; 16 of 128 3000 82 / 62, 4680 139 / 129, 8000 253 / 272;
-// 16 of 72 1500 34.4 / 26.5, 4680 109 / 100, 8000 193 / 204, 12 of 96 8000 193 / 187, 35 of 64 8000 325 / 316; window 256: 35 of 64
-// 8000 72 / 56, 12 of 96 8000 38 / 31, 20 of 112 16384 133 / 145.
+// 20 heads of 112 1500 tokens 38 / 30, 2000 59 / 48, 2560 66 / 66, 3000 70 / 88, 8000 294 / 351; 16 of 128 3000 70 / 60, 4680 123 / 122, 8000 231 / 261;
+// window 256: 20 of 112 16384 136 / 143.  Narrower heads (two tiles as they were when reads and products still took turns): 16 of 72 1500
+// 34.4 / 26.5, 4680 109 / 100, 8000 193 / 204, 12 of 96 8000 193 / 187, 35 of 64 8000 325 / 316; window 256: 35 of 64 8000 72 / 56, 12 of 96 8000 38 / 31.
 int query_tiles(int B, int N, int H, int d) { return d <= 96 || (int64_t)B * H * ((N + 127) / 128) <= 400 ? 1 : 2; }
 // Parts of a prompt's keys: where the blocks of queries leave compute units idle and have tiles of keys enough to pay for a second launch
 // (600 tokens, 20 heads of 112, ten tiles: whole 13.9 us, in two parts over 20; 128 of 1128 keys 22.7 / 17.0 (four parts), 300 of 4300 67 / 32 (five), 1 of
