@@ -265,7 +265,8 @@ __global__ __launch_bounds__(64 * NW, QT == 1 && DK < 4 ? 3 : 2) void window_att
     }
   }
   // ---- Values that are not finite: the products with V once more, so that they reach the queries that see them and no others.  32 keys at a
-  // time straight from memory, the finite values; the others counted, and their signs summed, over the keys that are seen.
+  // time straight from memory, the finite values; the others counted, and their signs summed, over the keys that are seen.  (All blocks of 16384
+  // tokens with a window of 4096: 5.9 ms where finite values take 0.65 - 0.78.)
   bool odd = false;
 #pragma unroll
   for (int q = 0; q < QT; ++q)
