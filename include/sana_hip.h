@@ -501,9 +501,10 @@ int sana_hip_block(const sana_block_args* args, void* stream);
  *   lengths       int32 [B] or NULL: entry b has lengths[b] tokens (0 .. N, values outside are clamped); what lies behind is
  *                 neither read nor written, and a stream of 0 tokens keeps its state
  *   workspace     at least sana_hip_decay_attention_workspace_bytes(...) bytes, 16-byte aligned (NULL where that is 0)
- * d % 8 == 0, d <= 128; B * H <= 2^24; q, k, v and the states 16-byte aligned, out 8; token strides from H*d to 2^23 - 1.
- * The state is summed in fp32 in a fixed order.  out must not overlap q, k or v.  A token's inf or NaN reaches its own
- * output, later ones, and those of up to 63 tokens in front of it.
+ * d % 8 == 0, d <= 128; B * H < 2^24 and, for N > 1, B * ceil(H / 4) <= 2^22 - 8; q, k, v and the states 16-byte aligned, out 8; token
+ * strides from H*d to 2^23 - 1.  The state is summed in fp32 in a fixed order.  out must not overlap q, k or v.  A value of inf or
+ * NaN leaves its channel (of outputs and state) inf or NaN from its token on, a key of them its head's outputs; nothing in front
+ * of it changes.
  */
 size_t sana_hip_decay_attention_workspace_bytes(int B, int N, int H, int d);
 int sana_hip_decay_attention(const void* q, const void* k, const void* v, const float* log_decay, const float* state_in,
@@ -524,8 +525,8 @@ int sana_hip_decay_attention(const void* q, const void* k, const void* v, const 
  *   workspace  at least sana_hip_window_attention_workspace_bytes(...) bytes, 16-byte aligned (NULL where that is 0): few queries
  *           of many keys are split over the keys
  * scale > 0; window >= 1; d % 8 == 0, d <= 128; q, k, v 16-byte aligned, out 8; token strides of k and v below 2^23.
- * Probabilities are rounded to the io dtype before they multiply v; maxima, sums and outputs are fp32.  A key whose value is
- * inf or NaN may reach the queries that see any of the 64 aligned keys around it.
+ * Probabilities are rounded to the io dtype before they multiply v; maxima, sums and outputs are fp32.  A key or a value of
+ * inf or NaN reaches the queries that see it, and no others.
  */
 size_t sana_hip_window_attention_workspace_bytes(int B, int N, int Nk, int H, int d, int window, int sinks);
 int sana_hip_window_attention(const void* q, const void* k, const void* v, void* out, const int32_t* lengths, void* workspace,
