@@ -31,7 +31,7 @@ class GraphedCall:
         self._inputs = list(example)   # the example tensors ARE the captured input buffers
         with torch.no_grad():
             # One stream of this object's own for the warm-up AND the capture.  The library keeps its scratch buffer
-            # per (device, stream): warming up on the stream that is captured afterwards creates that buffer eagerly,
+            # per (device, stream, host thread): warming up on the stream that is captured afterwards creates that buffer eagerly,
             # in the ordinary memory pool, before the capture begins (allocated during the capture it would belong to
             # this graph's private pool while other graphs used it), and a stream per object gives every graph a
             # scratch buffer of its own, so two graphs replayed on different streams do not share one.

@@ -5,6 +5,7 @@ checks, without a launch: empty outputs, and an all-zero state for no tokens.
 """
 from __future__ import annotations
 
+import threading
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -17,12 +18,15 @@ IO16 = (torch.bfloat16, torch.float16)   # the 16-bit io dtypes of the GEMMs and
 HEAD_DIM = 32
 HEAD_DIMS = (32, 112)   # head dims with kernels: 32 (all dtypes), 112 (bf16; the video configurations)
 
-# Scratch buffers (attention partial states, split-k planes): one per (device, stream), so calls on different
-# streams never share scratch memory; calls on one stream are ordered by it.  A buffer that has become too small
+# Scratch buffers (attention partial states, split-k planes): one per (device, stream, host thread), so calls on different
+# streams never share scratch memory; one thread's calls on one stream are ordered by it.  Two threads' are not: a call of
+# several launches leaves the interpreter's lock while it issues them, and another thread's launches may go in between.
+# A buffer that has become too small
 # is RETIRED, never freed: a captured HIP graph (or work still queued) may hold its address, and the allocator
 # would hand freed memory to the next tensor.  Sizes grow in powers of two, so everything retired on a stream is
-# smaller than its current buffer.
-_workspaces = {}     # (device index, raw stream handle) -> list of uint8 tensors, the last one current
+# smaller than its current buffer.  (A thread that has ended leaves its buffers to the next one of its identity.)
+_MAIN_THREAD = threading.main_thread().ident
+_workspaces = {}     # (device index, raw stream handle[, thread other than the main one]) -> list of uint8 tensors, the last one current
 _chunk_tables = {}   # (device index, tuple) -> int32 tensor
 _CACHE_LIMIT = 256   # small derived device tensors (chunk tables, frame flags) kept per process
 
@@ -59,6 +63,9 @@ def _workspace(device: torch.device, nbytes: int, stream: Optional[int] = None) 
     if nbytes == 0:
         return None
     key = (device.index, _stream() if stream is None else stream)
+    thread = threading.get_ident()
+    if thread != _MAIN_THREAD:
+        key = (*key, thread)
     bufs = _workspaces.get(key)
     if bufs is None:
         bufs = _workspaces[key] = []
@@ -906,7 +913,7 @@ def _lengths_arg(t: Optional[torch.Tensor], B: int, what: str = "lengths") -> Op
 
 
 def _call_scratch(device: torch.device, nbytes: int) -> Optional[torch.Tensor]:
-    """Scratch that holds nothing between calls: the stream's buffer, or, under capture and where it is too large to be kept,
+    """Scratch that holds nothing between calls: this thread's buffer of the stream, or, under capture and where it is too large to be kept,
     one of this call's own (graphs that are captured on one stream and replayed side by side must not share it)."""
     if nbytes and (nbytes > STATE_SCRATCH_KEPT or torch._C._cuda_isCurrentStreamCapturing()):
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
