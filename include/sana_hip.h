@@ -529,6 +529,8 @@ int sana_hip_decay_attention(const void* q, const void* k, const void* v, const 
  * inf or NaN reaches the queries that see it, and no others.
  */
 size_t sana_hip_window_attention_workspace_bytes(int B, int N, int Nk, int H, int d, int window, int sinks);
+/* The tiles of 16 queries that a wave takes (1 or 2: 64 or 128 queries a workgroup): a query for tests and measurements. */
+int sana_hip_window_attention_query_tiles(int B, int N, int H, int d);
 int sana_hip_window_attention(const void* q, const void* k, const void* v, void* out, const int32_t* lengths, void* workspace,
                               size_t workspace_bytes, int B, int N, int Nk, int H, int Hkv, int d, int window, int sinks,
                               int64_t q_stride_b, int64_t q_stride_n, int64_t k_stride_b, int64_t k_stride_n,

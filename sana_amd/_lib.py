@@ -112,6 +112,7 @@ SIGNATURES = {
                                          c_void_p, c_size_t, c_int, c_int, c_int, c_int, c_int64, c_int64, c_int64, c_int64,
                                          c_int64, c_int64, c_int64, c_int64, c_float, c_int, c_void_p]),
     "sana_hip_window_attention_workspace_bytes": (c_size_t, [c_int] * 7),
+    "sana_hip_window_attention_query_tiles": (c_int, [c_int] * 4),
     "sana_hip_window_attention": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
                                           c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int64, c_int64, c_int64,
                                           c_int64, c_int64, c_int64, c_int64, c_int64, c_float, c_int, c_void_p]),

@@ -689,6 +689,10 @@ SANA_API size_t sana_hip_window_attention_workspace_bytes(int B, int N, int Nk, 
   return part_bytes(prompt_splits(B, N, Nk, H, d, window, sinks), (int64_t)B * N * H, d);
 }
 
+SANA_API int sana_hip_window_attention_query_tiles(int B, int N, int H, int d) {
+  return B <= 0 || N <= 0 || H <= 0 || d <= 0 || d > 128 ? 0 : query_tiles(B, N, H, d);
+}
+
 SANA_API int sana_hip_window_attention(const void* q, const void* k, const void* v, void* out, const int32_t* lengths, void* workspace,
                                        size_t workspace_bytes, int B, int N, int Nk, int H, int Hkv, int d, int window, int sinks,
                                        int64_t q_stride_b, int64_t q_stride_n, int64_t k_stride_b, int64_t k_stride_n,
