@@ -384,7 +384,10 @@ __global__ __launch_bounds__(256) void window_join_kernel(const WindowArgs a) {
       const float f = __shfl(mine, s0 + s, 32);  // (0 behind the last part, whose values are repeated there: they may be inf)
       l = fmaf(f, __shfl(ml[1], s0 + s, 32), l);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) o[r] = fmaf(f, f == 0.f ? 0.f : x[s][r], o[r]);
+      for (int r = 0; r < 4; ++r) {  // a part whose weight is 0 in fp32 gives what is not finite all the same: its keys are seen
+        const float y = s0 + s < a.splits ? x[s][r] : 0.f;
+        o[r] = fmaf(f == 0.f && !(fabsf(y) < INFINITY) ? 1.f : f, y, o[r]);
+      }
     }
   }
   const float inv = 1.0f / l;
