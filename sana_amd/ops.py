@@ -9,6 +9,7 @@ import threading
 from typing import Optional, Sequence, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import DT_BF16, DT_F16, DT_F32, SanaHipError
@@ -882,7 +883,7 @@ def gate_residual(y: torch.Tensor, gate: torch.Tensor, residual: torch.Tensor) -
 # --------------------------------------------------------------------------- streams whose memory does not grow
 
 def _here(ts, what: str) -> int:
-    """The device index on which all tensors of the call have to be (None entries aside); no gradients are asked for."""
+    """The device index on which all tensors of the call have to be (None entries aside); no derivatives are asked for, of neither mode."""
     dev = ts[0].get_device()
     for t in ts:
         if t is not None and t.get_device() != dev or dev < 0:
@@ -892,6 +893,10 @@ def _here(ts, what: str) -> int:
         for t in ts:
             if t is not None and t.requires_grad:
                 raise SanaHipError(f"{what} is forward only: call it under torch.no_grad() or on detached tensors")
+    if forward_ad._current_level >= 0:   # (dual tensors want no gradients, and the output would come without a tangent)
+        for t in ts:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise SanaHipError(f"{what} has no forward-mode derivative: call it on the primals")
     return dev
 
 

@@ -1,0 +1,38 @@
+"""What the streams' calls refuse, and what they take in the place of a number."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+import sana_amd
+from sana_amd import ops
+
+gpu = pytest.mark.gpu
+BF16 = torch.bfloat16
+
+
+def stream(cuda):
+    g = torch.Generator().manual_seed(0)
+    q, k, v = (torch.randn(1, 8, 64, generator=g).to(BF16).to(cuda) for _ in range(3))
+    cache = [torch.zeros(1, 20, 64, dtype=BF16, device=cuda) for _ in range(2)]
+    return q, k, v, torch.tensor([-0.1, -0.2], device=cuda), cache, torch.zeros(1, dtype=torch.int32, device=cuda)
+
+
+@gpu
+def test_forward_mode_derivatives_are_refused(cuda):
+    """A dual tensor wants no gradient, so only its tangent tells it: an output without one would be a wrong derivative of zero."""
+    q, k, v, g, (ck, cv), pos = stream(cuda)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        one = slice(0, 1)
+        bad = [lambda: ops.decay_linear_attention(dual(q), k, v, g), lambda: ops.decay_linear_attention(q, k, v, dual(g)),
+               lambda: ops.decay_linear_attention(q, k, v, g, state=dual(torch.zeros(1, 2, 32, 32, device=cuda))),
+               lambda: ops.window_attention(q, dual(k), v, 2, 5), lambda: ops.window_cache_append_(ck, cv, k, dual(v), pos),
+               lambda: ops.window_attention_step_(q[:, one], k[:, one], dual(v[:, one]), ck, cv, pos, 2),
+               lambda: ops.window_attention_step_(q[:, one], k[:, one], v[:, one], dual(ck), cv, pos, 2)]
+        for i, f in enumerate(bad):
+            with pytest.raises(sana_amd.SanaHipError):
+                f()
+                pytest.fail(f"case {i} was taken")
+        want = ops.window_attention(q, k, v, 2, 5)   # primals are fine within a level
+        assert torch.equal(ops.window_attention(forward_ad.unpack_dual(dual(q)).primal, k, v, 2, 5), want)
+    assert not ck.any() and not cv.any()
