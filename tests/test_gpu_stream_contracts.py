@@ -1,4 +1,5 @@
 """What the streams' calls refuse, and what they take in the place of a number."""
+import numpy as np
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -36,3 +37,16 @@ def test_forward_mode_derivatives_are_refused(cuda):
         want = ops.window_attention(q, k, v, 2, 5)   # primals are fine within a level
         assert torch.equal(ops.window_attention(forward_ad.unpack_dual(dual(q)).primal, k, v, 2, 5), want)
     assert not ck.any() and not cv.any()
+
+
+@gpu
+@pytest.mark.parametrize("tokens", [1, 8])
+def test_a_scale_is_any_number(cuda, tokens):
+    q, k, v, g, (ck, cv), pos = stream(cuda)
+    q, k, v = (t[:, :tokens] for t in (q, k, v))
+    want = ops.decay_linear_attention(q, k, v, g, 0.5)[0]
+    wide = ops.window_attention(q, k, v, 2, 5, scale=0.5)
+    for scale in (np.float32(0.5), np.float64(0.5), torch.tensor(0.5), torch.tensor(0.5, device=cuda)):
+        assert torch.equal(ops.decay_linear_attention(q, k, v, g, scale)[0], want)
+        assert torch.equal(ops.window_attention(q, k, v, 2, 5, scale=scale), wide)
+    assert torch.equal(ops.decay_linear_attention(q, k, v, g, 2)[0], ops.decay_linear_attention(q, k, v, g, 2.0)[0])
