@@ -624,7 +624,7 @@ SANA_API int sana_hip_decay_attention(const void* q, const void* k, const void* 
   }
   for (const int64_t sb : {q_stride_b, k_stride_b, v_stride_b, o_stride_b})
     if (sb < 0) return SANA_ERR_ARG;
-  if (B > 1 && o_stride_b == 0) return SANA_ERR_ARG;  // (entries that would write the same rows)
+  if (B > 1 && o_stride_b < (int64_t)H * d) return SANA_ERR_ARG;  // (entries that would write the same elements)
   for (const void* p : {q, k, v, (const void*)state_in, (const void*)state_out})
     if (!aligned16(p)) return SANA_ERR_ALIGN;
   for (const int64_t st : {q_stride_b, q_stride_n, k_stride_b, k_stride_n, v_stride_b, v_stride_n})

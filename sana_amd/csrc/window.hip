@@ -709,7 +709,7 @@ SANA_API int sana_hip_window_attention(const void* q, const void* k, const void*
     return SANA_ERR_ARG;
   for (const int64_t sb : {q_stride_b, k_stride_b, v_stride_b, o_stride_b})
     if (sb < 0) return SANA_ERR_ARG;
-  if (B > 1 && o_stride_b == 0) return SANA_ERR_ARG;  // (entries that would write the same rows)
+  if (B > 1 && o_stride_b < (int64_t)H * d) return SANA_ERR_ARG;  // (entries that would write the same elements)
   if (k_stride_n >= (1 << 23) || v_stride_n >= (1 << 23)) return SANA_ERR_SHAPE;  // 32-bit byte offsets within a tile
   if (misaligned({q, k, v}, {q_stride_b, q_stride_n, k_stride_b, k_stride_n, v_stride_b, v_stride_n}) ||
       (reinterpret_cast<uintptr_t>(out) & 7u) || o_stride_b % 4 || o_stride_n % 4 || off4(lengths))
@@ -744,7 +744,7 @@ SANA_API int sana_hip_window_cache_append(void* cache_k, void* cache_v, const vo
   if (ck_stride_n < C || cv_stride_n < C || k_stride_n < C || v_stride_n < C) return SANA_ERR_ARG;
   for (const int64_t sb : {ck_stride_b, cv_stride_b, k_stride_b, v_stride_b})
     if (sb < 0) return SANA_ERR_ARG;
-  if (B > 1 && (ck_stride_b == 0 || cv_stride_b == 0)) return SANA_ERR_ARG;  // (streams that would write the same rows)
+  if (B > 1 && (ck_stride_b < C || cv_stride_b < C)) return SANA_ERR_ARG;  // (streams that would write the same elements)
   if ((int64_t)window + sinks > (1 << 30)) return SANA_ERR_SHAPE;
   if (C % 8 || groups >= WA_MAX_BLOCKS || B > 65535) return SANA_ERR_SHAPE;
   if (misaligned({cache_k, cache_v, k, v}, {ck_stride_b, ck_stride_n, cv_stride_b, cv_stride_n, k_stride_b, k_stride_n, v_stride_b, v_stride_n}) ||
@@ -777,7 +777,7 @@ SANA_API int sana_hip_window_step(const void* q, const void* k, const void* v, v
   if (ck_stride_n < C || cv_stride_n < C) return SANA_ERR_ARG;
   for (const int64_t sb : {q_stride_b, k_stride_b, v_stride_b, ck_stride_b, cv_stride_b, o_stride_b})
     if (sb < 0) return SANA_ERR_ARG;
-  if (B > 1 && (o_stride_b == 0 || ck_stride_b == 0 || cv_stride_b == 0)) return SANA_ERR_ARG;  // (streams that would write the same rows)
+  if (B > 1 && (o_stride_b < (int64_t)H * d || ck_stride_b < C || cv_stride_b < C)) return SANA_ERR_ARG;  // (streams that would write the same elements)
   if ((int64_t)window + sinks > (1 << 30)) return SANA_ERR_SHAPE;
   if (misaligned({q, k, v, cache_k, cache_v}, {q_stride_b, k_stride_b, v_stride_b, ck_stride_b, ck_stride_n, cv_stride_b, cv_stride_n}) ||
       (reinterpret_cast<uintptr_t>(out) & 7u) || o_stride_b % 4 || off4(positions))

@@ -5,7 +5,7 @@ import torch
 from torch.autograd import forward_ad
 
 import sana_amd
-from sana_amd import ops
+from sana_amd import _lib, ops
 
 gpu = pytest.mark.gpu
 BF16 = torch.bfloat16
@@ -50,3 +50,20 @@ def test_a_scale_is_any_number(cuda, tokens):
         assert torch.equal(ops.decay_linear_attention(q, k, v, g, scale)[0], want)
         assert torch.equal(ops.window_attention(q, k, v, 2, 5, scale=scale), wide)
     assert torch.equal(ops.decay_linear_attention(q, k, v, g, 2)[0], ops.decay_linear_attention(q, k, v, g, 2.0)[0])
+
+
+def test_entries_whose_rows_overlap_are_refused_before_any_launch():
+    """Host checks (the pointers are never followed): two batch entries of an output or of a cache that are less than a row apart."""
+    lib, P, bf16 = _lib.load(), 0x10000, _lib.DT_BF16
+    ARG = -1
+    decay = lambda o_b, B=2: lib.sana_hip_decay_attention(P, P, P, P, None, P, P + 4, None, None, 0, B, 8, 3, 32, *[8 * 96, 96] * 3, o_b, 96,  # noqa: E731
+                                                         1.0, bf16, None)
+    assert decay(88) == ARG and decay(96) == -3 and decay(0, 1) == -3   # (-3: an output of 4-byte alignment, found behind this)
+    window = lambda o_b: lib.sana_hip_window_attention(P, P, P, P, None, None, 0, 2, 8, 8, 4, 2, 32, 5, 0, *[8 * 128, 128] * 3, o_b, 128, 0.1,  # noqa: E731
+                                                       bf16, None)
+    assert window(120) == ARG and window(0) == ARG
+    step = lambda ck=20 * 64, cv=20 * 64, o=128: lib.sana_hip_window_step(P, P, P, P, P, P, P, None, 0, 2, 4, 2, 32, 20, 0, 128, 64, 64, ck, 64, cv, 64,  # noqa: E731
+                                                                          o, 0.1, bf16, None)
+    assert step(o=120) == ARG and step(ck=56) == ARG and step(cv=56) == ARG
+    put = lambda ck, cv: lib.sana_hip_window_cache_append(P, P, P, P, P, None, 2, 8, 64, 20, 0, ck, 64, cv, 64, 512, 64, 512, 64, bf16, None)  # noqa: E731
+    assert put(56, 20 * 64) == ARG and put(20 * 64, 56) == ARG
