@@ -604,7 +604,7 @@ using namespace sana;
 #define SANA_API extern "C" __attribute__((visibility("default")))
 
 SANA_API size_t sana_hip_decay_attention_workspace_bytes(int B, int N, int H, int d) {
-  if (B <= 0 || N <= 1 || H <= 0 || d <= 0 || d > 128 || (int64_t)B * H >= (1 << 24)) return 0;
+  if (B <= 0 || N <= 1 || N > (1 << 30) || H <= 0 || d <= 0 || d > 128 || (int64_t)B * H >= (1 << 24)) return 0;
   int tokens;
   const int nseg = segment_count(B, N, H, d, &tokens);
   return nseg > 1 ? (size_t)B * H * nseg * d * d * sizeof(float) : 0;

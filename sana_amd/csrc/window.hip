@@ -571,6 +571,10 @@ __global__ __launch_bounds__(256) void window_append_kernel(const WindowArgs a) 
 
 constexpr int WA_NW = 4;
 constexpr int64_t WA_MAX_BLOCKS = 1 << 24;  // of 256 threads: a launch has fewer than 2^32 threads an axis
+// What the rules below take without leaving 64 bits, and what a launch could take at most: a block for each (batch entry, head).
+bool prompt_fits(int B, int N, int Nk, int H, int d) {
+  return Nk <= (1 << 30) && N <= Nk && d <= 128 && (int64_t)B * H <= WA_MAX_BLOCKS - 8;
+}
 // 16-query tiles of a wave, 64 or 128 queries a workgroup.  Two feed twice the MFMAs with a read of K or V and pay where heads are wide
 // and the blocks many; one gives more and shorter workgroups, and up to 96 channels three and more waves a SIMD.  us, two / one, window 4096:
 // 20 heads of 112 1500 tokens 38 / 30, 2000 59 / 48, 2560 66 / 66, 3000 70 / 88, 8000 294 / 351; 16 of 128 3000 70 / 60, 4680 123 / 122, 8000 231 / 261;
@@ -637,7 +641,6 @@ int launch_prompt(WindowArgs a, hipStream_t s) {
 template <typename T, int DK, int DT>
 int launch_step(const WindowArgs& a, hipStream_t s) {
   const int64_t groups = step_groups(a.B, a.H, a.Hkv);
-  if (groups >= WA_MAX_BLOCKS) return SANA_ERR_SHAPE;
   // (eight waves where a cache is not split and the chip has room for them: 20 key heads of 112 x 772 rows 13.7 us, four 15.3; 320 x 516 29.8 / 28.3)
   if (a.splits == 1 && groups <= 256)
     hipLaunchKernelGGL((window_step_kernel<T, DK, DT, 8>), dim3((unsigned)groups), dim3(512), 0, s, a);
@@ -688,12 +691,12 @@ using namespace sana;
 #define SANA_API extern "C" __attribute__((visibility("default")))
 
 SANA_API size_t sana_hip_window_attention_workspace_bytes(int B, int N, int Nk, int H, int d, int window, int sinks) {
-  if (B <= 0 || N <= 0 || Nk < N || H <= 0 || d <= 0 || window <= 0 || sinks < 0) return 0;
+  if (B <= 0 || N <= 0 || H <= 0 || d <= 0 || window <= 0 || sinks < 0 || !prompt_fits(B, N, Nk, H, d)) return 0;
   return part_bytes(prompt_splits(B, N, Nk, H, d, window, sinks), (int64_t)B * N * H, d);
 }
 
 SANA_API int sana_hip_window_attention_query_tiles(int B, int N, int H, int d) {
-  return B <= 0 || N <= 0 || H <= 0 || d <= 0 || d > 128 ? 0 : query_tiles(B, N, H, d);
+  return B <= 0 || N <= 0 || H <= 0 || d <= 0 || !prompt_fits(B, N, N, H, d) ? 0 : query_tiles(B, N, H, d);
 }
 
 SANA_API int sana_hip_window_attention(const void* q, const void* k, const void* v, void* out, const int32_t* lengths, void* workspace,
@@ -704,7 +707,7 @@ SANA_API int sana_hip_window_attention(const void* q, const void* k, const void*
   if (!q || !k || !v || !out || Nk < N || !(scale > 0.f && scale * 1.44269504088896341f < INFINITY)) return SANA_ERR_ARG;
   const int rc = check_sizes(B, N, H, Hkv, d, window, sinks, io_dtype);
   if (rc != SANA_OK) return rc;
-  if (Nk > (1 << 30)) return SANA_ERR_SHAPE;
+  if (!prompt_fits(B, N, Nk, H, d)) return SANA_ERR_SHAPE;
   if (q_stride_n < (int64_t)H * d || o_stride_n < (int64_t)H * d || k_stride_n < (int64_t)Hkv * d || v_stride_n < (int64_t)Hkv * d)
     return SANA_ERR_ARG;
   for (const int64_t sb : {q_stride_b, k_stride_b, v_stride_b, o_stride_b})
@@ -761,7 +764,8 @@ SANA_API int sana_hip_window_cache_append(void* cache_k, void* cache_v, const vo
 }
 
 SANA_API size_t sana_hip_window_step_workspace_bytes(int B, int H, int Hkv, int d, int window, int sinks) {
-  if (B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || d <= 0 || window <= 0 || sinks < 0 || (int64_t)window + sinks > (1 << 30)) return 0;
+  if (B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || d <= 0 || d > 128 || window <= 0 || sinks < 0 || (int64_t)window + sinks > (1 << 30)) return 0;
+  if (step_groups(B, H, Hkv) >= WA_MAX_BLOCKS) return 0;
   return part_bytes(step_splits(B, H, Hkv, window + sinks, d), (int64_t)B * H, d);
 }
 
@@ -778,7 +782,7 @@ SANA_API int sana_hip_window_step(const void* q, const void* k, const void* v, v
   for (const int64_t sb : {q_stride_b, k_stride_b, v_stride_b, ck_stride_b, cv_stride_b, o_stride_b})
     if (sb < 0) return SANA_ERR_ARG;
   if (B > 1 && (o_stride_b < (int64_t)H * d || ck_stride_b < C || cv_stride_b < C)) return SANA_ERR_ARG;  // (streams that would write the same elements)
-  if ((int64_t)window + sinks > (1 << 30)) return SANA_ERR_SHAPE;
+  if ((int64_t)window + sinks > (1 << 30) || step_groups(B, H, Hkv) >= WA_MAX_BLOCKS) return SANA_ERR_SHAPE;
   if (misaligned({q, k, v, cache_k, cache_v}, {q_stride_b, k_stride_b, v_stride_b, ck_stride_b, ck_stride_n, cv_stride_b, cv_stride_n}) ||
       (reinterpret_cast<uintptr_t>(out) & 7u) || o_stride_b % 4 || off4(positions))
     return SANA_ERR_ALIGN;

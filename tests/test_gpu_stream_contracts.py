@@ -1,4 +1,8 @@
 """What the streams' calls refuse, and what they take in the place of a number."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -67,3 +71,32 @@ def test_entries_whose_rows_overlap_are_refused_before_any_launch():
     assert step(o=120) == ARG and step(ck=56) == ARG and step(cv=56) == ARG
     put = lambda ck, cv: lib.sana_hip_window_cache_append(P, P, P, P, P, None, 2, 8, 64, 20, 0, ck, 64, cv, 64, 512, 64, 512, 64, bf16, None)  # noqa: E731
     assert put(56, 20 * 64) == ARG and put(20 * 64, 56) == ARG
+
+
+HUGE = """
+import sys
+sys.path.insert(0, sys.argv[1])
+from sana_amd import _lib
+lib, P, bf16 = _lib.load(), 0x10000, _lib.DT_BF16
+M = 2 ** 31 - 1
+# batches x heads x blocks of queries that pass 2^63, to the multiples of 2^64 that a product in 64 bits calls 0
+assert lib.sana_hip_window_attention_workspace_bytes(1 << 30, 1024, 2048, 1 << 30, 8, 4000, 0) == 0
+assert lib.sana_hip_window_attention_workspace_bytes(1 << 30, 1 << 22, 1 << 22, 1 << 18, 8, 4000, 0) == 0
+assert lib.sana_hip_window_attention_query_tiles(1 << 30, 1024, 1 << 30, 8) == 0
+assert lib.sana_hip_window_attention(P, P, P, P, None, None, 0, 1 << 30, 1 << 22, 1 << 22, 1 << 18, 1 << 18, 8, 4000, 0, *[1 << 43, 1 << 21] * 4, 0.1, bf16, None) == -2
+# counts next to the type's end
+for f, n in ((lib.sana_hip_window_attention_workspace_bytes, 7), (lib.sana_hip_window_step_workspace_bytes, 6),
+             (lib.sana_hip_decay_attention_workspace_bytes, 4)):
+    assert f(*[M] * n) == 0
+assert lib.sana_hip_window_attention_query_tiles(1, M, 1, 8) == 0 and lib.sana_hip_window_attention_workspace_bytes(1, M, M, 1, 8, M, 0) == 0
+assert lib.sana_hip_decay_attention_workspace_bytes(1, M, 1, 8) == 0
+assert lib.sana_hip_window_step_workspace_bytes(M, M, M, M, 1 << 29, 1 << 29) == 0
+print("whole")
+"""
+
+
+def test_sizes_beyond_all_memory_end_no_process():
+    """(In a process of its own: a division by a wrapped product of 0 ends it.)"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", HUGE, root], capture_output=True, text=True, timeout=100)
+    assert run.returncode == 0 and run.stdout.strip().endswith("whole"), (run.returncode, run.stderr[-400:])
