@@ -273,7 +273,18 @@ __global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) 
           for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
             for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(st[vt][kt][r]));
-        sfit = dc_fit(max_wave(most));
+        most = max_wave(most);
+        if (__builtin_expect(most == INFINITY, 0)) {  // (a carried inf: the other channels go in by their own maximum)
+          most = 0.f;
+#pragma unroll
+          for (int vt = 0; vt < VT; ++vt)
+#pragma unroll
+            for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(st[vt][kt][r]) < INFINITY ? fabsf(st[vt][kt][r]) : 0.f);
+          most = max_wave(most);
+        }
+        sfit = dc_fit(most);
       }
 #pragma unroll
       for (int vt = 0; vt < VT; ++vt)

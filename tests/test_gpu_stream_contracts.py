@@ -10,6 +10,7 @@ from torch.autograd import forward_ad
 
 import sana_amd
 from sana_amd import _lib, ops
+from test_gpu_decay_attention import check, definition, make
 
 gpu = pytest.mark.gpu
 BF16 = torch.bfloat16
@@ -100,3 +101,29 @@ def test_sizes_beyond_all_memory_end_no_process():
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     run = subprocess.run([sys.executable, "-c", HUGE, root], capture_output=True, text=True, timeout=100)
     assert run.returncode == 0 and run.stdout.strip().endswith("whole"), (run.returncode, run.stderr[-400:])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, torch.float16])
+@pytest.mark.parametrize("N,H,d", [(1, 3, 64), (100, 3, 32), (150, 3, 64), (90, 3, 112), (1500, 2, 112)])
+@pytest.mark.parametrize("size", [1e7, 1e-4])
+def test_a_carried_inf_stays_in_its_channel(cuda, N, H, d, dtype, size):
+    """An inf of the state in front: its channel is not finite, all others are what they are without it, f16 states beyond and far below the type's
+    range among them (the power of two that takes a wave's states there must not come from the inf)."""
+    q, k, v, log_decay, state = make(1, N, H, d, dtype, carried=True)
+    q, v, state, scale = q * 1e-3, (v * 3e-5 * size).to(dtype), state * size, 1e3 / size
+    state[0, 0, 5, 7], state[0, H - 1, d - 2, 0] = float("inf"), -float("inf")
+    clean = torch.where(torch.isfinite(state), state, torch.zeros_like(state))
+    odd, odd_state = torch.zeros(1, N, H, d, dtype=torch.bool), torch.zeros(1, H, d, d, dtype=torch.bool)
+    for h, c in ((0, 5), (H - 1, d - 2)):
+        odd[0, :, h, c], odd_state[0, h, c] = True, True
+    want = definition(q, k, v, log_decay, scale, clean, None)
+    out, last = ops.decay_linear_attention(q.cuda(), k.cuda(), v.cuda(), log_decay.cuda(), scale, state.cuda())
+    out, last = out.double().cpu(), last.double().cpu()
+    odd = odd.reshape(1, N, H * d)
+    assert not torch.isfinite(out[0, 0][odd[0, 0]]).any()
+    # A state whose terms sum to less than fp32's smallest normal number, 2^-126, has no half step relative to itself: 0.5^150 * 1e-4 of the first head
+    # is 7e-50 where fp32 ends at 1.4e-45, so it is off by itself; by 2^-126 at most.
+    small = want[3] < 2.0 ** -126
+    assert ((last - want[1]).abs() <= 2.0 ** -126)[small & ~odd_state].all()
+    check((torch.where(odd, want[0], out), torch.where(odd_state | small, want[1], last)), want, q, N)
