@@ -502,9 +502,12 @@ int sana_hip_block(const sana_block_args* args, void* stream);
  *                 neither read nor written, and a stream of 0 tokens keeps its state
  *   workspace     at least sana_hip_decay_attention_workspace_bytes(...) bytes, 16-byte aligned (NULL where that is 0)
  * d % 8 == 0, d <= 128; B * H < 2^24 and, for N > 1, B * ceil(H / 4) <= 2^22 - 8; q, k, v and the states 16-byte aligned, out 8; token
- * strides from H*d to 2^23 - 1.  The state is summed in fp32 in a fixed order.  out must not overlap q, k or v.  A value of inf or
- * NaN leaves its channel (of outputs and state) inf or NaN from its token on, a key of them its head's outputs; nothing in front
- * of it changes.
+ * strides from H*d to 2^23 - 1, batch strides of out at least H*d for B > 1.  The state is summed in fp32 in a fixed order.  For N > 1
+ * one operand of each product of an output is rounded to the io dtype once: the state where it meets q, q . k (with its decay) where it meets
+ * v; against 64 bits outputs are off by 1.4 times the rounding of the result alone.  out must not overlap q, k or v, nor its entries
+ * each other.  A value of inf or
+ * NaN (or a state's, in state_in) leaves its channel (of outputs and state) inf or NaN from its token on, a key of them its head's outputs;
+ * nothing in front of it changes.
  */
 size_t sana_hip_decay_attention_workspace_bytes(int B, int N, int H, int d);
 int sana_hip_decay_attention(const void* q, const void* k, const void* v, const float* log_decay, const float* state_in,
@@ -524,9 +527,12 @@ int sana_hip_decay_attention(const void* q, const void* k, const void* v, const 
  *           what lies behind is neither read nor written
  *   workspace  at least sana_hip_window_attention_workspace_bytes(...) bytes, 16-byte aligned (NULL where that is 0): few queries
  *           of many keys are split over the keys
- * scale > 0; window >= 1; d % 8 == 0, d <= 128; q, k, v 16-byte aligned, out 8; token strides of k and v below 2^23.
+ * scale > 0; window >= 1; d % 8 == 0, d <= 128; q, k, v 16-byte aligned, out 8; token strides of each at least the width of its rows
+ * (H*d, Hkv*d), those of k and v below 2^23; batch strides of out at least H*d for B > 1.
+ * Nk, window and sinks at most 2^30, H*d at most 2^22, and B * H * ceil(N / queries of a workgroup) * parts at most 2^24 - 8, else
+ * SANA_ERR_SHAPE: 64 or 128 queries (below), parts 1 where there are 256 workgroups and more without them.
  * Probabilities are rounded to the io dtype before they multiply v; maxima, sums and outputs are fp32.  A key or a value of
- * inf or NaN reaches the queries that see it, and no others.
+ * inf or NaN reaches the queries that see it, and no others.  out must not overlap q, k or v, nor its entries each other.
  */
 size_t sana_hip_window_attention_workspace_bytes(int B, int N, int Nk, int H, int d, int window, int sinks);
 /* The tiles of 16 queries that a wave takes (1 or 2: 64 or 128 queries a workgroup): a query for tests and measurements. */
@@ -541,7 +547,10 @@ int sana_hip_window_attention(const void* q, const void* k, const void* v, void*
  * row sinks + (p - sinks) % window.  Appends N new tokens (lengths[b] of them) at positions[b], positions[b] + 1, ...
  *   cache_k, cache_v [B][sinks + window][C], k, v [B][N][C] views, 16-bit; C % 8 == 0, all 16-byte aligned; B <= 65535
  *   positions int32 [B]: tokens that the stream has seen before; negative: an idle stream, nothing is written
- * Rows of positions that hold no token yet, and tokens that later ones of the call push out, are not written. */
+ * window + sinks at most 2^30, N * C / 2048 below 2^24; strides of tokens, and of the caches' entries for B > 1, at least C.  Caches must
+ * not overlap k or v, nor their entries each other.
+ * Rows of positions that hold no token yet, and tokens that later ones of the call push out, are not written.  A call of many queries over such
+ * a cache does not exist: sana_hip_window_attention reads rows in the order of their tokens. */
 int sana_hip_window_cache_append(void* cache_k, void* cache_v, const void* k, const void* v, const int32_t* positions,
                                  const int32_t* lengths, int B, int N, int C, int window, int sinks, int64_t ck_stride_b,
                                  int64_t ck_stride_n, int64_t cv_stride_b, int64_t cv_stride_n, int64_t k_stride_b,
@@ -549,7 +558,8 @@ int sana_hip_window_cache_append(void* cache_k, void* cache_v, const void* k, co
 
 /* One token of each stream: its key and value go into the cache as above (position positions[b]), and its queries attend to
  * what the cache then holds.  q, out [B][H*d] rows, k, v [B][Hkv*d] rows; an idle stream (negative position) gets zeros and its
- * cache is left alone.  Workspace, types and alignment as in sana_hip_window_attention. */
+ * cache is left alone.  Workspace, types, roundings and alignment as in sana_hip_window_attention; window + sinks at most 2^30, H*d at most 2^22,
+ * B * Hkv * ceil(H / Hkv / 16) below 2^24; for B > 1 batch strides of out at least H*d, of the caches at least Hkv*d. */
 size_t sana_hip_window_step_workspace_bytes(int B, int H, int Hkv, int d, int window, int sinks);
 int sana_hip_window_step(const void* q, const void* k, const void* v, void* cache_k, void* cache_v, const int32_t* positions,
                          void* out, void* workspace, size_t workspace_bytes, int B, int H, int Hkv, int d, int window,

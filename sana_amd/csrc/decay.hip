@@ -58,14 +58,16 @@ enum { DC_SUMS, DC_OUT, DC_WHOLE };
 // Roundings.  Each product of the output has one operand of 16 bits that is rounded, P or S, as attention kernels round P: with the rounding of
 // the result the error is 1.4 times that of the result's rounding alone.  The weighted values a^(C-1-j) v_j enter the state as a sum of
 // 16-bit values: three of bf16 where the state is given back (fp32's accuracy; with two it is 1.3e-6 off after 32760
-// tokens), two of bf16 where it only goes on to outputs, two of f16 (22 bits), the second times 2^11, so that it stays a normal number.
+// tokens), two of bf16 where it only goes on to outputs, two of f16, the second times 2^11 (22 bits from 2^-14 on; smaller values end at 2^-36, as f16
+// values themselves end at 2^-25).
 // f16 ends at 65504: S goes in scaled by a power of two for each wave, P for each query.
 // A value that is not finite must not reach the queries in front of it (0 * inf): it is staged as 0, and its channel is set to NaN from its
 // token on.
-// What bounds it: where all compute units work, memory (32760 tokens x 20 heads of 112, 25 segments: sums 78 us = 318 MB at 4.1 TB/s, outputs 155 us =
-// 563 MB at 3.6 TB/s; rows of 224 bytes come at 3.8 - 4.1 TB/s to any kernel here); few chunks, the chain of a chunk's steps, some 2 us
+// What bounds it: where all compute units work, memory (32760 tokens x 20 heads of 112, 25 segments, rows of 224 bytes: sums 80 us = 318 MB at 4.0 TB/s;
+// outputs 159 us = 612 MB at 3.8 TB/s, of which their loads and stores alone take 132, 4.6 TB/s) and, for the rest, the chain of a chunk's steps;
+// few chunks, that chain alone, some 2 us
 // (32 channels) to 4 us (112) each: three barriers, each with the LDS and MFMA latencies in front of it (300 tokens x 70 heads of 32: five
-// chunks, 12 us).  Two chunks requested ahead, three workgroups a compute unit and eight waves a workgroup were no faster.
+// chunks, 12 us; 2 x 4680 tokens, one stream half as long: outputs 48 us, their loads and stores alone 36).  Two chunks requested ahead, three workgroups a compute unit and eight waves a workgroup were no faster.
 template <typename T, int DK, int KT, int VT, int NV, int MODE>
 __global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) {
   constexpr bool OUT = MODE != DC_SUMS, F = is_f16<T>;
@@ -274,7 +276,7 @@ __global__ __launch_bounds__(256, 2) void decay_chunk_kernel(const DecayArgs a) 
 #pragma unroll
             for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(st[vt][kt][r]));
         most = max_wave(most);
-        if (__builtin_expect(most == INFINITY, 0)) {  // (a carried inf: the other channels go in by their own maximum)
+        if (__builtin_expect(most == INFINITY, 0)) {  // (a carried inf: the other channels go in by their own maximum.  1 - 1.5 % of an f16 call)
           most = 0.f;
 #pragma unroll
           for (int vt = 0; vt < VT; ++vt)

@@ -6,8 +6,9 @@ namespace sana {
 
 typedef __attribute__((address_space(3))) unsigned char lds_t;  // (pointers, not integers: the compiler sees which array is read)
 
-// 16-byte slots of an LDS row of DK * 64 bytes are exchanged by a key of the row: 16 consecutive rows of one slot, and the 16 rows of a
-// transposing read, cover all banks.  The key of row 16 i + r is that of r.
+// 16-byte slots of an LDS row of DK * 64 bytes are exchanged by a key of the row, which spreads 16 consecutive rows of one slot over the banks.
+// The key of row 16 i + r is that of r.  LDS cycles of a wave's instruction, by the counters: a plain read of 16 rows 4 without conflicts for DK = 2 and
+// 4, 8 of which 4 are conflicts for DK = 1 and 3 (two bits of key); a transposing read 4 of which 2 are conflicts at every DK; a 16-byte write 8, none.
 template <int DK>
 __device__ __forceinline__ int row_key(int row) {
   return DK == 4 ? (row & 15) : DK == 2 ? ((row >> 1) & 7) : ((row >> 2) & 3);

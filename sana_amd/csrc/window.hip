@@ -35,8 +35,9 @@ template <typename T> inline constexpr float kShift = is_f16<T> ? 6.f : 0.f;
 // the order of keys that this gives.  The running maximum moves only when some score is 2^8 above it: until then p <= 2^8 and nothing is
 // rescaled (the 16-bit p keeps its relative step, l and o are fp32).  f16: p times 2^6, the small ones away from its subnormal numbers.
 // Of a tile of 64 keys x 32 queries x 112 channels the matrix pipe takes 960 cycles, the vector unit some 1000 (half of them powers) and
-// the LDS 350 for each of four waves: with two waves a SIMD 16384 tokens x 20 heads over a window of 4096 run at 0.84 PFLOP/s (633 us), f16 with
-// shared key heads at 0.86.  Through registers instead of direct loads 705 us; each tile's scores in front of its own powers instead of those of the tile
+// the LDS 350 for each of four waves.  The time is the sum of the first two: the matrix pipes work 48 % of it (counters), the two waves of a SIMD, which come
+// from workgroups of no relation in phase, do not overlap.  16384 tokens x 20 heads over a window of 4096 run at 0.84 - 0.88 PFLOP/s (633 - 606 us), f16 with
+// shared key heads at 0.86 - 0.90.  Through registers instead of direct loads 705 us; each tile's scores in front of its own powers instead of those of the tile
 // before: 630 - 690, by how the compiler mixes them; each operand read from LDS where it is used instead of an MFMA group ahead, and the
 // maxima in front of the powers instead of beside the values' MFMAs: 653; where in a tile the rest of the vector work stands, wave priorities
 // and reads further ahead change it by less than 0.5 %; three or four query tiles a wave: the registers do not hold them.
@@ -578,8 +579,10 @@ bool prompt_fits(int B, int N, int Nk, int H, int d) {
 // 16-query tiles of a wave, 64 or 128 queries a workgroup.  Two feed twice the MFMAs with a read of K or V and pay where heads are wide
 // and the blocks many; one gives more and shorter workgroups, and up to 96 channels three and more waves a SIMD.  us, two / one, window 4096:
 // 20 heads of 112 1500 tokens 38 / 30, 2000 59 / 48, 2560 66 / 66, 3000 70 / 88, 8000 294 / 351; 16 of 128 3000 70 / 60, 4680 123 / 122, 8000 231 / 261;
-// window 256: 20 of 112 16384 136 / 143.  Narrower heads (two tiles as they were when reads and products still took turns): 16 of 72 1500
-// 34.4 / 26.5, 4680 109 / 100, 8000 193 / 204, 12 of 96 8000 193 / 187, 35 of 64 8000 325 / 316; window 256: 35 of 64 8000 72 / 56, 12 of 96 8000 38 / 31.
+// window 256: 20 of 112 16384 136 / 143.  Narrower heads have one: 70 of 32 3000 108 / 94, 8000 388 / 400; 35 of 64 3000 89 / 74, 8000 312 / 305,
+// 16384 657 / 676; 16 of 72 3000 55 / 51, 8000 175 / 185; 12 of 96 4680 99 / 86, 8000 182 / 184; window 256: 70 of 32 8000 91 / 81, 35 of 64 8000
+// 74 / 60, 16 of 72 8000 42 / 38, 12 of 96 8000 39 / 31.  (From 72 channels on, long prompts over a long window would be faster by two, which are not
+// built for them: 2 x 16384 of 16 of 72 732 / 872, 16384 of 12 of 96 316 / 373, 8000 of 20 of 80 232 / 261.)
 int query_tiles(int B, int N, int H, int d) { return d <= 96 || (int64_t)B * H * ((N + 127) / 128) <= 400 ? 1 : 2; }
 // Parts of a prompt's keys: where the blocks of queries leave compute units idle and have tiles of keys enough to pay for a second launch
 // (600 tokens, 20 heads of 112, ten tiles: whole 13.9 us, in two parts over 20; 128 of 1128 keys 22.7 / 17.0 (four parts), 300 of 4300 67 / 32 (five), 1 of

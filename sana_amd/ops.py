@@ -939,7 +939,8 @@ def decay_linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lo
     it is a new tensor.  ``lengths``: int32 [B] on the device, the tokens that each batch entry really has (clamped to 0 .. N);
     rows behind them are not read, and stay in ``out`` as they were (zeros in a new one); an entry without tokens
     keeps its state.  A value of inf or NaN leaves its channel inf or NaN from its token on, and nothing in front of it; a key, its
-    head.  ``out`` must not overlap the inputs.  Forward only."""
+    head.  Of many tokens, one operand of each product of an output (the state, the scores) is rounded to the inputs' dtype once; the state
+    itself stays fp32.  ``out`` must not overlap the inputs, nor its entries each other.  Forward only."""
     dev = _here((q, k, v, log_decay, state, lengths, out, state_out), "decay_linear_attention")
     if dev != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
@@ -1014,7 +1015,9 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, num_head
     what is kept, k and v hold the sinks and then, in order, at least the last window - 1 tokens in front of the queries.
     ``lengths``: int32 [B] on the device, the queries that each batch entry really has (clamped to 0 .. N; its keys end with its
     last query); rows behind them are not read, and stay in ``out`` as they were (zeros in a new one).
-    What a query does not see does not reach it, inf and NaN included.  Returns [B, N, H*d].  ``out`` must not overlap the inputs.
+    What a query does not see does not reach it, inf and NaN included.  Probabilities are rounded to the inputs' dtype before they
+    multiply v.  Returns [B, N, H*d].  ``out`` must not overlap the inputs, nor its entries each other.  k and v are rows in order: a cache of
+    :func:`window_cache_append_` that has wrapped is read by single tokens alone (:func:`window_attention_step_`).
     Forward only."""
     dev = _here((q, k, v, lengths, out), "window_attention")
     if dev != torch._C._cuda_getDevice():
