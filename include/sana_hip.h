@@ -567,6 +567,69 @@ int sana_hip_window_step(const void* q, const void* k, const void* v, void* cach
                          int64_t ck_stride_n, int64_t cv_stride_b, int64_t cv_stride_n, int64_t o_stride_b, float scale,
                          int io_dtype, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * The heads of a stream's queries and keys between their projection and the attention, and its cache in 8 bits; one pass:
+ *
+ *   norm      x' = x * rsqrt(mean(x^2) + eps) * weight over the d channels of a head (q_weight, k_weight [d], both or neither: no norm)
+ *   rotation  of channel pairs by position * freqs[i] radians, the first `rotary` channels of each head:
+ *             (a, b) -> magnitude * (a cos - b sin, a sin + b cos); pairs (2i, 2i + 1) (interleaved), else (i, i + rotary / 2)
+ *   cache     keys (normed and rotated) and values in 8 bits into the rows of a ring cache
+ *
+ * The per-head form of the q/k RMSNorm and the rotary embedding that the reference's attention classes apply one after the other
+ * (diffusion/model/nets/sana_blocks.py:88-92, :1572-1582).  In 32 bits, angles in 64, rounded once; into the cache from the unrounded key.
+ *   q, q_out  [B][N][H*d] views (NULL and H = 0: keys alone), k, v, k_out [B][N][Hkv*d] views, bf16 or f16, each its own strides (batch, token);
+ *             q_out may be q itself and k_out k (with its strides), else they must not overlap the inputs
+ *   k_out     may be NULL where there is a cache
+ *   weights   of the io dtype;  freqs  fp64 [rotary / 2] (any scaling for long contexts is in them)
+ *   positions int32 [B] or NULL (zeros): the position of each entry's first token; negative: an idle stream
+ *   lengths   int32 [B] or NULL: entry b has lengths[b] tokens (clamped to 0 .. N)
+ *             Rows of q_out and k_out without a token stay as they were, or are zeroed (zero_rest: 1 q_out, 2 k_out, 3 both).
+ *   codes_k, codes_v  int8 [B] times dense [Hkv][sinks + window][d'], d' = d rounded up to a multiple of 16 (what is behind d is neither read
+ *             nor written), or NULL: no cache;  scales fp32 [B] times dense [Hkv][sinks + window][2], of a row's key and of its value.
+ *             A head's row x is c = round(127 x / max|x|), ties to even, with the scale max|x| / 127; one of inf or NaN has the scale NaN.
+ *             Which row a token goes into, and which tokens are not written, as in sana_hip_window_cache_append.
+ * d % 8 == 0, d <= 128; rotary % 8 == 0, rotary <= d; H*d and Hkv*d at most 2^22; window + sinks at most 2^30; rows 16-byte aligned, their
+ * strides multiples of 8; codes 16-byte aligned, ck_b and cv_b multiples of 16; scales 8-byte aligned, sc_b even; for B > 1 the entries of what
+ * is written must not overlap. */
+typedef struct sana_heads_args {
+  const void *q, *k, *v;
+  void *q_out, *k_out;
+  const void *q_weight, *k_weight;
+  const double* freqs;
+  const int32_t *positions, *lengths;
+  int8_t *codes_k, *codes_v;
+  float* scales;
+  int64_t q_b, q_n, k_b, k_n, v_b, v_n, qo_b, qo_n, ko_b, ko_n, ck_b, cv_b, sc_b;
+  int B, N, H, Hkv, d, rotary, interleaved, window, sinks, zero_rest, io_dtype;
+  float eps, magnitude;
+} sana_heads_args;
+int sana_hip_heads(const sana_heads_args* args, void* stream);
+
+/* One token of each stream over a cache of 8 bits that holds it already (sana_hip_heads, at the same positions):
+ *   out = sum_j softmax_j(scale * sk_j (q . ck_j)) sv_j cv_j   over the rows of the last `window` tokens up to positions[b] and of the sinks.
+ *   q, out  [B][H*d] rows, bf16 or f16; an idle stream (negative position) gets zeros
+ * Codes meet q exactly; probabilities (with their row's scale) enter the product as two bf16 each (2^-16), maxima, sums and outputs are fp32.
+ * Workspace, limits and alignment as in sana_hip_window_step and sana_hip_heads. */
+size_t sana_hip_window_q8_workspace_bytes(int B, int H, int Hkv, int d, int window, int sinks);
+int sana_hip_window_q8(const void* q, const int8_t* codes_k, const int8_t* codes_v, const float* scales, const int32_t* positions, void* out,
+                       void* workspace, size_t workspace_bytes, int B, int H, int Hkv, int d, int window, int sinks, int64_t q_stride_b,
+                       int64_t o_stride_b, int64_t ck_stride_b, int64_t cv_stride_b, int64_t scales_stride_b, float scale, int io_dtype,
+                       void* stream);
+
+/* A cache's rows in the order of their tokens, as sana_hip_window_attention takes them: of a stream that has seen n = positions[b] tokens the
+ * tokens 0 .. n - 1 where n <= sinks + last, else 0 .. sinks - 1 and n - last .. n - 1; rows behind them stay as they were, or are
+ * zeroed (zero_rest).
+ *   cache_k, cache_v  16-bit rows as in sana_hip_window_cache_append (scales NULL; strides in elements: batch, row), or the codes of
+ *         sana_hip_heads (scales given; ck_stride_n, cv_stride_n unused)
+ *   out_k, out_v  [B][sinks + last][Hkv*d] views of the io dtype; last at most window, sinks + last at least 1
+ * d % 8 == 0, for codes d <= 128; Hkv*d at most 2^22; window + sinks at most 2^30; B * (sinks + last) below 2^25 for 16-bit rows,
+ * B * Hkv * ceil((sinks + last) / 16) for codes; rows 16-byte aligned, their strides multiples of 8.  The outputs must not overlap the caches,
+ * nor their entries each other. */
+int sana_hip_window_cache_read(const void* cache_k, const void* cache_v, const float* scales, const int32_t* positions, void* out_k, void* out_v,
+                               int B, int Hkv, int d, int window, int sinks, int last, int64_t ck_stride_b, int64_t ck_stride_n,
+                               int64_t cv_stride_b, int64_t cv_stride_n, int64_t scales_stride_b, int64_t ok_stride_b, int64_t ok_stride_n,
+                               int64_t ov_stride_b, int64_t ov_stride_n, int zero_rest, int io_dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -34,6 +34,10 @@ BLOCK_ARGS = struct.Struct("@" + "".join({c_void_p: "P", c_size_t: "N", c_int64:
                                          for _, t in BlockArgs._fields_) + "0q")
 assert BLOCK_ARGS.size == ctypes.sizeof(BlockArgs)
 
+# ``sana_heads_args`` of include/sana_hip.h, its fields in order: 13 pointers, 13 strides, 11 numbers, eps and the rotation's magnitude.  What it
+# packs is handed over as it is (a call spends a microsecond on it, three on a ctypes structure).
+HEADS_ARGS = struct.Struct("@13P13q11i2f0q")
+
 # name -> (restype, argtypes); must list every symbol include/sana_hip.h declares
 SIGNATURES = {
     "sana_hip_abi_version": (c_int, []),
@@ -123,6 +127,14 @@ SIGNATURES = {
     "sana_hip_window_step": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
                                      c_int, c_int, c_int, c_int, c_int, c_int, c_int64, c_int64, c_int64, c_int64, c_int64,
                                      c_int64, c_int64, c_int64, c_float, c_int, c_void_p]),
+    "sana_hip_heads": (c_int, [c_void_p, c_void_p]),
+    "sana_hip_window_q8_workspace_bytes": (c_size_t, [c_int] * 6),
+    "sana_hip_window_q8": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
+                                   c_int, c_int, c_int, c_int, c_int, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_float,
+                                   c_int, c_void_p]),
+    "sana_hip_window_cache_read": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
+                                           c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,
+                                           c_int, c_int, c_void_p]),
     "sana_hip_layernorm_modulate": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int,
                                             c_int64, c_int64, c_int, c_int64, c_float, c_int, c_void_p]),
 }

@@ -1,0 +1,259 @@
+// What happens to a stream's heads between their projection and the attention, in one pass over the rows:
+//
+//   norm      x' = x * rsqrt(mean(x^2) + eps) * w over the d channels of a head, queries and keys each their weights
+//   rotation  of channel pairs (a, b) by t = position * freqs[i], the first 2 * |freqs| channels of the head:
+//             (a, b) -> m * (a cos t - b sin t, a sin t + b cos t); pairs (2i, 2i + 1), or (i, i + rotary / 2)
+//   8 bits    a head's row of a key or a value as whole numbers c = round(127 x / max|x|), ties to even, and the scale max|x| / 127
+//
+// all in 32 bits and rounded once, from the unrounded values where a key is rotated and put into 8 bits in the same pass.
+#include "window_common.h"
+
+namespace sana {
+namespace {
+
+struct HeadArgs {
+  sana_heads_args a;
+  int gq, gk, gv, per, chunks;  // groups of heads of a token: of queries, of keys, of values; groups a wave takes; waves a token
+  int64_t items;                // workgroups with work
+  float inv_d;
+};
+
+// Combined over the LPH (4, 8, 16) lanes that hold a head: exchanges within 16 lanes on the vector unit.
+template <int LPH, typename V, typename Op>
+__device__ __forceinline__ V over_head(V x, Op op) {
+  const auto with = [&](V y, auto ctrl) {
+    return op(y, __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, y), decltype(ctrl)::value, 0xf, 0xf, false)));
+  };
+  x = with(x, std::integral_constant<int, 0xB1>{});   // lane ^ 1
+  x = with(x, std::integral_constant<int, 0x4E>{});   // lane ^ 2
+  if constexpr (LPH >= 8) x = with(x, std::integral_constant<int, 0x141>{});   // 7 - lane: the other four
+  if constexpr (LPH >= 16) x = with(x, std::integral_constant<int, 0x140>{});  // 15 - lane: the other eight
+  return x;
+}
+
+// x in 8 bits: 127 x / most to the nearest whole number, ties to even; inv is 1 / most up to 2 steps.  The first quotient is mended by what it leaves
+// of 127 x (which is exact for 16-bit x): a tie, which fp32 holds, comes out as itself, and a quotient of two 16-bit floats that is none
+// is at least 2^-19 of itself away from one.  (5 operations in the place of a division's 10.)
+__device__ __forceinline__ uint32_t code_bits(float x, float most, float inv) {
+  const float t = 127.0f * x, y = t * inv;
+  return __float_as_uint(fmaf(fmaf(-y, most, t), inv, y) + 12582912.0f);  // 1.5 * 2^23: the whole number in the low bits
+}
+__device__ __forceinline__ uint32_t pack_codes(const float* x, float most, float inv) {
+  const uint32_t lo = __builtin_amdgcn_perm(code_bits(x[1], most, inv), code_bits(x[0], most, inv), 0x0c0c0400u);
+  const uint32_t hi = __builtin_amdgcn_perm(code_bits(x[3], most, inv), code_bits(x[2], most, inv), 0x04000c0cu);
+  return lo | hi;
+}
+
+// A wave takes one token and runs over `per` groups of 64 / LPH heads, U of them at a time; LPH lanes hold a head, 8 channels each.  FAR: pairs
+// half of the rotated channels apart, a lane holds four channels of either half, so a pair never leaves its lane.
+template <typename T, int LPH, bool FAR>
+__global__ __launch_bounds__(256) void heads_kernel(const HeadArgs h) {
+  constexpr int HPW = 64 / LPH, U = 4;
+  const sana_heads_args& a = h.a;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, j = lane % LPH, sub = lane / LPH;
+  const int64_t per_xcd = (h.items + 7) >> 3, item = (int64_t)(blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+  if ((int64_t)(blockIdx.x >> 3) >= per_xcd || item >= h.items) return;
+  // (uniform: scalars) workgroup -> (stream, four tokens, chunk of the heads)
+  const int blocks = (a.N + 3) / 4, chunk = (int)(item % h.chunks);
+  const int64_t rest = item / h.chunks;
+  const int b = (int)(rest / blocks), t = 4 * (int)(rest - (int64_t)b * blocks) + wave;
+  if (t >= a.N) return;
+  const int pos = a.positions ? a.positions[b] : 0;
+  const int n = a.lengths ? min(max(a.lengths[b], 0), a.N) : a.N;
+  const bool live = pos >= 0 && t < n;
+  if (!live && !a.zero_rest) return;
+  const uint32_t p = (uint32_t)pos + (uint32_t)t;
+  const bool kept = live && a.codes_k && (p < (uint32_t)a.sinks || t >= n - a.window);  // (not pushed out by this call's own tokens)
+  const int rows = a.window + a.sinks, slot = p < (uint32_t)a.sinks ? (int)p : a.sinks + (int)((p - (uint32_t)a.sinks) % (uint32_t)a.window);
+  const int d = a.d, dp = (d + 15) & ~15, eighths = a.rotary / 8;
+
+  // this lane's channels: two runs of four
+  const bool turns = j < eighths, far_pair = FAR && turns;
+  const int e0 = FAR ? (far_pair ? 4 * j : 8 * j) : 8 * j, e1 = far_pair ? a.rotary / 2 + 4 * j : e0 + 4;
+  const bool in = 8 * j < d;
+  float c[4], s[4];
+  if (live && turns) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      // in turns and 64 bits: of far positions only the fraction counts
+      const double at = (double)p * (a.freqs[4 * j + i] * 0.15915494309189533577);
+      const float f = (float)(at - __builtin_rint(at));
+      sincospif(2.0f * f, &s[i], &c[i]);
+      c[i] *= a.magnitude, s[i] *= a.magnitude;
+    }
+  }
+  const int g0 = chunk * h.per, g1 = min(g0 + h.per, h.gq + h.gk + h.gv);
+  const auto kind_of = [&](int g) { return g < h.gq ? 0 : g < h.gq + h.gk ? 1 : 2; };
+  const auto head_of = [&](int g, int kind) { return (g - (kind == 0 ? 0 : kind == 1 ? h.gq : h.gq + h.gk)) * HPW + sub; };
+  float w[2][8] = {};  // the norms' weights
+  if (a.q_weight && live && in) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint16_t* from = static_cast<const uint16_t*>(k ? a.k_weight : a.q_weight);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t bits = from[i < 4 ? e0 + i : e1 + i - 4];
+        w[k][i] = is_f16<T> ? f16_bits_to_f32(bits) : bf16_bits_to_f32(bits);
+      }
+    }
+  }
+  const uint16_t* in_rows[3] = {static_cast<const uint16_t*>(a.q) + b * a.q_b + t * a.q_n, static_cast<const uint16_t*>(a.k) + b * a.k_b + t * a.k_n,
+                                static_cast<const uint16_t*>(a.v) + b * a.v_b + t * a.v_n};
+  uint16_t* out_rows[2] = {static_cast<uint16_t*>(a.q_out) + b * a.qo_b + t * a.qo_n, static_cast<uint16_t*>(a.k_out) + b * a.ko_b + t * a.ko_n};
+
+  for (int g = g0; g < g1; g += U) {
+    u32x2_t x0[U], x1[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int gu = min(g + u, g1 - 1), kind = kind_of(gu), head = head_of(gu, kind), heads = kind == 0 ? a.H : a.Hkv;
+      const uint16_t* row = (kind == 0 ? in_rows[0] : kind == 1 ? in_rows[1] : in_rows[2]) + head * d;
+      x0[u] = x1[u] = u32x2_t{0u, 0u};
+      if (!live || !in || head >= heads) continue;
+      const bool near8 = !FAR || kind == 2;
+      if (near8) {
+        const u32x4_t x = *reinterpret_cast<const u32x4_t*>(row + 8 * j);
+        x0[u] = u32x2_t{x[0], x[1]}, x1[u] = u32x2_t{x[2], x[3]};
+      } else {
+        x0[u] = *reinterpret_cast<const u32x2_t*>(row + e0), x1[u] = *reinterpret_cast<const u32x2_t*>(row + e1);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int gu = g + u;
+      if (gu >= g1) break;
+      const int kind = kind_of(gu), head = head_of(gu, kind), heads = kind == 0 ? a.H : a.Hkv;
+      const bool mine = in && head < heads;
+      const bool near8 = !FAR || kind == 2;
+      const int at0 = near8 ? 8 * j : e0, at1 = near8 ? 8 * j + 4 : e1;
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t v = i < 2 ? x0[u][i] : x1[u][i - 2];
+        x[2 * i] = lo16<T>(v), x[2 * i + 1] = hi16<T>(v);
+      }
+      if (kind < 2 && a.q_weight) {
+        float sq = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sq = fmaf(x[i], x[i], sq);
+        sq = over_head<LPH>(sq, [](float y, float z) { return y + z; });
+        const float r = __builtin_amdgcn_rsqf(sq * h.inv_d + a.eps);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = x[i] * r * (kind ? w[1][i] : w[0][i]);
+      }
+      if (kind < 2 && turns) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int i0 = FAR ? i : 2 * i, i1 = FAR ? 4 + i : 2 * i + 1;
+          const float y = x[i0], z = x[i1];
+          x[i0] = y * c[i] - z * s[i], x[i1] = y * s[i] + z * c[i];
+        }
+      }
+      uint16_t* to = kind == 0 ? out_rows[0] : out_rows[1];
+      if (kind < 2 && (kind == 0 || a.k_out) && mine && (live || (a.zero_rest >> kind & 1))) {
+        const u32x4_t o = live ? u32x4_t{pk16<T>(x[0], x[1]), pk16<T>(x[2], x[3]), pk16<T>(x[4], x[5]), pk16<T>(x[6], x[7])} : u32x4_t{0u, 0u, 0u, 0u};
+        if (near8) {
+          *reinterpret_cast<u32x4_t*>(to + head * d + 8 * j) = o;
+        } else {
+          *reinterpret_cast<u32x2_t*>(to + head * d + e0) = u32x2_t{o[0], o[1]};
+          *reinterpret_cast<u32x2_t*>(to + head * d + e1) = u32x2_t{o[2], o[3]};
+        }
+      }
+      if (kind > 0 && kept) {
+        uint32_t most = 0;  // the largest magnitude, by its bits: NaN above inf
+#pragma unroll
+        for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
+        most = over_head<LPH>(most, [](uint32_t y, uint32_t z) { return max(y, z); });
+        const bool bad = most >= 0x7f800000u;
+        const float m = __uint_as_float(most);
+        // (far from 1 in the range of whole powers: a reciprocal that stays a normal number)
+        const float lift = m < 0x1p-100f ? 0x1p100f : m > 0x1p100f ? 0x1p-100f : 1.0f;
+        const float inv = m > 0.f && !bad ? __builtin_amdgcn_rcpf(m * lift) : 0.f;
+        if (!bad) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] *= lift;
+        }
+        const uint32_t lo = bad ? 0u : pack_codes(x, m * lift, inv), hi = bad ? 0u : pack_codes(x + 4, m * lift, inv);
+        if (mine) {
+          int8_t* codes = (kind == 1 ? a.codes_k + b * a.ck_b : a.codes_v + b * a.cv_b) + ((int64_t)head * rows + slot) * dp;
+          if (near8) {
+            *reinterpret_cast<u32x2_t*>(codes + 8 * j) = u32x2_t{lo, hi};
+          } else {
+            *reinterpret_cast<uint32_t*>(codes + at0) = lo, *reinterpret_cast<uint32_t*>(codes + at1) = hi;
+          }
+          if (j == 0) a.scales[b * a.sc_b + 2 * ((int64_t)head * rows + slot) + (kind - 1)] = bad ? __uint_as_float(0x7fc00000u) : m / 127.0f;
+        }
+      }
+    }
+  }
+}
+
+// Groups of heads that a wave takes of a token: all, and their angles once, where there are tokens enough for every SIMD; else fewer.
+int groups_a_wave(int64_t tokens, int groups) {
+  const int64_t chunks = tokens >= 4096 ? 1 : (4096 + tokens - 1) / tokens;
+  return (int)((groups + (chunks < groups ? chunks : groups) - 1) / (chunks < groups ? chunks : groups));
+}
+
+template <typename T, int LPH>
+int launch_heads(const sana_heads_args& a, hipStream_t s) {
+  constexpr int HPW = 64 / LPH;
+  HeadArgs h = {};
+  h.a = a, h.inv_d = 1.0f / a.d;
+  h.gq = (a.H + HPW - 1) / HPW, h.gk = (a.Hkv + HPW - 1) / HPW, h.gv = a.codes_k ? h.gk : 0;
+  const int groups = h.gq + h.gk + h.gv;
+  h.per = groups_a_wave((int64_t)a.B * a.N, groups), h.chunks = (groups + h.per - 1) / h.per;
+  const int64_t tokens = (int64_t)a.B * ((a.N + 3) / 4);  // (below 2^61)
+  if (tokens >= WA_MAX_BLOCKS || tokens * h.chunks >= WA_MAX_BLOCKS - 8) return SANA_ERR_SHAPE;
+  h.items = tokens * h.chunks;
+  const dim3 grid((unsigned)((h.items + 7) / 8 * 8));
+  if (a.rotary && !a.interleaved) hipLaunchKernelGGL((heads_kernel<T, LPH, true>), grid, dim3(256), 0, s, h);
+  else hipLaunchKernelGGL((heads_kernel<T, LPH, false>), grid, dim3(256), 0, s, h);
+  return hipGetLastError() == hipSuccess ? SANA_OK : SANA_ERR_LAUNCH;
+}
+template <typename T>
+int heads_of(const sana_heads_args& a, hipStream_t s) {
+  return a.d <= 32 ? launch_heads<T, 4>(a, s) : a.d <= 64 ? launch_heads<T, 8>(a, s) : launch_heads<T, 16>(a, s);
+}
+
+}  // namespace
+}  // namespace sana
+
+using namespace sana;
+
+extern "C" __attribute__((visibility("default"))) int sana_hip_heads(const sana_heads_args* args, void* stream) {
+  if (!args) return SANA_ERR_ARG;
+  const sana_heads_args& a = *args;
+  const bool cached = a.codes_k || a.codes_v || a.scales;
+  if (!a.k || a.B <= 0 || a.N <= 0 || a.Hkv <= 0 || a.d <= 0 || a.H < 0 || a.rotary < 0 || (a.q == nullptr) != (a.H == 0) ||
+      (a.q == nullptr) != (a.q_out == nullptr))
+    return SANA_ERR_ARG;
+  if (cached ? !a.codes_k || !a.codes_v || !a.scales || !a.v || !a.positions || a.window <= 0 || a.sinks < 0 : !a.k_out) return SANA_ERR_ARG;
+  if ((a.q_weight == nullptr) != (a.k_weight == nullptr) || (a.freqs == nullptr) != (a.rotary == 0) || !(a.eps >= 0.f && a.eps < INFINITY) ||
+      !(fabsf(a.magnitude) < INFINITY))
+    return SANA_ERR_ARG;
+  if (a.io_dtype != SANA_DT_BF16 && a.io_dtype != SANA_DT_F16) return SANA_ERR_DTYPE;
+  if (a.d % 8 || a.d > 128 || a.rotary % 8 || a.rotary > a.d || a.N > (1 << 30) || (int64_t)a.H * a.d > (1 << 22) || (int64_t)a.Hkv * a.d > (1 << 22))
+    return SANA_ERR_SHAPE;
+  const int64_t wq = (int64_t)a.H * a.d, wk = (int64_t)a.Hkv * a.d;
+  if ((a.q && (a.q_n < wq || a.qo_n < wq || a.q_b < 0 || a.qo_b < 0)) || a.k_n < wk || a.k_b < 0 || (a.k_out && (a.ko_n < wk || a.ko_b < 0)) ||
+      (cached && (a.v_n < wk || a.v_b < 0)))
+    return SANA_ERR_ARG;
+  if (a.B > 1 && ((a.q && a.qo_b < wq) || (a.k_out && a.ko_b < wk))) return SANA_ERR_ARG;  // (entries that would write the same elements)
+  // in place: the lane that reads a channel writes it, so its place has to be the same one
+  if ((a.q && a.q == a.q_out && (a.q_n != a.qo_n || (a.B > 1 && a.q_b != a.qo_b))) ||
+      (a.k == a.k_out && (a.k_n != a.ko_n || (a.B > 1 && a.k_b != a.ko_b))))
+    return SANA_ERR_ARG;
+  if (cached) {
+    if (a.window > (1 << 30) || a.sinks > (1 << 30) || (int64_t)a.window + a.sinks > (1 << 30)) return SANA_ERR_SHAPE;
+    const int64_t rows = a.window + a.sinks, codes = a.Hkv * rows * ((a.d + 15) & ~15);
+    if (a.ck_b < 0 || a.cv_b < 0 || a.sc_b < 0 || (a.B > 1 && (a.ck_b < codes || a.cv_b < codes || a.sc_b < 2 * a.Hkv * rows))) return SANA_ERR_ARG;
+    if (misaligned({a.codes_k, a.codes_v, a.v}, {a.v_b, a.v_n}) || a.ck_b % 16 || a.cv_b % 16 || a.sc_b % 2 ||
+        (reinterpret_cast<uintptr_t>(a.scales) & 7u))
+      return SANA_ERR_ALIGN;
+  }
+  if (misaligned({a.q, a.k, a.q_out, a.k_out}, {a.k_b, a.k_n}) || (a.q && misaligned({}, {a.q_b, a.q_n, a.qo_b, a.qo_n})) ||
+      (a.k_out && misaligned({}, {a.ko_b, a.ko_n})) || off4(a.positions) || off4(a.lengths) ||
+      ((reinterpret_cast<uintptr_t>(a.q_weight) | reinterpret_cast<uintptr_t>(a.k_weight)) & 1u) || (reinterpret_cast<uintptr_t>(a.freqs) & 7u))
+    return SANA_ERR_ALIGN;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return a.io_dtype == SANA_DT_F16 ? heads_of<F16>(a, s) : heads_of<BF16>(a, s);
+}

@@ -1,0 +1,413 @@
+// A stream's ring cache in 8 bits (written by heads.hip): one token's softmax attention over it, and its rows in the order of their tokens.
+//
+//   out = sum_j softmax_j(scale * sk_j (q . ck_j)) sv_j cv_j,   c whole numbers of -127 .. 127, sk and sv fp32, one of each for a head's row
+//
+// A head's rows lie one behind the other, [key head][row][d'], d' = d rounded up to 16, their scales as pairs [key head][row][2].
+#include "window_common.h"
+
+namespace sana {
+namespace {
+
+struct Window8Args {
+  WindowArgs w;  // (its caches unused)
+  const int8_t *ck, *cv;
+  const float* scales;
+  int64_t ck_b, cv_b, sc_b;
+};
+
+// four codes of a word as floats
+__device__ __forceinline__ f32x4_t codes_f32(uint32_t x) {
+  return f32x4_t{(float)(int8_t)x, (float)(int8_t)(x >> 8), (float)(int8_t)(x >> 16), (float)((int32_t)x >> 24)};
+}
+// eight codes as 16-bit floats, which hold them exactly
+template <typename T>
+__device__ __forceinline__ u32x4_t codes16(uint32_t lo, uint32_t hi) {
+  const f32x4_t a = codes_f32(lo), b = codes_f32(hi);
+  if constexpr (is_f16<T>) {
+    const auto pk = [](float x, float y) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x, y)); };
+    return u32x4_t{pk(a[0], a[1]), pk(a[2], a[3]), pk(b[0], b[1]), pk(b[2], b[3])};
+  } else {
+    return u32x4_t{pack_bf16(a[0], a[1]), pack_bf16(a[2], a[3]), pack_bf16(b[0], b[1]), pack_bf16(b[2], b[3])};
+  }
+}
+
+// One token of each stream.  A workgroup takes a part of the rows of one (stream, key head), its NW waves in turn a tile of 16 * RT rows; the query
+// heads that share the key head are the 16 columns of the products (more than 16 in further workgroups).  K comes from memory as the operand it
+// is (16 channels a lane, two products), V through the wave's own LDS as bf16 to be transposed; its scale goes to the probability, and both as
+// the sum of two bf16 numbers into the product.
+template <typename T, int P, int NW, int RT>
+__global__ __launch_bounds__(64 * NW) void window_q8_kernel(const Window8Args x) {
+  const WindowArgs& a = x.w;
+  constexpr int DP = 16 * P, KS = (P + 3) / 4, DK = (P + 1) / 2, DT = P, PITCH = DK * 64, ROWS = 16 * RT, TILE = ROWS * PITCH;
+  constexpr int PV = (ROWS * P + 63) / 64, SUMS = 16 * 16 * DT * 4 + 128;  // PV: 16-byte pieces of V a lane
+  constexpr int OWN = (TILE + 2 * 4 * ROWS > SUMS ? TILE + 2 * 4 * ROWS : SUMS);
+  __shared__ __attribute__((aligned(16))) unsigned char smem[NW * OWN];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, fr = lane & 15, fg = lane >> 4;
+  unsigned char* mine = smem + wave * OWN;
+  float* my_scales = reinterpret_cast<float*>(mine + TILE);  // of the keys, then of the values
+  const int G = a.H / a.Hkv, blocks = (G + 15) / 16, d = a.d;
+  const int split = blockIdx.y, gb = blockIdx.x % blocks, bk = blockIdx.x / blocks, b = bk / a.Hkv, hk = bk - b * a.Hkv;
+  const int pos = a.positions[b];
+  if (pos < 0) {  // an idle stream: zeros
+    if (split == 0 && gb == 0)
+      for (int c = tid; c < G * d; c += 64 * NW) a.out[b * a.o_b + hk * G * d + c] = 0;
+    return;
+  }
+  const int rows = a.window + a.sinks, count = pos < rows ? pos + 1 : rows;
+  const int tiles = (count + ROWS - 1) / ROWS, t0 = (int)((int64_t)tiles * split / a.splits), t1 = (int)((int64_t)tiles * (split + 1) / a.splits);
+  const int64_t head_rows = (int64_t)hk * rows;
+  const int8_t *ck = x.ck + b * x.ck_b + head_rows * DP, *cv = x.cv + b * x.cv_b + head_rows * DP;
+  const float* scales = x.scales + b * x.sc_b + 2 * head_rows;
+
+  const int head = 16 * gb + fr, h = hk * G + min(head, G - 1);
+  u32x4_t qf[KS][2];
+#pragma unroll
+  for (int s = 0; s < KS; ++s)
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int c = 16 * (4 * s + fg) + 8 * half;
+      qf[s][half] = *reinterpret_cast<const u32x4_t*>(a.q + b * a.q_b + h * d + (c < d ? c : 0));
+      if (c >= d) qf[s][half] = u32x4_t{0u, 0u, 0u, 0u};  // (codes are finite: what lies behind d counts as nothing)
+    }
+
+  u32x4_t rk[RT][KS], rv[PV];
+  f32x2_t rs[(ROWS + 63) / 64];
+  auto request = [&](int t) {
+#pragma unroll
+    for (int kt = 0; kt < RT; ++kt) {
+      const int8_t* from = ck + (int64_t)min(ROWS * t + 16 * kt + fr, count - 1) * DP;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) rk[kt][s] = *reinterpret_cast<const u32x4_t*>(from + 16 * min(4 * s + fg, P - 1));
+    }
+#pragma unroll
+    for (int i = 0; i < PV; ++i) {
+      const int idx = lane + 64 * i, r = idx / P, c = idx - r * P;
+      rv[i] = *reinterpret_cast<const u32x4_t*>(cv + (int64_t)min(ROWS * t + r, count - 1) * DP + 16 * c);
+    }
+#pragma unroll
+    for (int i = 0; i < (ROWS + 63) / 64; ++i)
+      rs[i] = *reinterpret_cast<const f32x2_t*>(scales + 2 * (int64_t)min(ROWS * t + 64 * i + lane, count - 1));
+  };
+  f32x4_t oc[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) oc[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  float mx = -INFINITY, sub = 0.f, sum = 0.f;
+  const int trow = 4 * fg + (fr >> 2), tkey = row_key<DK>(trow), piece = fr & 3;
+  if (t0 + wave < t1) request(t0 + wave);
+#pragma unroll 1
+  for (int t = t0 + wave; t < t1; t += NW) {
+    f32x4_t sc[RT];
+#pragma unroll
+    for (int kt = 0; kt < RT; ++kt) sc[kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < (ROWS + 63) / 64; ++i)
+      if (64 * i + lane < ROWS) {  // (a row that is not there: a value's scale of 0, so that nothing of it counts)
+        const bool there = ROWS * t + 64 * i + lane < count;
+        my_scales[64 * i + lane] = rs[i].x * a.scale_log2e;
+        my_scales[ROWS + 64 * i + lane] = there ? rs[i].y : 0.f;
+      }
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int kt = 0; kt < RT; ++kt) {
+        sc[kt] = mfma_16x16x32<T>(codes16<T>(rk[kt][s][0], rk[kt][s][1]), qf[s][0], sc[kt]);
+        sc[kt] = mfma_16x16x32<T>(codes16<T>(rk[kt][s][2], rk[kt][s][3]), qf[s][1], sc[kt]);
+      }
+#pragma unroll
+    for (int i = 0; i < PV; ++i) {
+      const int idx = lane + 64 * i, r = idx / P, c = idx - r * P;
+      if (ROWS * P % 64 == 0 || r < ROWS) {
+        unsigned char* to = mine + r * PITCH;
+        *reinterpret_cast<u32x4_t*>(to + (((2 * c) ^ row_key<DK>(r & 15)) << 4)) = codes16<BF16>(rv[i][0], rv[i][1]);
+        *reinterpret_cast<u32x4_t*>(to + (((2 * c + 1) ^ row_key<DK>(r & 15)) << 4)) = codes16<BF16>(rv[i][2], rv[i][3]);
+      }
+    }
+    if (t + NW < t1) request(t + NW);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the wave's own scales and V are there)
+    float most = -INFINITY;
+#pragma unroll
+    for (int kt = 0; kt < RT; ++kt) {
+      const f32x4_t sk = *reinterpret_cast<const f32x4_t*>(my_scales + 16 * kt + 4 * fg);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        sc[kt][r] = ROWS * t + 16 * kt + 4 * fg + r < count ? sc[kt][r] * sk[r] : -INFINITY;
+        most = fmaxf(most, sc[kt][r]);
+      }
+    }
+    if (__any(most > mx + 8.f)) {
+      const float now = fmaxf(mx, max_groups(most));
+      const float f = __builtin_amdgcn_exp2f(mx - (now == -INFINITY ? 0.f : now));
+      mx = now, sub = now == -INFINITY ? 0.f : now;
+      sum *= f;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) oc[dt][r] *= f;
+    }
+#pragma unroll
+    for (int k2 = 0; k2 < RT / 2; ++k2) {
+      u32x4_t hi, lo;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        const f32x4_t sv = *reinterpret_cast<const f32x4_t*>(my_scales + ROWS + 16 * (2 * k2 + kt) + 4 * fg);
+        float p[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          p[r] = __builtin_amdgcn_exp2f(sc[2 * k2 + kt][r] - sub);
+          sum += p[r];
+          p[r] *= sv[r];
+        }
+        hi[2 * kt] = pack_bf16(p[0], p[1]), hi[2 * kt + 1] = pack_bf16(p[2], p[3]);
+        lo[2 * kt] = pack_bf16(p[0] - bf16_lo(hi[2 * kt]), p[1] - bf16_hi(hi[2 * kt]));
+        lo[2 * kt + 1] = pack_bf16(p[2] - bf16_lo(hi[2 * kt + 1]), p[3] - bf16_hi(hi[2 * kt + 1]));
+      }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        lds_t* from = (lds_t*)mine + (32 * k2 + trow) * PITCH + (((2 * dt + (piece >> 1)) ^ tkey) << 4) + 8 * (piece & 1);
+        const u32x2_t v0 = lds_read_tr(from), v1 = lds_read_tr(from + 16 * PITCH);
+        const u32x4_t vf = u32x4_t{v0.x, v0.y, v1.x, v1.y};
+        oc[dt] = mfma_16x16x32_bf16(vf, lo, oc[dt]);
+        oc[dt] = mfma_16x16x32_bf16(vf, hi, oc[dt]);
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+  // ---- the waves' parts, through LDS: [channel][head], then the maxima and sums
+  sum = sum_groups(sum);
+  float* po = reinterpret_cast<float*>(mine);
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) po[(16 * dt + 4 * fg + r) * 16 + fr] = oc[dt][r];
+  if (fg == 0) po[16 * 16 * DT + fr] = mx, po[16 * 16 * DT + 16 + fr] = sum;
+  lds_barrier();
+  auto part = [&](int w) { return reinterpret_cast<const float*>(smem + w * OWN); };
+  const int col = tid & 15, g = 16 * gb + col;
+  float m = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) m = fmaxf(m, part(w)[16 * 16 * DT + col]);
+  const float base = m == -INFINITY ? 0.f : m;
+  float f[NW], l = 0.f;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    f[w] = __builtin_amdgcn_exp2f(part(w)[16 * 16 * DT + col] - base);
+    l = fmaf(f[w], part(w)[16 * 16 * DT + 16 + col], l);
+  }
+  if (g >= G) return;
+  const int64_t at = ((int64_t)split * a.B + b) * a.H + hk * G + g;
+  const float inv = 1.0f / l;
+  for (int c = tid >> 4; c < d; c += 4 * NW) {
+    float o = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) o = fmaf(f[w], part(w)[c * 16 + col], o);
+    if (a.splits == 1) a.out[b * a.o_b + (hk * G + g) * d + c] = (uint16_t)pk16<T>(o * inv, 0.f);
+    else a.part_o[at * d + c] = o;
+  }
+  if (a.splits > 1 && tid < 16) a.part_ml[2 * at] = m, a.part_ml[2 * at + 1] = l;
+}
+
+// ---------------------------------------------------------------------------- rows in order
+
+struct ReadArgs {
+  const unsigned char *k, *v;  // 16-bit rows or codes
+  const float* scales;
+  const int* positions;
+  uint16_t *out_k, *out_v;
+  int B, Hkv, d, dp, window, sinks, last, blocks, zero_rest;
+  int64_t k_b, k_n, v_b, v_n, sc_b, ok_b, ok_n, ov_b, ov_n;  // k_b .. v_n in bytes
+  int64_t items;
+};
+
+// Row i of the output -> the cache's row, -1 behind the last one.
+__device__ __forceinline__ int read_slot(const ReadArgs& a, int pos, int i) {
+  const int held = a.sinks + a.last;
+  if (pos <= held) return i < pos ? (i < a.sinks ? i : a.sinks + (i - a.sinks) % a.window) : -1;
+  if (i < a.sinks) return i;
+  return a.sinks + (int)((uint32_t)(pos - a.last - a.sinks + (i - a.sinks)) % (uint32_t)a.window);
+}
+
+// 16-bit rows: a wave copies a row of keys or of values.
+__global__ __launch_bounds__(256) void read16_kernel(const ReadArgs a) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int64_t item = (int64_t)blockIdx.x * 4 + wave;
+  if (item >= a.items) return;
+  const int of_v = (int)(item & 1), held = a.sinks + a.last;
+  const int b = (int)((item >> 1) / held), i = (int)((item >> 1) - (int64_t)b * held);
+  const int slot = read_slot(a, a.positions[b], i), width = a.Hkv * a.d;
+  uint16_t* to = of_v ? a.out_v + b * a.ov_b + i * a.ov_n : a.out_k + b * a.ok_b + i * a.ok_n;
+  if (slot < 0) {
+    if (a.zero_rest)
+      for (int c = 8 * lane; c < width; c += 512) *reinterpret_cast<u32x4_t*>(to + c) = u32x4_t{0u, 0u, 0u, 0u};
+    return;
+  }
+  const unsigned char* from = of_v ? a.v + b * a.v_b + slot * a.v_n : a.k + b * a.k_b + slot * a.k_n;
+  for (int c0 = 8 * lane; c0 < width; c0 += 2048) {
+    u32x4_t x[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (c0 + 512 * u < width) x[u] = *reinterpret_cast<const u32x4_t*>(from + 2 * (c0 + 512 * u));
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (c0 + 512 * u < width) *reinterpret_cast<u32x4_t*>(to + c0 + 512 * u) = x[u];
+  }
+}
+
+// Codes: a wave takes RB rows of a head's keys or values, 8 channels a lane; the heads of a block of rows on one XCD, whose L2 puts the pieces of
+// an output row together.
+constexpr int RB = 16;
+template <typename T>
+__global__ __launch_bounds__(256) void read8_kernel(const ReadArgs a) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int64_t wgs = (a.items + 3) / 4, per_xcd = (wgs + 7) >> 3, wg = (int64_t)(blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3), item = 4 * wg + wave;
+  if ((int64_t)(blockIdx.x >> 3) >= per_xcd || item >= a.items) return;
+  const int pair = (int)(item % (2 * a.Hkv)), of_v = pair >= a.Hkv, hk = of_v ? pair - a.Hkv : pair;
+  const int64_t rest = item / (2 * a.Hkv);
+  const int b = (int)(rest / a.blocks), i0 = RB * (int)(rest - (int64_t)b * a.blocks);
+  const int held = a.sinks + a.last, rows = a.sinks + a.window, pos = a.positions[b], eighths = a.d / 8, n = min(RB, held - i0) * eighths;
+  const unsigned char* from = (of_v ? a.v + b * a.v_b : a.k + b * a.k_b) + (int64_t)hk * rows * a.dp;
+  const float* scales = a.scales + b * a.sc_b + 2 * (int64_t)hk * rows + of_v;
+  uint16_t* to = (of_v ? a.out_v + b * a.ov_b : a.out_k + b * a.ok_b) + hk * a.d;
+  const int64_t to_n = of_v ? a.ov_n : a.ok_n;
+  constexpr int U = RB * 16 / 64;
+  u32x2_t x[U];
+  float s[U];
+  int slot[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int idx = lane + 64 * u, r = idx / eighths, c = idx - r * eighths;
+    slot[u] = -1, x[u] = u32x2_t{0u, 0u}, s[u] = 0.f;
+    if (idx < n && (slot[u] = read_slot(a, pos, i0 + r)) >= 0) {
+      x[u] = *reinterpret_cast<const u32x2_t*>(from + (int64_t)slot[u] * a.dp + 8 * c);
+      s[u] = scales[2 * (int64_t)slot[u]];
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int idx = lane + 64 * u, r = idx / eighths, c = idx - r * eighths;
+    if (idx >= n || (slot[u] < 0 && !a.zero_rest)) continue;
+    const f32x4_t y = codes_f32(x[u].x), z = codes_f32(x[u].y);
+    *reinterpret_cast<u32x4_t*>(to + (i0 + r) * to_n + 8 * c) =
+        u32x4_t{pk16<T>(y[0] * s[u], y[1] * s[u]), pk16<T>(y[2] * s[u], y[3] * s[u]), pk16<T>(z[0] * s[u], z[1] * s[u]), pk16<T>(z[2] * s[u], z[3] * s[u])};
+  }
+}
+
+int q8_splits(int B, int H, int Hkv, int rows, int d) {
+  const int64_t groups = step_groups(B, H, Hkv), bytes = (int64_t)rows * d * 2;
+  if (bytes <= (groups <= 128 ? 256 << 10 : 1 << 20)) return 1;
+  const int most = rows / 128 < WA_MAX_SPLITS ? rows / 128 : WA_MAX_SPLITS;
+  for (int s = 1; s < most; ++s)
+    if (groups * s * 32 >= (groups * s + 255) / 256 * 256 * 25) return s;
+  return most > 1 ? most : 1;
+}
+
+template <typename T, int P>
+int launch_q8(const Window8Args& x, hipStream_t s) {
+  const WindowArgs& a = x.w;
+  const int64_t groups = step_groups(a.B, a.H, a.Hkv);
+  if (a.splits == 1 && groups <= 256)
+    hipLaunchKernelGGL((window_q8_kernel<T, P, 8, 2>), dim3((unsigned)groups), dim3(512), 0, s, x);
+  else
+    hipLaunchKernelGGL((window_q8_kernel<T, P, 4, 4>), dim3((unsigned)groups, (unsigned)a.splits), dim3(256), 0, s, x);
+  if (a.splits > 1) {
+    const int rc = launch_join<T>(a, s);
+    if (rc != SANA_OK) return rc;
+  }
+  return hipGetLastError() == hipSuccess ? SANA_OK : SANA_ERR_LAUNCH;
+}
+template <typename T>
+int q8_of(const Window8Args& x, hipStream_t s) {
+  switch ((x.w.d + 15) / 16) {
+    case 1: return launch_q8<T, 1>(x, s);
+    case 2: return launch_q8<T, 2>(x, s);
+    case 3: return launch_q8<T, 3>(x, s);
+    case 4: return launch_q8<T, 4>(x, s);
+    case 5: return launch_q8<T, 5>(x, s);
+    case 6: return launch_q8<T, 6>(x, s);
+    case 7: return launch_q8<T, 7>(x, s);
+    default: return launch_q8<T, 8>(x, s);
+  }
+}
+
+}  // namespace
+}  // namespace sana
+
+using namespace sana;
+
+#define SANA_API extern "C" __attribute__((visibility("default")))
+
+SANA_API size_t sana_hip_window_q8_workspace_bytes(int B, int H, int Hkv, int d, int window, int sinks) {
+  if (B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || d <= 0 || d > 128 || window <= 0 || sinks < 0 || (int64_t)window + sinks > (1 << 30)) return 0;
+  if (step_groups(B, H, Hkv) >= WA_MAX_BLOCKS) return 0;
+  return part_bytes(q8_splits(B, H, Hkv, window + sinks, d), (int64_t)B * H, d);
+}
+
+SANA_API int sana_hip_window_q8(const void* q, const int8_t* codes_k, const int8_t* codes_v, const float* scales, const int32_t* positions, void* out,
+                                void* workspace, size_t workspace_bytes, int B, int H, int Hkv, int d, int window, int sinks, int64_t q_stride_b,
+                                int64_t o_stride_b, int64_t ck_stride_b, int64_t cv_stride_b, int64_t scales_stride_b, float scale, int io_dtype,
+                                void* stream) {
+  if (!q || !codes_k || !codes_v || !scales || !positions || !out || !(scale > 0.f && scale * 1.44269504088896341f < INFINITY)) return SANA_ERR_ARG;
+  const int rc = check_sizes(B, 1, H, Hkv, d, window, sinks, io_dtype);
+  if (rc != SANA_OK) return rc;
+  for (const int64_t sb : {q_stride_b, o_stride_b, ck_stride_b, cv_stride_b, scales_stride_b})
+    if (sb < 0) return SANA_ERR_ARG;
+  if (B > 1 && o_stride_b < (int64_t)H * d) return SANA_ERR_ARG;  // (entries that would write the same elements)
+  if ((int64_t)window + sinks > (1 << 30) || step_groups(B, H, Hkv) >= WA_MAX_BLOCKS) return SANA_ERR_SHAPE;
+  if (misaligned({q, codes_k, codes_v}, {q_stride_b}) || ck_stride_b % 16 || cv_stride_b % 16 || scales_stride_b % 2 ||
+      (reinterpret_cast<uintptr_t>(scales) & 7u) || (reinterpret_cast<uintptr_t>(out) & 7u) || o_stride_b % 4 || off4(positions))
+    return SANA_ERR_ALIGN;
+  Window8Args x = {};
+  WindowArgs& a = x.w;
+  a.q = static_cast<const uint16_t*>(q), a.out = static_cast<uint16_t*>(out), a.positions = positions;
+  a.B = B, a.N = 1, a.Nk = 1, a.H = H, a.Hkv = Hkv, a.d = d, a.window = window, a.sinks = sinks, a.q_b = q_stride_b, a.o_b = o_stride_b;
+  a.scale_log2e = scale * 1.44269504088896341f;
+  x.ck = codes_k, x.cv = codes_v, x.scales = scales, x.ck_b = ck_stride_b, x.cv_b = cv_stride_b, x.sc_b = scales_stride_b;
+  a.splits = q8_splits(B, H, Hkv, window + sinks, d);
+  const int64_t rows = (int64_t)B * H;
+  if (a.splits > 1) {
+    if (!workspace || workspace_bytes < part_bytes(a.splits, rows, d)) return SANA_ERR_WORKSPACE;
+    if (!aligned16(workspace)) return SANA_ERR_ALIGN;
+    a.part_o = static_cast<float*>(workspace), a.part_ml = a.part_o + a.splits * rows * d;
+  }
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return io_dtype == SANA_DT_F16 ? q8_of<F16>(x, s) : q8_of<BF16>(x, s);
+}
+
+SANA_API int sana_hip_window_cache_read(const void* cache_k, const void* cache_v, const float* scales, const int32_t* positions, void* out_k,
+                                        void* out_v, int B, int Hkv, int d, int window, int sinks, int last, int64_t ck_stride_b,
+                                        int64_t ck_stride_n, int64_t cv_stride_b, int64_t cv_stride_n, int64_t scales_stride_b, int64_t ok_stride_b,
+                                        int64_t ok_stride_n, int64_t ov_stride_b, int64_t ov_stride_n, int zero_rest, int io_dtype, void* stream) {
+  if (!cache_k || !cache_v || !positions || !out_k || !out_v || last < 0 || last > window) return SANA_ERR_ARG;
+  // (16-bit rows are copied whole: no head's width)
+  const int rc = check_sizes(B, 1, Hkv, Hkv, scales ? d : 8, window, sinks, io_dtype);
+  if (rc != SANA_OK) return rc;
+  if ((int64_t)sinks + last < 1 || d <= 0) return SANA_ERR_ARG;
+  if (d % 8 || (int64_t)Hkv * d > (1 << 22) || (int64_t)window + sinks > (1 << 30)) return SANA_ERR_SHAPE;
+  const int64_t width = (int64_t)Hkv * d, held = (int64_t)sinks + last;
+  for (const int64_t sb : {ck_stride_b, cv_stride_b, scales_stride_b, ok_stride_b, ov_stride_b})
+    if (sb < 0) return SANA_ERR_ARG;
+  if (ok_stride_n < width || ov_stride_n < width || (!scales && (ck_stride_n < width || cv_stride_n < width))) return SANA_ERR_ARG;
+  if (B > 1 && (ok_stride_b < width || ov_stride_b < width)) return SANA_ERR_ARG;  // (entries that would write the same elements)
+  if (misaligned({cache_k, cache_v, out_k, out_v}, {ok_stride_b, ok_stride_n, ov_stride_b, ov_stride_n}) || off4(positions)) return SANA_ERR_ALIGN;
+  ReadArgs a = {};
+  a.k = static_cast<const unsigned char*>(cache_k), a.v = static_cast<const unsigned char*>(cache_v), a.scales = scales, a.positions = positions;
+  a.out_k = static_cast<uint16_t*>(out_k), a.out_v = static_cast<uint16_t*>(out_v);
+  a.B = B, a.Hkv = Hkv, a.d = d, a.dp = (d + 15) & ~15, a.window = window, a.sinks = sinks, a.last = last, a.zero_rest = zero_rest;
+  a.ok_b = ok_stride_b, a.ok_n = ok_stride_n, a.ov_b = ov_stride_b, a.ov_n = ov_stride_n;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (!scales) {
+    if (misaligned({}, {ck_stride_b, ck_stride_n, cv_stride_b, cv_stride_n})) return SANA_ERR_ALIGN;
+    a.k_b = 2 * ck_stride_b, a.k_n = 2 * ck_stride_n, a.v_b = 2 * cv_stride_b, a.v_n = 2 * cv_stride_n;
+    if (held >= (WA_MAX_BLOCKS << 1) / B) return SANA_ERR_SHAPE;
+    a.items = 2 * B * held;
+    hipLaunchKernelGGL(read16_kernel, dim3((unsigned)((a.items + 3) / 4)), dim3(256), 0, s, a);
+  } else {
+    if (ck_stride_b % 16 || cv_stride_b % 16 || scales_stride_b % 2 || (reinterpret_cast<uintptr_t>(scales) & 7u)) return SANA_ERR_ALIGN;
+    a.k_b = ck_stride_b, a.v_b = cv_stride_b, a.sc_b = scales_stride_b, a.blocks = (int)((held + RB - 1) / RB);
+    if ((int64_t)a.blocks * Hkv >= (WA_MAX_BLOCKS << 1) / B) return SANA_ERR_SHAPE;
+    a.items = (int64_t)B * a.blocks * 2 * Hkv;
+    const unsigned grid = (unsigned)(((a.items + 3) / 4 + 7) / 8 * 8);
+    if (io_dtype == SANA_DT_F16) hipLaunchKernelGGL(read8_kernel<F16>, dim3(grid), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL(read8_kernel<BF16>, dim3(grid), dim3(256), 0, s, a);
+  }
+  return hipGetLastError() == hipSuccess ? SANA_OK : SANA_ERR_LAUNCH;
+}

@@ -5,6 +5,7 @@ checks, without a launch: empty outputs, and an all-zero state for no tokens.
 """
 from __future__ import annotations
 
+import math
 import threading
 from typing import Optional, Sequence, Tuple
 
@@ -1119,3 +1120,287 @@ def window_attention_step_(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ca
     if code:
         _lib.check(code, "sana_hip_window_step")
     return out
+
+
+# --------------------------------------------------------------------------- a stream's heads, and its cache in 8 bits
+
+def rotary_frequencies(rotary_dim: int, base: float = 10000.0, factor: float = 1.0, trained: Optional[int] = None, slow: float = 1.0,
+                       fast: float = 32.0, device="cuda") -> torch.Tensor:
+    """Radians a position of each rotated pair of channels, fp64 [rotary_dim / 2]: ``base ** (-2 i / rotary_dim)``, for contexts ``factor`` times as
+    long as those of training divided by it -- all of them, or, with the ``trained`` length, only those that turn fewer than ``slow`` times over it;
+    ones that turn more than ``fast`` times stay as they are, and between the two lies a blend by the number of turns."""
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise SanaHipError(f"rotary_dim must be even and at least 2, got {rotary_dim}")
+    if not base > 0 or not factor > 0 or (trained is not None and not (trained > 0 and fast > slow)):
+        raise SanaHipError(f"base, factor and trained must be positive and fast above slow, got {base}, {factor}, {trained}, {fast}, {slow}")
+    f = base ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
+    keep = torch.zeros_like(f) if trained is None else ((trained * f / (2 * math.pi) - slow) / (fast - slow)).clamp(0, 1)
+    return (f * (keep + (1 - keep) / factor)).to(device)
+
+
+def window_cache_q8(batch: int, rows: int, kv_heads: int, head_dim: int, device="cuda") -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """An empty cache of 8 bits for ``batch`` streams: (codes of keys, codes of values, scales), int8 [batch, kv_heads, rows, d'] and fp32
+    [batch, kv_heads, rows, 2], ``rows`` = sinks + window, d' = head_dim rounded up to a multiple of 16 (what is behind head_dim is not looked at).
+    A head's row x lies in it as ``c = round(127 x / max|x|)``, ties to even, and the scale ``max|x| / 127`` (of the key, of the value); a row
+    with an inf or NaN has the scale NaN.  Tensors of these shapes whose streams are dense and do not overlap are a cache as well."""
+    if head_dim % 8 or not 0 < head_dim <= 128 or rows < 1 or kv_heads < 1:
+        raise SanaHipError(f"no cache of {rows} rows of {kv_heads} heads of {head_dim} (head dims: multiples of 8 up to 128)")
+    shape = (batch, kv_heads, rows, -(-head_dim // 16) * 16)
+    return (torch.zeros(shape, dtype=torch.int8, device=device), torch.zeros(shape, dtype=torch.int8, device=device),
+            torch.zeros(batch, kv_heads, rows, 2, dtype=torch.float32, device=device))
+
+
+def _q8_parts(cache, what: str):
+    if len(cache) != 3:
+        raise SanaHipError(f"{what}: a cache of 8 bits is (codes of keys, codes of values, scales)")
+    return cache
+
+
+def _q8_cache(cache, B: int, d: int, sinks: int, what: str) -> Tuple[int, int, Tuple[int, int, int], Tuple[int, int, int]]:
+    """-> (key heads, window, the three pointers, the three stream strides) of a cache of heads of d channels."""
+    ck, cv, sc = cache
+    shape = ck.shape
+    if len(shape) != 4 or ck.dtype is not torch.int8 or cv.dtype is not torch.int8 or cv.shape != shape or sc.dtype is not torch.float32 \
+            or sc.shape != (*shape[:3], 2) or shape[0] != B or shape[3] != (d + 15) // 16 * 16:
+        raise SanaHipError(f"{what}: codes int8 [{B}, kv_heads, rows, {(d + 15) // 16 * 16}] and scales fp32 [{B}, kv_heads, rows, 2] are a cache of "
+                           f"heads of {d}, got {ck.dtype} {tuple(shape)}, {cv.dtype} {tuple(cv.shape)}, {sc.dtype} {tuple(sc.shape)}")
+    _, G, R, width = shape
+    strides = []
+    for t, w in ((ck, width), (cv, width), (sc, 2)):
+        b, g, n, c = t.stride()
+        if c != 1 or (n != w and R > 1) or (g != R * w and G > 1):
+            raise SanaHipError(f"{what}: each stream of a cache must be dense, got strides {t.stride()} of {tuple(t.shape)}")
+        strides.append(b if B > 1 else 0)
+    if not 0 <= sinks < R:
+        raise SanaHipError(f"{what}: a cache of {R} rows holds {sinks} sinks and no window")
+    return G, R - sinks, (ck.data_ptr(), cv.data_ptr(), sc.data_ptr()), strides
+
+
+def _heads_checks(q, k, num_heads: int, q_weight, k_weight, freqs, what: str) -> Tuple[int, int]:
+    """-> (head_dim, rotated channels) of [B, N, num_heads * d] queries and [B, N, kv_heads * d] keys, their weights and frequencies."""
+    dt, qs, ks = q.dtype, q.shape, k.shape
+    if len(qs) != 3 or len(ks) != 3 or dt not in IO16 or k.dtype is not dt or qs[:2] != ks[:2]:
+        raise SanaHipError(f"{what} needs bf16 or fp16 q [B, N, H*d] and k [B, N, Hkv*d] of one dtype, got {dt} {tuple(qs)}, {k.dtype} {tuple(ks)}")
+    if num_heads < 1 or qs[2] == 0 or qs[2] % num_heads:
+        raise SanaHipError(f"{qs[2]} channels are not {num_heads} heads")
+    d = qs[2] // num_heads
+    if d % 8 or d > 128:
+        raise SanaHipError(f"head_dim {d} has no kernel (multiples of 8 up to 128)")
+    if ks[2] == 0 or ks[2] % d:
+        raise SanaHipError(f"k {tuple(ks)} does not match q {tuple(qs)} with {num_heads} heads of {d}")
+    if (q_weight is None) != (k_weight is None):
+        raise SanaHipError(f"{what}: q_weight and k_weight go together")
+    for t in (q_weight, k_weight):
+        if t is not None and (t.dtype is not dt or t.shape != (d,) or not t.is_contiguous()):
+            raise SanaHipError(f"{what}: the norms' weights must be contiguous {dt} [{d}], got {t.dtype} {tuple(t.shape)}")
+    if freqs is None:
+        return d, 0
+    r = 2 * freqs.numel()
+    if freqs.dtype is not torch.float64 or freqs.dim() != 1 or not freqs.is_contiguous() or r % 8 or not 0 < r <= d:
+        raise SanaHipError(f"{what}: freqs must be contiguous fp64 [rotary / 2], rotary a multiple of 8 up to {d}, got {freqs.dtype} {tuple(freqs.shape)}")
+    return d, r
+
+
+def _out_like(t: torch.Tensor, out: Optional[torch.Tensor], what: str) -> torch.Tensor:
+    if out is None:
+        return torch.empty_like(t, memory_format=torch.contiguous_format)
+    if out.shape != t.shape or out.dtype is not t.dtype:
+        raise SanaHipError(f"{what} has the wrong shape or dtype")
+    return out
+
+
+def _heads(q, k, v, d, rotary, q_weight, k_weight, eps, freqs, interleaved, magnitude, positions, lengths, q_out, k_out, cache, window, sinks,
+           zero_rest) -> None:
+    """The call itself; all tensors checked.  ``cache``: the pointers and stream strides of :func:`_q8_cache`, or None."""
+    B, N, C = k.shape
+    ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    rows = lambda t, what: (0, 0) if t is None else _token_rows(t, what)  # noqa: E731
+    pointers, strides = cache or ((0, 0, 0), (0, 0, 0))
+    args = _lib.HEADS_ARGS.pack(
+        ptr(q), k.data_ptr(), ptr(v), ptr(q_out), ptr(k_out), ptr(q_weight), ptr(k_weight), ptr(freqs), positions or 0, lengths or 0, *pointers,
+        *rows(q, "q"), *_token_rows(k, "k"), *rows(v, "v"), *rows(q_out, "q_out"), *rows(k_out, "k_out"), *strides,
+        B, N, 0 if q is None else q.shape[2] // d, C // d, d, rotary, 1 if interleaved else 0, window, sinks, zero_rest, _DT[k.dtype], eps, magnitude)
+    code = _lib.load().sana_hip_heads(args, _stream())
+    if code:
+        _lib.check(code, "sana_hip_heads")
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, num_heads: int, q_weight: Optional[torch.Tensor] = None,
+                 k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, freqs: Optional[torch.Tensor] = None, interleaved: bool = True,
+                 magnitude: float = 1.0, positions: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
+                 q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Norms of queries and keys for each head and the rotation by their position, in one pass.  q: [B, N, H*d], k: [B, N, Hkv*d] token-major views,
+    bf16 or fp16 of one dtype, d a multiple of 8 up to 128.
+
+    ``q_weight``, ``k_weight`` [d] (of q's dtype, None: no norm): ``x * rsqrt(mean(x^2) + eps) * weight`` over each head.  ``freqs``: fp64
+    [rotary / 2] on the device (:func:`rotary_frequencies`; None: no rotation), radians a position of the pairs of each head's first ``rotary``
+    channels (a multiple of 8), pairs (2i, 2i + 1), or (i, i + rotary / 2) with ``interleaved=False``:
+    ``(a, b) -> magnitude * (a cos - b sin, a sin + b cos)``.  ``positions``: int32 [B] on the device, the position of each entry's first token
+    (None: 0; negative: an idle stream), ``lengths``: int32 [B], the tokens it really has (clamped to 0 .. N); rows without a token stay in
+    ``q_out`` / ``k_out`` as they were (zeros in new ones).  ``q_out`` may be q and ``k_out`` k, else they must not overlap the inputs.  Sums,
+    products and rotations are fp32, angles fp64; the outputs are rounded once.  Returns (q, k) of the inputs' shapes.  Forward only."""
+    dev = _here((q, k, q_weight, k_weight, freqs, positions, lengths, q_out, k_out), "qk_norm_rope")
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            return qk_norm_rope(q, k, num_heads, q_weight, k_weight, eps, freqs, interleaved, magnitude, positions, lengths, q_out, k_out)
+    d, rotary = _heads_checks(q, k, num_heads, q_weight, k_weight, freqs, "qk_norm_rope")
+    B, N, _ = q.shape
+    position_ptr = _lengths_arg(positions, B, "positions")
+    length_ptr = _lengths_arg(lengths, B)
+    zero_rest = (1 if q_out is None else 0) + (2 if k_out is None else 0)
+    q_out, k_out = _out_like(q, q_out, "q_out"), _out_like(k, k_out, "k_out")
+    if B * N:
+        _heads(q, k, None, d, rotary, q_weight, k_weight, eps, freqs, interleaved, magnitude, position_ptr, length_ptr, q_out, k_out, None, 0, 0,
+               zero_rest)
+    return q_out, k_out
+
+
+def window_cache_append_q8_(cache: Sequence[torch.Tensor], k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, sinks: int = 0,
+                            lengths: Optional[torch.Tensor] = None) -> None:
+    """:func:`window_cache_append_` into a cache of 8 bits (:func:`window_cache_q8`): k, v [B, N, kv_heads * d], each head's row by its largest
+    magnitude.  ``positions`` and ``lengths`` as there.  The cache must not overlap k and v.  Forward only."""
+    ck, cv, sc = _q8_parts(cache, "window_cache_append_q8_")
+    dev = _here((ck, cv, sc, k, v, positions, lengths), "window_cache_append_q8_")
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            return window_cache_append_q8_(cache, k, v, positions, sinks, lengths)
+    if k.dim() != 3 or k.shape != v.shape or k.dtype not in IO16 or v.dtype is not k.dtype:
+        raise SanaHipError(f"window_cache_append_q8_ needs bf16 or fp16 k and v [B, N, C] of one dtype, got {tuple(k.shape)}, {tuple(v.shape)}")
+    B, N, C = k.shape
+    G = ck.shape[1] if ck.dim() == 4 else 0
+    if G < 1 or C % G or C // G % 8 or not 0 < C // G <= 128:
+        raise SanaHipError(f"window_cache_append_q8_: k {tuple(k.shape)} is not the heads of a cache {tuple(ck.shape)}")
+    _, window, *parts = _q8_cache(cache, B, C // G, sinks, "window_cache_append_q8_")
+    position_ptr, length_ptr = _lengths_arg(positions, B, "positions"), _lengths_arg(lengths, B)
+    if B * N:
+        _heads(None, k, v, C // G, 0, None, None, 0.0, None, True, 1.0, position_ptr, length_ptr, None, None, parts, window, sinks, 0)
+
+
+def qk_norm_rope_append_q8_(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: Sequence[torch.Tensor], positions: torch.Tensor, num_heads: int,
+                            q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                            freqs: Optional[torch.Tensor] = None, interleaved: bool = True, magnitude: float = 1.0, sinks: int = 0,
+                            lengths: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None,
+                            ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """:func:`qk_norm_rope` and :func:`window_cache_append_q8_` in one pass over the rows of a projection: the queries come back, the keys go into the
+    cache unrounded in between, the values beside them.  A prompt whose own attention needs the keys in 16 bits too hands over a ``k_out``.
+    Returns (q, ``k_out``).  Forward only."""
+    ck, cv, sc = _q8_parts(cache, "qk_norm_rope_append_q8_")
+    dev = _here((q, k, v, ck, cv, sc, positions, q_weight, k_weight, freqs, lengths, q_out, k_out), "qk_norm_rope_append_q8_")
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            return qk_norm_rope_append_q8_(q, k, v, cache, positions, num_heads, q_weight, k_weight, eps, freqs, interleaved, magnitude, sinks,
+                                           lengths, q_out, k_out)
+    d, rotary = _heads_checks(q, k, num_heads, q_weight, k_weight, freqs, "qk_norm_rope_append_q8_")
+    B, N, _ = q.shape
+    if v.shape != k.shape or v.dtype is not k.dtype:
+        raise SanaHipError(f"v {v.dtype} {tuple(v.shape)} does not match k {k.dtype} {tuple(k.shape)}")
+    G, window, *parts = _q8_cache(cache, B, d, sinks, "qk_norm_rope_append_q8_")
+    if G * d != k.shape[2]:
+        raise SanaHipError(f"a cache of {G} heads does not match k {tuple(k.shape)} with heads of {d}")
+    position_ptr, length_ptr = _lengths_arg(positions, B, "positions"), _lengths_arg(lengths, B)
+    zero_rest = 1 if q_out is None else 0
+    q_out = _out_like(q, q_out, "q_out")
+    if k_out is not None:
+        _out_like(k, k_out, "k_out")
+    if B * N:
+        _heads(q, k, v, d, rotary, q_weight, k_weight, eps, freqs, interleaved, magnitude, position_ptr, length_ptr, q_out, k_out, parts, window, sinks,
+               zero_rest)
+    return q_out, k_out
+
+
+def window_attention_q8(q: torch.Tensor, cache: Sequence[torch.Tensor], positions: torch.Tensor, num_heads: int, sinks: int = 0,
+                        scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One token of each stream over its cache of 8 bits (:func:`window_cache_q8`), which holds the token's own key and value already
+    (:func:`qk_norm_rope_append_q8_` or :func:`window_cache_append_q8_` at the same ``positions``): q [B, 1, H*d], bf16 or fp16, H a multiple of the
+    cache's heads, attends to the last ``window`` tokens up to itself and to the first ``sinks``.  ``positions``: int32 [B] on the device, the tokens seen
+    before this one; a negative one is an idle stream, whose output is zero.  A row of the scale NaN makes its head's outputs NaN.  Products with the
+    codes are exact up to fp32 sums; the output is rounded once.  ``out`` must not overlap q or the cache.  Returns [B, 1, H*d].  Forward only."""
+    ck, cv, sc = _q8_parts(cache, "window_attention_q8")
+    dev = _here((q, ck, cv, sc, positions, out), "window_attention_q8")
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            return window_attention_q8(q, cache, positions, num_heads, sinks, scale, out)
+    if q.dim() != 3 or q.shape[1] != 1 or q.dtype not in IO16:
+        raise SanaHipError(f"window_attention_q8 takes one token of each stream, bf16 or fp16 [B, 1, H*d], got {q.dtype} {tuple(q.shape)}")
+    B, _, C = q.shape
+    if num_heads < 1 or C == 0 or C % num_heads:
+        raise SanaHipError(f"{C} channels are not {num_heads} heads")
+    d = C // num_heads
+    if d % 8 or d > 128:
+        raise SanaHipError(f"head_dim {d} has no kernel (multiples of 8 up to 128)")
+    G, window, pointers, strides = _q8_cache(cache, B, d, sinks, "window_attention_q8")
+    if num_heads % G:
+        raise SanaHipError(f"{num_heads} query heads do not share {G} key heads")
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise SanaHipError(f"scale must be positive, got {scale}")
+    position_ptr = _lengths_arg(positions, B, "positions")
+    out = _out_like(q, out, "out")
+    if B == 0:
+        return out
+    lib = _lib.load()
+    nbytes = lib.sana_hip_window_q8_workspace_bytes(B, num_heads, G, d, window, sinks)
+    ws = _call_scratch(q.device, nbytes) if nbytes else None
+    code = lib.sana_hip_window_q8(q.data_ptr(), *pointers, position_ptr, out.data_ptr(), None if ws is None else ws.data_ptr(), nbytes, B, num_heads, G,
+                                  d, window, sinks, _token_rows(q, "q")[0], _token_rows(out, "out")[0], *strides, scale, _DT[q.dtype], _stream())
+    if code:
+        _lib.check(code, "sana_hip_window_q8")
+    return out
+
+
+def window_cache_read(cache: Sequence[torch.Tensor], positions: torch.Tensor, sinks: int = 0, last: Optional[int] = None, dim: Optional[int] = None,
+                      dtype: Optional[torch.dtype] = None, out: Optional[Sequence[torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The rows of a ring cache in the order of their tokens, as :func:`window_attention` takes the past of a chunk: of a stream that has seen
+    ``positions[b]`` = n tokens (int32 [B] on the device), tokens 0 .. n - 1 where those are at most ``sinks + last``, else the ``sinks`` first
+    and the ``last`` ones (None: the window; a chunk needs window - 1).  ``cache``: (keys, values) of :func:`window_cache_append_`, or (codes, codes,
+    scales) of :func:`window_cache_q8`, with heads of ``dim`` channels (None: the codes' width) and the ``dtype`` to read them as
+    (bf16 or fp16, None: bf16).  Returns (k, v) [B, sinks + last, C]; ``out``: a pair to fill, e.g. the front rows of buffers whose last rows
+    are the chunk's.  Rows behind a stream's last token stay in ``out`` as they were (zeros in new ones).  ``out`` must not overlap the cache.  Forward only."""
+    what = "window_cache_read"
+    if len(cache) not in (2, 3) or (out is not None and len(out) != 2):
+        raise SanaHipError(f"{what} reads (keys, values) or (codes, codes, scales) into a pair")
+    dev = _here((*cache, positions, *(out or ())), what)
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            return window_cache_read(cache, positions, sinks, last, dim, dtype, out)
+    ck, cv = cache[0], cache[1]
+    if len(cache) == 2:
+        if ck.dim() != 3 or cv.shape != ck.shape or ck.dtype not in IO16 or cv.dtype is not ck.dtype or dtype not in (None, ck.dtype):
+            raise SanaHipError(f"{what}: a 16-bit cache is bf16 or fp16 [B, rows, C], twice, and read in its dtype, got {ck.dtype} {tuple(ck.shape)}, "
+                               f"{cv.dtype} {tuple(cv.shape)}, {dtype}")
+        B, R, C = ck.shape
+        G, width, dtype = 1, C, ck.dtype
+        if C == 0 or C % 8:
+            raise SanaHipError(f"{what}: rows of {C} channels have no kernel (multiples of 8)")
+        if not 0 <= sinks < R:
+            raise SanaHipError(f"{what}: a cache of {R} rows holds {sinks} sinks and no window")
+        window, pointers = R - sinks, (ck.data_ptr(), cv.data_ptr(), None)
+        strides = (*_token_rows(ck, "cache_k"), *_token_rows(cv, "cache_v"), 0)
+    else:
+        dtype = torch.bfloat16 if dtype is None else dtype
+        if ck.dim() != 4 or dtype not in IO16:
+            raise SanaHipError(f"{what}: codes [B, kv_heads, rows, d'] are read as bf16 or fp16, got {tuple(ck.shape)}, {dtype}")
+        B, width = ck.shape[0], ck.shape[3] if dim is None else dim
+        if width % 8 or not 0 < width <= 128:
+            raise SanaHipError(f"head_dim {width} has no kernel (multiples of 8 up to 128)")
+        G, window, pointers, (kb, vb, sb) = _q8_cache(cache, B, width, sinks, what)
+        strides = (kb, 0, vb, 0, sb)
+    last = window if last is None else last
+    if not 0 <= last <= window or sinks + last < 1:
+        raise SanaHipError(f"{what}: the last {last} tokens of a window of {window} and {sinks} sinks")
+    position_ptr = _lengths_arg(positions, B, "positions")
+    shape = (B, sinks + last, G * width)
+    zero_rest = 1 if out is None else 0
+    if out is None:
+        out = (torch.empty(shape, dtype=dtype, device=ck.device), torch.empty(shape, dtype=dtype, device=ck.device))
+    for t in out:
+        if t.shape != shape or t.dtype is not dtype:
+            raise SanaHipError(f"{what}: out must be two {dtype} {shape}, got {t.dtype} {tuple(t.shape)}")
+    k, v = out
+    if B == 0:
+        return k, v
+    code = _lib.load().sana_hip_window_cache_read(*pointers, position_ptr, k.data_ptr(), v.data_ptr(), B, G, width, window, sinks, last, *strides,
+                                                  *_token_rows(k, "out"), *_token_rows(v, "out"), zero_rest, _DT[dtype], _stream())
+    if code:
+        _lib.check(code, "sana_hip_window_cache_read")
+    return k, v
