@@ -623,7 +623,7 @@ int sana_hip_window_q8(const void* q, const int8_t* codes_k, const int8_t* codes
  *         sana_hip_heads (scales given; ck_stride_n, cv_stride_n unused)
  *   out_k, out_v  [B][sinks + last][Hkv*d] views of the io dtype; last at most window, sinks + last at least 1
  * d % 8 == 0, for codes d <= 128; Hkv*d at most 2^22; window + sinks at most 2^30; B * (sinks + last) below 2^25 for 16-bit rows,
- * B * Hkv * ceil((sinks + last) / 16) for codes; rows 16-byte aligned, their strides multiples of 8.  The outputs must not overlap the caches,
+ * B * Hkv * ceil((sinks + last) / 32) for codes; rows 16-byte aligned, their strides multiples of 8.  The outputs must not overlap the caches,
  * nor their entries each other. */
 int sana_hip_window_cache_read(const void* cache_k, const void* cache_v, const float* scales, const int32_t* positions, void* out_k, void* out_v,
                                int B, int Hkv, int d, int window, int sinks, int last, int64_t ck_stride_b, int64_t ck_stride_n,

@@ -13,8 +13,8 @@ namespace {
 
 struct HeadArgs {
   sana_heads_args a;
-  int gq, gk, gv, per, chunks;  // groups of heads of a token: of queries, of keys, of values; groups a wave takes; waves a token
-  int64_t items;                // workgroups with work
+  int gq, gk, gv, per;  // groups of heads of a token: of queries, of keys, of values; groups that a wave takes
+  uint32_t chunks;      // waves a token
   float inv_d;
 };
 
@@ -45,48 +45,62 @@ __device__ __forceinline__ uint32_t pack_codes(const float* x, float most, float
 }
 
 // A wave takes one token and runs over `per` groups of 64 / LPH heads, U of them at a time; LPH lanes hold a head, 8 channels each.  FAR: pairs
-// half of the rotated channels apart, a lane holds four channels of either half, so a pair never leaves its lane.
+// half of the rotated channels apart, a lane holds four channels of either half, so that a pair never leaves its lane.  Loads are under no condition
+// (a lane without a head or a channel repeats another's): the compiler puts what follows a conditional load, and the wait for it, into the same branch.
 template <typename T, int LPH, bool FAR>
 __global__ __launch_bounds__(256) void heads_kernel(const HeadArgs h) {
   constexpr int HPW = 64 / LPH, U = 4;
   const sana_heads_args& a = h.a;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, j = lane % LPH, sub = lane / LPH;
-  const int64_t per_xcd = (h.items + 7) >> 3, item = (int64_t)(blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
-  if ((int64_t)(blockIdx.x >> 3) >= per_xcd || item >= h.items) return;
   // (uniform: scalars) workgroup -> (stream, four tokens, chunk of the heads)
-  const int blocks = (a.N + 3) / 4, chunk = (int)(item % h.chunks);
-  const int64_t rest = item / h.chunks;
-  const int b = (int)(rest / blocks), t = 4 * (int)(rest - (int64_t)b * blocks) + wave;
+  const uint32_t blocks = ((uint32_t)a.N + 3) / 4, rest = blockIdx.x / h.chunks, chunk = blockIdx.x - rest * h.chunks;
+  const int b = rest / blocks, t = 4 * (rest - b * blocks) + wave;
   if (t >= a.N) return;
   const int pos = a.positions ? a.positions[b] : 0;
   const int n = a.lengths ? min(max(a.lengths[b], 0), a.N) : a.N;
-  const bool live = pos >= 0 && t < n;
-  if (!live && !a.zero_rest) return;
-  const uint32_t p = (uint32_t)pos + (uint32_t)t;
-  const bool kept = live && a.codes_k && (p < (uint32_t)a.sinks || t >= n - a.window);  // (not pushed out by this call's own tokens)
-  const int rows = a.window + a.sinks, slot = p < (uint32_t)a.sinks ? (int)p : a.sinks + (int)((p - (uint32_t)a.sinks) % (uint32_t)a.window);
-  const int d = a.d, dp = (d + 15) & ~15, eighths = a.rotary / 8;
-
-  // this lane's channels: two runs of four
-  const bool turns = j < eighths, far_pair = FAR && turns;
-  const int e0 = FAR ? (far_pair ? 4 * j : 8 * j) : 8 * j, e1 = far_pair ? a.rotary / 2 + 4 * j : e0 + 4;
-  const bool in = 8 * j < d;
-  float c[4], s[4];
-  if (live && turns) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      // in turns and 64 bits: of far positions only the fraction counts
-      const double at = (double)p * (a.freqs[4 * j + i] * 0.15915494309189533577);
-      const float f = (float)(at - __builtin_rint(at));
-      sincospif(2.0f * f, &s[i], &c[i]);
-      c[i] *= a.magnitude, s[i] *= a.magnitude;
-    }
-  }
-  const int g0 = chunk * h.per, g1 = min(g0 + h.per, h.gq + h.gk + h.gv);
+  const int g0 = chunk * h.per, d = a.d;
+  int g1 = min(g0 + h.per, h.gq + h.gk + h.gv);
   const auto kind_of = [&](int g) { return g < h.gq ? 0 : g < h.gq + h.gk ? 1 : 2; };
   const auto head_of = [&](int g, int kind) { return (g - (kind == 0 ? 0 : kind == 1 ? h.gq : h.gq + h.gk)) * HPW + sub; };
-  float w[2][8] = {};  // the norms' weights
-  if (a.q_weight && live && in) {
+  uint16_t* out_rows[2] = {static_cast<uint16_t*>(a.q_out) + b * a.qo_b + t * a.qo_n, static_cast<uint16_t*>(a.k_out) + b * a.ko_b + t * a.ko_n};
+  const bool in = 8 * j < d;
+  if (pos < 0 || t >= n) {  // no token
+    for (int g = g0; g < min(g1, h.gq + h.gk); ++g) {
+      const int kind = kind_of(g), head = head_of(g, kind);
+      if ((a.zero_rest >> kind & 1) && in && head < (kind ? a.Hkv : a.H))
+        *reinterpret_cast<u32x4_t*>((kind ? out_rows[1] : out_rows[0]) + head * d + 8 * j) = u32x4_t{0u, 0u, 0u, 0u};
+    }
+    return;
+  }
+  const uint32_t p = (uint32_t)pos + (uint32_t)t;
+  const bool kept = a.codes_k && (p < (uint32_t)a.sinks || t >= n - a.window);  // (not pushed out by this call's own tokens)
+  if (!kept) g1 = min(g1, a.k_out ? h.gq + h.gk : h.gq);
+  if (g0 >= g1) return;
+  const int rows = a.window + a.sinks, dp = (d + 15) & ~15;
+
+  // this lane's channels: two runs of four
+  const bool turns = 8 * j < a.rotary, far_pair = FAR && turns;
+  const int at8 = in ? 8 * j : 0, e0 = far_pair ? 4 * j : at8, e1 = far_pair ? a.rotary / 2 + 4 * j : at8 + 4;
+  const uint16_t* in_rows[3] = {static_cast<const uint16_t*>(a.q) + b * a.q_b + t * a.q_n, static_cast<const uint16_t*>(a.k) + b * a.k_b + t * a.k_n,
+                                static_cast<const uint16_t*>(a.v) + b * a.v_b + t * a.v_n};
+  u32x2_t x0[U], x1[U];
+  const auto request = [&](int g) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int gu = min(g + u, g1 - 1), kind = kind_of(gu), head = min(head_of(gu, kind), (kind == 0 ? a.H : a.Hkv) - 1);
+      const uint16_t* row = (kind == 0 ? in_rows[0] : kind == 1 ? in_rows[1] : in_rows[2]) + head * d;
+      if constexpr (FAR) {
+        x0[u] = *reinterpret_cast<const u32x2_t*>(row + (kind == 2 ? at8 : e0)), x1[u] = *reinterpret_cast<const u32x2_t*>(row + (kind == 2 ? at8 + 4 : e1));
+      } else {
+        const u32x4_t x = *reinterpret_cast<const u32x4_t*>(row + at8);
+        x0[u] = u32x2_t{x[0], x[1]}, x1[u] = u32x2_t{x[2], x[3]};
+      }
+    }
+  };
+  request(g0);
+
+  float w[2][8];  // the norms' weights
+  if (a.q_weight) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const uint16_t* from = static_cast<const uint16_t*>(k ? a.k_weight : a.q_weight);
@@ -97,90 +111,84 @@ __global__ __launch_bounds__(256) void heads_kernel(const HeadArgs h) {
       }
     }
   }
-  const uint16_t* in_rows[3] = {static_cast<const uint16_t*>(a.q) + b * a.q_b + t * a.q_n, static_cast<const uint16_t*>(a.k) + b * a.k_b + t * a.k_n,
-                                static_cast<const uint16_t*>(a.v) + b * a.v_b + t * a.v_n};
-  uint16_t* out_rows[2] = {static_cast<uint16_t*>(a.q_out) + b * a.qo_b + t * a.qo_n, static_cast<uint16_t*>(a.k_out) + b * a.ko_b + t * a.ko_n};
-
-  for (int g = g0; g < g1; g += U) {
-    u32x2_t x0[U], x1[U];
+  float c[4], s[4];
+  if (turns) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int gu = min(g + u, g1 - 1), kind = kind_of(gu), head = head_of(gu, kind), heads = kind == 0 ? a.H : a.Hkv;
-      const uint16_t* row = (kind == 0 ? in_rows[0] : kind == 1 ? in_rows[1] : in_rows[2]) + head * d;
-      x0[u] = x1[u] = u32x2_t{0u, 0u};
-      if (!live || !in || head >= heads) continue;
-      const bool near8 = !FAR || kind == 2;
-      if (near8) {
-        const u32x4_t x = *reinterpret_cast<const u32x4_t*>(row + 8 * j);
-        x0[u] = u32x2_t{x[0], x[1]}, x1[u] = u32x2_t{x[2], x[3]};
-      } else {
-        x0[u] = *reinterpret_cast<const u32x2_t*>(row + e0), x1[u] = *reinterpret_cast<const u32x2_t*>(row + e1);
-      }
+    for (int i = 0; i < 4; ++i) {
+      // in turns and 64 bits: of far positions only the fraction counts
+      const double at = (double)p * (a.freqs[4 * j + i] * 0.15915494309189533577);
+      sincospif(2.0f * (float)(at - __builtin_rint(at)), &s[i], &c[i]);
+      c[i] *= a.magnitude, s[i] *= a.magnitude;
     }
+  }
+  const int slot = !kept ? 0 : p < (uint32_t)a.sinks ? (int)p : a.sinks + (int)((p - (uint32_t)a.sinks) % (uint32_t)a.window);
+
+#pragma unroll 1
+  for (int g = g0; g < g1; g += U) {
+    float x[U][8];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t v = !in ? 0u : i < 2 ? x0[u][i] : x1[u][i - 2];
+        x[u][2 * i] = lo16<T>(v), x[u][2 * i + 1] = hi16<T>(v);
+      }
+    if (g + U < g1) request(g + U);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int gu = g + u;
       if (gu >= g1) break;
-      const int kind = kind_of(gu), head = head_of(gu, kind), heads = kind == 0 ? a.H : a.Hkv;
-      const bool mine = in && head < heads;
-      const bool near8 = !FAR || kind == 2;
-      const int at0 = near8 ? 8 * j : e0, at1 = near8 ? 8 * j + 4 : e1;
-      float x[8];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t v = i < 2 ? x0[u][i] : x1[u][i - 2];
-        x[2 * i] = lo16<T>(v), x[2 * i + 1] = hi16<T>(v);
-      }
+      const int kind = kind_of(gu), head = head_of(gu, kind);
+      const bool mine = in && head < (kind == 0 ? a.H : a.Hkv), near8 = !FAR || kind == 2;
       if (kind < 2 && a.q_weight) {
         float sq = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sq = fmaf(x[i], x[i], sq);
+        for (int i = 0; i < 8; ++i) sq = fmaf(x[u][i], x[u][i], sq);
         sq = over_head<LPH>(sq, [](float y, float z) { return y + z; });
         const float r = __builtin_amdgcn_rsqf(sq * h.inv_d + a.eps);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = x[i] * r * (kind ? w[1][i] : w[0][i]);
+        for (int i = 0; i < 8; ++i) x[u][i] = x[u][i] * r * (kind ? w[1][i] : w[0][i]);
       }
       if (kind < 2 && turns) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int i0 = FAR ? i : 2 * i, i1 = FAR ? 4 + i : 2 * i + 1;
-          const float y = x[i0], z = x[i1];
-          x[i0] = y * c[i] - z * s[i], x[i1] = y * s[i] + z * c[i];
+          const float y = x[u][i0], z = x[u][i1];
+          x[u][i0] = y * c[i] - z * s[i], x[u][i1] = y * s[i] + z * c[i];
         }
       }
-      uint16_t* to = kind == 0 ? out_rows[0] : out_rows[1];
-      if (kind < 2 && (kind == 0 || a.k_out) && mine && (live || (a.zero_rest >> kind & 1))) {
-        const u32x4_t o = live ? u32x4_t{pk16<T>(x[0], x[1]), pk16<T>(x[2], x[3]), pk16<T>(x[4], x[5]), pk16<T>(x[6], x[7])} : u32x4_t{0u, 0u, 0u, 0u};
-        if (near8) {
-          *reinterpret_cast<u32x4_t*>(to + head * d + 8 * j) = o;
+      if (mine && (kind == 0 || (kind == 1 && a.k_out))) {
+        uint16_t* to = (kind == 0 ? out_rows[0] : out_rows[1]) + head * d;
+        const u32x4_t o = {pk16<T>(x[u][0], x[u][1]), pk16<T>(x[u][2], x[u][3]), pk16<T>(x[u][4], x[u][5]), pk16<T>(x[u][6], x[u][7])};
+        if constexpr (FAR) {
+          *reinterpret_cast<u32x2_t*>(to + e0) = u32x2_t{o[0], o[1]};
+          *reinterpret_cast<u32x2_t*>(to + e1) = u32x2_t{o[2], o[3]};
         } else {
-          *reinterpret_cast<u32x2_t*>(to + head * d + e0) = u32x2_t{o[0], o[1]};
-          *reinterpret_cast<u32x2_t*>(to + head * d + e1) = u32x2_t{o[2], o[3]};
+          *reinterpret_cast<u32x4_t*>(to + at8) = o;
         }
       }
       if (kind > 0 && kept) {
         uint32_t most = 0;  // the largest magnitude, by its bits: NaN above inf
 #pragma unroll
-        for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(x[i]) & 0x7fffffffu);
+        for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(x[u][i]) & 0x7fffffffu);
         most = over_head<LPH>(most, [](uint32_t y, uint32_t z) { return max(y, z); });
         const bool bad = most >= 0x7f800000u;
         const float m = __uint_as_float(most);
-        // (far from 1 in the range of whole powers: a reciprocal that stays a normal number)
-        const float lift = m < 0x1p-100f ? 0x1p100f : m > 0x1p100f ? 0x1p-100f : 1.0f;
-        const float inv = m > 0.f && !bad ? __builtin_amdgcn_rcpf(m * lift) : 0.f;
-        if (!bad) {
+        // (far from 1 by a power of two towards it: a reciprocal that is a normal number)
+        const float lift = m < 0x1p-100f ? 0x1p100f : m > 0x1p100f ? 0x1p-100f : 1.0f, ml = m * lift;
+        const float inv = m > 0.f && !bad ? __builtin_amdgcn_rcpf(ml) : 0.f;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] *= lift;
-        }
-        const uint32_t lo = bad ? 0u : pack_codes(x, m * lift, inv), hi = bad ? 0u : pack_codes(x + 4, m * lift, inv);
+        for (int i = 0; i < 8; ++i) x[u][i] *= lift;
+        const uint32_t lo = bad ? 0u : pack_codes(x[u], ml, inv), hi = bad ? 0u : pack_codes(x[u] + 4, ml, inv);
         if (mine) {
-          int8_t* codes = (kind == 1 ? a.codes_k + b * a.ck_b : a.codes_v + b * a.cv_b) + ((int64_t)head * rows + slot) * dp;
+          const int64_t row = (int64_t)head * rows + slot;
+          int8_t* codes = (kind == 1 ? a.codes_k + b * a.ck_b : a.codes_v + b * a.cv_b) + row * dp;
           if (near8) {
-            *reinterpret_cast<u32x2_t*>(codes + 8 * j) = u32x2_t{lo, hi};
+            *reinterpret_cast<u32x2_t*>(codes + at8) = u32x2_t{lo, hi};
           } else {
-            *reinterpret_cast<uint32_t*>(codes + at0) = lo, *reinterpret_cast<uint32_t*>(codes + at1) = hi;
+            *reinterpret_cast<uint32_t*>(codes + e0) = lo, *reinterpret_cast<uint32_t*>(codes + e1) = hi;
           }
-          if (j == 0) a.scales[b * a.sc_b + 2 * ((int64_t)head * rows + slot) + (kind - 1)] = bad ? __uint_as_float(0x7fc00000u) : m / 127.0f;
+          if (j == 0) a.scales[b * a.sc_b + 2 * row + (kind - 1)] = bad ? __uint_as_float(0x7fc00000u) : m / 127.0f;
         }
       }
     }
@@ -202,9 +210,8 @@ int launch_heads(const sana_heads_args& a, hipStream_t s) {
   const int groups = h.gq + h.gk + h.gv;
   h.per = groups_a_wave((int64_t)a.B * a.N, groups), h.chunks = (groups + h.per - 1) / h.per;
   const int64_t tokens = (int64_t)a.B * ((a.N + 3) / 4);  // (below 2^61)
-  if (tokens >= WA_MAX_BLOCKS || tokens * h.chunks >= WA_MAX_BLOCKS - 8) return SANA_ERR_SHAPE;
-  h.items = tokens * h.chunks;
-  const dim3 grid((unsigned)((h.items + 7) / 8 * 8));
+  if (tokens >= WA_MAX_BLOCKS || tokens * h.chunks >= WA_MAX_BLOCKS) return SANA_ERR_SHAPE;
+  const dim3 grid((unsigned)(tokens * h.chunks));
   if (a.rotary && !a.interleaved) hipLaunchKernelGGL((heads_kernel<T, LPH, true>), grid, dim3(256), 0, s, h);
   else hipLaunchKernelGGL((heads_kernel<T, LPH, false>), grid, dim3(256), 0, s, h);
   return hipGetLastError() == hipSuccess ? SANA_OK : SANA_ERR_LAUNCH;

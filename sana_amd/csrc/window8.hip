@@ -213,81 +213,80 @@ struct ReadArgs {
   const float* scales;
   const int* positions;
   uint16_t *out_k, *out_v;
-  int B, Hkv, d, dp, window, sinks, last, blocks, zero_rest;
+  int B, Hkv, d, dp, window, sinks, last, rows, blocks, zero_rest;  // rows: of a head that a wave takes
   int64_t k_b, k_n, v_b, v_n, sc_b, ok_b, ok_n, ov_b, ov_n;  // k_b .. v_n in bytes
   int64_t items;
 };
 
-// Row i of the output -> the cache's row, -1 behind the last one.
-__device__ __forceinline__ int read_slot(const ReadArgs& a, int pos, int i) {
+// A stream's rows in order (uniform): how many it has, and by how much its tokens lie further in the ring than their output rows behind the sinks.
+struct InOrder {
+  int count, turned;
+};
+__device__ __forceinline__ InOrder in_order(const ReadArgs& a, int pos) {
   const int held = a.sinks + a.last;
-  if (pos <= held) return i < pos ? (i < a.sinks ? i : a.sinks + (i - a.sinks) % a.window) : -1;
-  if (i < a.sinks) return i;
-  return a.sinks + (int)((uint32_t)(pos - a.last - a.sinks + (i - a.sinks)) % (uint32_t)a.window);
+  if (pos <= held) return {max(pos, 0), 0};  // tokens 0 .. pos - 1, none pushed out: row i is row i
+  return {held, (int)((uint32_t)(pos - held) % (uint32_t)a.window)};
+}
+__device__ __forceinline__ int read_slot(const ReadArgs& a, InOrder o, int i) {
+  const int row = i + o.turned;
+  return i < a.sinks ? i : row < a.sinks + a.window ? row : row - a.window;  // (last <= window: once round at most)
 }
 
 // 16-bit rows: a wave copies a row of keys or of values.
 __global__ __launch_bounds__(256) void read16_kernel(const ReadArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int64_t item = (int64_t)blockIdx.x * 4 + wave;
-  if (item >= a.items) return;
-  const int of_v = (int)(item & 1), held = a.sinks + a.last;
-  const int b = (int)((item >> 1) / held), i = (int)((item >> 1) - (int64_t)b * held);
-  const int slot = read_slot(a, a.positions[b], i), width = a.Hkv * a.d;
+  const uint32_t item = 4 * blockIdx.x + wave, held = a.sinks + a.last, rest = item >> 1;
+  if (item >= (uint32_t)a.items) return;
+  const int of_v = item & 1, b = rest / held, i = rest - b * held, width = a.Hkv * a.d;
+  const InOrder o = in_order(a, a.positions[b]);
   uint16_t* to = of_v ? a.out_v + b * a.ov_b + i * a.ov_n : a.out_k + b * a.ok_b + i * a.ok_n;
-  if (slot < 0) {
+  if (i >= o.count) {
     if (a.zero_rest)
       for (int c = 8 * lane; c < width; c += 512) *reinterpret_cast<u32x4_t*>(to + c) = u32x4_t{0u, 0u, 0u, 0u};
     return;
   }
+  const int64_t slot = read_slot(a, o, i);
   const unsigned char* from = of_v ? a.v + b * a.v_b + slot * a.v_n : a.k + b * a.k_b + slot * a.k_n;
   for (int c0 = 8 * lane; c0 < width; c0 += 2048) {
     u32x4_t x[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (c0 + 512 * u < width) x[u] = *reinterpret_cast<const u32x4_t*>(from + 2 * (c0 + 512 * u));
+    for (int u = 0; u < 4; ++u) x[u] = *reinterpret_cast<const u32x4_t*>(from + 2 * min(c0 + 512 * u, width - 8));
 #pragma unroll
     for (int u = 0; u < 4; ++u)
       if (c0 + 512 * u < width) *reinterpret_cast<u32x4_t*>(to + c0 + 512 * u) = x[u];
   }
 }
 
-// Codes: a wave takes RB rows of a head's keys or values, 8 channels a lane; the heads of a block of rows on one XCD, whose L2 puts the pieces of
-// an output row together.
-constexpr int RB = 16;
+// Codes: a wave takes READ_STEPS * R rows of a head's keys or values, R = 64 / (d / 8) in a step, 8 channels a lane.
+constexpr int READ_STEPS = 4;
 template <typename T>
 __global__ __launch_bounds__(256) void read8_kernel(const ReadArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int64_t wgs = (a.items + 3) / 4, per_xcd = (wgs + 7) >> 3, wg = (int64_t)(blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3), item = 4 * wg + wave;
-  if ((int64_t)(blockIdx.x >> 3) >= per_xcd || item >= a.items) return;
-  const int pair = (int)(item % (2 * a.Hkv)), of_v = pair >= a.Hkv, hk = of_v ? pair - a.Hkv : pair;
-  const int64_t rest = item / (2 * a.Hkv);
-  const int b = (int)(rest / a.blocks), i0 = RB * (int)(rest - (int64_t)b * a.blocks);
-  const int held = a.sinks + a.last, rows = a.sinks + a.window, pos = a.positions[b], eighths = a.d / 8, n = min(RB, held - i0) * eighths;
-  const unsigned char* from = (of_v ? a.v + b * a.v_b : a.k + b * a.k_b) + (int64_t)hk * rows * a.dp;
-  const float* scales = a.scales + b * a.sc_b + 2 * (int64_t)hk * rows + of_v;
-  uint16_t* to = (of_v ? a.out_v + b * a.ov_b : a.out_k + b * a.ok_b) + hk * a.d;
+  const uint32_t item = 4 * blockIdx.x + wave, pairs = 2 * a.Hkv, rest = item / pairs, pair = item - rest * pairs;
+  if (item >= (uint32_t)a.items) return;
+  const int of_v = pair >= (uint32_t)a.Hkv, hk = of_v ? pair - a.Hkv : pair, b = rest / a.blocks, i0 = a.rows * (rest - b * a.blocks);
+  const int eighths = a.d / 8, step = 64 / eighths, r = lane / eighths, c = lane - r * eighths;
+  const int end = min(i0 + a.rows, a.sinks + a.last), cached = a.sinks + a.window;
+  const InOrder o = in_order(a, a.positions[b]);
+  const unsigned char* from = (of_v ? a.v + b * a.v_b : a.k + b * a.k_b) + (int64_t)hk * cached * a.dp + 8 * c;
+  const float* scales = a.scales + b * a.sc_b + 2 * (int64_t)hk * cached + of_v;
+  uint16_t* to = (of_v ? a.out_v + b * a.ov_b : a.out_k + b * a.ok_b) + hk * a.d + 8 * c;
   const int64_t to_n = of_v ? a.ov_n : a.ok_n;
-  constexpr int U = RB * 16 / 64;
-  u32x2_t x[U];
-  float s[U];
-  int slot[U];
+  u32x2_t x[READ_STEPS];
+  float s[READ_STEPS];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int idx = lane + 64 * u, r = idx / eighths, c = idx - r * eighths;
-    slot[u] = -1, x[u] = u32x2_t{0u, 0u}, s[u] = 0.f;
-    if (idx < n && (slot[u] = read_slot(a, pos, i0 + r)) >= 0) {
-      x[u] = *reinterpret_cast<const u32x2_t*>(from + (int64_t)slot[u] * a.dp + 8 * c);
-      s[u] = scales[2 * (int64_t)slot[u]];
-    }
+  for (int u = 0; u < READ_STEPS; ++u) {  // (under no condition, so that none waits for another: lanes without a row repeat one)
+    const int64_t slot = read_slot(a, o, min(i0 + u * step + r, end - 1));
+    x[u] = *reinterpret_cast<const u32x2_t*>(from + slot * a.dp);
+    s[u] = scales[2 * slot];
   }
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int idx = lane + 64 * u, r = idx / eighths, c = idx - r * eighths;
-    if (idx >= n || (slot[u] < 0 && !a.zero_rest)) continue;
+  for (int u = 0; u < READ_STEPS; ++u) {
+    const int i = i0 + u * step + r;
     const f32x4_t y = codes_f32(x[u].x), z = codes_f32(x[u].y);
-    *reinterpret_cast<u32x4_t*>(to + (i0 + r) * to_n + 8 * c) =
-        u32x4_t{pk16<T>(y[0] * s[u], y[1] * s[u]), pk16<T>(y[2] * s[u], y[3] * s[u]), pk16<T>(z[0] * s[u], z[1] * s[u]), pk16<T>(z[2] * s[u], z[3] * s[u])};
+    u32x4_t v = {pk16<T>(y[0] * s[u], y[1] * s[u]), pk16<T>(y[2] * s[u], y[3] * s[u]), pk16<T>(z[0] * s[u], z[1] * s[u]), pk16<T>(z[2] * s[u], z[3] * s[u])};
+    if (i >= o.count) v = u32x4_t{0u, 0u, 0u, 0u};
+    if (r < step && i < end && (i < o.count || a.zero_rest)) *reinterpret_cast<u32x4_t*>(to + i * to_n) = v;
   }
 }
 
@@ -402,10 +401,11 @@ SANA_API int sana_hip_window_cache_read(const void* cache_k, const void* cache_v
     hipLaunchKernelGGL(read16_kernel, dim3((unsigned)((a.items + 3) / 4)), dim3(256), 0, s, a);
   } else {
     if (ck_stride_b % 16 || cv_stride_b % 16 || scales_stride_b % 2 || (reinterpret_cast<uintptr_t>(scales) & 7u)) return SANA_ERR_ALIGN;
-    a.k_b = ck_stride_b, a.v_b = cv_stride_b, a.sc_b = scales_stride_b, a.blocks = (int)((held + RB - 1) / RB);
+    a.k_b = ck_stride_b, a.v_b = cv_stride_b, a.sc_b = scales_stride_b;
+    a.rows = READ_STEPS * (64 / (d / 8)), a.blocks = (int)((held + a.rows - 1) / a.rows);
     if ((int64_t)a.blocks * Hkv >= (WA_MAX_BLOCKS << 1) / B) return SANA_ERR_SHAPE;
     a.items = (int64_t)B * a.blocks * 2 * Hkv;
-    const unsigned grid = (unsigned)(((a.items + 3) / 4 + 7) / 8 * 8);
+    const unsigned grid = (unsigned)((a.items + 3) / 4);
     if (io_dtype == SANA_DT_F16) hipLaunchKernelGGL(read8_kernel<F16>, dim3(grid), dim3(256), 0, s, a);
     else hipLaunchKernelGGL(read8_kernel<BF16>, dim3(grid), dim3(256), 0, s, a);
   }
