@@ -14,7 +14,8 @@ namespace {
 struct HeadArgs {
   sana_heads_args a;
   int gq, gk, gv, per;  // groups of heads of a token: of queries, of keys, of values; groups that a wave takes
-  uint32_t chunks;      // waves a token
+  uint32_t chunks;      // workgroups of a tile of tokens
+  int whole, skipped;   // tiles behind the first `whole` ones that are left out: nothing of them stays in the cache
   float inv_d;
 };
 
@@ -44,50 +45,57 @@ __device__ __forceinline__ uint32_t pack_codes(const float* x, float most, float
   return lo | hi;
 }
 
-// A wave takes one token and runs over `per` groups of 64 / LPH heads, U of them at a time; LPH lanes hold a head, 8 channels each.  FAR: pairs
-// half of the rotated channels apart, a lane holds four channels of either half, so that a pair never leaves its lane.  Loads are under no condition
-// (a lane without a head or a channel repeats another's): the compiler puts what follows a conditional load, and the wait for it, into the same branch.
-template <typename T, int LPH, bool FAR>
+// LPH lanes hold a head, 8 channels each.  FAR: pairs half of the rotated channels apart, a lane holds four channels of either half, so that a pair never
+// leaves its lane.  A wave takes one token and `per` groups of 64 / LPH of its heads, or (TOKENS) `per` heads of 64 / LPH consecutive tokens, whose rows
+// in the cache lie side by side; U of them are on their way at a time.  Loads are under no condition (a lane without a head, a channel or a token repeats
+// another's): the compiler puts what follows a conditional load, and the wait for it, into the same branch.
+template <typename T, int LPH, bool FAR, bool TOKENS>
 __global__ __launch_bounds__(256) void heads_kernel(const HeadArgs h) {
-  constexpr int HPW = 64 / LPH, U = 4;
+  constexpr int AT_ONCE = 64 / LPH, U = TOKENS ? 2 : 4, TW = TOKENS ? AT_ONCE : 1;  // TW: tokens of a wave
   const sana_heads_args& a = h.a;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, j = lane % LPH, sub = lane / LPH;
-  // (uniform: scalars) workgroup -> (stream, four tokens, chunk of the heads)
-  const uint32_t blocks = ((uint32_t)a.N + 3) / 4, rest = blockIdx.x / h.chunks, chunk = blockIdx.x - rest * h.chunks;
-  const int b = rest / blocks, t = 4 * (rest - b * blocks) + wave;
-  if (t >= a.N) return;
+  // (uniform: scalars) workgroup -> (stream, tokens, chunk of the heads)
+  const uint32_t blocks = ((uint32_t)a.N + 4 * TW - 1) / (4 * TW) - h.skipped, rest = blockIdx.x / h.chunks, chunk = blockIdx.x - rest * h.chunks;
+  const int b = rest / blocks, tile = rest - b * blocks, first = TW * (4 * (tile + (tile >= h.whole ? h.skipped : 0)) + wave), t = TOKENS ? first + sub : first;
+  if (first >= a.N) return;
   const int pos = a.positions ? a.positions[b] : 0;
-  const int n = a.lengths ? min(max(a.lengths[b], 0), a.N) : a.N;
+  const int n = pos < 0 ? 0 : a.lengths ? min(max(a.lengths[b], 0), a.N) : a.N;  // tokens that there are
   const int g0 = chunk * h.per, d = a.d;
   int g1 = min(g0 + h.per, h.gq + h.gk + h.gv);
-  const auto kind_of = [&](int g) { return g < h.gq ? 0 : g < h.gq + h.gk ? 1 : 2; };
-  const auto head_of = [&](int g, int kind) { return (g - (kind == 0 ? 0 : kind == 1 ? h.gq : h.gq + h.gk)) * HPW + sub; };
-  uint16_t* out_rows[2] = {static_cast<uint16_t*>(a.q_out) + b * a.qo_b + t * a.qo_n, static_cast<uint16_t*>(a.k_out) + b * a.ko_b + t * a.ko_n};
-  const bool in = 8 * j < d;
-  if (pos < 0 || t >= n) {  // no token
-    for (int g = g0; g < min(g1, h.gq + h.gk); ++g) {
+  // groups: those of the queries, of the keys, of the values; heads one by one: the queries', then key and value in turns
+  const auto kind_of = [&](int g) { return g < h.gq ? 0 : !TOKENS ? (g < h.gq + h.gk ? 1 : 2) : h.gv ? 1 + (g - h.gq) % 2 : 1; };
+  const auto head_of = [&](int g, int kind) {
+    if constexpr (TOKENS) return kind == 0 ? g : h.gv ? (g - h.gq) / 2 : g - h.gq;
+    else return (g - (kind == 0 ? 0 : kind == 1 ? h.gq : h.gq + h.gk)) * AT_ONCE + sub;
+  };
+  const bool live = t < n, in = 8 * j < d;
+  const int tc = min(t, a.N - 1);
+  uint16_t* out_rows[2] = {static_cast<uint16_t*>(a.q_out) + b * a.qo_b + tc * a.qo_n, static_cast<uint16_t*>(a.k_out) + b * a.ko_b + tc * a.ko_n};
+  if (first + TW > n && a.zero_rest) {  // rows without a token
+    for (int g = g0; g < g1; ++g) {
       const int kind = kind_of(g), head = head_of(g, kind);
-      if ((a.zero_rest >> kind & 1) && in && head < (kind ? a.Hkv : a.H))
+      if (kind < 2 && (a.zero_rest >> kind & 1) && in && t >= n && t < a.N && head < (kind ? a.Hkv : a.H))
         *reinterpret_cast<u32x4_t*>((kind ? out_rows[1] : out_rows[0]) + head * d + 8 * j) = u32x4_t{0u, 0u, 0u, 0u};
     }
-    return;
   }
+  if (first >= n) return;
   const uint32_t p = (uint32_t)pos + (uint32_t)t;
-  const bool kept = a.codes_k && (p < (uint32_t)a.sinks || t >= n - a.window);  // (not pushed out by this call's own tokens)
-  if (!kept) g1 = min(g1, a.k_out ? h.gq + h.gk : h.gq);
+  const bool kept = live && a.codes_k && (p < (uint32_t)a.sinks || t >= n - a.window);  // (not pushed out by this call's own tokens)
+  const bool any_kept = TOKENS ? __any(kept) : kept;
+  if (!any_kept && !a.k_out) g1 = min(g1, h.gq);
   if (g0 >= g1) return;
   const int rows = a.window + a.sinks, dp = (d + 15) & ~15;
 
   // this lane's channels: two runs of four
   const bool turns = 8 * j < a.rotary, far_pair = FAR && turns;
   const int at8 = in ? 8 * j : 0, e0 = far_pair ? 4 * j : at8, e1 = far_pair ? a.rotary / 2 + 4 * j : at8 + 4;
-  const uint16_t* in_rows[3] = {static_cast<const uint16_t*>(a.q) + b * a.q_b + t * a.q_n, static_cast<const uint16_t*>(a.k) + b * a.k_b + t * a.k_n,
-                                static_cast<const uint16_t*>(a.v) + b * a.v_b + t * a.v_n};
+  const uint16_t* in_rows[3] = {static_cast<const uint16_t*>(a.q) + b * a.q_b + tc * a.q_n, static_cast<const uint16_t*>(a.k) + b * a.k_b + tc * a.k_n,
+                                static_cast<const uint16_t*>(a.v) + b * a.v_b + tc * a.v_n};
   u32x2_t x0[U], x1[U];
   const auto request = [&](int g) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int gu = min(g + u, g1 - 1), kind = kind_of(gu), head = min(head_of(gu, kind), (kind == 0 ? a.H : a.Hkv) - 1);
+      const int gu = min(g + u, g1 - 1), kind = kind_of(gu), head = TOKENS ? head_of(gu, kind) : min(head_of(gu, kind), (kind == 0 ? a.H : a.Hkv) - 1);
       const uint16_t* row = (kind == 0 ? in_rows[0] : kind == 1 ? in_rows[1] : in_rows[2]) + head * d;
       if constexpr (FAR) {
         x0[u] = *reinterpret_cast<const u32x2_t*>(row + (kind == 2 ? at8 : e0)), x1[u] = *reinterpret_cast<const u32x2_t*>(row + (kind == 2 ? at8 + 4 : e1));
@@ -139,7 +147,7 @@ __global__ __launch_bounds__(256) void heads_kernel(const HeadArgs h) {
       const int gu = g + u;
       if (gu >= g1) break;
       const int kind = kind_of(gu), head = head_of(gu, kind);
-      const bool mine = in && head < (kind == 0 ? a.H : a.Hkv), near8 = !FAR || kind == 2;
+      const bool mine = in && live && (TOKENS || head < (kind == 0 ? a.H : a.Hkv)), near8 = !FAR || kind == 2;
       if (kind < 2 && a.q_weight) {
         float sq = 0.f;
 #pragma unroll
@@ -157,6 +165,10 @@ __global__ __launch_bounds__(256) void heads_kernel(const HeadArgs h) {
           x[u][i0] = y * c[i] - z * s[i], x[u][i1] = y * s[i] + z * c[i];
         }
       }
+      // The values as they are in 32 bits: f16's conversion would otherwise be one operation with the product in front of it here, where nothing else
+      // needs the product, and two there, where it goes into 8 bits as well, and the same call with and without a cache differ in a bit.
+#pragma unroll
+      for (int i = 0; i < 8; ++i) asm("" : "+v"(x[u][i]));
       if (mine && (kind == 0 || (kind == 1 && a.k_out))) {
         uint16_t* to = (kind == 0 ? out_rows[0] : out_rows[1]) + head * d;
         const u32x4_t o = {pk16<T>(x[u][0], x[u][1]), pk16<T>(x[u][2], x[u][3]), pk16<T>(x[u][4], x[u][5]), pk16<T>(x[u][6], x[u][7])};
@@ -167,7 +179,7 @@ __global__ __launch_bounds__(256) void heads_kernel(const HeadArgs h) {
           *reinterpret_cast<u32x4_t*>(to + at8) = o;
         }
       }
-      if (kind > 0 && kept) {
+      if (kind > 0 && any_kept) {
         uint32_t most = 0;  // the largest magnitude, by its bits: NaN above inf
 #pragma unroll
         for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(x[u][i]) & 0x7fffffffu);
@@ -180,7 +192,7 @@ __global__ __launch_bounds__(256) void heads_kernel(const HeadArgs h) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[u][i] *= lift;
         const uint32_t lo = bad ? 0u : pack_codes(x[u], ml, inv), hi = bad ? 0u : pack_codes(x[u] + 4, ml, inv);
-        if (mine) {
+        if (mine && kept) {
           const int64_t row = (int64_t)head * rows + slot;
           int8_t* codes = (kind == 1 ? a.codes_k + b * a.ck_b : a.codes_v + b * a.cv_b) + row * dp;
           if (near8) {
@@ -195,30 +207,37 @@ __global__ __launch_bounds__(256) void heads_kernel(const HeadArgs h) {
   }
 }
 
-// Groups of heads that a wave takes of a token: all, and their angles once, where there are tokens enough for every SIMD; else fewer.
-int groups_a_wave(int64_t tokens, int groups) {
-  const int64_t chunks = tokens >= 4096 ? 1 : (4096 + tokens - 1) / tokens;
+// Heads, or groups of them, that a wave takes: many, and their angles once, where there are waves enough.
+int heads_a_wave(int64_t waves, int groups) {
+  const int64_t chunks = waves >= 4096 ? 1 : (4096 + waves - 1) / waves;
   return (int)((groups + (chunks < groups ? chunks : groups) - 1) / (chunks < groups ? chunks : groups));
 }
 
-template <typename T, int LPH>
+template <typename T, int LPH, bool TOKENS>
 int launch_heads(const sana_heads_args& a, hipStream_t s) {
-  constexpr int HPW = 64 / LPH;
+  constexpr int AT_ONCE = 64 / LPH, TW = TOKENS ? AT_ONCE : 1, HW = TOKENS ? 1 : AT_ONCE;
   HeadArgs h = {};
   h.a = a, h.inv_d = 1.0f / a.d;
-  h.gq = (a.H + HPW - 1) / HPW, h.gk = (a.Hkv + HPW - 1) / HPW, h.gv = a.codes_k ? h.gk : 0;
+  h.gq = (a.H + HW - 1) / HW, h.gk = (a.Hkv + HW - 1) / HW, h.gv = a.codes_k ? h.gk : 0;
   const int groups = h.gq + h.gk + h.gv;
-  h.per = groups_a_wave((int64_t)a.B * a.N, groups), h.chunks = (groups + h.per - 1) / h.per;
-  const int64_t tokens = (int64_t)a.B * ((a.N + 3) / 4);  // (below 2^61)
-  if (tokens >= WA_MAX_BLOCKS || tokens * h.chunks >= WA_MAX_BLOCKS) return SANA_ERR_SHAPE;
-  const dim3 grid((unsigned)(tokens * h.chunks));
-  if (a.rotary && !a.interleaved) hipLaunchKernelGGL((heads_kernel<T, LPH, true>), grid, dim3(256), 0, s, h);
-  else hipLaunchKernelGGL((heads_kernel<T, LPH, false>), grid, dim3(256), 0, s, h);
+  // (four heads of TW tokens: us of 2, 4, 8, 16)
+  h.per = TOKENS ? (groups < 4 ? groups : 4) : heads_a_wave((int64_t)a.B * a.N, groups), h.chunks = (groups + h.per - 1) / h.per;
+  constexpr int TILE = 4 * TW;
+  h.whole = (a.sinks + TILE - 1) / TILE;
+  h.skipped = a.codes_k && !a.q && !a.k_out && !a.lengths && a.N > a.window ? (a.N - a.window) / TILE - h.whole : 0;
+  h.skipped = h.skipped < 0 ? 0 : h.skipped;
+  const int64_t tiles = (int64_t)a.B * ((a.N + TILE - 1) / TILE - h.skipped);  // (below 2^61)
+  if (tiles >= WA_MAX_BLOCKS || tiles * h.chunks >= WA_MAX_BLOCKS) return SANA_ERR_SHAPE;
+  const dim3 grid((unsigned)(tiles * h.chunks));
+  if (a.rotary && !a.interleaved) hipLaunchKernelGGL((heads_kernel<T, LPH, true, TOKENS>), grid, dim3(256), 0, s, h);
+  else hipLaunchKernelGGL((heads_kernel<T, LPH, false, TOKENS>), grid, dim3(256), 0, s, h);
   return hipGetLastError() == hipSuccess ? SANA_OK : SANA_ERR_LAUNCH;
 }
+template <typename T, int LPH>
+int heads_as(const sana_heads_args& a, hipStream_t s) { return a.N >= 16 ? launch_heads<T, LPH, true>(a, s) : launch_heads<T, LPH, false>(a, s); }
 template <typename T>
 int heads_of(const sana_heads_args& a, hipStream_t s) {
-  return a.d <= 32 ? launch_heads<T, 4>(a, s) : a.d <= 64 ? launch_heads<T, 8>(a, s) : launch_heads<T, 16>(a, s);
+  return a.d <= 32 ? heads_as<T, 4>(a, s) : a.d <= 64 ? heads_as<T, 8>(a, s) : heads_as<T, 16>(a, s);
 }
 
 }  // namespace

@@ -72,21 +72,24 @@ __global__ __launch_bounds__(64 * NW) void window_q8_kernel(const Window8Args x)
 
   u32x4_t rk[RT][KS], rv[PV];
   f32x2_t rs[(ROWS + 63) / 64];
+  // (scalar bases and 32-bit offsets within a tile; the hint: what is read once leaves the caches to others)
   auto request = [&](int t) {
+    const int left = count - 1 - ROWS * t;
+    const int8_t *k0 = ck + (int64_t)(ROWS * DP) * t, *v0 = cv + (int64_t)(ROWS * DP) * t;
+    const float* s0 = scales + (int64_t)(2 * ROWS) * t;
 #pragma unroll
-    for (int kt = 0; kt < RT; ++kt) {
-      const int8_t* from = ck + (int64_t)min(ROWS * t + 16 * kt + fr, count - 1) * DP;
+    for (int kt = 0; kt < RT; ++kt)
 #pragma unroll
-      for (int s = 0; s < KS; ++s) rk[kt][s] = *reinterpret_cast<const u32x4_t*>(from + 16 * min(4 * s + fg, P - 1));
-    }
+      for (int s = 0; s < KS; ++s)
+        rk[kt][s] = load_stream<true>(reinterpret_cast<const u32x4_t*>(k0 + (uint32_t)(min(16 * kt + fr, left) * DP + 16 * min(4 * s + fg, P - 1))));
 #pragma unroll
     for (int i = 0; i < PV; ++i) {
       const int idx = lane + 64 * i, r = idx / P, c = idx - r * P;
-      rv[i] = *reinterpret_cast<const u32x4_t*>(cv + (int64_t)min(ROWS * t + r, count - 1) * DP + 16 * c);
+      rv[i] = load_stream<true>(reinterpret_cast<const u32x4_t*>(v0 + (uint32_t)(min(r, left) * DP + 16 * c)));
     }
 #pragma unroll
     for (int i = 0; i < (ROWS + 63) / 64; ++i)
-      rs[i] = *reinterpret_cast<const f32x2_t*>(scales + 2 * (int64_t)min(ROWS * t + 64 * i + lane, count - 1));
+      rs[i] = *reinterpret_cast<const f32x2_t*>(s0 + (uint32_t)(2 * min(64 * i + lane, left)));
   };
   f32x4_t oc[DT];
 #pragma unroll
@@ -206,6 +209,42 @@ __global__ __launch_bounds__(64 * NW) void window_q8_kernel(const Window8Args x)
   if (a.splits > 1 && tid < 16) a.part_ml[2 * at] = m, a.part_ml[2 * at + 1] = l;
 }
 
+// The parts of a query head, a workgroup a head: weights 2^(m_s - m) from a lane a part, then eight parts at a time, 32 lanes of four channels each,
+// all of a lane's parts on their way at once; sums in a fixed order.
+constexpr int Q8_MAX_SPLITS = 64;
+template <typename T>
+__global__ __launch_bounds__(256) void q8_join_kernel(const WindowArgs a) {
+  __shared__ float sums[8][128];
+  const int row = blockIdx.x, b = row / a.H, h = row - b * a.H, lane = threadIdx.x & 63, part = threadIdx.x >> 5, c = 4 * (threadIdx.x & 31);
+  if (a.positions[b] < 0) return;
+  const int64_t rows = (int64_t)a.B * a.H;
+  const f32x2_t ml = *reinterpret_cast<const f32x2_t*>(a.part_ml + 2 * (min(lane, a.splits - 1) * rows + row));
+  f32x4_t x[Q8_MAX_SPLITS / 8];
+#pragma unroll
+  for (int i = 0; i < Q8_MAX_SPLITS / 8; ++i)
+    x[i] = *reinterpret_cast<const f32x4_t*>(a.part_o + (min(8 * i + part, a.splits - 1) * rows + row) * a.d + min(c, a.d - 4));
+  const float m = max_wave(ml[0]), f = lane < a.splits ? __builtin_amdgcn_exp2f(ml[0] - m) : 0.f;
+  float l = f == 0.f && ml[1] == ml[1] ? 0.f : f * ml[1];
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) l += __shfl_xor(l, o);
+  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < Q8_MAX_SPLITS / 8; ++i) {
+    const float fi = __shfl(f, 8 * i + part);
+    if (8 * i + part < a.splits)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[r] = fmaf(fi, x[i][r], o[r]);
+  }
+  *reinterpret_cast<f32x4_t*>(&sums[part][c]) = o;
+  __syncthreads();
+  if (threadIdx.x >= 32 || c >= a.d) return;
+  f32x4_t sum = *reinterpret_cast<const f32x4_t*>(&sums[0][c]);
+#pragma unroll
+  for (int i = 1; i < 8; ++i) sum += *reinterpret_cast<const f32x4_t*>(&sums[i][c]);
+  const float inv = 1.0f / l;
+  *reinterpret_cast<u32x2_t*>(a.out + b * a.o_b + h * a.d + c) = u32x2_t{pk16<T>(sum[0] * inv, sum[1] * inv), pk16<T>(sum[2] * inv, sum[3] * inv)};
+}
+
 // ---------------------------------------------------------------------------- rows in order
 
 struct ReadArgs {
@@ -293,7 +332,7 @@ __global__ __launch_bounds__(256) void read8_kernel(const ReadArgs a) {
 int q8_splits(int B, int H, int Hkv, int rows, int d) {
   const int64_t groups = step_groups(B, H, Hkv), bytes = (int64_t)rows * d * 2;
   if (bytes <= (groups <= 128 ? 256 << 10 : 1 << 20)) return 1;
-  const int most = rows / 128 < WA_MAX_SPLITS ? rows / 128 : WA_MAX_SPLITS;
+  const int most = rows / 128 < Q8_MAX_SPLITS ? rows / 128 : Q8_MAX_SPLITS;
   for (int s = 1; s < most; ++s)
     if (groups * s * 32 >= (groups * s + 255) / 256 * 256 * 25) return s;
   return most > 1 ? most : 1;
@@ -303,13 +342,9 @@ template <typename T, int P>
 int launch_q8(const Window8Args& x, hipStream_t s) {
   const WindowArgs& a = x.w;
   const int64_t groups = step_groups(a.B, a.H, a.Hkv);
-  if (a.splits == 1 && groups <= 256)
-    hipLaunchKernelGGL((window_q8_kernel<T, P, 8, 2>), dim3((unsigned)groups), dim3(512), 0, s, x);
-  else
-    hipLaunchKernelGGL((window_q8_kernel<T, P, 4, 4>), dim3((unsigned)groups, (unsigned)a.splits), dim3(256), 0, s, x);
+  hipLaunchKernelGGL((window_q8_kernel<T, P, 8, 2>), dim3((unsigned)groups, (unsigned)a.splits), dim3(512), 0, s, x);
   if (a.splits > 1) {
-    const int rc = launch_join<T>(a, s);
-    if (rc != SANA_OK) return rc;
+    hipLaunchKernelGGL(q8_join_kernel<T>, dim3((unsigned)(a.B * a.H)), dim3(256), 0, s, a);
   }
   return hipGetLastError() == hipSuccess ? SANA_OK : SANA_ERR_LAUNCH;
 }

@@ -1213,13 +1213,17 @@ def _heads(q, k, v, d, rotary, q_weight, k_weight, eps, freqs, interleaved, magn
            zero_rest) -> None:
     """The call itself; all tensors checked.  ``cache``: the pointers and stream strides of :func:`_q8_cache`, or None."""
     B, N, C = k.shape
-    ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
-    rows = lambda t, what: (0, 0) if t is None else _token_rows(t, what)  # noqa: E731
+    no_rows = (0, 0)
+    qp, H, q_rows, qo_rows = (0, 0, no_rows, no_rows) if q is None else (q.data_ptr(), q.shape[2] // d, _token_rows(q, "q"), _token_rows(q_out, "q_out"))
+    qo = 0 if q is None else q_out.data_ptr()
+    ko, ko_rows = (0, no_rows) if k_out is None else (k_out.data_ptr(), _token_rows(k_out, "k_out"))
+    vp, v_rows = (0, no_rows) if v is None else (v.data_ptr(), _token_rows(v, "v"))
+    qw, kw = (0, 0) if q_weight is None else (q_weight.data_ptr(), k_weight.data_ptr())
     pointers, strides = cache or ((0, 0, 0), (0, 0, 0))
     args = _lib.HEADS_ARGS.pack(
-        ptr(q), k.data_ptr(), ptr(v), ptr(q_out), ptr(k_out), ptr(q_weight), ptr(k_weight), ptr(freqs), positions or 0, lengths or 0, *pointers,
-        *rows(q, "q"), *_token_rows(k, "k"), *rows(v, "v"), *rows(q_out, "q_out"), *rows(k_out, "k_out"), *strides,
-        B, N, 0 if q is None else q.shape[2] // d, C // d, d, rotary, 1 if interleaved else 0, window, sinks, zero_rest, _DT[k.dtype], eps, magnitude)
+        qp, k.data_ptr(), vp, qo, ko, qw, kw, freqs.data_ptr() if rotary else 0, positions or 0, lengths or 0, *pointers,
+        *q_rows, *_token_rows(k, "k"), *v_rows, *qo_rows, *ko_rows, *strides,
+        B, N, H, C // d, d, rotary, 1 if interleaved else 0, window, sinks, zero_rest, _DT[k.dtype], eps, magnitude)
     code = _lib.load().sana_hip_heads(args, _stream())
     if code:
         _lib.check(code, "sana_hip_heads")
