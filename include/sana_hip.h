@@ -580,7 +580,7 @@ int sana_hip_window_step(const void* q, const void* k, const void* v, void* cach
  *   q, q_out  [B][N][H*d] views (NULL and H = 0: keys alone), k, v, k_out [B][N][Hkv*d] views, bf16 or f16, each its own strides (batch, token);
  *             q_out may be q itself and k_out k (with its strides), else they must not overlap the inputs
  *   k_out     may be NULL where there is a cache
- *   weights   of the io dtype;  freqs  fp64 [rotary / 2] (any scaling for long contexts is in them)
+ *   weights   of the io dtype, 8-byte aligned;  freqs  fp64 [rotary / 2] (any scaling for long contexts is in them)
  *   positions int32 [B] or NULL (zeros): the position of each entry's first token; negative: an idle stream
  *   lengths   int32 [B] or NULL: entry b has lengths[b] tokens (clamped to 0 .. N)
  *             Rows of q_out and k_out without a token stay as they were, or are zeroed (zero_rest: 1 q_out, 2 k_out, 3 both).

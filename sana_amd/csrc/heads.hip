@@ -35,14 +35,21 @@ __device__ __forceinline__ V over_head(V x, Op op) {
 // x in 8 bits: 127 x / most to the nearest whole number, ties to even; inv is 1 / most up to 2 steps.  The first quotient is mended by what it leaves
 // of 127 x (which is exact for 16-bit x): a tie, which fp32 holds, comes out as itself, and a quotient of two 16-bit floats that is none
 // is at least 2^-19 of itself away from one.  (5 operations in the place of a division's 10.)
-__device__ __forceinline__ uint32_t code_bits(float x, float most, float inv) {
-  const float t = 127.0f * x, y = t * inv;
+// (Of numbers far from 1 all three may be lifted by a power of two: t = 127 x and most by the same.)
+__device__ __forceinline__ uint32_t code_bits(float t, float most, float inv) {
+  const float y = t * inv;
   return __float_as_uint(fmaf(fmaf(-y, most, t), inv, y) + 12582912.0f);  // 1.5 * 2^23: the whole number in the low bits
 }
-__device__ __forceinline__ uint32_t pack_codes(const float* x, float most, float inv) {
-  const uint32_t lo = __builtin_amdgcn_perm(code_bits(x[1], most, inv), code_bits(x[0], most, inv), 0x0c0c0400u);
-  const uint32_t hi = __builtin_amdgcn_perm(code_bits(x[3], most, inv), code_bits(x[2], most, inv), 0x04000c0cu);
+__device__ __forceinline__ uint32_t pack_codes(const float* x, float c127, float most, float inv) {
+  const auto code = [&](int i) { return code_bits(x[i] * c127, most, inv); };
+  const uint32_t lo = __builtin_amdgcn_perm(code(1), code(0), 0x0c0c0400u), hi = __builtin_amdgcn_perm(code(3), code(2), 0x04000c0cu);
   return lo | hi;
+}
+// m / 127, rounded once: the product with 1 / 127, mended by what it leaves (3 operations; a division takes 10).
+__device__ __forceinline__ float scale_of(float m) {
+  constexpr float inv = 1.0f / 127.0f;
+  const float y = m * inv;
+  return m < 0x1p-100f ? m / 127.0f : fmaf(fmaf(-y, 127.0f, m), inv, y);
 }
 
 // LPH lanes hold a head, 8 channels each.  FAR: pairs half of the rotated channels apart, a lane holds four channels of either half, so that a pair never
@@ -112,10 +119,11 @@ __global__ __launch_bounds__(256) void heads_kernel(const HeadArgs h) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const uint16_t* from = static_cast<const uint16_t*>(k ? a.k_weight : a.q_weight);
+      const u32x2_t lo = *reinterpret_cast<const u32x2_t*>(from + e0), hi = *reinterpret_cast<const u32x2_t*>(from + e1);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t bits = from[i < 4 ? e0 + i : e1 + i - 4];
-        w[k][i] = is_f16<T> ? f16_bits_to_f32(bits) : bf16_bits_to_f32(bits);
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t v = i < 2 ? lo[i] : hi[i - 2];
+        w[k][2 * i] = lo16<T>(v), w[k][2 * i + 1] = hi16<T>(v);
       }
     }
   }
@@ -123,13 +131,16 @@ __global__ __launch_bounds__(256) void heads_kernel(const HeadArgs h) {
   if (turns) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      // in turns and 64 bits: of far positions only the fraction counts
+      // in turns and 64 bits: of far positions only the fraction counts.  (Sine and cosine of -1/2 .. 1/2 turn are off by 2.1 2^-24 at most here.)
       const double at = (double)p * (a.freqs[4 * j + i] * 0.15915494309189533577);
-      sincospif(2.0f * (float)(at - __builtin_rint(at)), &s[i], &c[i]);
-      c[i] *= a.magnitude, s[i] *= a.magnitude;
+      const float turn = (float)(at - __builtin_rint(at));
+      c[i] = __builtin_amdgcn_cosf(turn) * a.magnitude, s[i] = __builtin_amdgcn_sinf(turn) * a.magnitude;
     }
   }
   const int slot = !kept ? 0 : p < (uint32_t)a.sinks ? (int)p : a.sinks + (int)((p - (uint32_t)a.sinks) % (uint32_t)a.window);
+  const int64_t head_codes = (int64_t)rows * dp;
+  int8_t *codes_k = a.codes_k + b * a.ck_b + (int64_t)slot * dp, *codes_v = a.codes_v + b * a.cv_b + (int64_t)slot * dp;
+  float* scales = a.scales + b * a.sc_b + 2 * (int64_t)slot;
 
 #pragma unroll 1
   for (int g = g0; g < g1; g += U) {
@@ -180,27 +191,26 @@ __global__ __launch_bounds__(256) void heads_kernel(const HeadArgs h) {
         }
       }
       if (kind > 0 && any_kept) {
-        uint32_t most = 0;  // the largest magnitude, by its bits: NaN above inf
+        float most = 0.f, odd = 0.f;  // odd: NaN if any of them is not finite
 #pragma unroll
-        for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(x[u][i]) & 0x7fffffffu);
-        most = over_head<LPH>(most, [](uint32_t y, uint32_t z) { return max(y, z); });
-        const bool bad = most >= 0x7f800000u;
-        const float m = __uint_as_float(most);
+        for (int i = 0; i < 8; i += 2) most = fmaxf(fmaxf(fabsf(x[u][i]), fabsf(x[u][i + 1])), most);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) odd = fmaf(x[u][i], 0.f, odd);
+        most = over_head<LPH>(most, [](float y, float z) { return fmaxf(y, z); });
+        odd = over_head<LPH>(odd, [](float y, float z) { return y + z; });
+        const bool bad = odd != odd;
         // (far from 1 by a power of two towards it: a reciprocal that is a normal number)
-        const float lift = m < 0x1p-100f ? 0x1p100f : m > 0x1p100f ? 0x1p-100f : 1.0f, ml = m * lift;
-        const float inv = m > 0.f && !bad ? __builtin_amdgcn_rcpf(ml) : 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[u][i] *= lift;
-        const uint32_t lo = bad ? 0u : pack_codes(x[u], ml, inv), hi = bad ? 0u : pack_codes(x[u] + 4, ml, inv);
+        const float lift = most < 0x1p-100f ? 0x1p100f : most > 0x1p100f ? 0x1p-100f : 1.0f, lifted = most * lift;
+        const float inv = most > 0.f ? __builtin_amdgcn_rcpf(lifted) : 0.f, c127 = 127.0f * lift;
+        const uint32_t lo = bad ? 0u : pack_codes(x[u], c127, lifted, inv), hi = bad ? 0u : pack_codes(x[u] + 4, c127, lifted, inv);
         if (mine && kept) {
-          const int64_t row = (int64_t)head * rows + slot;
-          int8_t* codes = (kind == 1 ? a.codes_k + b * a.ck_b : a.codes_v + b * a.cv_b) + row * dp;
+          int8_t* codes = (kind == 1 ? codes_k : codes_v) + head * head_codes;
           if (near8) {
             *reinterpret_cast<u32x2_t*>(codes + at8) = u32x2_t{lo, hi};
           } else {
             *reinterpret_cast<uint32_t*>(codes + e0) = lo, *reinterpret_cast<uint32_t*>(codes + e1) = hi;
           }
-          if (j == 0) a.scales[b * a.sc_b + 2 * row + (kind - 1)] = bad ? __uint_as_float(0x7fc00000u) : m / 127.0f;
+          if (j == 0) scales[(int64_t)head * (2 * rows) + (kind - 1)] = bad ? __uint_as_float(0x7fc00000u) : scale_of(most);
         }
       }
     }
@@ -278,7 +288,7 @@ extern "C" __attribute__((visibility("default"))) int sana_hip_heads(const sana_
   }
   if (misaligned({a.q, a.k, a.q_out, a.k_out}, {a.k_b, a.k_n}) || (a.q && misaligned({}, {a.q_b, a.q_n, a.qo_b, a.qo_n})) ||
       (a.k_out && misaligned({}, {a.ko_b, a.ko_n})) || off4(a.positions) || off4(a.lengths) ||
-      ((reinterpret_cast<uintptr_t>(a.q_weight) | reinterpret_cast<uintptr_t>(a.k_weight)) & 1u) || (reinterpret_cast<uintptr_t>(a.freqs) & 7u))
+      ((reinterpret_cast<uintptr_t>(a.q_weight) | reinterpret_cast<uintptr_t>(a.k_weight)) & 7u) || (reinterpret_cast<uintptr_t>(a.freqs) & 7u))
     return SANA_ERR_ALIGN;
   hipStream_t s = static_cast<hipStream_t>(stream);
   return a.io_dtype == SANA_DT_F16 ? heads_of<F16>(a, s) : heads_of<BF16>(a, s);

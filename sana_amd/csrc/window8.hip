@@ -47,14 +47,7 @@ __global__ __launch_bounds__(64 * NW) void window_q8_kernel(const Window8Args x)
   float* my_scales = reinterpret_cast<float*>(mine + TILE);  // of the keys, then of the values
   const int G = a.H / a.Hkv, blocks = (G + 15) / 16, d = a.d;
   const int split = blockIdx.y, gb = blockIdx.x % blocks, bk = blockIdx.x / blocks, b = bk / a.Hkv, hk = bk - b * a.Hkv;
-  const int pos = a.positions[b];
-  if (pos < 0) {  // an idle stream: zeros
-    if (split == 0 && gb == 0)
-      for (int c = tid; c < G * d; c += 64 * NW) a.out[b * a.o_b + hk * G * d + c] = 0;
-    return;
-  }
-  const int rows = a.window + a.sinks, count = pos < rows ? pos + 1 : rows;
-  const int tiles = (count + ROWS - 1) / ROWS, t0 = (int)((int64_t)tiles * split / a.splits), t1 = (int)((int64_t)tiles * (split + 1) / a.splits);
+  const int pos = a.positions[b], rows = a.window + a.sinks;
   const int64_t head_rows = (int64_t)hk * rows;
   const int8_t *ck = x.ck + b * x.ck_b + head_rows * DP, *cv = x.cv + b * x.cv_b + head_rows * DP;
   const float* scales = x.scales + b * x.sc_b + 2 * head_rows;
@@ -72,9 +65,9 @@ __global__ __launch_bounds__(64 * NW) void window_q8_kernel(const Window8Args x)
 
   u32x4_t rk[RT][KS], rv[PV];
   f32x2_t rs[(ROWS + 63) / 64];
-  // (scalar bases and 32-bit offsets within a tile; the hint: what is read once leaves the caches to others)
+  // (scalar bases and 32-bit offsets within a tile; rows that hold no token yet are read, and count as nothing; the hint: what is read once leaves the caches to others)
   auto request = [&](int t) {
-    const int left = count - 1 - ROWS * t;
+    const int left = rows - 1 - ROWS * t;
     const int8_t *k0 = ck + (int64_t)(ROWS * DP) * t, *v0 = cv + (int64_t)(ROWS * DP) * t;
     const float* s0 = scales + (int64_t)(2 * ROWS) * t;
 #pragma unroll
@@ -91,12 +84,23 @@ __global__ __launch_bounds__(64 * NW) void window_q8_kernel(const Window8Args x)
     for (int i = 0; i < (ROWS + 63) / 64; ++i)
       rs[i] = *reinterpret_cast<const f32x2_t*>(s0 + (uint32_t)(2 * min(64 * i + lane, left)));
   };
+  // A whole cache's first tiles are on their way before the position has come; of parts it says where they begin.
+  const bool whole = a.splits == 1;
+  if (whole) request(min(wave, (rows - 1) / ROWS));
+  if (pos < 0) {  // an idle stream: zeros
+    if (split == 0 && gb == 0)
+      for (int c = tid; c < G * d; c += 64 * NW) a.out[b * a.o_b + hk * G * d + c] = 0;
+    return;
+  }
+  const int count = pos < rows ? pos + 1 : rows;
+  const int tiles = (count + ROWS - 1) / ROWS, t0 = whole ? 0 : (int)((int64_t)tiles * split / a.splits);
+  const int t1 = whole ? tiles : (int)((int64_t)tiles * (split + 1) / a.splits);
+  if (!whole && t0 + wave < t1) request(t0 + wave);
   f32x4_t oc[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) oc[dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   float mx = -INFINITY, sub = 0.f, sum = 0.f;
   const int trow = 4 * fg + (fr >> 2), tkey = row_key<DK>(trow), piece = fr & 3;
-  if (t0 + wave < t1) request(t0 + wave);
 #pragma unroll 1
   for (int t = t0 + wave; t < t1; t += NW) {
     f32x4_t sc[RT];
@@ -297,8 +301,10 @@ __global__ __launch_bounds__(256) void read16_kernel(const ReadArgs a) {
 }
 
 // Codes: a wave takes READ_STEPS * R rows of a head's keys or values, R = 64 / (d / 8) in a step, 8 channels a lane.
+// Stores that stay in the caches: a chunk's attention reads the rows next, and takes 12 us longer where they were streamed past (2 x 10920 rows of 20 heads
+// of 112, in front of 1 to 4680 queries), though the call alone, behind the one that wrote the codes, is up to 15 % shorter.
 constexpr int READ_STEPS = 4;
-template <typename T>
+template <typename T, bool NT>
 __global__ __launch_bounds__(256) void read8_kernel(const ReadArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const uint32_t item = 4 * blockIdx.x + wave, pairs = 2 * a.Hkv, rest = item / pairs, pair = item - rest * pairs;
@@ -316,7 +322,7 @@ __global__ __launch_bounds__(256) void read8_kernel(const ReadArgs a) {
 #pragma unroll
   for (int u = 0; u < READ_STEPS; ++u) {  // (under no condition, so that none waits for another: lanes without a row repeat one)
     const int64_t slot = read_slot(a, o, min(i0 + u * step + r, end - 1));
-    x[u] = *reinterpret_cast<const u32x2_t*>(from + slot * a.dp);
+    x[u] = load_stream<NT>(reinterpret_cast<const u32x2_t*>(from + slot * a.dp));
     s[u] = scales[2 * slot];
   }
 #pragma unroll
@@ -329,13 +335,20 @@ __global__ __launch_bounds__(256) void read8_kernel(const ReadArgs a) {
   }
 }
 
+template <typename T, bool NT>
+void read8(const ReadArgs& a, unsigned grid, hipStream_t s) { hipLaunchKernelGGL((read8_kernel<T, NT>), dim3(grid), dim3(256), 0, s, a); }
+
+// Parts of a cache's rows.  Short caches are taken whole: parts cost a second launch, 2 us on the device and 3.5 of the host's where calls are issued one by
+// one.  Longer ones of few streams in as many parts as the 256 compute units take at once, one each, but of 64 rows and more; where a few workgroups
+// more than that leave most of a second round idle, in three.  us on the device, whole / by this rule (best of up to 64 parts): 8 key heads of
+// 128 x 1028 rows 13.2 / whole (16 parts 8.8), x 4100 34.6 / 10.3, x 16388 122 / 14.0; 20 of 112 x 4100 33.5 / 12.8; 80 x 4100 35.8 / 21.3; 120 x 4100 37.3 / 27.8; 160 39.0 /
+// whole (3 parts 36.9), 200 41.3 / whole; 260 73.4 / 65.6, 300 x 8200 135 / 113, 400 x 4100 79 / whole (3 parts 83).
 int q8_splits(int B, int H, int Hkv, int rows, int d) {
   const int64_t groups = step_groups(B, H, Hkv), bytes = (int64_t)rows * d * 2;
-  if (bytes <= (groups <= 128 ? 256 << 10 : 1 << 20)) return 1;
-  const int most = rows / 128 < Q8_MAX_SPLITS ? rows / 128 : Q8_MAX_SPLITS;
-  for (int s = 1; s < most; ++s)
-    if (groups * s * 32 >= (groups * s + 255) / 256 * 256 * 25) return s;
-  return most > 1 ? most : 1;
+  if (bytes <= (groups <= 128 ? 256 << 10 : 384 << 10)) return 1;
+  const int most = rows / 64 < Q8_MAX_SPLITS ? rows / 64 : Q8_MAX_SPLITS;
+  const int64_t want = groups <= 256 ? 256 / groups : groups * 100 < (groups + 255) / 256 * 256 * 65 ? 3 : 1;
+  return (int)(want > most ? most : want < 1 ? 1 : want);
 }
 
 template <typename T, int P>
@@ -441,8 +454,11 @@ SANA_API int sana_hip_window_cache_read(const void* cache_k, const void* cache_v
     if ((int64_t)a.blocks * Hkv >= (WA_MAX_BLOCKS << 1) / B) return SANA_ERR_SHAPE;
     a.items = (int64_t)B * a.blocks * 2 * Hkv;
     const unsigned grid = (unsigned)((a.items + 3) / 4);
-    if (io_dtype == SANA_DT_F16) hipLaunchKernelGGL(read8_kernel<F16>, dim3(grid), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL(read8_kernel<BF16>, dim3(grid), dim3(256), 0, s, a);
+    // Codes beyond the 32 MB of the L2s are read once and past them.  us, written and read back, kept / streamed: 24 MB 26 / 30; 34 MB 47 / 41, 56 MB 40 / 36, 98 MB
+    // 116 / 118 (and in front of a chunk's attention 143 / 138).
+    const bool nt = 2 * B * held * Hkv * a.dp > (32 << 20);
+    if (io_dtype == SANA_DT_F16) nt ? read8<F16, true>(a, grid, s) : read8<F16, false>(a, grid, s);
+    else nt ? read8<BF16, true>(a, grid, s) : read8<BF16, false>(a, grid, s);
   }
   return hipGetLastError() == hipSuccess ? SANA_OK : SANA_ERR_LAUNCH;
 }

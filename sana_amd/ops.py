@@ -5,6 +5,7 @@ checks, without a launch: empty outputs, and an all-zero state for no tokens.
 """
 from __future__ import annotations
 
+import functools
 import math
 import threading
 from typing import Optional, Sequence, Tuple
@@ -1165,12 +1166,15 @@ def _q8_cache(cache, B: int, d: int, sinks: int, what: str) -> Tuple[int, int, T
         raise SanaHipError(f"{what}: codes int8 [{B}, kv_heads, rows, {(d + 15) // 16 * 16}] and scales fp32 [{B}, kv_heads, rows, 2] are a cache of "
                            f"heads of {d}, got {ck.dtype} {tuple(shape)}, {cv.dtype} {tuple(cv.shape)}, {sc.dtype} {tuple(sc.shape)}")
     _, G, R, width = shape
-    strides = []
-    for t, w in ((ck, width), (cv, width), (sc, 2)):
-        b, g, n, c = t.stride()
-        if c != 1 or (n != w and R > 1) or (g != R * w and G > 1):
-            raise SanaHipError(f"{what}: each stream of a cache must be dense, got strides {t.stride()} of {tuple(t.shape)}")
-        strides.append(b if B > 1 else 0)
+    if ck.is_contiguous() and cv.is_contiguous() and sc.is_contiguous():
+        strides = (G * R * width, G * R * width, 2 * G * R) if B > 1 else (0, 0, 0)
+    else:
+        strides = []
+        for t, w in ((ck, width), (cv, width), (sc, 2)):
+            b, g, n, c = t.stride()
+            if c != 1 or (n != w and R > 1) or (g != R * w and G > 1):
+                raise SanaHipError(f"{what}: each stream of a cache must be dense, got strides {t.stride()} of {tuple(t.shape)}")
+            strides.append(b if B > 1 else 0)
     if not 0 <= sinks < R:
         raise SanaHipError(f"{what}: a cache of {R} rows holds {sinks} sinks and no window")
     return G, R - sinks, (ck.data_ptr(), cv.data_ptr(), sc.data_ptr()), strides
@@ -1312,6 +1316,11 @@ def qk_norm_rope_append_q8_(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, c
     return q_out, k_out
 
 
+@functools.lru_cache(maxsize=256)
+def _q8_bytes(*sizes: int) -> int:
+    return _lib.load().sana_hip_window_q8_workspace_bytes(*sizes)
+
+
 def window_attention_q8(q: torch.Tensor, cache: Sequence[torch.Tensor], positions: torch.Tensor, num_heads: int, sinks: int = 0,
                         scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """One token of each stream over its cache of 8 bits (:func:`window_cache_q8`), which holds the token's own key and value already
@@ -1343,7 +1352,7 @@ def window_attention_q8(q: torch.Tensor, cache: Sequence[torch.Tensor], position
     if B == 0:
         return out
     lib = _lib.load()
-    nbytes = lib.sana_hip_window_q8_workspace_bytes(B, num_heads, G, d, window, sinks)
+    nbytes = _q8_bytes(B, num_heads, G, d, window, sinks)
     ws = _call_scratch(q.device, nbytes) if nbytes else None
     code = lib.sana_hip_window_q8(q.data_ptr(), *pointers, position_ptr, out.data_ptr(), None if ws is None else ws.data_ptr(), nbytes, B, num_heads, G,
                                   d, window, sinks, _token_rows(q, "q")[0], _token_rows(out, "out")[0], *strides, scale, _DT[q.dtype], _stream())
@@ -1396,7 +1405,7 @@ def window_cache_read(cache: Sequence[torch.Tensor], positions: torch.Tensor, si
     shape = (B, sinks + last, G * width)
     zero_rest = 1 if out is None else 0
     if out is None:
-        out = (torch.empty(shape, dtype=dtype, device=ck.device), torch.empty(shape, dtype=dtype, device=ck.device))
+        out = (cache[0].new_empty(shape), cache[1].new_empty(shape)) if len(cache) == 2 else (ck.new_empty(shape, dtype=dtype), cv.new_empty(shape, dtype=dtype))
     for t in out:
         if t.shape != shape or t.dtype is not dtype:
             raise SanaHipError(f"{what}: out must be two {dtype} {shape}, got {t.dtype} {tuple(t.shape)}")
