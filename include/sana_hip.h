@@ -611,24 +611,37 @@ int sana_hip_heads(const sana_heads_args* args, void* stream);
  * Codes meet q exactly; probabilities (with their row's scale) enter the product as two bf16 each (2^-16), maxima, sums and outputs are fp32.
  * Workspace, limits and alignment as in sana_hip_window_step and sana_hip_heads. */
 size_t sana_hip_window_q8_workspace_bytes(int B, int H, int Hkv, int d, int window, int sinks);
-int sana_hip_window_q8(const void* q, const int8_t* codes_k, const int8_t* codes_v, const float* scales, const int32_t* positions, void* out,
-                       void* workspace, size_t workspace_bytes, int B, int H, int Hkv, int d, int window, int sinks, int64_t q_stride_b,
-                       int64_t o_stride_b, int64_t ck_stride_b, int64_t cv_stride_b, int64_t scales_stride_b, float scale, int io_dtype,
-                       void* stream);
+typedef struct sana_window_q8_args {
+  const void* q;
+  const int8_t *codes_k, *codes_v;
+  const float* scales;
+  const int32_t* positions;
+  void *out, *workspace;
+  size_t workspace_bytes;
+  int64_t q_b, o_b, ck_b, cv_b, sc_b;
+  int B, H, Hkv, d, window, sinks, io_dtype;
+  float scale;
+} sana_window_q8_args;
+int sana_hip_window_q8(const sana_window_q8_args* args, void* stream);
 
 /* A cache's rows in the order of their tokens, as sana_hip_window_attention takes them: of a stream that has seen n = positions[b] tokens the
  * tokens 0 .. n - 1 where n <= sinks + last, else 0 .. sinks - 1 and n - last .. n - 1; rows behind them stay as they were, or are
  * zeroed (zero_rest).
  *   cache_k, cache_v  16-bit rows as in sana_hip_window_cache_append (scales NULL; strides in elements: batch, row), or the codes of
- *         sana_hip_heads (scales given; ck_stride_n, cv_stride_n unused)
+ *         sana_hip_heads (scales given; ck_n and cv_n unused)
  *   out_k, out_v  [B][sinks + last][Hkv*d] views of the io dtype; last at most window, sinks + last at least 1
  * d % 8 == 0, for codes d <= 128; Hkv*d at most 2^22; window + sinks at most 2^30; B * (sinks + last) below 2^25 for 16-bit rows,
  * B * Hkv * ceil((sinks + last) / 32) for codes; rows 16-byte aligned, their strides multiples of 8.  The outputs must not overlap the caches,
  * nor their entries each other. */
-int sana_hip_window_cache_read(const void* cache_k, const void* cache_v, const float* scales, const int32_t* positions, void* out_k, void* out_v,
-                               int B, int Hkv, int d, int window, int sinks, int last, int64_t ck_stride_b, int64_t ck_stride_n,
-                               int64_t cv_stride_b, int64_t cv_stride_n, int64_t scales_stride_b, int64_t ok_stride_b, int64_t ok_stride_n,
-                               int64_t ov_stride_b, int64_t ov_stride_n, int zero_rest, int io_dtype, void* stream);
+typedef struct sana_cache_read_args {
+  const void *cache_k, *cache_v;
+  const float* scales;
+  const int32_t* positions;
+  void *out_k, *out_v;
+  int64_t ck_b, ck_n, cv_b, cv_n, sc_b, ok_b, ok_n, ov_b, ov_n;
+  int B, Hkv, d, window, sinks, last, zero_rest, io_dtype;
+} sana_cache_read_args;
+int sana_hip_window_cache_read(const sana_cache_read_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -34,9 +34,11 @@ BLOCK_ARGS = struct.Struct("@" + "".join({c_void_p: "P", c_size_t: "N", c_int64:
                                          for _, t in BlockArgs._fields_) + "0q")
 assert BLOCK_ARGS.size == ctypes.sizeof(BlockArgs)
 
-# ``sana_heads_args`` of include/sana_hip.h, its fields in order: 13 pointers, 13 strides, 11 numbers, eps and the rotation's magnitude.  What it
-# packs is handed over as it is (a call spends a microsecond on it, three on a ctypes structure).
-HEADS_ARGS = struct.Struct("@13P13q11i2f0q")
+# ``sana_heads_args``, ``sana_window_q8_args`` and ``sana_cache_read_args`` of include/sana_hip.h, their fields in order.  What these pack is handed over as
+# it is: a call spends half a microsecond on it, more than one on as many arguments and three on a ctypes structure.
+HEADS_ARGS = struct.Struct("@13P13q11i2f0q")    # pointers, strides, numbers, eps and the rotation's magnitude
+WINDOW_Q8_ARGS = struct.Struct("@7PN5q7if0q")   # pointers, workspace bytes, strides, numbers, scale
+CACHE_READ_ARGS = struct.Struct("@6P9q8i0q")    # pointers, strides, numbers
 
 # name -> (restype, argtypes); must list every symbol include/sana_hip.h declares
 SIGNATURES = {
@@ -129,12 +131,8 @@ SIGNATURES = {
                                      c_int64, c_int64, c_int64, c_float, c_int, c_void_p]),
     "sana_hip_heads": (c_int, [c_void_p, c_void_p]),
     "sana_hip_window_q8_workspace_bytes": (c_size_t, [c_int] * 6),
-    "sana_hip_window_q8": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
-                                   c_int, c_int, c_int, c_int, c_int, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_float,
-                                   c_int, c_void_p]),
-    "sana_hip_window_cache_read": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
-                                           c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,
-                                           c_int, c_int, c_void_p]),
+    "sana_hip_window_q8": (c_int, [c_void_p, c_void_p]),
+    "sana_hip_window_cache_read": (c_int, [c_void_p, c_void_p]),
     "sana_hip_layernorm_modulate": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int,
                                             c_int64, c_int64, c_int, c_int64, c_float, c_int, c_void_p]),
 }

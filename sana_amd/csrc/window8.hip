@@ -388,10 +388,15 @@ SANA_API size_t sana_hip_window_q8_workspace_bytes(int B, int H, int Hkv, int d,
   return part_bytes(q8_splits(B, H, Hkv, window + sinks, d), (int64_t)B * H, d);
 }
 
-SANA_API int sana_hip_window_q8(const void* q, const int8_t* codes_k, const int8_t* codes_v, const float* scales, const int32_t* positions, void* out,
-                                void* workspace, size_t workspace_bytes, int B, int H, int Hkv, int d, int window, int sinks, int64_t q_stride_b,
-                                int64_t o_stride_b, int64_t ck_stride_b, int64_t cv_stride_b, int64_t scales_stride_b, float scale, int io_dtype,
-                                void* stream) {
+SANA_API int sana_hip_window_q8(const sana_window_q8_args* args, void* stream) {
+  if (!args) return SANA_ERR_ARG;
+  const void *q = args->q, *codes_k = args->codes_k, *codes_v = args->codes_v;
+  const float* scales = args->scales;
+  const int32_t* positions = args->positions;
+  void *out = args->out, *workspace = args->workspace;
+  const int B = args->B, H = args->H, Hkv = args->Hkv, d = args->d, window = args->window, sinks = args->sinks, io_dtype = args->io_dtype;
+  const int64_t q_stride_b = args->q_b, o_stride_b = args->o_b, ck_stride_b = args->ck_b, cv_stride_b = args->cv_b, scales_stride_b = args->sc_b;
+  const float scale = args->scale;
   if (!q || !codes_k || !codes_v || !scales || !positions || !out || !(scale > 0.f && scale * 1.44269504088896341f < INFINITY)) return SANA_ERR_ARG;
   const int rc = check_sizes(B, 1, H, Hkv, d, window, sinks, io_dtype);
   if (rc != SANA_OK) return rc;
@@ -407,11 +412,11 @@ SANA_API int sana_hip_window_q8(const void* q, const int8_t* codes_k, const int8
   a.q = static_cast<const uint16_t*>(q), a.out = static_cast<uint16_t*>(out), a.positions = positions;
   a.B = B, a.N = 1, a.Nk = 1, a.H = H, a.Hkv = Hkv, a.d = d, a.window = window, a.sinks = sinks, a.q_b = q_stride_b, a.o_b = o_stride_b;
   a.scale_log2e = scale * 1.44269504088896341f;
-  x.ck = codes_k, x.cv = codes_v, x.scales = scales, x.ck_b = ck_stride_b, x.cv_b = cv_stride_b, x.sc_b = scales_stride_b;
+  x.ck = args->codes_k, x.cv = args->codes_v, x.scales = scales, x.ck_b = ck_stride_b, x.cv_b = cv_stride_b, x.sc_b = scales_stride_b;
   a.splits = q8_splits(B, H, Hkv, window + sinks, d);
   const int64_t rows = (int64_t)B * H;
   if (a.splits > 1) {
-    if (!workspace || workspace_bytes < part_bytes(a.splits, rows, d)) return SANA_ERR_WORKSPACE;
+    if (!workspace || args->workspace_bytes < part_bytes(a.splits, rows, d)) return SANA_ERR_WORKSPACE;
     if (!aligned16(workspace)) return SANA_ERR_ALIGN;
     a.part_o = static_cast<float*>(workspace), a.part_ml = a.part_o + a.splits * rows * d;
   }
@@ -419,10 +424,15 @@ SANA_API int sana_hip_window_q8(const void* q, const int8_t* codes_k, const int8
   return io_dtype == SANA_DT_F16 ? q8_of<F16>(x, s) : q8_of<BF16>(x, s);
 }
 
-SANA_API int sana_hip_window_cache_read(const void* cache_k, const void* cache_v, const float* scales, const int32_t* positions, void* out_k,
-                                        void* out_v, int B, int Hkv, int d, int window, int sinks, int last, int64_t ck_stride_b,
-                                        int64_t ck_stride_n, int64_t cv_stride_b, int64_t cv_stride_n, int64_t scales_stride_b, int64_t ok_stride_b,
-                                        int64_t ok_stride_n, int64_t ov_stride_b, int64_t ov_stride_n, int zero_rest, int io_dtype, void* stream) {
+SANA_API int sana_hip_window_cache_read(const sana_cache_read_args* args, void* stream) {
+  if (!args) return SANA_ERR_ARG;
+  const void *cache_k = args->cache_k, *cache_v = args->cache_v;
+  const float* scales = args->scales;
+  const int32_t* positions = args->positions;
+  void *out_k = args->out_k, *out_v = args->out_v;
+  const int B = args->B, Hkv = args->Hkv, d = args->d, window = args->window, sinks = args->sinks, last = args->last, io_dtype = args->io_dtype;
+  const int64_t ck_stride_b = args->ck_b, ck_stride_n = args->ck_n, cv_stride_b = args->cv_b, cv_stride_n = args->cv_n, scales_stride_b = args->sc_b;
+  const int64_t ok_stride_b = args->ok_b, ok_stride_n = args->ok_n, ov_stride_b = args->ov_b, ov_stride_n = args->ov_n;
   if (!cache_k || !cache_v || !positions || !out_k || !out_v || last < 0 || last > window) return SANA_ERR_ARG;
   // (16-bit rows are copied whole: no head's width)
   const int rc = check_sizes(B, 1, Hkv, Hkv, scales ? d : 8, window, sinks, io_dtype);
@@ -438,7 +448,7 @@ SANA_API int sana_hip_window_cache_read(const void* cache_k, const void* cache_v
   ReadArgs a = {};
   a.k = static_cast<const unsigned char*>(cache_k), a.v = static_cast<const unsigned char*>(cache_v), a.scales = scales, a.positions = positions;
   a.out_k = static_cast<uint16_t*>(out_k), a.out_v = static_cast<uint16_t*>(out_v);
-  a.B = B, a.Hkv = Hkv, a.d = d, a.dp = (d + 15) & ~15, a.window = window, a.sinks = sinks, a.last = last, a.zero_rest = zero_rest;
+  a.B = B, a.Hkv = Hkv, a.d = d, a.dp = (d + 15) & ~15, a.window = window, a.sinks = sinks, a.last = last, a.zero_rest = args->zero_rest;
   a.ok_b = ok_stride_b, a.ok_n = ok_stride_n, a.ov_b = ov_stride_b, a.ov_n = ov_stride_n;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (!scales) {

@@ -1205,9 +1205,12 @@ def _heads_checks(q, k, num_heads: int, q_weight, k_weight, freqs, what: str) ->
     return d, r
 
 
+_CONTIGUOUS = torch.contiguous_format
+
+
 def _out_like(t: torch.Tensor, out: Optional[torch.Tensor], what: str) -> torch.Tensor:
     if out is None:
-        return torch.empty_like(t, memory_format=torch.contiguous_format)
+        return torch.empty_like(t, memory_format=_CONTIGUOUS)
     if out.shape != t.shape or out.dtype is not t.dtype:
         raise SanaHipError(f"{what} has the wrong shape or dtype")
     return out
@@ -1218,9 +1221,13 @@ def _heads(q, k, v, d, rotary, q_weight, k_weight, eps, freqs, interleaved, magn
     """The call itself; all tensors checked.  ``cache``: the pointers and stream strides of :func:`_q8_cache`, or None."""
     B, N, C = k.shape
     no_rows = (0, 0)
-    qp, H, q_rows, qo_rows = (0, 0, no_rows, no_rows) if q is None else (q.data_ptr(), q.shape[2] // d, _token_rows(q, "q"), _token_rows(q_out, "q_out"))
-    qo = 0 if q is None else q_out.data_ptr()
-    ko, ko_rows = (0, no_rows) if k_out is None else (k_out.data_ptr(), _token_rows(k_out, "k_out"))
+    if q is None:
+        qp, qo, H, q_rows, qo_rows = 0, 0, 0, no_rows, no_rows
+    else:
+        width = q.shape[2]
+        qp, qo, H, q_rows = q.data_ptr(), q_out.data_ptr(), width // d, _token_rows(q, "q")
+        qo_rows = (N * width if B > 1 else 0, width) if zero_rest & 1 else _token_rows(q_out, "q_out")     # (new ones are contiguous)
+    ko, ko_rows = (0, no_rows) if k_out is None else (k_out.data_ptr(), (N * C if B > 1 else 0, C) if zero_rest & 2 else _token_rows(k_out, "k_out"))
     vp, v_rows = (0, no_rows) if v is None else (v.data_ptr(), _token_rows(v, "v"))
     qw, kw = (0, 0) if q_weight is None else (q_weight.data_ptr(), k_weight.data_ptr())
     pointers, strides = cache or ((0, 0, 0), (0, 0, 0))
@@ -1351,11 +1358,14 @@ def window_attention_q8(q: torch.Tensor, cache: Sequence[torch.Tensor], position
     out = _out_like(q, out, "out")
     if B == 0:
         return out
-    lib = _lib.load()
+    if q.stride(2) != 1 or out.stride(2) != 1:   # (C is a multiple of 8)
+        raise SanaHipError(f"q and out must have unit channel stride, got strides {q.stride()} and {out.stride()}")
     nbytes = _q8_bytes(B, num_heads, G, d, window, sinks)
     ws = _call_scratch(q.device, nbytes) if nbytes else None
-    code = lib.sana_hip_window_q8(q.data_ptr(), *pointers, position_ptr, out.data_ptr(), None if ws is None else ws.data_ptr(), nbytes, B, num_heads, G,
-                                  d, window, sinks, _token_rows(q, "q")[0], _token_rows(out, "out")[0], *strides, scale, _DT[q.dtype], _stream())
+    args = _lib.WINDOW_Q8_ARGS.pack(q.data_ptr(), *pointers, position_ptr, out.data_ptr(), 0 if ws is None else ws.data_ptr(), nbytes,
+                                    q.stride(0) if B > 1 else 0, out.stride(0) if B > 1 else 0, *strides, B, num_heads, G, d, window, sinks,
+                                    _DT[q.dtype], scale)
+    code = _lib.load().sana_hip_window_q8(args, _stream())
     if code:
         _lib.check(code, "sana_hip_window_q8")
     return out
@@ -1387,7 +1397,7 @@ def window_cache_read(cache: Sequence[torch.Tensor], positions: torch.Tensor, si
             raise SanaHipError(f"{what}: rows of {C} channels have no kernel (multiples of 8)")
         if not 0 <= sinks < R:
             raise SanaHipError(f"{what}: a cache of {R} rows holds {sinks} sinks and no window")
-        window, pointers = R - sinks, (ck.data_ptr(), cv.data_ptr(), None)
+        window, pointers = R - sinks, (ck.data_ptr(), cv.data_ptr(), 0)
         strides = (*_token_rows(ck, "cache_k"), *_token_rows(cv, "cache_v"), 0)
     else:
         dtype = torch.bfloat16 if dtype is None else dtype
@@ -1412,8 +1422,9 @@ def window_cache_read(cache: Sequence[torch.Tensor], positions: torch.Tensor, si
     k, v = out
     if B == 0:
         return k, v
-    code = _lib.load().sana_hip_window_cache_read(*pointers, position_ptr, k.data_ptr(), v.data_ptr(), B, G, width, window, sinks, last, *strides,
-                                                  *_token_rows(k, "out"), *_token_rows(v, "out"), zero_rest, _DT[dtype], _stream())
+    args = _lib.CACHE_READ_ARGS.pack(*pointers, position_ptr, k.data_ptr(), v.data_ptr(), *strides, *_token_rows(k, "out"), *_token_rows(v, "out"),
+                                     B, G, width, window, sinks, last, zero_rest, _DT[dtype])
+    code = _lib.load().sana_hip_window_cache_read(args, _stream())
     if code:
         _lib.check(code, "sana_hip_window_cache_read")
     return k, v

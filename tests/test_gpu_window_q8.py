@@ -340,11 +340,12 @@ def test_a_cache_of_more_than_32_bits_of_bytes(cuda):
 def test_calls_that_are_refused_before_any_launch():
     lib, P, bf16 = _lib.load(), 0x10000, _lib.DT_BF16
     ARG, SHAPE, ALIGN, WORK, DTYPE = -1, -2, -3, -4, -6
-    base = dict(q=P, ck=P, cv=P, sc=P, pos=P, out=P, ws=None, bytes=0, B=2, H=4, G=2, d=64, window=20, sinks=0, q_b=256, o_b=256, ck_b=2 * 20 * 64, cv_b=2 * 20 * 64,
-                sc_b=80, scale=0.1, dt=bf16)
-    step = lambda **c: lib.sana_hip_window_q8(*{**base, **c}.values(), None)  # noqa: E731
+    base = dict(q=P, ck=P, cv=P, sc=P, pos=P, out=P, ws=0, bytes=0, q_b=256, o_b=256, ck_b=2 * 20 * 64, cv_b=2 * 20 * 64, sc_b=80, B=2, H=4, G=2, d=64, window=20, sinks=0,
+                dt=bf16, scale=0.1)
+    step = lambda **c: lib.sana_hip_window_q8(_lib.WINDOW_Q8_ARGS.pack(*{**base, **c}.values()), None)  # noqa: E731
+    assert lib.sana_hip_window_q8(None, None) == ARG and lib.sana_hip_window_cache_read(None, None) == ARG
     for n in ("q", "ck", "cv", "sc", "pos", "out"):
-        assert step(**{n: None}) == ARG
+        assert step(**{n: 0}) == ARG
         assert step(**{n: P + 2}) == ALIGN
     for c in (dict(B=0), dict(H=3), dict(G=0), dict(d=0), dict(window=0), dict(sinks=-1), dict(scale=0.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(o_b=248),
               dict(ck_b=-16), dict(q_b=-8)):
@@ -359,17 +360,17 @@ def test_calls_that_are_refused_before_any_launch():
     assert step(window=9000) == WORK and step(window=9000, ws=P, bytes=need - 1) == WORK and step(window=9000, ws=P + 8, bytes=need) == ALIGN
     M = 2 ** 31 - 1
     assert lib.sana_hip_window_q8_workspace_bytes(M, M, M, M, M, M) == 0 and lib.sana_hip_window_q8_workspace_bytes(M, M, 1, 128, 1 << 29, 1 << 29) == 0
-    base2 = dict(ck=P, cv=P, sc=P, pos=P, ok=P, ov=P, B=2, G=2, d=64, window=20, sinks=4, last=20, ck_b=4 << 10, ck_n=128, cv_b=4 << 10, cv_n=128, sc_b=96, ok_b=24 * 128,
-                 ok_n=128, ov_b=24 * 128, ov_n=128, zero=0, dt=bf16)
-    read = lambda **c: lib.sana_hip_window_cache_read(*{**base2, **c}.values(), None)  # noqa: E731
+    base2 = dict(ck=P, cv=P, sc=P, pos=P, ok=P, ov=P, ck_b=4 << 10, ck_n=128, cv_b=4 << 10, cv_n=128, sc_b=96, ok_b=24 * 128, ok_n=128, ov_b=24 * 128, ov_n=128,
+                 B=2, G=2, d=64, window=20, sinks=4, last=20, zero=0, dt=bf16)
+    read = lambda **c: lib.sana_hip_window_cache_read(_lib.CACHE_READ_ARGS.pack(*{**base2, **c}.values()), None)  # noqa: E731
     for n in ("ck", "cv", "pos", "ok", "ov"):
-        assert read(**{n: None}) == ARG
-    for c in (dict(last=21), dict(last=-1), dict(last=0, sinks=0), dict(ok_n=120), dict(ov_b=120), dict(B=0), dict(sc=None, ck_n=120), dict(ck_b=-16), dict(d=0), dict(d=0, sc=None)):
+        assert read(**{n: 0}) == ARG
+    for c in (dict(last=21), dict(last=-1), dict(last=0, sinks=0), dict(ok_n=120), dict(ov_b=120), dict(B=0), dict(sc=0, ck_n=120), dict(ck_b=-16), dict(d=0), dict(d=0, sc=0)):
         assert read(**c) == ARG, c
-    for c in (dict(d=60), dict(d=60, sc=None), dict(d=136), dict(window=1 << 30, last=1 << 30, sinks=4), dict(B=1 << 26), dict(B=1 << 26, sc=None, G=1),
-              dict(d=1 << 22, sc=None, ck_n=1 << 23, cv_n=1 << 23, ok_n=1 << 23, ov_n=1 << 23, ok_b=1 << 30, ov_b=1 << 30)):
+    for c in (dict(d=60), dict(d=60, sc=0), dict(d=136), dict(window=1 << 30, last=1 << 30, sinks=4), dict(B=1 << 26), dict(B=1 << 26, sc=0, G=1),
+              dict(d=1 << 22, sc=0, ck_n=1 << 23, cv_n=1 << 23, ok_n=1 << 23, ov_n=1 << 23, ok_b=1 << 30, ov_b=1 << 30)):
         assert read(**c) == SHAPE, c
-    for c in (dict(ck=P + 8), dict(ok=P + 2), dict(pos=P + 2), dict(sc=P + 4), dict(ck_b=24), dict(sc_b=97), dict(ok_n=132), dict(sc=None, ck_n=132)):
+    for c in (dict(ck=P + 8), dict(ok=P + 2), dict(pos=P + 2), dict(sc=P + 4), dict(ck_b=24), dict(sc_b=97), dict(ok_n=132), dict(sc=0, ck_n=132)):
         assert read(**c) == ALIGN, c
     assert read(dt=0) == DTYPE
 
