@@ -243,8 +243,13 @@ int launch_heads(const sana_heads_args& a, hipStream_t s) {
   else hipLaunchKernelGGL((heads_kernel<T, LPH, false, TOKENS>), grid, dim3(256), 0, s, h);
   return hipGetLastError() == hipSuccess ? SANA_OK : SANA_ERR_LAUNCH;
 }
+// Runs of tokens for many tokens, else heads of one token.  us of all in one pass, heads / tokens: 20 + 20 + 20 heads of 112 1 token 4.0 / 5.3, 64 x 1
+// 4.9 / 6.2, 1000 x 1 12.6 / 27.6, 64 x 16 10.3 / 10.2, 64 x 64 22.6 / 24.2, 2 x 4680 60 / 56; 32 + 8 + 8 of 128 64 x 64 19.5 / 20.6; 16384 tokens of 20 + 20
+// of 112 without a cache 60 / 61, 8 x 2047 of 32 + 8 of 128 in far pairs 64 / 60; into a cache alone 2 x 4680 of 5 of 112 16 / 12, 16 x 4096 of 4 of 128 40 / 23.
 template <typename T, int LPH>
-int heads_as(const sana_heads_args& a, hipStream_t s) { return a.N >= 16 ? launch_heads<T, LPH, true>(a, s) : launch_heads<T, LPH, false>(a, s); }
+int heads_as(const sana_heads_args& a, hipStream_t s) {
+  return a.N >= 64 && (int64_t)a.B * a.N >= 8192 ? launch_heads<T, LPH, true>(a, s) : launch_heads<T, LPH, false>(a, s);
+}
 template <typename T>
 int heads_of(const sana_heads_args& a, hipStream_t s) {
   return a.d <= 32 ? heads_as<T, 4>(a, s) : a.d <= 64 ? heads_as<T, 8>(a, s) : heads_as<T, 16>(a, s);

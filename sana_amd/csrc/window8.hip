@@ -110,7 +110,7 @@ __global__ __launch_bounds__(64 * NW) void window_q8_kernel(const Window8Args x)
     for (int i = 0; i < (ROWS + 63) / 64; ++i)
       if (64 * i + lane < ROWS) {  // (a row that is not there: a value's scale of 0, so that nothing of it counts)
         const bool there = ROWS * t + 64 * i + lane < count;
-        my_scales[64 * i + lane] = rs[i].x * a.scale_log2e;
+        my_scales[64 * i + lane] = rs[i].x;
         my_scales[ROWS + 64 * i + lane] = there ? rs[i].y : 0.f;
       }
 #pragma unroll
@@ -137,7 +137,7 @@ __global__ __launch_bounds__(64 * NW) void window_q8_kernel(const Window8Args x)
       const f32x4_t sk = *reinterpret_cast<const f32x4_t*>(my_scales + 16 * kt + 4 * fg);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        sc[kt][r] = ROWS * t + 16 * kt + 4 * fg + r < count ? sc[kt][r] * sk[r] : -INFINITY;
+        sc[kt][r] = ROWS * t + 16 * kt + 4 * fg + r < count ? sc[kt][r] * a.scale_log2e * sk[r] : -INFINITY;
         most = fmaxf(most, sc[kt][r]);
       }
     }

@@ -330,6 +330,57 @@ def test_all_in_one_pass(cuda, B, N, H, G, d, rotary, window, sinks, interleaved
                 assert (err <= s[:, None] * (0.5 + 2.0 ** -16) + 3 * far[:, None] + 2.0 ** -22 * most[:, None]).all()
 
 
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("B,N,H,G,d,rotary", [(1, 8229, 3, 1, 72, 72), (3, 2999, 2, 2, 32, 16), (2, 4100, 5, 5, 112, 112), (90, 97, 4, 2, 128, 64), (1, 9000, 1, 3, 8, 8), (2, 5000, 3, 2, 64, 0)])
+def test_many_tokens_are_what_they_are_in_pieces(cuda, B, N, H, G, d, rotary, interleaved, dtype):
+    """Runs of tokens a wave and heads of one token a wave: the same numbers, one call or many, with and without a cache."""
+    q, k, v, qw, kw = (t.cuda() for t in make(B, N, H, G, d, dtype, seed=N))
+    f = freqs_of(rotary)
+    args = (qw, kw, 1e-6, None if f is None else f.cuda(), interleaved, 0.9)
+    positions = torch.arange(B) * 1000003 + 5
+    positions[B // 2] = -1 if B > 2 else 17
+    lengths = N - torch.arange(B) * (N // (B + 3))
+    window, sinks, pieces = 600, 130, 1000
+    whole, parts = ([t.cuda() for t in filled(B, G, window + sinks, d)] for _ in range(2))
+    got = ops.qk_norm_rope_append_q8_(q, k, v, whole, i32(positions.tolist()), H, *args, sinks, i32(lengths.tolist()), k_out=torch.zeros_like(k))
+    alone = ops.qk_norm_rope(q, k, H, *args, i32(positions.tolist()), i32(lengths.tolist()))
+    want = torch.zeros_like(q), torch.zeros_like(k)
+    for at in range(0, N, pieces):
+        now = slice(at, min(at + pieces, N))
+        pos = torch.where(positions < 0, positions, positions + at)
+        for b in range(B):     # (piece by piece and stream by stream)
+            one = slice(b, b + 1)
+            n = max(0, min(int(lengths[b]) - at, pieces))
+            outs = ops.qk_norm_rope_append_q8_(q[one, now], k[one, now], v[one, now], [t[one] for t in parts], i32([int(pos[b])]), H, *args, sinks, i32([n]),
+                                               k_out=torch.zeros_like(k[one, now]))
+            want[0][one, now], want[1][one, now] = outs
+    for g, a, w in zip(got, alone, want):
+        assert torch.equal(g, w) and torch.equal(a, w)
+    assert all(torch.equal(a.view(torch.int8 if a.dtype == torch.int8 else torch.int32), b.view(torch.int8 if b.dtype == torch.int8 else torch.int32)) for a, b in zip(whole, parts))
+
+
+@gpu
+@pytest.mark.parametrize("window,sinks,N", [(500, 70, 9000), (5, 0, 8192), (8000, 3, 8300), (9000, 100, 9001), (64, 9500, 9000), (1, 1, 20000)])
+def test_long_appends_leave_out_what_does_not_stay(cuda, window, sinks, N):
+    """All tokens of a call without lengths: those between the sinks and the last window are not even looked at (they are NaN here)."""
+    B, G, d = 3, 2, 40
+    _, k, v, _, _ = (t.cuda() for t in make(B, N, 1, G, d, BF16, seed=window))
+    positions = [0, 50, 1000000]
+    whole, parts = ([t.cuda() for t in filled(B, G, window + sinks, d)] for _ in range(2))
+    for at in range(0, N, 1000):
+        n = min(1000, N - at)
+        ops.window_cache_append_q8_(parts, k[:, at:at + n], v[:, at:at + n], i32([p + at for p in positions]), sinks)
+    for b, p in enumerate(positions):
+        gone = torch.arange(N, device="cuda")
+        gone = (gone + p >= sinks) & (gone < N - window)
+        k[b, gone], v[b, gone] = math.nan, math.nan
+    ops.window_cache_append_q8_(whole, k, v, i32(positions), sinks)
+    # a row of NaN has the scale NaN: none is there, and all are those of the pieces
+    assert all(torch.equal(a, b) for a, b in zip(whole, parts))
+
+
 # --------------------------------------------------------------------------- refusals
 
 def test_calls_that_are_refused_before_any_launch():
