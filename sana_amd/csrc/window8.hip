@@ -46,7 +46,8 @@ __global__ __launch_bounds__(64 * NW) void window_q8_kernel(const Window8Args x)
   unsigned char* mine = smem + wave * OWN;
   float* my_scales = reinterpret_cast<float*>(mine + TILE);  // of the keys, then of the values
   const int G = a.H / a.Hkv, blocks = (G + 15) / 16, d = a.d;
-  const int split = blockIdx.y, gb = blockIdx.x % blocks, bk = blockIdx.x / blocks, b = bk / a.Hkv, hk = bk - b * a.Hkv;
+  const uint32_t split = blockIdx.y, bk = blockIdx.x / (uint32_t)blocks;
+  const int gb = blockIdx.x - bk * blocks, b = bk / (uint32_t)a.Hkv, hk = bk - b * a.Hkv;
   const int pos = a.positions[b], rows = a.window + a.sinks;
   const int64_t head_rows = (int64_t)hk * rows;
   const int8_t *ck = x.ck + b * x.ck_b + head_rows * DP, *cv = x.cv + b * x.cv_b + head_rows * DP;
@@ -93,8 +94,8 @@ __global__ __launch_bounds__(64 * NW) void window_q8_kernel(const Window8Args x)
     return;
   }
   const int count = pos < rows ? pos + 1 : rows;
-  const int tiles = (count + ROWS - 1) / ROWS, t0 = whole ? 0 : (int)((int64_t)tiles * split / a.splits);
-  const int t1 = whole ? tiles : (int)((int64_t)tiles * (split + 1) / a.splits);
+  const int tiles = (count + ROWS - 1) / ROWS;  // (2^25 at most, and 64 parts)
+  const int t0 = whole ? 0 : (int)((uint32_t)tiles * split / a.splits), t1 = whole ? tiles : (int)((uint32_t)tiles * (split + 1) / a.splits);
   if (!whole && t0 + wave < t1) request(t0 + wave);
   f32x4_t oc[DT];
 #pragma unroll
