@@ -11,11 +11,13 @@
 namespace sana {
 namespace {
 
+constexpr int MAX_TILES = 1 << 15;
+
 struct HeadArgs {
   sana_heads_args a;
   int gq, gk, gv, per;  // groups of heads of a token: of queries, of keys, of values; groups that a wave takes
-  uint32_t chunks;      // workgroups of a tile of tokens
   int whole, skipped;   // tiles behind the first `whole` ones that are left out: nothing of them stays in the cache
+  int layers;           // of the grid, of MAX_TILES tiles each, that a stream takes
   float inv_d;
 };
 
@@ -61,12 +63,11 @@ __global__ __launch_bounds__(256) void heads_kernel(const HeadArgs h) {
   constexpr int AT_ONCE = 64 / LPH, U = TOKENS ? 2 : 4, TW = TOKENS ? AT_ONCE : 1;  // TW: tokens of a wave
   const sana_heads_args& a = h.a;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, j = lane % LPH, sub = lane / LPH;
-  // (uniform: scalars) workgroup -> (stream, tokens, chunk of the heads)
-  const uint32_t blocks = ((uint32_t)a.N + 4 * TW - 1) / (4 * TW) - h.skipped, rest = blockIdx.x / h.chunks, chunk = blockIdx.x - rest * h.chunks;
-  const int b = rest / blocks, tile = rest - b * blocks, first = TW * (4 * (tile + (tile >= h.whole ? h.skipped : 0)) + wave), t = TOKENS ? first + sub : first;
+  // workgroup -> (chunk of the heads, tile of tokens, stream); the tiles of a stream in several layers of the grid if they are very many
+  int b = blockIdx.z, tile = blockIdx.y;
+  if (h.layers > 1) b = blockIdx.z / h.layers, tile += (blockIdx.z - b * h.layers) * MAX_TILES;
+  const int chunk = blockIdx.x, first = TW * (4 * (tile + (tile >= h.whole ? h.skipped : 0)) + wave), t = TOKENS ? first + sub : first;
   if (first >= a.N) return;
-  const int pos = a.positions ? a.positions[b] : 0;
-  const int n = pos < 0 ? 0 : a.lengths ? min(max(a.lengths[b], 0), a.N) : a.N;  // tokens that there are
   const int g0 = chunk * h.per, d = a.d;
   int g1 = min(g0 + h.per, h.gq + h.gk + h.gv);
   // groups: those of the queries, of the keys, of the values; heads one by one: the queries', then key and value in turns
@@ -75,27 +76,10 @@ __global__ __launch_bounds__(256) void heads_kernel(const HeadArgs h) {
     if constexpr (TOKENS) return kind == 0 ? g : h.gv ? (g - h.gq) / 2 : g - h.gq;
     else return (g - (kind == 0 ? 0 : kind == 1 ? h.gq : h.gq + h.gk)) * AT_ONCE + sub;
   };
-  const bool live = t < n, in = 8 * j < d;
-  const int tc = min(t, a.N - 1);
-  uint16_t* out_rows[2] = {static_cast<uint16_t*>(a.q_out) + b * a.qo_b + tc * a.qo_n, static_cast<uint16_t*>(a.k_out) + b * a.ko_b + tc * a.ko_n};
-  if (first + TW > n && a.zero_rest) {  // rows without a token
-    for (int g = g0; g < g1; ++g) {
-      const int kind = kind_of(g), head = head_of(g, kind);
-      if (kind < 2 && (a.zero_rest >> kind & 1) && in && t >= n && t < a.N && head < (kind ? a.Hkv : a.H))
-        *reinterpret_cast<u32x4_t*>((kind ? out_rows[1] : out_rows[0]) + head * d + 8 * j) = u32x4_t{0u, 0u, 0u, 0u};
-    }
-  }
-  if (first >= n) return;
-  const uint32_t p = (uint32_t)pos + (uint32_t)t;
-  const bool kept = live && a.codes_k && (p < (uint32_t)a.sinks || t >= n - a.window);  // (not pushed out by this call's own tokens)
-  const bool any_kept = TOKENS ? __any(kept) : kept;
-  if (!any_kept && !a.k_out) g1 = min(g1, h.gq);
-  if (g0 >= g1) return;
-  const int rows = a.window + a.sinks, dp = (d + 15) & ~15;
-
   // this lane's channels: two runs of four
-  const bool turns = 8 * j < a.rotary, far_pair = FAR && turns;
+  const bool in = 8 * j < d, turns = 8 * j < a.rotary, far_pair = FAR && turns;
   const int at8 = in ? 8 * j : 0, e0 = far_pair ? 4 * j : at8, e1 = far_pair ? a.rotary / 2 + 4 * j : at8 + 4;
+  const int tc = min(t, a.N - 1);
   const uint16_t* in_rows[3] = {static_cast<const uint16_t*>(a.q) + b * a.q_b + tc * a.q_n, static_cast<const uint16_t*>(a.k) + b * a.k_b + tc * a.k_n,
                                 static_cast<const uint16_t*>(a.v) + b * a.v_b + tc * a.v_n};
   u32x2_t x0[U], x1[U];
@@ -112,7 +96,28 @@ __global__ __launch_bounds__(256) void heads_kernel(const HeadArgs h) {
       }
     }
   };
-  request(g0);
+  // (before the position has come, unless there may be rows without a token)
+  if (!a.lengths) request(g0);
+
+  const int pos = a.positions ? a.positions[b] : 0;
+  const int n = pos < 0 ? 0 : a.lengths ? min(max(a.lengths[b], 0), a.N) : a.N;  // tokens that there are
+  const bool live = t < n;
+  uint16_t* out_rows[2] = {static_cast<uint16_t*>(a.q_out) + b * a.qo_b + tc * a.qo_n, static_cast<uint16_t*>(a.k_out) + b * a.ko_b + tc * a.ko_n};
+  if (first + TW > n && a.zero_rest) {  // rows without a token
+    for (int g = g0; g < g1; ++g) {
+      const int kind = kind_of(g), head = head_of(g, kind);
+      if (kind < 2 && (a.zero_rest >> kind & 1) && in && t >= n && t < a.N && head < (kind ? a.Hkv : a.H))
+        *reinterpret_cast<u32x4_t*>((kind ? out_rows[1] : out_rows[0]) + head * d + 8 * j) = u32x4_t{0u, 0u, 0u, 0u};
+    }
+  }
+  if (first >= n) return;
+  const uint32_t p = (uint32_t)pos + (uint32_t)t;
+  const bool kept = live && a.codes_k && (p < (uint32_t)a.sinks || t >= n - a.window);  // (not pushed out by this call's own tokens)
+  const bool any_kept = TOKENS ? __any(kept) : kept;
+  if (!any_kept && !a.k_out) g1 = min(g1, h.gq);
+  if (g0 >= g1) return;
+  const int rows = a.window + a.sinks, dp = (d + 15) & ~15;
+  if (a.lengths) request(g0);
 
   float w[2][8];  // the norms' weights
   if (a.q_weight) {
@@ -231,14 +236,15 @@ int launch_heads(const sana_heads_args& a, hipStream_t s) {
   h.gq = (a.H + HW - 1) / HW, h.gk = (a.Hkv + HW - 1) / HW, h.gv = a.codes_k ? h.gk : 0;
   const int groups = h.gq + h.gk + h.gv;
   // (four heads of TW tokens: us of 2, 4, 8, 16)
-  h.per = TOKENS ? (groups < 4 ? groups : 4) : heads_a_wave((int64_t)a.B * a.N, groups), h.chunks = (groups + h.per - 1) / h.per;
+  h.per = TOKENS ? (groups < 4 ? groups : 4) : heads_a_wave((int64_t)a.B * a.N, groups);
   constexpr int TILE = 4 * TW;
   h.whole = (a.sinks + TILE - 1) / TILE;
   h.skipped = a.codes_k && !a.q && !a.k_out && !a.lengths && a.N > a.window ? (a.N - a.window) / TILE - h.whole : 0;
   h.skipped = h.skipped < 0 ? 0 : h.skipped;
-  const int64_t tiles = (int64_t)a.B * ((a.N + TILE - 1) / TILE - h.skipped);  // (below 2^61)
-  if (tiles >= WA_MAX_BLOCKS || tiles * h.chunks >= WA_MAX_BLOCKS) return SANA_ERR_SHAPE;
-  const dim3 grid((unsigned)(tiles * h.chunks));
+  const int chunks = (groups + h.per - 1) / h.per, tiles = (a.N + TILE - 1) / TILE - h.skipped;
+  h.layers = (tiles + MAX_TILES - 1) / MAX_TILES;
+  if ((int64_t)a.B * h.layers > 65535 || (int64_t)chunks * tiles >= WA_MAX_BLOCKS / a.B) return SANA_ERR_SHAPE;
+  const dim3 grid((unsigned)chunks, (unsigned)(h.layers > 1 ? MAX_TILES : tiles), (unsigned)(a.B * h.layers));
   if (a.rotary && !a.interleaved) hipLaunchKernelGGL((heads_kernel<T, LPH, true, TOKENS>), grid, dim3(256), 0, s, h);
   else hipLaunchKernelGGL((heads_kernel<T, LPH, false, TOKENS>), grid, dim3(256), 0, s, h);
   return hipGetLastError() == hipSuccess ? SANA_OK : SANA_ERR_LAUNCH;

@@ -257,7 +257,7 @@ struct ReadArgs {
   const float* scales;
   const int* positions;
   uint16_t *out_k, *out_v;
-  int B, Hkv, d, dp, window, sinks, last, rows, blocks, zero_rest;  // rows: of a head that a wave takes
+  int B, Hkv, d, dp, window, sinks, last, rows, by_eighths, zero_rest;  // rows: of a head that a wave takes; by_eighths: 2^16 / (d / 8), rounded up
   int64_t k_b, k_n, v_b, v_n, sc_b, ok_b, ok_n, ov_b, ov_n;  // k_b .. v_n in bytes
   int64_t items;
 };
@@ -308,10 +308,11 @@ constexpr int READ_STEPS = 4;
 template <typename T, bool NT>
 __global__ __launch_bounds__(256) void read8_kernel(const ReadArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const uint32_t item = 4 * blockIdx.x + wave, pairs = 2 * a.Hkv, rest = item / pairs, pair = item - rest * pairs;
+  // wave -> (head of keys or of values, block of rows); grid -> (four waves, stream)
+  const uint32_t item = 4 * blockIdx.x + wave, pairs = 2 * a.Hkv, block = item / pairs, pair = item - block * pairs;
   if (item >= (uint32_t)a.items) return;
-  const int of_v = pair >= (uint32_t)a.Hkv, hk = of_v ? pair - a.Hkv : pair, b = rest / a.blocks, i0 = a.rows * (rest - b * a.blocks);
-  const int eighths = a.d / 8, step = 64 / eighths, r = lane / eighths, c = lane - r * eighths;
+  const int of_v = pair >= (uint32_t)a.Hkv, hk = of_v ? pair - a.Hkv : pair, b = blockIdx.y, i0 = a.rows * block;
+  const int eighths = a.d / 8, step = 64 / eighths, r = lane * a.by_eighths >> 16, c = lane - r * eighths;
   const int end = min(i0 + a.rows, a.sinks + a.last), cached = a.sinks + a.window;
   const InOrder o = in_order(a, a.positions[b]);
   const unsigned char* from = (of_v ? a.v + b * a.v_b : a.k + b * a.k_b) + (int64_t)hk * cached * a.dp + 8 * c;
@@ -337,7 +338,7 @@ __global__ __launch_bounds__(256) void read8_kernel(const ReadArgs a) {
 }
 
 template <typename T, bool NT>
-void read8(const ReadArgs& a, unsigned grid, hipStream_t s) { hipLaunchKernelGGL((read8_kernel<T, NT>), dim3(grid), dim3(256), 0, s, a); }
+void read8(const ReadArgs& a, dim3 grid, hipStream_t s) { hipLaunchKernelGGL((read8_kernel<T, NT>), grid, dim3(256), 0, s, a); }
 
 // Parts of a cache's rows.  Short caches are taken whole: parts cost a second launch, 2 us on the device and 3.5 of the host's where calls are issued one by
 // one.  Longer ones of few streams in as many parts as the 256 compute units take at once, one each, but of 64 rows and more; where a few workgroups
@@ -461,10 +462,11 @@ SANA_API int sana_hip_window_cache_read(const sana_cache_read_args* args, void* 
   } else {
     if (ck_stride_b % 16 || cv_stride_b % 16 || scales_stride_b % 2 || (reinterpret_cast<uintptr_t>(scales) & 7u)) return SANA_ERR_ALIGN;
     a.k_b = ck_stride_b, a.v_b = cv_stride_b, a.sc_b = scales_stride_b;
-    a.rows = READ_STEPS * (64 / (d / 8)), a.blocks = (int)((held + a.rows - 1) / a.rows);
-    if ((int64_t)a.blocks * Hkv >= (WA_MAX_BLOCKS << 1) / B) return SANA_ERR_SHAPE;
-    a.items = (int64_t)B * a.blocks * 2 * Hkv;
-    const unsigned grid = (unsigned)((a.items + 3) / 4);
+    a.rows = READ_STEPS * (64 / (d / 8));
+    a.by_eighths = (65536 + d / 8 - 1) / (d / 8);
+    a.items = (held + a.rows - 1) / a.rows * 2 * Hkv;
+    if (B > 65535 || a.items >= (WA_MAX_BLOCKS << 2) / B) return SANA_ERR_SHAPE;
+    const dim3 grid((unsigned)((a.items + 3) / 4), (unsigned)B);
     // Codes beyond the 32 MB of the L2s are read once and past them.  us, written and read back, kept / streamed: 24 MB 26 / 30; 34 MB 47 / 41, 56 MB 40 / 36, 98 MB
     // 116 / 118 (and in front of a chunk's attention 143 / 138).
     const bool nt = 2 * B * held * Hkv * a.dp > (32 << 20);
