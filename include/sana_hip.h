@@ -550,7 +550,7 @@ int sana_hip_window_attention(const void* q, const void* k, const void* v, void*
  * window + sinks at most 2^30, N * C / 2048 below 2^24; strides of tokens, and of the caches' entries for B > 1, at least C.  Caches must
  * not overlap k or v, nor their entries each other.
  * Rows of positions that hold no token yet, and tokens that later ones of the call push out, are not written.  A call of many queries over such
- * a cache does not exist: sana_hip_window_attention reads rows in the order of their tokens. */
+ * a cache does not exist: sana_hip_window_attention reads rows in the order of their tokens, into which sana_hip_window_cache_read puts them. */
 int sana_hip_window_cache_append(void* cache_k, void* cache_v, const void* k, const void* v, const int32_t* positions,
                                  const int32_t* lengths, int B, int N, int C, int window, int sinks, int64_t ck_stride_b,
                                  int64_t ck_stride_n, int64_t cv_stride_b, int64_t cv_stride_n, int64_t k_stride_b,
@@ -576,7 +576,7 @@ int sana_hip_window_step(const void* q, const void* k, const void* v, void* cach
  *   cache     keys (normed and rotated) and values in 8 bits into the rows of a ring cache
  *
  * The per-head form of the q/k RMSNorm and the rotary embedding that the reference's attention classes apply one after the other
- * (diffusion/model/nets/sana_blocks.py:88-92, :1572-1582).  In 32 bits, angles in 64, rounded once; into the cache from the unrounded key.
+ * (diffusion/model/norms.py:182-231, diffusion/model/nets/sana_blocks.py:1572-1582).  In 32 bits, angles in 64, rounded once; into the cache from the unrounded key.
  *   q, q_out  [B][N][H*d] views (NULL and H = 0: keys alone), k, v, k_out [B][N][Hkv*d] views, bf16 or f16, each its own strides (batch, token);
  *             q_out may be q itself and k_out k (with its strides), else they must not overlap the inputs
  *   k_out     may be NULL where there is a cache
@@ -588,7 +588,8 @@ int sana_hip_window_step(const void* q, const void* k, const void* v, void* cach
  *             nor written), or NULL: no cache;  scales fp32 [B] times dense [Hkv][sinks + window][2], of a row's key and of its value.
  *             A head's row x is c = round(127 x / max|x|), ties to even, with the scale max|x| / 127; one of inf or NaN has the scale NaN.
  *             Which row a token goes into, and which tokens are not written, as in sana_hip_window_cache_append.
- * d % 8 == 0, d <= 128; rotary % 8 == 0, rotary <= d; H*d and Hkv*d at most 2^22; window + sinks at most 2^30; rows 16-byte aligned, their
+ * d % 8 == 0, d <= 128; rotary % 8 == 0, rotary <= d; H*d and Hkv*d at most 2^22; window + sinks at most 2^30; B * ceil(N / 2^19) at most 65535 and
+ * B * N * (H + 2 Hkv) below 2^28; rows 16-byte aligned, their
  * strides multiples of 8; codes 16-byte aligned, ck_b and cv_b multiples of 16; scales 8-byte aligned, sc_b even; for B > 1 the entries of what
  * is written must not overlap. */
 typedef struct sana_heads_args {
@@ -631,7 +632,7 @@ int sana_hip_window_q8(const sana_window_q8_args* args, void* stream);
  *         sana_hip_heads (scales given; ck_n and cv_n unused)
  *   out_k, out_v  [B][sinks + last][Hkv*d] views of the io dtype; last at most window, sinks + last at least 1
  * d % 8 == 0, for codes d <= 128; Hkv*d at most 2^22; window + sinks at most 2^30; B * (sinks + last) below 2^25 for 16-bit rows,
- * B * Hkv * ceil((sinks + last) / 32) for codes; rows 16-byte aligned, their strides multiples of 8.  The outputs must not overlap the caches,
+ * B * Hkv * ceil((sinks + last) / 16) for codes, B at most 65535; rows 16-byte aligned, their strides multiples of 8.  The outputs must not overlap the caches,
  * nor their entries each other. */
 typedef struct sana_cache_read_args {
   const void *cache_k, *cache_v;

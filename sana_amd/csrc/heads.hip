@@ -57,7 +57,11 @@ __device__ __forceinline__ float scale_of(float m) {
 // LPH lanes hold a head, 8 channels each.  FAR: pairs half of the rotated channels apart, a lane holds four channels of either half, so that a pair never
 // leaves its lane.  A wave takes one token and `per` groups of 64 / LPH of its heads, or (TOKENS) `per` heads of 64 / LPH consecutive tokens, whose rows
 // in the cache lie side by side; U of them are on their way at a time.  Loads are under no condition (a lane without a head, a channel or a token repeats
-// another's): the compiler puts what follows a conditional load, and the wait for it, into the same branch.
+// another's): the compiler puts what follows a conditional load, and the wait for it, into the same branch (16384 tokens of 20 + 20 heads of 112 78 us that
+// way, 60 now).  Memory bounds it, behind some 5 us of ramp and tail a launch: those tokens 294 MB in 51 us = 5.7 TB/s; keys and values of 2 x 4680 tokens
+// into the cache 126 MB in 29; queries as well 210 MB in 51 = 4.1 TB/s, of which either the stores of the queries or those of the codes are 4 (the six
+// streams of rows in and out are what is slow, not the vector unit: without half of a rotation's or of a code's operations the time is the same).  Many
+// short waves beat few long ones: angles in LDS for tiles of 8 to 32 tokens a workgroup 77 us, workgroups in ranges by XCD 69 to 78.
 template <typename T, int LPH, bool FAR, bool TOKENS>
 __global__ __launch_bounds__(256) void heads_kernel(const HeadArgs h) {
   constexpr int AT_ONCE = 64 / LPH, U = TOKENS ? 2 : 4, TW = TOKENS ? AT_ONCE : 1;  // TW: tokens of a wave
@@ -235,7 +239,8 @@ int launch_heads(const sana_heads_args& a, hipStream_t s) {
   h.a = a, h.inv_d = 1.0f / a.d;
   h.gq = (a.H + HW - 1) / HW, h.gk = (a.Hkv + HW - 1) / HW, h.gv = a.codes_k ? h.gk : 0;
   const int groups = h.gq + h.gk + h.gv;
-  // (four heads of TW tokens: us of 2, 4, 8, 16)
+  // (TOKENS: four heads.  us of 2 / 4 / 6 / 8: 16384 tokens - / 60 / 63 / 64, all in one pass 70 / 54 / 53 / 54, 16 x 4096 tokens into short caches 26 / 23 / 28 / 25; and two
+  // of them on their way: 1 / 2 / 4 57 / 55 / 57)
   h.per = TOKENS ? (groups < 4 ? groups : 4) : heads_a_wave((int64_t)a.B * a.N, groups);
   constexpr int TILE = 4 * TW;
   h.whole = (a.sinks + TILE - 1) / TILE;

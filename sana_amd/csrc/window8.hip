@@ -34,7 +34,11 @@ __device__ __forceinline__ u32x4_t codes16(uint32_t lo, uint32_t hi) {
 // One token of each stream.  A workgroup takes a part of the rows of one (stream, key head), its NW waves in turn a tile of 16 * RT rows; the query
 // heads that share the key head are the 16 columns of the products (more than 16 in further workgroups).  K comes from memory as the operand it
 // is (16 channels a lane, two products), V through the wave's own LDS as bf16 to be transposed; its scale goes to the probability, and both as
-// the sum of two bf16 numbers into the product.
+// the sum of two bf16 numbers into the product.  (bf16 for f16 too: a value's scale may be of any size.)
+// Every compute unit busy, memory bounds it: 64 streams x 8196 rows x 8 key heads of 128, 1.06 GB 164 us = 6.4 TB/s, reads alone (179 with loads that stay in the
+// caches; 4, 6, 12 waves 169, 175, 173; 64 rows a wave 185).  One stream of 131136 rows 277 MB in 32 parts 49 us with the join (25 parts 55, 48 parts 60: a part
+// a compute unit).  A short cache is what one compute unit takes in, some 30 bytes a ns behind 6 us of launch, first loads and the waves' sum: 16 key heads of
+// 72 x 1028 rows 165 KB each, 11 us; products of 8-bit numbers in the place of the conversions (q in three slices) 4 % less there and nothing elsewhere.
 template <typename T, int P, int NW, int RT>
 __global__ __launch_bounds__(64 * NW) void window_q8_kernel(const Window8Args x) {
   const WindowArgs& a = x.w;
@@ -214,7 +218,7 @@ __global__ __launch_bounds__(64 * NW) void window_q8_kernel(const Window8Args x)
   if (a.splits > 1 && tid < 16) a.part_ml[2 * at] = m, a.part_ml[2 * at + 1] = l;
 }
 
-// The parts of a query head, a workgroup a head: weights 2^(m_s - m) from a lane a part, then eight parts at a time, 32 lanes of four channels each,
+// The parts of a query head (32 heads in 32 parts 4.4 us), a workgroup a head: weights 2^(m_s - m) from a lane a part, then eight parts at a time, 32 lanes of four channels each,
 // all of a lane's parts on their way at once; sums in a fixed order.
 constexpr int Q8_MAX_SPLITS = 64;
 template <typename T>
@@ -301,7 +305,8 @@ __global__ __launch_bounds__(256) void read16_kernel(const ReadArgs a) {
   }
 }
 
-// Codes: a wave takes READ_STEPS * R rows of a head's keys or values, R = 64 / (d / 8) in a step, 8 channels a lane.
+// Codes: a wave takes READ_STEPS * R rows of a head's keys or values, R = 64 / (d / 8) in a step, 8 channels a lane.  Memory bounds it: 2 x 10920 rows of 20
+// heads of 112, 297 MB 55 - 61 us = 5.2 TB/s (2, 3, 4, 6, 8 steps 64, 62, 62, 63, 64 us a call; with loads under a condition 86).
 // Stores that stay in the caches: a chunk's attention reads the rows next, and takes 12 us longer where they were streamed past (2 x 10920 rows of 20 heads
 // of 112, in front of 1 to 4680 queries), though the call alone, behind the one that wrote the codes, is up to 15 % shorter.
 constexpr int READ_STEPS = 4;

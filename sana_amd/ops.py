@@ -1019,7 +1019,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, num_head
     last query); rows behind them are not read, and stay in ``out`` as they were (zeros in a new one).
     What a query does not see does not reach it, inf and NaN included.  Probabilities are rounded to the inputs' dtype before they
     multiply v.  Returns [B, N, H*d].  ``out`` must not overlap the inputs, nor its entries each other.  k and v are rows in order: a cache of
-    :func:`window_cache_append_` that has wrapped is read by single tokens alone (:func:`window_attention_step_`).
+    :func:`window_cache_append_` that has wrapped is put in order by :func:`window_cache_read` (single tokens take it as it is,
+    :func:`window_attention_step_`).
     Forward only."""
     dev = _here((q, k, v, lengths, out), "window_attention")
     if dev != torch._C._cuda_getDevice():

@@ -103,6 +103,32 @@ def test_the_same_call_again_is_the_same(cuda):
         assert all(torch.equal(a, b) for a, b in zip(turn(s), first)) and all(torch.equal(a, b) for a, b in zip(s[5], held))
 
 
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, torch.float16])
+def test_a_chunk_behind_the_rows_of_its_cache(cuda, dtype):
+    """The past read into the front of a buffer, the chunk's keys normed and rotated into its end and into the cache in one pass: the attention over the
+    buffer is what it is over the same rows put together by single calls."""
+    B, N, H, G, d, window, sinks = 2, 150, 4, 2, 72, 200, 5
+    cache, f = ops.window_cache_q8(B, sinks + window, G, d), ops.rotary_frequencies(d)
+    positions, past = torch.zeros(B, dtype=torch.int32, device="cuda"), 0
+    for chunk in range(4):
+        q, k, v, qw, kw = (t.cuda() for t in make(B, N, H, G, d, dtype, seed=chunk))
+        past = min(past, sinks + window - 1)
+        rows = torch.full((2, B, past + N, G * d), float("nan"), dtype=dtype, device="cuda")
+        if past:
+            ops.window_cache_read(cache, positions, sinks, past - sinks, d, dtype, out=rows[:, :, :past].unbind(0))
+            front = ops.window_cache_read(cache, positions, sinks, past - sinks, d, dtype)
+            assert torch.equal(front[0], rows[0, :, :past]) and torch.equal(front[1], rows[1, :, :past])
+        rows[1, :, past:] = v
+        alone = ops.qk_norm_rope(q, k, H, qw, kw, 1e-6, f, positions=positions)
+        want = ops.window_attention(alone[0], torch.cat([rows[0, :, :past], alone[1]], 1), rows[1].clone(), H, window, sinks)
+        q, back = ops.qk_norm_rope_append_q8_(q, k, v, cache, positions, H, qw, kw, 1e-6, f, sinks=sinks, k_out=rows[0, :, past:])
+        assert torch.equal(back, alone[1]) and torch.equal(q, alone[0]) and not torch.isnan(rows).any()
+        assert torch.equal(ops.window_attention(q, rows[0], rows[1], H, window, sinks), want)
+        positions += N
+        past += N
+
+
 def test_no_cpu_tensors():
     q, k, v, qw, kw = make(1, 1, 2, 1, 32, BF16)
     cache, pos = ops.window_cache_q8(1, 9, 1, 32, device="cpu"), torch.zeros(1, dtype=torch.int32)
