@@ -886,14 +886,13 @@ def gate_residual(y: torch.Tensor, gate: torch.Tensor, residual: torch.Tensor) -
 
 def _here(ts, what: str) -> int:
     """The device index on which all tensors of the call have to be (None entries aside); no derivatives are asked for, of neither mode."""
-    dev = ts[0].get_device()
+    dev, grads = ts[0].get_device(), torch.is_grad_enabled()
     for t in ts:
-        if t is not None and t.get_device() != dev or dev < 0:
-            _need_cuda(*ts)
-            raise SanaHipError(f"{what}: all tensors must be on one device")
-    if torch.is_grad_enabled():
-        for t in ts:
-            if t is not None and t.requires_grad:
+        if t is not None:
+            if t.get_device() != dev or dev < 0:
+                _need_cuda(*ts)
+                raise SanaHipError(f"{what}: all tensors must be on one device")
+            if grads and t.requires_grad:
                 raise SanaHipError(f"{what} is forward only: call it under torch.no_grad() or on detached tensors")
     if forward_ad._current_level >= 0:   # (dual tensors want no gradients, and the output would come without a tangent)
         for t in ts:
@@ -1184,7 +1183,7 @@ def _q8_cache(cache, B: int, d: int, sinks: int, what: str) -> Tuple[int, int, T
 def _heads_checks(q, k, num_heads: int, q_weight, k_weight, freqs, what: str) -> Tuple[int, int]:
     """-> (head_dim, rotated channels) of [B, N, num_heads * d] queries and [B, N, kv_heads * d] keys, their weights and frequencies."""
     dt, qs, ks = q.dtype, q.shape, k.shape
-    if len(qs) != 3 or len(ks) != 3 or dt not in IO16 or k.dtype is not dt or qs[:2] != ks[:2]:
+    if len(qs) != 3 or len(ks) != 3 or dt not in IO16 or k.dtype is not dt or qs[0] != ks[0] or qs[1] != ks[1]:
         raise SanaHipError(f"{what} needs bf16 or fp16 q [B, N, H*d] and k [B, N, Hkv*d] of one dtype, got {dt} {tuple(qs)}, {k.dtype} {tuple(ks)}")
     if num_heads < 1 or qs[2] == 0 or qs[2] % num_heads:
         raise SanaHipError(f"{qs[2]} channels are not {num_heads} heads")
@@ -1195,9 +1194,10 @@ def _heads_checks(q, k, num_heads: int, q_weight, k_weight, freqs, what: str) ->
         raise SanaHipError(f"k {tuple(ks)} does not match q {tuple(qs)} with {num_heads} heads of {d}")
     if (q_weight is None) != (k_weight is None):
         raise SanaHipError(f"{what}: q_weight and k_weight go together")
-    for t in (q_weight, k_weight):
-        if t is not None and (t.dtype is not dt or t.shape != (d,) or not t.is_contiguous()):
-            raise SanaHipError(f"{what}: the norms' weights must be contiguous {dt} [{d}], got {t.dtype} {tuple(t.shape)}")
+    if q_weight is not None:
+        for t in (q_weight, k_weight):
+            if t.dtype is not dt or t.numel() != d or t.dim() != 1 or not t.is_contiguous():
+                raise SanaHipError(f"{what}: the norms' weights must be contiguous {dt} [{d}], got {t.dtype} {tuple(t.shape)}")
     if freqs is None:
         return d, 0
     r = 2 * freqs.numel()
@@ -1261,8 +1261,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, num_heads: int, q_weight: Opt
             return qk_norm_rope(q, k, num_heads, q_weight, k_weight, eps, freqs, interleaved, magnitude, positions, lengths, q_out, k_out)
     d, rotary = _heads_checks(q, k, num_heads, q_weight, k_weight, freqs, "qk_norm_rope")
     B, N, _ = q.shape
-    position_ptr = _lengths_arg(positions, B, "positions")
-    length_ptr = _lengths_arg(lengths, B)
+    position_ptr = None if positions is None else _lengths_arg(positions, B, "positions")
+    length_ptr = None if lengths is None else _lengths_arg(lengths, B)
     zero_rest = (1 if q_out is None else 0) + (2 if k_out is None else 0)
     q_out, k_out = _out_like(q, q_out, "q_out"), _out_like(k, k_out, "k_out")
     if B * N:
@@ -1416,7 +1416,7 @@ def window_cache_read(cache: Sequence[torch.Tensor], positions: torch.Tensor, si
     shape = (B, sinks + last, G * width)
     zero_rest = 1 if out is None else 0
     if out is None:
-        out = (cache[0].new_empty(shape), cache[1].new_empty(shape)) if len(cache) == 2 else (ck.new_empty(shape, dtype=dtype), cv.new_empty(shape, dtype=dtype))
+        out = (ck.new_empty(shape, dtype=dtype), ck.new_empty(shape, dtype=dtype)) if len(cache) == 3 else (ck.new_empty(shape), ck.new_empty(shape))
     for t in out:
         if t.shape != shape or t.dtype is not dtype:
             raise SanaHipError(f"{what}: out must be two {dtype} {shape}, got {t.dtype} {tuple(t.shape)}")
