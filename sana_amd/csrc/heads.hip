@@ -173,7 +173,7 @@ __global__ __launch_bounds__(256) void heads_kernel(const HeadArgs h) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) sq = fmaf(x[u][i], x[u][i], sq);
         sq = over_head<LPH>(sq, [](float y, float z) { return y + z; });
-        const float r = __builtin_amdgcn_rsqf(sq * h.inv_d + a.eps);
+        const float r = rsqrtf(sq * h.inv_d + a.eps);  // (of subnormal numbers too, where eps is 0)
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[u][i] = x[u][i] * r * (kind ? w[1][i] : w[0][i]);
       }

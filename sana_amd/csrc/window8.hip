@@ -363,9 +363,7 @@ int launch_q8(const Window8Args& x, hipStream_t s) {
   const WindowArgs& a = x.w;
   const int64_t groups = step_groups(a.B, a.H, a.Hkv);
   hipLaunchKernelGGL((window_q8_kernel<T, P, 8, 2>), dim3((unsigned)groups, (unsigned)a.splits), dim3(512), 0, s, x);
-  if (a.splits > 1) {
-    hipLaunchKernelGGL(q8_join_kernel<T>, dim3((unsigned)(a.B * a.H)), dim3(256), 0, s, a);
-  }
+  if (a.splits > 1) hipLaunchKernelGGL(q8_join_kernel<T>, dim3((unsigned)(a.B * a.H)), dim3(256), 0, s, a);
   return hipGetLastError() == hipSuccess ? SANA_OK : SANA_ERR_LAUNCH;
 }
 template <typename T>

@@ -133,6 +133,20 @@ def test_scaled_frequencies(cuda):
 
 
 @gpu
+@pytest.mark.parametrize("power", [-64, -60, 0, 55])
+def test_rows_of_any_size_without_eps(cuda, power):
+    """bf16 rows whose squares are far from 1, down to the subnormal numbers of fp32: there a square is off by 2^-150, and so is the mean, of some 2^-128."""
+    H, d = 4, 64
+    q, k, _, qw, kw = make(2, 5, H, 2, d, BF16)
+    q, k = (t.contiguous() * 2.0 ** power for t in (q, k))
+    got = ops.qk_norm_rope(q.cuda(), k.cuda(), H, qw.cuda(), kw.cuda(), 0.0)
+    for g, x, n, w in ((got[0], q, H, qw), (got[1], k, 2, kw)):
+        want, off = definition(x, n, w, 0.0, None, True, 1.0, None)
+        mean = x.double().reshape(2, 5, n, d).square().mean(-1, keepdim=True)
+        near(g, want, off + want.abs() * (2.0 ** -150 + 2.0 ** -150) / mean)
+
+
+@gpu
 @pytest.mark.parametrize("interleaved", [True, False])
 def test_lengths_and_idle_streams(cuda, interleaved):
     """Rows without a token: zeros in new outputs, left as they were in given ones, NaN of the inputs there not looked at."""
