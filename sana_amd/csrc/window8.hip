@@ -31,19 +31,20 @@ __device__ __forceinline__ u32x4_t codes16(uint32_t lo, uint32_t hi) {
   }
 }
 
-// One token of each stream.  A workgroup takes a part of the rows of one (stream, key head), its NW waves in turn a tile of 16 * RT rows; the query
-// heads that share the key head are the 16 columns of the products (more than 16 in further workgroups).  K comes from memory as the operand it
-// is (16 channels a lane, two products), V through the wave's own LDS as bf16 to be transposed; its scale goes to the probability, and both as
+// One token of each stream.  A workgroup takes a part of the rows of one (stream, key head) and 16 * VP channels of its values, its NW waves in turn a
+// tile of 16 * RT rows; the query heads that share the key head are the 16 columns of the products (more than 16 in further workgroups).  K comes from
+// memory as the operand it is (16 channels a lane, two products), V through the wave's own LDS as bf16 to be transposed; its scale goes to the probability, and both as
 // the sum of two bf16 numbers into the product.  (bf16 for f16 too: a value's scale may be of any size.)
 // Every compute unit busy, memory bounds it: 64 streams x 8196 rows x 8 key heads of 128, 1.06 GB 164 us = 6.4 TB/s, reads alone (179 with loads that stay in the
 // caches; 4, 6, 12 waves 169, 175, 173; 64 rows a wave 185).  One stream of 131136 rows 277 MB in 32 parts 49 us with the join (25 parts 55, 48 parts 60: a part
-// a compute unit).  A short cache is what one compute unit takes in, some 30 bytes a ns behind 6 us of launch, first loads and the waves' sum: 16 key heads of
-// 72 x 1028 rows 165 KB each, 11 us; products of 8-bit numbers in the place of the conversions (q in three slices) 4 % less there and nothing elsewhere.
-template <typename T, int P, int NW, int RT>
+// a compute unit).  A short cache is what one compute unit takes in, 37 bytes a ns at most whatever is asked for (two tiles ahead no faster) behind
+// 6 us of launch, first loads and the waves' sum, so the values' channels go to several: 16 key heads of 72 x 1028 rows 11.3 us whole, 9.0 by three.  Products of
+// 8-bit numbers in the place of the conversions (q in three slices): 4 % less for a cache that one compute unit takes, nothing elsewhere.
+template <typename T, int P, int VP, int NW, int RT>
 __global__ __launch_bounds__(64 * NW) void window_q8_kernel(const Window8Args x) {
   const WindowArgs& a = x.w;
-  constexpr int DP = 16 * P, KS = (P + 3) / 4, DK = (P + 1) / 2, DT = P, PITCH = DK * 64, ROWS = 16 * RT, TILE = ROWS * PITCH;
-  constexpr int PV = (ROWS * P + 63) / 64, SUMS = 16 * 16 * DT * 4 + 128;  // PV: 16-byte pieces of V a lane
+  constexpr int DP = 16 * P, KS = (P + 3) / 4, DK = (VP + 1) / 2, DT = VP, PITCH = DK * 64, ROWS = 16 * RT, TILE = ROWS * PITCH;
+  constexpr int PV = (ROWS * VP + 63) / 64, SUMS = 16 * 16 * DT * 4 + 128;  // PV: 16-byte pieces of V a lane
   constexpr int OWN = (TILE + 2 * 4 * ROWS > SUMS ? TILE + 2 * 4 * ROWS : SUMS);
   __shared__ __attribute__((aligned(16))) unsigned char smem[NW * OWN];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, fr = lane & 15, fg = lane >> 4;
@@ -52,7 +53,7 @@ __global__ __launch_bounds__(64 * NW) void window_q8_kernel(const Window8Args x)
   const int G = a.H / a.Hkv, blocks = (G + 15) / 16, d = a.d;
   const uint32_t split = blockIdx.y, bk = blockIdx.x / (uint32_t)blocks;
   const int gb = blockIdx.x - bk * blocks, b = bk / (uint32_t)a.Hkv, hk = bk - b * a.Hkv;
-  const int pos = a.positions[b], rows = a.window + a.sinks;
+  const int pos = a.positions[b], rows = a.window + a.sinks, v0_piece = VP < P ? VP * blockIdx.z : 0;
   const int64_t head_rows = (int64_t)hk * rows;
   const int8_t *ck = x.ck + b * x.ck_b + head_rows * DP, *cv = x.cv + b * x.cv_b + head_rows * DP;
   const float* scales = x.scales + b * x.sc_b + 2 * head_rows;
@@ -82,8 +83,8 @@ __global__ __launch_bounds__(64 * NW) void window_q8_kernel(const Window8Args x)
         rk[kt][s] = load_stream<true>(reinterpret_cast<const u32x4_t*>(k0 + (uint32_t)(min(16 * kt + fr, left) * DP + 16 * min(4 * s + fg, P - 1))));
 #pragma unroll
     for (int i = 0; i < PV; ++i) {
-      const int idx = lane + 64 * i, r = idx / P, c = idx - r * P;
-      rv[i] = load_stream<true>(reinterpret_cast<const u32x4_t*>(v0 + (uint32_t)(min(r, left) * DP + 16 * c)));
+      const int idx = lane + 64 * i, r = idx / VP, c = idx - r * VP;
+      rv[i] = load_stream<true>(reinterpret_cast<const u32x4_t*>(v0 + (uint32_t)(min(r, left) * DP + 16 * (VP < P ? min(v0_piece + c, P - 1) : c))));
     }
 #pragma unroll
     for (int i = 0; i < (ROWS + 63) / 64; ++i)
@@ -93,7 +94,7 @@ __global__ __launch_bounds__(64 * NW) void window_q8_kernel(const Window8Args x)
   const bool whole = a.splits == 1;
   if (whole) request(min(wave, (rows - 1) / ROWS));
   if (pos < 0) {  // an idle stream: zeros
-    if (split == 0 && gb == 0)
+    if (split == 0 && gb == 0 && blockIdx.z == 0)
       for (int c = tid; c < G * d; c += 64 * NW) a.out[b * a.o_b + hk * G * d + c] = 0;
     return;
   }
@@ -127,8 +128,8 @@ __global__ __launch_bounds__(64 * NW) void window_q8_kernel(const Window8Args x)
       }
 #pragma unroll
     for (int i = 0; i < PV; ++i) {
-      const int idx = lane + 64 * i, r = idx / P, c = idx - r * P;
-      if (ROWS * P % 64 == 0 || r < ROWS) {
+      const int idx = lane + 64 * i, r = idx / VP, c = idx - r * VP;
+      if (ROWS * VP % 64 == 0 || r < ROWS) {
         unsigned char* to = mine + r * PITCH;
         *reinterpret_cast<u32x4_t*>(to + (((2 * c) ^ row_key<DK>(r & 15)) << 4)) = codes16<BF16>(rv[i][0], rv[i][1]);
         *reinterpret_cast<u32x4_t*>(to + (((2 * c + 1) ^ row_key<DK>(r & 15)) << 4)) = codes16<BF16>(rv[i][2], rv[i][3]);
@@ -208,14 +209,14 @@ __global__ __launch_bounds__(64 * NW) void window_q8_kernel(const Window8Args x)
   if (g >= G) return;
   const int64_t at = ((int64_t)split * a.B + b) * a.H + hk * G + g;
   const float inv = 1.0f / l;
-  for (int c = tid >> 4; c < d; c += 4 * NW) {
+  for (int c = 16 * v0_piece + (tid >> 4); c < min(d, 16 * (v0_piece + VP)); c += 4 * NW) {
     float o = 0.f;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) o = fmaf(f[w], part(w)[c * 16 + col], o);
+    for (int w = 0; w < NW; ++w) o = fmaf(f[w], part(w)[(c - 16 * v0_piece) * 16 + col], o);
     if (a.splits == 1) a.out[b * a.o_b + (hk * G + g) * d + c] = (uint16_t)pk16<T>(o * inv, 0.f);
     else a.part_o[at * d + c] = o;
   }
-  if (a.splits > 1 && tid < 16) a.part_ml[2 * at] = m, a.part_ml[2 * at + 1] = l;
+  if (a.splits > 1 && tid < 16 && blockIdx.z == 0) a.part_ml[2 * at] = m, a.part_ml[2 * at + 1] = l;
 }
 
 // The parts of a query head (32 heads in 32 parts 4.4 us), a workgroup a head: weights 2^(m_s - m) from a lane a part, then eight parts at a time, 32 lanes of four channels each,
@@ -347,12 +348,13 @@ void read8(const ReadArgs& a, dim3 grid, hipStream_t s) { hipLaunchKernelGGL((re
 
 // Parts of a cache's rows.  Short caches are taken whole: parts cost a second launch, 2 us on the device and 3.5 of the host's where calls are issued one by
 // one.  Longer ones of few streams in as many parts as the 256 compute units take at once, one each, but of 64 rows and more; where a few workgroups
-// more than that leave most of a second round idle, in three.  us on the device, whole / by this rule (best of up to 64 parts): 8 key heads of
-// 128 x 1028 rows 13.2 / whole (16 parts 8.8), x 4100 34.6 / 10.3, x 16388 122 / 14.0; 20 of 112 x 4100 33.5 / 12.8; 80 x 4100 35.8 / 21.3; 120 x 4100 37.3 / 27.8; 160 39.0 /
-// whole (3 parts 36.9), 200 41.3 / whole; 260 73.4 / 65.6, 300 x 8200 135 / 113, 400 x 4100 79 / whole (3 parts 83).
+// more than that leave most of a second round idle, in three.  us a call, whole / in these parts: 8 key heads of 128 x 1600 rows 12.1 / 13.5, x 2052 15.7 /
+// 13.7, x 4100 34.7 / 15.0, x 16388 122 / 14.7; 20 of 112 x 1500 13.0 / 13.7, x 2052 16.2 / 13.5; 80 x 1300 13.2 / 14.0, x 1700 16.1 / 14.9, x 4100 35.3 / 21.1; 120 x
+// 1300 13.6 / 16.2, x 2052 19.9 / 19.2; 70 of 64 x 2052 12.8 / 14.1, x 3000 16.6 / 14.2; 70 of 32 x 1028 10 / 14.7, x 4100 19.2 / 13.7; 160 of 112 x 4100 38 / whole; 260 x
+// 2052 40 / 42, x 4100 73 / 65, 300 x 8200 135 / 113, 400 x 4100 79 / whole (in three 83).
 int q8_splits(int B, int H, int Hkv, int rows, int d) {
-  const int64_t groups = step_groups(B, H, Hkv), bytes = (int64_t)rows * d * 2;
-  if (bytes <= (groups <= 128 ? 256 << 10 : 384 << 10)) return 1;
+  const int64_t groups = step_groups(B, H, Hkv);
+  if (groups <= 256 ? rows <= (d <= 64 ? 2048 : 1600) : (int64_t)rows * d * 2 <= (768 << 10)) return 1;
   const int most = rows / 64 < Q8_MAX_SPLITS ? rows / 64 : Q8_MAX_SPLITS;
   const int64_t want = groups <= 256 ? 256 / groups : groups * 100 < (groups + 255) / 256 * 256 * 65 ? 3 : 1;
   return (int)(want > most ? most : want < 1 ? 1 : want);
@@ -362,7 +364,26 @@ template <typename T, int P>
 int launch_q8(const Window8Args& x, hipStream_t s) {
   const WindowArgs& a = x.w;
   const int64_t groups = step_groups(a.B, a.H, a.Hkv);
-  hipLaunchKernelGGL((window_q8_kernel<T, P, 8, 2>), dim3((unsigned)groups, (unsigned)a.splits), dim3(512), 0, s, x);
+  const int64_t workgroups = groups * a.splits;
+  const auto launch = [&](auto tiles) {
+    constexpr int VP = decltype(tiles)::value;
+    hipLaunchKernelGGL((window_q8_kernel<T, P, VP, 8, 2>), dim3((unsigned)groups, (unsigned)a.splits, (P + VP - 1) / VP), dim3(512), 0, s, x);
+  };
+  // The values' channels over several workgroups where compute units are left: each takes all keys and 32 channels, or half, of the values, which is 5/8
+  // or 3/4 of what one would have to take in.  us on the device of one / two / four a key head, caches taken whole: 16 heads of 72 x 1028 rows 11.3 / 10.1 /
+  // 9.0 (three), 20 of 112 x 1028 13.5 / 11.6 / 10.4, x 516 9.6 / 8.5 / 7.6, 8 of 128 x 260 7.6 / 6.7 / 6.5, 80 of 112 x 1028 14.2 / 11.8 / 17.4, 35 of 64 x
+  // 1028 9.4 / 8.4 / 9.1 (16 channels each), 36 of 32 x 1028 8.1 / 8.0 (16 each).
+  if constexpr (P >= 3) {
+    if (workgroups * ((P + 1) / 2) <= 256) {
+      launch(std::integral_constant<int, 2>{});
+    } else if (P >= 5 && workgroups * 2 <= 256) {
+      launch(std::integral_constant<int, (P + 1) / 2>{});
+    } else {
+      launch(std::integral_constant<int, P>{});
+    }
+  } else {
+    launch(std::integral_constant<int, P>{});
+  }
   if (a.splits > 1) hipLaunchKernelGGL(q8_join_kernel<T>, dim3((unsigned)(a.B * a.H)), dim3(256), 0, s, a);
   return hipGetLastError() == hipSuccess ? SANA_OK : SANA_ERR_LAUNCH;
 }

@@ -100,6 +100,14 @@ def test_parts_and_whole(cuda, B, H, G, d, rows):
 
 
 @gpu
+@pytest.mark.parametrize("d", [16, 40, 64, 72, 96, 104, 128])
+@pytest.mark.parametrize("B,H,G,rows", [(40, 4, 2, 60), (33, 3, 3, 100), (100, 2, 2, 37), (1, 3, 1, 9000), (2, 2, 1, 7000)])
+def test_values_over_several_workgroups(cuda, B, H, G, rows, d):
+    """64, 80, 99 and 200 workgroups of whole caches, few of long ones in parts: a workgroup takes 32 channels of the values, half of them, or all; idle streams' zeros too."""
+    compare(B, H, G, d, rows - 2, 2, [-1 if i % 7 == 3 else (rows // 2 + 11 * i) % (3 * rows) for i in range(B)], BF16, seed=d)
+
+
+@gpu
 def test_scores_of_thousands(cuda):
     compare(2, 2, 1, 64, 500, 4, [400, 800], BF16, scale=20.0)
     compare(2, 2, 1, 64, 5000, 4, [400, 8000], F16, scale=20.0)
