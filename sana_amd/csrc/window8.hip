@@ -262,7 +262,7 @@ struct ReadArgs {
   const float* scales;
   const int* positions;
   uint16_t *out_k, *out_v;
-  int B, Hkv, d, dp, window, sinks, last, rows, by_eighths, zero_rest;  // rows: of a head that a wave takes; by_eighths: 2^16 / (d / 8), rounded up
+  int B, Hkv, d, dp, window, sinks, last, rows, by_eighths, zero_rest;  // rows: that a wave takes; by_eighths: 2^16 over a row's pieces of 8 channels, rounded up
   int64_t k_b, k_n, v_b, v_n, sc_b, ok_b, ok_n, ov_b, ov_n;  // k_b .. v_n in bytes
   int64_t items;
 };
@@ -306,11 +306,34 @@ __global__ __launch_bounds__(256) void read16_kernel(const ReadArgs a) {
   }
 }
 
+constexpr int READ_STEPS = 4;
+
+// Narrow 16-bit rows (up to 256 channels): a wave copies READ_STEPS times as many rows of keys or of values as it has lanes for.  292968 rows of 64 channels of two
+// streams 266 us by a wave a row, 56 so; 146484 of 128 144 and 56.
+__global__ __launch_bounds__(256) void read16_narrow_kernel(const ReadArgs a) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const uint32_t item = 4 * blockIdx.x + wave;
+  if (item >= (uint32_t)a.items) return;
+  const int of_v = item & 1, b = blockIdx.y, i0 = a.rows * (item >> 1);
+  const int eighths = a.Hkv * a.d / 8, step = 64 / eighths, r = lane * a.by_eighths >> 16, c = lane - r * eighths, end = min(i0 + a.rows, a.sinks + a.last);
+  const InOrder o = in_order(a, a.positions[b]);
+  const unsigned char* from = (of_v ? a.v + b * a.v_b : a.k + b * a.k_b) + 16 * c;
+  uint16_t* to = (of_v ? a.out_v + b * a.ov_b : a.out_k + b * a.ok_b) + 8 * c;
+  const int64_t from_n = of_v ? a.v_n : a.k_n, to_n = of_v ? a.ov_n : a.ok_n;
+  u32x4_t x[READ_STEPS];
+#pragma unroll
+  for (int u = 0; u < READ_STEPS; ++u) x[u] = *reinterpret_cast<const u32x4_t*>(from + read_slot(a, o, min(i0 + u * step + r, end - 1)) * from_n);
+#pragma unroll
+  for (int u = 0; u < READ_STEPS; ++u) {
+    const int i = i0 + u * step + r;
+    if (r < step && i < end && (i < o.count || a.zero_rest)) *reinterpret_cast<u32x4_t*>(to + i * to_n) = i < o.count ? x[u] : u32x4_t{0u, 0u, 0u, 0u};
+  }
+}
+
 // Codes: a wave takes READ_STEPS * R rows of a head's keys or values, R = 64 / (d / 8) in a step, 8 channels a lane.  Memory bounds it: 2 x 10920 rows of 20
 // heads of 112, 297 MB 55 - 61 us = 5.2 TB/s (2, 3, 4, 6, 8 steps 64, 62, 62, 63, 64 us a call; with loads under a condition 86).
 // Stores that stay in the caches: a chunk's attention reads the rows next, and takes 12 us longer where they were streamed past (2 x 10920 rows of 20 heads
 // of 112, in front of 1 to 4680 queries), though the call alone, behind the one that wrote the codes, is up to 15 % shorter.
-constexpr int READ_STEPS = 4;
 template <typename T, bool NT>
 __global__ __launch_bounds__(256) void read8_kernel(const ReadArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -481,6 +504,12 @@ SANA_API int sana_hip_window_cache_read(const sana_cache_read_args* args, void* 
     if (misaligned({}, {ck_stride_b, ck_stride_n, cv_stride_b, cv_stride_n})) return SANA_ERR_ALIGN;
     a.k_b = 2 * ck_stride_b, a.k_n = 2 * ck_stride_n, a.v_b = 2 * cv_stride_b, a.v_n = 2 * cv_stride_n;
     if (held >= (WA_MAX_BLOCKS << 1) / B) return SANA_ERR_SHAPE;
+    if (width <= 256 && B <= 65535) {
+      a.rows = READ_STEPS * (64 / (int)(width / 8)), a.by_eighths = (65536 + (int)width / 8 - 1) / (int)(width / 8);
+      a.items = (held + a.rows - 1) / a.rows * 2;
+      hipLaunchKernelGGL(read16_narrow_kernel, dim3((unsigned)((a.items + 3) / 4), (unsigned)B), dim3(256), 0, s, a);
+      return hipGetLastError() == hipSuccess ? SANA_OK : SANA_ERR_LAUNCH;
+    }
     a.items = 2 * B * held;
     hipLaunchKernelGGL(read16_kernel, dim3((unsigned)((a.items + 3) / 4)), dim3(256), 0, s, a);
   } else {

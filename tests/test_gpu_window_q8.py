@@ -169,7 +169,7 @@ def in_order(cache, positions, sinks, last, fill, rows_of):
 @gpu
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("bits", [8, 16])
-@pytest.mark.parametrize("G,d,window,sinks,last", [(2, 72, 37, 5, None), (3, 32, 64, 0, 63), (1, 128, 1, 3, 0), (5, 112, 200, 1, 40), (2, 8, 16, 16, 16), (7, 40, 100, 0, 1)])
+@pytest.mark.parametrize("G,d,window,sinks,last", [(2, 72, 37, 5, None), (3, 32, 64, 0, 63), (1, 128, 1, 3, 0), (5, 112, 200, 1, 40), (2, 8, 16, 16, 16), (7, 40, 100, 0, 1), (1, 8, 300, 7, 299), (2, 128, 90, 0, 90), (1, 104, 500, 3, 411), (3, 88, 64, 1, 60)])
 def test_rows_in_order(cuda, G, d, window, sinks, last, bits, dtype):
     R = window + sinks
     cache = realistic(9, G, R, d)
