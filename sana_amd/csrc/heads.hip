@@ -254,12 +254,23 @@ int launch_heads(const sana_heads_args& a, hipStream_t s) {
   else hipLaunchKernelGGL((heads_kernel<T, LPH, false, TOKENS>), grid, dim3(256), 0, s, h);
   return hipGetLastError() == hipSuccess ? SANA_OK : SANA_ERR_LAUNCH;
 }
-// Runs of tokens for many tokens, else heads of one token.  us of all in one pass, heads / tokens: 20 + 20 + 20 heads of 112 1 token 4.0 / 5.3, 64 x 1
-// 4.9 / 6.2, 1000 x 1 12.6 / 27.6, 64 x 16 10.3 / 10.2, 64 x 64 22.6 / 24.2, 2 x 4680 60 / 56; 32 + 8 + 8 of 128 64 x 64 19.5 / 20.6; 16384 tokens of 20 + 20
-// of 112 without a cache 60 / 61, 8 x 2047 of 32 + 8 of 128 in far pairs 64 / 60; into a cache alone 2 x 4680 of 5 of 112 16 / 12, 16 x 4096 of 4 of 128 40 / 23.
+// Heads of one token, or runs of tokens where there are many.  us of all in one pass, heads / tokens: 20 + 20 + 20 heads of 112 1 token 4.0 / 5.3, 64 x 1
+// 4.9 / 6.2, 1000 x 1 12.6 / 27.6, 64 x 16 10.3 / 10.2, 64 x 64 22.6 / 24.2, 2 x 4680 60 / 56; 32 + 8 + 8 of 128 64 x 64 19.5 / 20.6; 8 x 2047 of 32 + 8 of
+// 128 in far pairs without a cache 64 / 60; into a cache alone 2 x 4680 of 5 of 112 16 / 12, 16 x 4096 of 4 of 128 40 / 23, 70 of 32 62 / 38.
+// Many tokens stay heads of one where queries are among them and six groups or more of heads fill their lanes: the rows of a token are whole lines that
+// one wave reads and writes.  Without a cache, near pairs (far pairs), 250 MB: 70 + 70 of 32 45.0 / 49.7 (48.7 / 63.0), 48 44.6 / 50.7 (51.4 / 62.2), 64
+// 43.7 / 42.9 (48.3 / 49.6), 16 + 16 of 72 48.2 / 55.4 (54.0 / 64.1), 96 44.6 / 46.9 (52.1 / 52.8), 112 43.6 / 45.4 (48.5 / 49.3), but of 128 42.6 / 42.2
+// (42.5 / 43.3), of 16 69 / 27, and with fewer groups 16 + 4 of 72 46.9 / 46.0 (57.2 / 53.3), 4 + 4 47.5 / 33.6.  With a cache its rows of codes, which lie
+// by head, outweigh that up to 64 channels and from 112: 32 85.0 / 75.1, 48 84.1 / 78.0, 64 68.1 / 62.8, 72 80.9 / 91.0, 80 71.8 / 77.4, 96 72.7 / 75.9, 104
+// 62.1 / 65.6, 112 65.3 / 67.2 and 52.5 / 51.3, 128 47.0 / 48.6 and 60 / 56.
 template <typename T, int LPH>
 int heads_as(const sana_heads_args& a, hipStream_t s) {
-  return a.N >= 64 && (int64_t)a.B * a.N >= 8192 ? launch_heads<T, LPH, true>(a, s) : launch_heads<T, LPH, false>(a, s);
+  constexpr int AT_ONCE = 64 / LPH;
+  if (a.N < 64 || (int64_t)a.B * a.N < 8192) return launch_heads<T, LPH, false>(a, s);
+  const int kv = a.codes_k ? 2 : 1, groups = (a.H + AT_ONCE - 1) / AT_ONCE + kv * ((a.Hkv + AT_ONCE - 1) / AT_ONCE);
+  const bool full = groups >= 6 && 10 * ((int64_t)a.H + (int64_t)kv * a.Hkv) >= 7 * (int64_t)AT_ONCE * groups;
+  const bool heads = a.q && full && (a.codes_k ? a.d > 64 && a.d < 112 : a.d > 16 && a.d < 128);
+  return heads ? launch_heads<T, LPH, false>(a, s) : launch_heads<T, LPH, true>(a, s);
 }
 template <typename T>
 int heads_of(const sana_heads_args& a, hipStream_t s) {

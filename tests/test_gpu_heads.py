@@ -347,7 +347,7 @@ def test_all_in_one_pass(cuda, B, N, H, G, d, rotary, window, sinks, interleaved
 @gpu
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("interleaved", [True, False])
-@pytest.mark.parametrize("B,N,H,G,d,rotary", [(1, 8229, 3, 1, 72, 72), (3, 2999, 2, 2, 32, 16), (2, 4100, 5, 5, 112, 112), (90, 97, 4, 2, 128, 64), (1, 9000, 1, 3, 8, 8), (2, 5000, 3, 2, 64, 0)])
+@pytest.mark.parametrize("B,N,H,G,d,rotary", [(1, 8229, 3, 1, 72, 72), (3, 2999, 2, 2, 32, 16), (2, 4100, 5, 5, 112, 112), (90, 97, 4, 2, 128, 64), (1, 9000, 1, 3, 8, 8), (2, 5000, 3, 2, 64, 0), (2, 4100, 15, 13, 72, 40)])
 def test_many_tokens_are_what_they_are_in_pieces(cuda, B, N, H, G, d, rotary, interleaved, dtype):
     """Runs of tokens a wave and heads of one token a wave: the same numbers, one call or many, with and without a cache."""
     q, k, v, qw, kw = (t.cuda() for t in make(B, N, H, G, d, dtype, seed=N))
