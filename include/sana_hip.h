@@ -583,7 +583,8 @@ int sana_hip_window_step(const void* q, const void* k, const void* v, void* cach
  *   weights   of the io dtype, 8-byte aligned;  freqs  fp64 [rotary / 2] (any scaling for long contexts is in them)
  *   positions int32 [B] or NULL (zeros): the position of each entry's first token; negative: an idle stream
  *   lengths   int32 [B] or NULL: entry b has lengths[b] tokens (clamped to 0 .. N)
- *             Rows of q_out and k_out without a token stay as they were, or are zeroed (zero_rest: 1 q_out, 2 k_out, 3 both).
+ *             Rows of q_out and k_out without a token stay as they were, or are zeroed (zero_rest: 1 q_out, 2 k_out, 3 both; of outputs that are
+ *             there: any other value is refused).
  *   codes_k, codes_v  int8 [B] times dense [Hkv][sinks + window][d'], d' = d rounded up to a multiple of 16 (what is behind d is neither read
  *             nor written), or NULL: no cache;  scales fp32 [B] times dense [Hkv][sinks + window][2], of a row's key and of its value.
  *             A head's row x is c = round(127 x / max|x|), ties to even, with the scale max|x| / 127; one of inf or NaN has the scale NaN.

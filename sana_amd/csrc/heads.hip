@@ -290,6 +290,7 @@ extern "C" __attribute__((visibility("default"))) int sana_hip_heads(const sana_
       (a.q == nullptr) != (a.q_out == nullptr))
     return SANA_ERR_ARG;
   if (cached ? !a.codes_k || !a.codes_v || !a.scales || !a.v || !a.positions || a.window <= 0 || a.sinks < 0 : !a.k_out) return SANA_ERR_ARG;
+  if (a.zero_rest & ~((a.q_out ? 1 : 0) | (a.k_out ? 2 : 0))) return SANA_ERR_ARG;  // (rows of an output that is not there)
   if ((a.q_weight == nullptr) != (a.k_weight == nullptr) || (a.freqs == nullptr) != (a.rotary == 0) || !(a.eps >= 0.f && a.eps < INFINITY) ||
       !(fabsf(a.magnitude) < INFINITY))
     return SANA_ERR_ARG;

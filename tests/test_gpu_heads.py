@@ -428,6 +428,44 @@ def test_calls_that_are_refused_before_any_launch():
     assert call(io_dtype=0) == DTYPE and call(io_dtype=7) == DTYPE
 
 
+def test_rows_of_an_output_that_is_not_there_cannot_be_zeroed():
+    """``zero_rest`` names q_out and k_out: what it names has to be there (the pointers are never followed)."""
+    lib, P = _lib.load(), 0x10000
+
+    def call(q, k_out, zero_rest):
+        pointers = dict(q=P if q else 0, k=2 * P, v=3 * P, q_out=4 * P if q else 0, k_out=5 * P if k_out else 0, q_weight=0, k_weight=0, freqs=0, positions=P, lengths=P,
+                        codes_k=6 * P, codes_v=7 * P, scales=8 * P)
+        strides = [8 * 256, 256, 8 * 128, 128, 8 * 128, 128, 8 * 256, 256, 8 * 128, 128, 2 * 20 * 64, 2 * 20 * 64, 2 * 20 * 2]
+        return lib.sana_hip_heads(_lib.HEADS_ARGS.pack(*pointers.values(), *strides, 2, 8, 4 if q else 0, 2, 64, 0, 1, 16, 4, zero_rest, _lib.DT_BF16, 1e-6, 1.0), None)
+
+    for zero_rest in (2, 3):
+        assert call(True, False, zero_rest) == -1 and call(False, False, zero_rest) == -1
+    for zero_rest in (1, 3):
+        assert call(False, True, zero_rest) == -1
+    for zero_rest in (-1, 4, 7):
+        assert call(True, True, zero_rest) == -1
+
+
+@gpu
+@pytest.mark.parametrize("N", [1, 6, 8192])
+@pytest.mark.parametrize("zero_rest", [0, 1])
+def test_one_pass_with_idle_streams_and_no_key_output(cuda, zero_rest, N):
+    """The C entry, keys into the cache alone: queries' rows without a token are zeros or as they were, and nothing else of the call depends on ``zero_rest``."""
+    B, H, G, d, W, S = 4, 4, 2, 64, 20, 2
+    q, k, v, _, _ = (t.contiguous().cuda() for t in make(B, N, H, G, d, BF16, seed=N))
+    pos, lens = i32([3, -1, 0, 40]), i32([N, N, 0, max(N - 2, 0)])
+    cache, ref = ([t.cuda() for t in filled(B, G, W + S, d)] for _ in range(2))
+    out = torch.full_like(q, 7.0)
+    rows_q, rows_k, codes = [N * H * d, H * d], [N * G * d, G * d], G * (W + S) * d
+    args = _lib.HEADS_ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0, 0, 0, 0, pos.data_ptr(), lens.data_ptr(), *(t.data_ptr() for t in cache),
+                                *rows_q, *rows_k, *rows_k, *rows_q, 0, 0, codes, codes, 2 * G * (W + S), B, N, H, G, d, 0, 1, W, S, zero_rest, _lib.DT_BF16, 1e-6, 1.0)
+    assert _lib.load().sana_hip_heads(args, torch.cuda.current_stream().cuda_stream) == 0
+    want, _ = ops.qk_norm_rope_append_q8_(q, k, v, ref, pos, H, sinks=S, lengths=lens)
+    live = torch.tensor([[p >= 0 and t < n for t in range(N)] for p, n in zip(pos.tolist(), lens.tolist())], device="cuda")[..., None]
+    assert torch.equal(out, torch.where(live, want, 0.0 if zero_rest else 7.0))
+    assert all(torch.equal(a, b) for a, b in zip(cache, ref))
+
+
 def test_no_cpu_tensors():
     q, k, v, qw, kw = make(1, 2, 2, 1, 32, BF16)
     cache = ops.window_cache_q8(1, 8, 1, 32, device="cpu")
