@@ -13,6 +13,10 @@ namespace {
 
 constexpr int MAX_TILES = 1 << 15;
 
+// The scales of a head's rows in a cache begin here: (key, value) pairs, in 64 bits, since two scales each for 2^30 rows are no 32-bit number.
+__host__ __device__ constexpr int64_t scales_of_head(int head, int rows) { return 2 * (int64_t)rows * head; }
+static_assert(scales_of_head(1, 1 << 30) == int64_t{1} << 31 && scales_of_head(3, 1 << 30) == 3 * (int64_t{1} << 31), "the largest cache's second and last heads");
+
 struct HeadArgs {
   sana_heads_args a;
   int gq, gk, gv, per;  // groups of heads of a token: of queries, of keys, of values; groups that a wave takes
@@ -219,7 +223,7 @@ __global__ __launch_bounds__(256) void heads_kernel(const HeadArgs h) {
           } else {
             *reinterpret_cast<uint32_t*>(codes + e0) = lo, *reinterpret_cast<uint32_t*>(codes + e1) = hi;
           }
-          if (j == 0) scales[(int64_t)head * (2 * rows) + (kind - 1)] = bad ? __uint_as_float(0x7fc00000u) : scale_of(most);
+          if (j == 0) scales[scales_of_head(head, rows) + (kind - 1)] = bad ? __uint_as_float(0x7fc00000u) : scale_of(most);
         }
       }
     }

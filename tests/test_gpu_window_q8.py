@@ -343,6 +343,36 @@ def test_a_cache_of_more_than_32_bits_of_bytes(cuda):
             assert ((out[b, 0, h * d:(h + 1) * d].double() - ref).abs() <= tol).all()
 
 
+@gpu
+def test_the_longest_cache(cuda):
+    """2^30 rows of two heads, 80 GiB: a head's scales are 2^31 numbers, its codes 2^34 bytes.  What is written is what a short cache holds of the same tokens, in
+    both heads; the first rows, then the last ones and those that the ring goes on with."""
+    G, d, S, R, n = 2, 8, 4, 1 << 30, 7
+    cache = (*(torch.empty(1, G, R, 16, dtype=torch.int8, device="cuda") for _ in range(2)), torch.empty(1, G, R, 2, device="cuda"))
+    g = torch.Generator().manual_seed(5)
+    k, v, q = (torch.randn(1, n, G * d, generator=g).to(BF16).cuda() for _ in range(3))
+    small = ops.window_cache_q8(1, 2 * n, G, d)
+    ops.window_cache_append_q8_(small, k, v, i32([0]), S)
+
+    def rows_are(at):
+        for a, b, width in zip(cache, small, (d, d, 2)):
+            for head in range(G):
+                assert torch.equal(torch.stack([a[0, head, r, :width] for r in at]), b[0, head, :n, :width])
+
+    ops.window_cache_append_q8_(cache, k, v, i32([0]), S)
+    rows_are(list(range(n)))
+    got, want = (ops.window_attention_q8(q[:, -1:], c, i32([n - 1]), G, S) for c in (cache, small))
+    check(got, definition(q[:, -1:].cpu(), [t.cpu() for t in small], [n - 1], G, S, d ** -0.5), n)
+    check(want, definition(q[:, -1:].cpu(), [t.cpu() for t in small], [n - 1], G, S, d ** -0.5), n)
+    first = R - 3
+    ops.window_cache_append_q8_(cache, k, v, i32([first]), S)
+    rows_are([row_of(first + t, S, R - S) for t in range(n)])
+    for a, b in zip(ops.window_cache_read(cache, i32([first + n]), S, n, d), ops.window_cache_read(small, i32([n]), 0, n, d)):
+        assert torch.equal(a[:, S:], b)
+    del cache, got, want
+    torch.cuda.empty_cache()
+
+
 # --------------------------------------------------------------------------- refusals
 
 def test_calls_that_are_refused_before_any_launch():
