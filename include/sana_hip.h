@@ -611,6 +611,8 @@ int sana_hip_heads(const sana_heads_args* args, void* stream);
  *   out = sum_j softmax_j(scale * sk_j (q . ck_j)) sv_j cv_j   over the rows of the last `window` tokens up to positions[b] and of the sinks.
  *   q, out  [B][H*d] rows, bf16 or f16; an idle stream (negative position) gets zeros
  * Codes meet q exactly; probabilities (with their row's scale) enter the product as two bf16 each (2^-16), maxima, sums and outputs are fp32.
+ * Values may be of any size: no sum of them leaves fp32 where their average does not, and small ones keep those 2^-16 (down to 2^-62 where others of
+ * over 2^80 are seen).  A query's products are summed before their scales: q up to 2^113.
  * Workspace, limits and alignment as in sana_hip_window_step and sana_hip_heads. */
 size_t sana_hip_window_q8_workspace_bytes(int B, int H, int Hkv, int d, int window, int sinks);
 typedef struct sana_window_q8_args {

@@ -35,6 +35,9 @@ __device__ __forceinline__ u32x4_t codes16(uint32_t lo, uint32_t hi) {
 // tile of 16 * RT rows; the query heads that share the key head are the 16 columns of the products (more than 16 in further workgroups).  K comes from
 // memory as the operand it is (16 channels a lane, two products), V through the wave's own LDS as bf16 to be transposed; its scale goes to the probability, and both as
 // the sum of two bf16 numbers into the product.  (bf16 for f16 too: a value's scale may be of any size.)
+// A probability is 2^(score - reference), and the reference moves only where a score is 8 above it.  It lies 48 above the scores of a tile with a value's scale over
+// 2^80, so that sums of up to 2^30 rows, of 2^8 times 127 times any scale each, stay below 2^127; 48 below those of a tile whose values' scales are all under 2^-64,
+// so that neither bf16 number is a subnormal one; weights and sums of parts are relative to their reference, whatever it is.
 // Every compute unit busy, memory bounds it: 64 streams x 8196 rows x 8 key heads of 128, 1.06 GB 164 us = 6.4 TB/s, reads alone (179 with loads that stay in the
 // caches; 4, 6, 12 waves 169, 175, 173; 64 rows a wave 185).  One stream of 131136 rows 277 MB in 32 parts 49 us with the join (25 parts 55, 48 parts 60: a part
 // a compute unit).  A short cache is what one compute unit takes in, 37 bytes a ns at most whatever is asked for (two tiles ahead no faster) behind
@@ -112,12 +115,14 @@ __global__ __launch_bounds__(64 * NW) void window_q8_kernel(const Window8Args x)
     f32x4_t sc[RT];
 #pragma unroll
     for (int kt = 0; kt < RT; ++kt) sc[kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    bool over = false, ordinary = false;  // of the values' scales
 #pragma unroll
     for (int i = 0; i < (ROWS + 63) / 64; ++i)
       if (64 * i + lane < ROWS) {  // (a row that is not there: a value's scale of 0, so that nothing of it counts)
-        const bool there = ROWS * t + 64 * i + lane < count;
+        const float sv = ROWS * t + 64 * i + lane < count ? rs[i].y : 0.f;
         my_scales[64 * i + lane] = rs[i].x;
-        my_scales[ROWS + 64 * i + lane] = there ? rs[i].y : 0.f;
+        my_scales[ROWS + 64 * i + lane] = sv;
+        over |= sv > 0x1p80f, ordinary |= sv >= 0x1p-64f;
       }
 #pragma unroll
     for (int s = 0; s < KS; ++s)
@@ -137,6 +142,7 @@ __global__ __launch_bounds__(64 * NW) void window_q8_kernel(const Window8Args x)
     }
     if (t + NW < t1) request(t + NW);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the wave's own scales and V are there)
+    const float lift = __any(over) ? 48.f : __any(ordinary) ? 0.f : -48.f;
     float most = -INFINITY;
 #pragma unroll
     for (int kt = 0; kt < RT; ++kt) {
@@ -147,6 +153,7 @@ __global__ __launch_bounds__(64 * NW) void window_q8_kernel(const Window8Args x)
         most = fmaxf(most, sc[kt][r]);
       }
     }
+    most += lift;
     if (__any(most > mx + 8.f)) {
       const float now = fmaxf(mx, max_groups(most));
       const float f = __builtin_amdgcn_exp2f(mx - (now == -INFINITY ? 0.f : now));

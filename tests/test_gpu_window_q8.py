@@ -131,6 +131,38 @@ def test_a_row_that_is_not_finite_reaches_its_head(cuda, rows, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("scale", [None, 3.0])
+@pytest.mark.parametrize("B,H,G,d,rows", [(2, 4, 2, 64, 40), (1, 4, 4, 72, 700), (2, 20, 1, 128, 700), (2, 4, 2, 64, 9000), (130, 2, 2, 40, 100)])
+@pytest.mark.parametrize("kind", ["huge", "tiny", "zeros", "any", "huge last", "huge first", "tiny first"])
+def test_values_of_any_size(cuda, kind, B, H, G, d, rows, scale):
+    """Values next to the largest number of their type, next to the smallest, of all sizes side by side: averages of them, which are finite.
+
+    Where some rows are huge, they are zero in every other channel, whose outputs are those of the other rows.  A score's distance from its reference is
+    up to 56 + 8 larger than without (the lift and the lazy maximum), which is rounded: 64 ln 2 U of a probability, in it and in the sums.  An output that is
+    no normal number is off by half of the smallest bf16 number, and what it is rounded from by half of the smallest fp32 number."""
+    g = torch.Generator().manual_seed(rows)
+    q = torch.randn(B, 1, H * d, generator=g).clamp(-6, 6).to(BF16)
+    k, v = (torch.randn(B, rows, G * d, generator=g).clamp(-1, 1) for _ in range(2))
+    at, huge, tiny = torch.arange(rows), 3.3e38, 2.0 ** -122
+    size = {"huge": torch.full((rows,), huge), "tiny": torch.full((rows,), tiny), "zeros": torch.zeros(rows),
+            "any": 2.0 ** (torch.rand(rows, generator=g) * 187 - 60), "huge last": torch.where(at >= rows - rows // 4, huge, 1.0),
+            "huge first": torch.where(at < rows // 4, huge, 1.0), "tiny first": torch.where(at < rows // 4, tiny, 1.0)}[kind]
+    v = v * size[:, None]
+    if kind.startswith("huge "):
+        v[..., ::2] *= (size[:, None] <= 1)
+    v = v.clamp(-huge, huge).to(BF16)
+    cache = [t.cuda() for t in filled(B, G, rows, d)]
+    ops.window_cache_append_q8_(cache, k.to(BF16).cuda(), v.cuda(), i32([0] * B))
+    positions = [rows - 1 - i % 3 for i in range(B)]
+    got = ops.window_attention_q8(q.cuda(), cache, i32(positions), H, 0, scale)
+    assert torch.isfinite(got).all()
+    ref, ref_abs, most = definition(q, [t.cpu() for t in cache], positions, H, 0, scale or d ** -0.5)
+    tol = 2.0 ** -8 * ref.abs() + (2.0 ** -16 + U * (rows / 2 + 100 + 2 * 26 * 1.45 * most + 2 * 64 * math.log(2))) * ref_abs + 2.0 ** -134 + 2.0 ** -150
+    off = (got.double().cpu() - ref).abs()
+    assert (off <= tol).all(), (off / tol).max().item()
+
+
+@gpu
 def test_streams_of_a_pool(cuda):
     """Every other stream of a larger cache, outputs and queries among other rows."""
     B, H, G, d, R = 3, 4, 2, 40, 200
