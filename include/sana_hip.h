@@ -613,7 +613,7 @@ int sana_hip_heads(const sana_heads_args* args, void* stream);
  * Codes meet q exactly; probabilities (with their row's scale) enter the product as two bf16 each (2^-16), maxima, sums and outputs are fp32.
  * Values may be of any size: no sum of them leaves fp32 where their average does not, and small ones keep those 2^-16 (down to 2^-62 where others of
  * over 2^80 are seen).  A query's products are summed before their scales: q up to 2^113.
- * Workspace, limits and alignment as in sana_hip_window_step and sana_hip_heads. */
+ * Workspace, limits and alignment as in sana_hip_window_step and sana_hip_heads, but B * Hkv * ceil(H / Hkv / 16) below 2^23. */
 size_t sana_hip_window_q8_workspace_bytes(int B, int H, int Hkv, int d, int window, int sinks);
 typedef struct sana_window_q8_args {
   const void* q;
@@ -634,8 +634,8 @@ int sana_hip_window_q8(const sana_window_q8_args* args, void* stream);
  *   cache_k, cache_v  16-bit rows as in sana_hip_window_cache_append (scales NULL; strides in elements: batch, row), or the codes of
  *         sana_hip_heads (scales given; ck_n and cv_n unused)
  *   out_k, out_v  [B][sinks + last][Hkv*d] views of the io dtype; last at most window, sinks + last at least 1
- * d % 8 == 0, for codes d <= 128; Hkv*d at most 2^22; window + sinks at most 2^30; B * (sinks + last) below 2^25 for 16-bit rows,
- * B * Hkv * ceil((sinks + last) / 16) for codes, B at most 65535; rows 16-byte aligned, their strides multiples of 8.  The outputs must not overlap the caches,
+ * d % 8 == 0, for codes d <= 128; Hkv*d at most 2^22; window + sinks at most 2^30; B * (sinks + last) for 16-bit rows and
+ * B * Hkv * ceil((sinks + last) / 16) for codes at most 2^25 - 2, for codes B at most 65535; rows 16-byte aligned, their strides multiples of 8.  The outputs must not overlap the caches,
  * nor their entries each other. */
 typedef struct sana_cache_read_args {
   const void *cache_k, *cache_v;

@@ -229,6 +229,8 @@ __global__ __launch_bounds__(64 * NW) void window_q8_kernel(const Window8Args x)
 // The parts of a query head (32 heads in 32 parts 4.4 us), a workgroup a head: weights 2^(m_s - m) from a lane a part, then eight parts at a time, 32 lanes of four channels each,
 // all of a lane's parts on their way at once; sums in a fixed order.
 constexpr int Q8_MAX_SPLITS = 64;
+constexpr int Q8_NW = 8;
+constexpr int64_t Q8_MAX_GROUPS = WA_MAX_BLOCKS * 256 / (64 * Q8_NW);  // (of 512 threads)
 template <typename T>
 __global__ __launch_bounds__(256) void q8_join_kernel(const WindowArgs a) {
   __shared__ float sums[8][128];
@@ -397,7 +399,7 @@ int launch_q8(const Window8Args& x, hipStream_t s) {
   const int64_t workgroups = groups * a.splits;
   const auto launch = [&](auto tiles) {
     constexpr int VP = decltype(tiles)::value;
-    hipLaunchKernelGGL((window_q8_kernel<T, P, VP, 8, 2>), dim3((unsigned)groups, (unsigned)a.splits, (P + VP - 1) / VP), dim3(512), 0, s, x);
+    hipLaunchKernelGGL((window_q8_kernel<T, P, VP, Q8_NW, 2>), dim3((unsigned)groups, (unsigned)a.splits, (P + VP - 1) / VP), dim3(64 * Q8_NW), 0, s, x);
   };
   // The values' channels over several workgroups where compute units are left: each takes all keys and 32 channels, or half, of the values, which is 5/8
   // or 3/4 of what one would have to take in.  us on the device of one / two / four a key head, caches taken whole: 16 heads of 72 x 1028 rows 11.3 / 10.1 /
@@ -440,7 +442,7 @@ using namespace sana;
 
 SANA_API size_t sana_hip_window_q8_workspace_bytes(int B, int H, int Hkv, int d, int window, int sinks) {
   if (B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || d <= 0 || d > 128 || window <= 0 || sinks < 0 || (int64_t)window + sinks > (1 << 30)) return 0;
-  if (step_groups(B, H, Hkv) >= WA_MAX_BLOCKS) return 0;
+  if (step_groups(B, H, Hkv) >= Q8_MAX_GROUPS) return 0;
   return part_bytes(q8_splits(B, H, Hkv, window + sinks, d), (int64_t)B * H, d);
 }
 
@@ -459,7 +461,7 @@ SANA_API int sana_hip_window_q8(const sana_window_q8_args* args, void* stream) {
   for (const int64_t sb : {q_stride_b, o_stride_b, ck_stride_b, cv_stride_b, scales_stride_b})
     if (sb < 0) return SANA_ERR_ARG;
   if (B > 1 && o_stride_b < (int64_t)H * d) return SANA_ERR_ARG;  // (entries that would write the same elements)
-  if ((int64_t)window + sinks > (1 << 30) || step_groups(B, H, Hkv) >= WA_MAX_BLOCKS) return SANA_ERR_SHAPE;
+  if ((int64_t)window + sinks > (1 << 30) || step_groups(B, H, Hkv) >= Q8_MAX_GROUPS) return SANA_ERR_SHAPE;
   if (misaligned({q, codes_k, codes_v}, {q_stride_b}) || ck_stride_b % 16 || cv_stride_b % 16 || scales_stride_b % 2 ||
       (reinterpret_cast<uintptr_t>(scales) & 7u) || (reinterpret_cast<uintptr_t>(out) & 7u) || o_stride_b % 4 || off4(positions))
     return SANA_ERR_ALIGN;
@@ -510,7 +512,7 @@ SANA_API int sana_hip_window_cache_read(const sana_cache_read_args* args, void* 
   if (!scales) {
     if (misaligned({}, {ck_stride_b, ck_stride_n, cv_stride_b, cv_stride_n})) return SANA_ERR_ALIGN;
     a.k_b = 2 * ck_stride_b, a.k_n = 2 * ck_stride_n, a.v_b = 2 * cv_stride_b, a.v_n = 2 * cv_stride_n;
-    if (held >= (WA_MAX_BLOCKS << 1) / B) return SANA_ERR_SHAPE;
+    if (B * held >= WA_MAX_BLOCKS << 1) return SANA_ERR_SHAPE;
     if (width <= 256 && B <= 65535) {
       a.rows = READ_STEPS * (64 / (int)(width / 8)), a.by_eighths = (65536 + (int)width / 8 - 1) / (int)(width / 8);
       a.items = (held + a.rows - 1) / a.rows * 2;
@@ -518,6 +520,7 @@ SANA_API int sana_hip_window_cache_read(const sana_cache_read_args* args, void* 
       return hipGetLastError() == hipSuccess ? SANA_OK : SANA_ERR_LAUNCH;
     }
     a.items = 2 * B * held;
+    if ((a.items + 3) / 4 >= WA_MAX_BLOCKS) return SANA_ERR_SHAPE;
     hipLaunchKernelGGL(read16_kernel, dim3((unsigned)((a.items + 3) / 4)), dim3(256), 0, s, a);
   } else {
     if (ck_stride_b % 16 || cv_stride_b % 16 || scales_stride_b % 2 || (reinterpret_cast<uintptr_t>(scales) & 7u)) return SANA_ERR_ALIGN;
@@ -525,7 +528,7 @@ SANA_API int sana_hip_window_cache_read(const sana_cache_read_args* args, void* 
     a.rows = READ_STEPS * (64 / (d / 8));
     a.by_eighths = (65536 + d / 8 - 1) / (d / 8);
     a.items = (held + a.rows - 1) / a.rows * 2 * Hkv;
-    if (B > 65535 || a.items >= (WA_MAX_BLOCKS << 2) / B) return SANA_ERR_SHAPE;
+    if (B > 65535 || B * a.items >= WA_MAX_BLOCKS << 2 || (a.items + 3) / 4 >= WA_MAX_BLOCKS) return SANA_ERR_SHAPE;
     const dim3 grid((unsigned)((a.items + 3) / 4), (unsigned)B);
     // Codes beyond the 32 MB of the L2s are read once and past them.  us, written and read back, kept / streamed: 24 MB 26 / 30; 34 MB 47 / 41, 56 MB 40 / 36, 98 MB
     // 116 / 118 (and in front of a chunk's attention 143 / 138).

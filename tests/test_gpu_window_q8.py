@@ -445,6 +445,26 @@ def test_calls_that_are_refused_before_any_launch():
     assert read(dt=0) == DTYPE
 
 
+def test_sizes_that_no_launch_takes_are_refused():
+    """An axis of a launch has fewer than 2^32 threads: 2^23 workgroups of 512 (a token), 2^24 of 256 (rows in order) are one too many.  (The pointers are never followed.)"""
+    lib, P, bf16, SHAPE = _lib.load(), 0x10000, _lib.DT_BF16, -2
+    codes = 20 * 16
+    for B, H, G in ((1 << 23, 1, 1), (1 << 22, 2, 2), (1 << 20, 68, 4), (1 << 4, 1 << 19, 1 << 19)):
+        args = _lib.WINDOW_Q8_ARGS.pack(P, P, P, P, P, P, 0, 0, H * 8, H * 8, G * codes, G * codes, G * 40, B, H, G, 8, 20, 0, bf16, 0.1)
+        assert lib.sana_hip_window_q8(args, None) == SHAPE, (B, H, G)
+        assert lib.sana_hip_window_q8_workspace_bytes(B, H, G, 8, 20, 0) == 0
+
+    def read(B, G, d, last, bits):
+        width, held = G * d, last + 1
+        row = width if bits == 16 else 0
+        return lib.sana_hip_window_cache_read(_lib.CACHE_READ_ARGS.pack(P, P, 0 if bits == 16 else P, P, P, P, row * held, row, row * held, row, 0, width * held, width,
+                                                                        width * held, width, B, G, d, last, 1, last, 0, bf16), None)
+
+    for bits, B, G, d, held in ((16, 1, 1, 512, (1 << 25) - 1), (16, 1, 1, 512, 1 << 25), (16, 3, 1, 512, 11184811), (16, 1, 1, 64, 1 << 25), (8, 1, 1, 128, (1 << 29) - 16),
+                                (8, 1, (1 << 15) - 1, 128, 16 * ((1 << 10) + 1)), (8, 3, 1, 128, 16 * 11184811)):
+        assert read(B, G, d, held - 1, bits) == SHAPE, (bits, B, G, d, held)
+
+
 @gpu
 def test_refusals(cuda):
     B, H, G, d, R = 2, 4, 2, 40, 30
