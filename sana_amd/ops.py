@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import functools
 import math
+import struct
 import threading
 from typing import Optional, Sequence, Tuple
 
@@ -1162,7 +1163,7 @@ def _q8_cache(cache, B: int, d: int, sinks: int, what: str) -> Tuple[int, int, T
     ck, cv, sc = cache
     shape = ck.shape
     if len(shape) != 4 or ck.dtype is not torch.int8 or cv.dtype is not torch.int8 or cv.shape != shape or sc.dtype is not torch.float32 \
-            or sc.shape != (*shape[:3], 2) or shape[0] != B or shape[3] != (d + 15) // 16 * 16:
+            or sc.shape != (*shape[:3], 2) or shape[0] != B or shape[1] < 1 or shape[3] != (d + 15) // 16 * 16:
         raise SanaHipError(f"{what}: codes int8 [{B}, kv_heads, rows, {(d + 15) // 16 * 16}] and scales fp32 [{B}, kv_heads, rows, 2] are a cache of "
                            f"heads of {d}, got {ck.dtype} {tuple(shape)}, {cv.dtype} {tuple(cv.shape)}, {sc.dtype} {tuple(sc.shape)}")
     _, G, R, width = shape
@@ -1207,6 +1208,7 @@ def _heads_checks(q, k, num_heads: int, q_weight, k_weight, freqs, what: str) ->
 
 
 _CONTIGUOUS = torch.contiguous_format
+_NO_NUMBER = (struct.error, OverflowError)    # of an argument that is missing, or beyond what its field of a call's arguments holds
 
 
 def _out_like(t: torch.Tensor, out: Optional[torch.Tensor], what: str) -> torch.Tensor:
@@ -1232,10 +1234,14 @@ def _heads(q, k, v, d, rotary, q_weight, k_weight, eps, freqs, interleaved, magn
     vp, v_rows = (0, no_rows) if v is None else (v.data_ptr(), _token_rows(v, "v"))
     qw, kw = (0, 0) if q_weight is None else (q_weight.data_ptr(), k_weight.data_ptr())
     pointers, strides = cache or ((0, 0, 0), (0, 0, 0))
-    args = _lib.HEADS_ARGS.pack(
-        qp, k.data_ptr(), vp, qo, ko, qw, kw, freqs.data_ptr() if rotary else 0, positions or 0, lengths or 0, *pointers,
-        *q_rows, *_token_rows(k, "k"), *v_rows, *qo_rows, *ko_rows, *strides,
-        B, N, H, C // d, d, rotary, 1 if interleaved else 0, window, sinks, zero_rest, _DT[k.dtype], eps, magnitude)
+    k_rows = _token_rows(k, "k")
+    try:
+        args = _lib.HEADS_ARGS.pack(
+            qp, k.data_ptr(), vp, qo, ko, qw, kw, freqs.data_ptr() if rotary else 0, positions or 0, lengths or 0, *pointers,
+            *q_rows, *k_rows, *v_rows, *qo_rows, *ko_rows, *strides,
+            B, N, H, C // d, d, rotary, 1 if interleaved else 0, window, sinks, zero_rest, _DT[k.dtype], eps, magnitude)
+    except _NO_NUMBER as e:
+        raise SanaHipError(f"no call with eps {eps}, magnitude {magnitude}, window {window} and {sinks} sinks: {e}") from None
     code = _lib.load().sana_hip_heads(args, _stream())
     if code:
         _lib.check(code, "sana_hip_heads")
@@ -1363,9 +1369,12 @@ def window_attention_q8(q: torch.Tensor, cache: Sequence[torch.Tensor], position
         raise SanaHipError(f"q and out must have unit channel stride, got strides {q.stride()} and {out.stride()}")
     nbytes = _q8_bytes(B, num_heads, G, d, window, sinks)
     ws = _call_scratch(q.device, nbytes) if nbytes else None
-    args = _lib.WINDOW_Q8_ARGS.pack(q.data_ptr(), *pointers, position_ptr, out.data_ptr(), 0 if ws is None else ws.data_ptr(), nbytes,
-                                    q.stride(0) if B > 1 else 0, out.stride(0) if B > 1 else 0, *strides, B, num_heads, G, d, window, sinks,
-                                    _DT[q.dtype], scale)
+    try:
+        args = _lib.WINDOW_Q8_ARGS.pack(q.data_ptr(), *pointers, position_ptr, out.data_ptr(), 0 if ws is None else ws.data_ptr(), nbytes,
+                                        q.stride(0) if B > 1 else 0, out.stride(0) if B > 1 else 0, *strides, B, num_heads, G, d, window, sinks,
+                                        _DT[q.dtype], scale)
+    except _NO_NUMBER as e:
+        raise SanaHipError(f"window_attention_q8: no call without positions, or with scale {scale} and a window of {window}: {e}") from None
     code = _lib.load().sana_hip_window_q8(args, _stream())
     if code:
         _lib.check(code, "sana_hip_window_q8")
@@ -1423,8 +1432,12 @@ def window_cache_read(cache: Sequence[torch.Tensor], positions: torch.Tensor, si
     k, v = out
     if B == 0:
         return k, v
-    args = _lib.CACHE_READ_ARGS.pack(*pointers, position_ptr, k.data_ptr(), v.data_ptr(), *strides, *_token_rows(k, "out"), *_token_rows(v, "out"),
-                                     B, G, width, window, sinks, last, zero_rest, _DT[dtype])
+    out_rows = (*_token_rows(k, "out"), *_token_rows(v, "out"))
+    try:
+        args = _lib.CACHE_READ_ARGS.pack(*pointers, position_ptr, k.data_ptr(), v.data_ptr(), *strides, *out_rows, B, G, width, window, sinks, last, zero_rest,
+                                         _DT[dtype])
+    except _NO_NUMBER as e:
+        raise SanaHipError(f"{what}: no call without positions, or with a window of {window} and the last {last}: {e}") from None
     code = _lib.load().sana_hip_window_cache_read(args, _stream())
     if code:
         _lib.check(code, "sana_hip_window_cache_read")

@@ -493,3 +493,25 @@ def test_refusals(cuda):
     for bad in (lambda: ops.window_cache_q8(1, 0, 1, 64), lambda: ops.window_cache_q8(1, 5, 1, 60), lambda: ops.window_cache_q8(1, 5, 1, 136), lambda: ops.window_cache_q8(1, 5, 0, 64)):
         with pytest.raises(sana_amd.SanaHipError):
             bad()
+
+
+@gpu
+def test_refusals_of_what_no_call_holds(cuda):
+    """No positions, numbers beyond 32 bits, a cache without heads: the library's own error, and nothing is written."""
+    B, H, G, d, R = 2, 4, 2, 40, 30
+    cache, pos, far = [t.cuda() for t in realistic(B, G, R, d)], i32([3, 50]), 1e39
+    q, k, v, _, _ = (t.cuda() for t in make(B, 1, H, G, d, BF16))
+    w = torch.ones(d, dtype=BF16, device="cuda")
+    f = freqs_of(40).cuda()
+    before = [t.clone() for t in cache]
+    none = [t[:, :0] for t in cache]
+    for call in (lambda: ops.window_attention_q8(q, cache, None, H), lambda: ops.window_attention_q8(q, cache, pos, H, scale=far), lambda: ops.window_attention_q8(q, none, pos, H),
+                 lambda: ops.window_cache_read(cache, None, dim=d), lambda: ops.window_cache_read(cache, None, dim=d, out=[torch.zeros(B, R, G * d, dtype=BF16, device="cuda")] * 2),
+                 lambda: ops.window_cache_read(none, pos, dim=d), lambda: ops.window_cache_read([t[..., :16].flatten(2).to(BF16) for t in cache[:2]], None),
+                 lambda: ops.window_cache_append_q8_(cache, k, v, None), lambda: ops.window_cache_append_q8_(none, k, v, pos), lambda: ops.qk_norm_rope(q, k, H, w, w, eps=far),
+                 lambda: ops.qk_norm_rope(q, k, H, freqs=f, magnitude=far), lambda: ops.qk_norm_rope(q, k, H, freqs=f, magnitude=-far),
+                 lambda: ops.qk_norm_rope_append_q8_(q, k, v, cache, None, H), lambda: ops.qk_norm_rope_append_q8_(q, k, v, cache, pos, H, w, w, far),
+                 lambda: ops.qk_norm_rope_append_q8_(q, k, v, none, pos, H)):
+        with pytest.raises(sana_amd.SanaHipError):
+            call()
+    assert all(torch.equal(a, b) for a, b in zip(cache, before))
