@@ -1,5 +1,8 @@
 """Norms and rotation of a stream's heads, and their keys and values in 8 bits, against the formulas in 64 bits."""
+import ctypes
 import math
+import os
+import re
 
 import pytest
 import torch
@@ -464,6 +467,33 @@ def test_one_pass_with_idle_streams_and_no_key_output(cuda, zero_rest, N):
     live = torch.tensor([[p >= 0 and t < n for t in range(N)] for p, n in zip(pos.tolist(), lens.tolist())], device="cuda")[..., None]
     assert torch.equal(out, torch.where(live, want, 0.0 if zero_rest else 7.0))
     assert all(torch.equal(a, b) for a, b in zip(cache, ref))
+
+
+def header_fields(name):
+    """The (type, field) pairs of a structure of include/sana_hip.h, in order."""
+    text = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "sana_hip.h")).read()
+    body = re.sub(r"/\*.*?\*/", "", re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), text, re.S).group(1), flags=re.S)
+    fields = []
+    for line in filter(None, (x.strip().replace("* ", " *") for x in body.split(";"))):
+        kind, names = re.match(r"((?:const )?\w+)\s+(.*)", line, re.S).groups()
+        for n in names.split(","):
+            n = n.strip()
+            fields.append((ctypes.c_void_p, n[1:].strip()) if n.startswith("*") else
+                          ({"size_t": ctypes.c_size_t, "int64_t": ctypes.c_int64, "int": ctypes.c_int, "float": ctypes.c_float}[kind], n))
+    return fields
+
+
+@pytest.mark.parametrize("name,layout", [("sana_heads_args", "HEADS_ARGS"), ("sana_window_q8_args", "WINDOW_Q8_ARGS"), ("sana_cache_read_args", "CACHE_READ_ARGS")])
+def test_packed_arguments_lie_as_in_the_header(name, layout):
+    """Each field in turn holds something, the others nothing: the packed bytes are those of the C structure."""
+    fields, layout = header_fields(name), getattr(_lib, layout)
+    args = type(name, (ctypes.Structure,), {"_fields_": [(n, t) for t, n in fields]})
+    assert layout.size == ctypes.sizeof(args)
+    for i, (kind, n) in enumerate(fields):
+        held = args()
+        value = 1.5 if kind is ctypes.c_float else 0x01020304
+        setattr(held, n, value)
+        assert layout.pack(*[value if j == i else 0.0 if t is ctypes.c_float else 0 for j, (t, _) in enumerate(fields)]) == bytes(held), n
 
 
 def test_no_cpu_tensors():
