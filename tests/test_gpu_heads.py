@@ -398,6 +398,55 @@ def test_long_appends_leave_out_what_does_not_stay(cuda, window, sinks, N):
     assert all(torch.equal(a, b) for a, b in zip(whole, parts))
 
 
+@gpu
+@pytest.mark.parametrize("cached", [False, True])
+def test_more_tokens_than_a_layer_of_the_grid(cuda, cached):
+    """Heads of one token a wave, 2^17 tokens of a stream a layer: bit for bit the two calls that the second layer's tokens divide it into."""
+    B, N, at, H, G, d, W, S = 2, (1 << 17) + 203, 1 << 17, (8 if cached else 16), (8 if cached else 16), 72, 700, 5
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q, k, v = (torch.randn(B, N, n * d, generator=g, device="cuda", dtype=BF16) for n in (H, G, G))
+    w = [(1 + 0.3 * torch.randn(d, generator=g, device="cuda")).to(BF16) for _ in range(2)]
+    args, positions = (*w, 1e-6, freqs_of(72).cuda()), [3, 1 << 20]
+    whole, parts = ([t.cuda() for t in filled(B, G, W + S, d)] for _ in range(2))
+
+    def call(now, positions, lengths, cache, outs):
+        if not cached:
+            return ops.qk_norm_rope(q[:, now], k[:, now], H, *args, positions=i32(positions), lengths=i32(lengths), q_out=outs[0][:, now], k_out=outs[1][:, now])
+        return ops.qk_norm_rope_append_q8_(q[:, now], k[:, now], v[:, now], cache, i32(positions), H, *args, sinks=S, lengths=i32(lengths), q_out=outs[0][:, now],
+                                           k_out=outs[1][:, now])
+
+    for lengths in ([N, at + 100], [at - 1, N], [N, at + 1]):
+        got, want = ([torch.full_like(t, 7.0) for t in (q, k)] for _ in range(2))
+        call(slice(0, N), positions, lengths, whole, got)
+        call(slice(0, at), positions, [min(n, at) for n in lengths], parts, want)
+        call(slice(at, N), [p + at for p in positions], [max(n - at, 0) for n in lengths], parts, want)
+        assert all(torch.equal(a, b) for a, b in zip(got, want)) and all(torch.equal(a, b) for a, b in zip(whole, parts))
+        assert (got[0][0, lengths[0]:] == 7).all() and (got[1][1, lengths[1]:] == 7).all()
+
+
+@gpu
+@pytest.mark.parametrize("lengths", [None, [640003, 524289]])
+def test_more_runs_of_tokens_than_a_layer_of_the_grid(cuda, lengths):
+    """Runs of tokens a wave, 2^19 tokens of a stream a layer, into the cache alone; without lengths those between the sinks and the last window are left out
+    (NaN here), and two layers of tiles are left."""
+    B, N, G, d, W, S = 2, 640003, 1, 80, 540001, 1000
+    k, v = (torch.randn(B, N, G * d, generator=torch.Generator(device="cuda").manual_seed(i), device="cuda", dtype=BF16) for i in (0, 1))
+    positions = [0, 77777]
+    whole, parts = ([t.cuda() for t in filled(B, G, W + S, d)] for _ in range(2))
+    for at in range(0, N, 100000):
+        n = min(100000, N - at)
+        ops.window_cache_append_q8_(parts, k[:, at:at + n], v[:, at:at + n], i32([p + at for p in positions]), S, i32([max(0, min(n, x - at)) for x in lengths or [N] * B]))
+    if lengths is None:
+        for b, p in enumerate(positions):
+            gone = torch.arange(N, device="cuda")
+            gone = (gone + p >= S) & (gone < N - W)
+            assert gone.sum() > 90000
+            k[b, gone], v[b, gone] = math.nan, math.nan
+    ops.window_cache_append_q8_(whole, k, v, i32(positions), S, i32(lengths))
+    # a row of NaN has the scale NaN: none is there, and all are those of the pieces
+    assert all(torch.equal(a, b) for a, b in zip(whole, parts))
+
+
 # --------------------------------------------------------------------------- refusals
 
 def test_calls_that_are_refused_before_any_launch():
