@@ -150,7 +150,7 @@ __global__ __launch_bounds__(256) void heads_kernel(const HeadArgs h) {
       c[i] = __builtin_amdgcn_cosf(turn) * a.magnitude, s[i] = __builtin_amdgcn_sinf(turn) * a.magnitude;
     }
   }
-  const int slot = !kept ? 0 : p < (uint32_t)a.sinks ? (int)p : a.sinks + (int)((p - (uint32_t)a.sinks) % (uint32_t)a.window);
+  const int slot = kept ? wa_slot(p, a.sinks, a.window) : 0;
   const int64_t head_codes = (int64_t)rows * dp;
   int8_t *codes_k = a.codes_k + b * a.ck_b + (int64_t)slot * dp, *codes_v = a.codes_v + b * a.cv_b + (int64_t)slot * dp;
   float* scales = a.scales + b * a.sc_b + 2 * (int64_t)slot;

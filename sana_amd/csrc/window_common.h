@@ -1,4 +1,5 @@
-// What the kernels over a window share (window.hip: 16-bit rows; window8.hip: a cache of 8 bits): sizes, the ring's rows, the join of parts of the keys.
+// What the kernels of a stream's window and its ring cache share (window.hip: 16-bit rows; window8.hip and heads.hip: a cache of 8 bits): arguments, the
+// ring's rows, sizes and alignment.
 #pragma once
 #include <initializer_list>
 
@@ -6,8 +7,6 @@
 
 namespace sana {
 namespace {
-
-constexpr int WA_MAX_SPLITS = 32;  // parts that the keys of a query are split into
 
 struct WindowArgs {
   const uint16_t *q, *k, *v;
@@ -19,62 +18,16 @@ struct WindowArgs {
   float scale_log2e;
 };
 
-// The parts of a query and head: weights 2^(m_s - m), sums and outputs added up in the order of the parts.  Half a wave a (query, head):
-// a lane reads the maximum and the sum of one part, then four channels of all.  A launch and two loads in a row: 3.4 us for 16 heads in 13 parts.
-template <typename T>
-__global__ __launch_bounds__(256) void window_join_kernel(const WindowArgs a) {
-  static_assert(WA_MAX_SPLITS <= 32, "");
-  const int64_t rows = (int64_t)a.B * a.N * a.H, row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (row >= rows) return;
-  const int lane = threadIdx.x & 31, c = 4 * lane;
-  const int64_t bn = row / a.H;
-  const int h = (int)(row - bn * a.H), b = (int)(bn / a.N), i = (int)(bn - (int64_t)b * a.N);
-  if ((a.lengths && i >= a.lengths[b]) || (a.positions && a.positions[b] < 0)) return;
-  f32x2_t ml = {-INFINITY, 0.f};
-  if (lane < a.splits) ml = *reinterpret_cast<const f32x2_t*>(a.part_ml + 2 * (lane * rows + row));
-  float m = ml[0];
-#pragma unroll
-  for (int x = 1; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor(m, x, 32));
-  const float mine = lane < a.splits ? __builtin_amdgcn_exp2f(ml[0] - m) : 0.f;
-  const float* from = a.part_o + row * a.d + (c < a.d ? c : 0);
-  float l = 0.f;
-  f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-  for (int s0 = 0; s0 < a.splits; s0 += 8) {
-    f32x4_t x[8];
-#pragma unroll
-    for (int s = 0; s < 8; ++s) x[s] = *reinterpret_cast<const f32x4_t*>(from + min(s0 + s, a.splits - 1) * rows * a.d);
-#pragma unroll
-    for (int s = 0; s < 8; ++s) {
-      const float f = __shfl(mine, s0 + s, 32);  // (0 behind the last part, whose values are repeated there: they may be inf)
-      l = fmaf(f, __shfl(ml[1], s0 + s, 32), l);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {  // a part whose weight is 0 in fp32 gives what is not finite all the same: its keys are seen
-        const float y = s0 + s < a.splits ? x[s][r] : 0.f;
-        o[r] = fmaf(f == 0.f && !(fabsf(y) < INFINITY) ? 1.f : f, y, o[r]);
-      }
-    }
-  }
-  const float inv = 1.0f / l;
-  if (c < a.d)
-    *reinterpret_cast<u32x2_t*>(a.out + b * a.o_b + (int64_t)i * a.o_n + h * a.d + c) =
-        u32x2_t{pk16<T>(o[0] * inv, o[1] * inv), pk16<T>(o[2] * inv, o[3] * inv)};
+// The row of the token at position p (below 2^32) in a cache of sinks + window rows.
+__device__ __forceinline__ int wa_slot(uint32_t p, int sinks, int window) {
+  return (int)(p < (uint32_t)sinks ? p : (uint32_t)sinks + (p - (uint32_t)sinks) % (uint32_t)window);
 }
-
-__device__ __forceinline__ int wa_slot(int64_t p, int sinks, int window) { return (int)(p < sinks ? p : sinks + (p - sinks) % window); }
 
 constexpr int64_t WA_MAX_BLOCKS = 1 << 24;  // of 256 threads: a launch has fewer than 2^32 threads an axis
 
 // One token: the workgroups of a whole cache, one a (stream, key head, 16 query heads).
 int64_t step_groups(int B, int H, int Hkv) { return (int64_t)B * Hkv * ((H / Hkv + 15) / 16); }
 size_t part_bytes(int splits, int64_t rows, int d) { return splits > 1 ? (size_t)splits * rows * (d + 2) * sizeof(float) : 0; }
-
-template <typename T>
-int launch_join(const WindowArgs& a, hipStream_t s) {
-  const int64_t groups = ((int64_t)a.B * a.N * a.H + 7) / 8;
-  if (groups >= WA_MAX_BLOCKS) return SANA_ERR_SHAPE;
-  hipLaunchKernelGGL(window_join_kernel<T>, dim3((unsigned)groups), dim3(256), 0, s, a);
-  return SANA_OK;
-}
 
 bool misaligned(std::initializer_list<const void*> rows, std::initializer_list<int64_t> strides) {
   for (const void* p : rows)
