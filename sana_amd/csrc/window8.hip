@@ -115,15 +115,12 @@ __global__ __launch_bounds__(64 * NW) void window_q8_kernel(const Window8Args x)
     f32x4_t sc[RT];
 #pragma unroll
     for (int kt = 0; kt < RT; ++kt) sc[kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    bool over = false, ordinary = false;  // of the values' scales
+    float sv[(ROWS + 63) / 64];  // the values' scales, 0 of a row that is not there, so that nothing of it counts
 #pragma unroll
-    for (int i = 0; i < (ROWS + 63) / 64; ++i)
-      if (64 * i + lane < ROWS) {  // (a row that is not there: a value's scale of 0, so that nothing of it counts)
-        const float sv = ROWS * t + 64 * i + lane < count ? rs[i].y : 0.f;
-        my_scales[64 * i + lane] = rs[i].x;
-        my_scales[ROWS + 64 * i + lane] = sv;
-        over |= sv > 0x1p80f, ordinary |= sv >= 0x1p-64f;
-      }
+    for (int i = 0; i < (ROWS + 63) / 64; ++i) {
+      sv[i] = 64 * i + lane < min(ROWS, count - ROWS * t) ? rs[i].y : 0.f;
+      if (64 * i + lane < ROWS) my_scales[64 * i + lane] = rs[i].x, my_scales[ROWS + 64 * i + lane] = sv[i];
+    }
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
@@ -142,7 +139,11 @@ __global__ __launch_bounds__(64 * NW) void window_q8_kernel(const Window8Args x)
     }
     if (t + NW < t1) request(t + NW);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the wave's own scales and V are there)
-    const float lift = __any(over) ? 48.f : __any(ordinary) ? 0.f : -48.f;
+    uint64_t over = 0, ordinary = 0;  // rows
+#pragma unroll
+    for (int i = 0; i < (ROWS + 63) / 64; ++i)
+      over |= __builtin_amdgcn_ballot_w64(sv[i] > 0x1p80f), ordinary |= __builtin_amdgcn_ballot_w64(sv[i] >= 0x1p-64f);
+    const float lift = over ? 48.f : ordinary ? 0.f : -48.f;
     float most = -INFINITY;
 #pragma unroll
     for (int kt = 0; kt < RT; ++kt) {
@@ -169,13 +170,13 @@ __global__ __launch_bounds__(64 * NW) void window_q8_kernel(const Window8Args x)
       u32x4_t hi, lo;
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
-        const f32x4_t sv = *reinterpret_cast<const f32x4_t*>(my_scales + ROWS + 16 * (2 * k2 + kt) + 4 * fg);
+        const f32x4_t scale = *reinterpret_cast<const f32x4_t*>(my_scales + ROWS + 16 * (2 * k2 + kt) + 4 * fg);
         float p[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           p[r] = __builtin_amdgcn_exp2f(sc[2 * k2 + kt][r] - sub);
           sum += p[r];
-          p[r] *= sv[r];
+          p[r] *= scale[r];
         }
         hi[2 * kt] = pack_bf16(p[0], p[1]), hi[2 * kt + 1] = pack_bf16(p[2], p[3]);
         lo[2 * kt] = pack_bf16(p[0] - bf16_lo(hi[2 * kt]), p[1] - bf16_hi(hi[2 * kt]));
