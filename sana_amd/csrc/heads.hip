@@ -176,8 +176,17 @@ __global__ __launch_bounds__(256) void heads_kernel(const HeadArgs h) {
         float sq = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) sq = fmaf(x[u][i], x[u][i], sq);
-        sq = over_head<LPH>(sq, [](float y, float z) { return y + z; });
-        const float r = rsqrtf(sq * h.inv_d + a.eps);  // (of subnormal numbers too, where eps is 0)
+        const auto plus = [](float y, float z) { return y + z; };
+        sq = over_head<LPH>(sq, plus);
+        float eps = a.eps;
+        if (!is_f16<T> && __any(sq == INFINITY)) {  // (heads whose squares leave fp32, from some 2^61 on: all of it 2^68 times smaller)
+          const float by = sq == INFINITY ? 0x1p-68f : 1.0f;
+          eps *= by * by, sq = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[u][i] *= by, sq = fmaf(x[u][i], x[u][i], sq);
+          sq = over_head<LPH>(sq, plus);
+        }
+        const float r = rsqrtf(sq * h.inv_d + eps);  // (of subnormal numbers too, where eps is 0)
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[u][i] = x[u][i] * r * (kind ? w[1][i] : w[0][i]);
       }

@@ -150,6 +150,25 @@ def test_rows_of_any_size_without_eps(cuda, power):
 
 
 @gpu
+@pytest.mark.parametrize("d", [8, 64, 128])
+@pytest.mark.parametrize("eps", [0.0, 1e-6, 1e38])
+@pytest.mark.parametrize("power", [60, 64, 90, 124])
+def test_rows_whose_squares_leave_32_bits(cuda, power, eps, d):
+    """bf16 heads of up to the largest numbers beside ordinary ones, of one token and of others: each by its own mean."""
+    H, G, N = 5, 3, 7
+    q, k, _, qw, kw = make(2, N, H, G, d, BF16, seed=power)
+    big = (torch.arange(N)[:, None] + torch.arange(H)) % 3 == 0
+    f = freqs_of(d)
+    q, k = (torch.where(big[:, :n, None], t.reshape(2, N, n, d).float() * 2.0 ** power, t.reshape(2, N, n, d).float()).clamp(-3.3e38, 3.3e38).flatten(2).to(BF16)
+            for t, n in ((q, H), (k, G)))
+    got = ops.qk_norm_rope(q.cuda(), k.cuda(), H, qw.cuda(), kw.cuda(), eps, f.cuda(), positions=i32([3, 70]))
+    for g, x, n, w in ((got[0], q, H, qw), (got[1], k, G, kw)):
+        want, off = definition(x, n, w, float(torch.tensor(eps)), f, True, 1.0, [3, 70])
+        assert torch.isfinite(g).all()
+        near(g, want, off)
+
+
+@gpu
 @pytest.mark.parametrize("interleaved", [True, False])
 def test_lengths_and_idle_streams(cuda, interleaved):
     """Rows without a token: zeros in new outputs, left as they were in given ones, NaN of the inputs there not looked at."""
