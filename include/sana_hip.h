@@ -575,8 +575,10 @@ int sana_hip_window_step(const void* q, const void* k, const void* v, void* cach
  *             (a, b) -> magnitude * (a cos - b sin, a sin + b cos); pairs (2i, 2i + 1) (interleaved), else (i, i + rotary / 2)
  *   cache     keys (normed and rotated) and values in 8 bits into the rows of a ring cache
  *
- * The per-head form of the q/k RMSNorm and the rotary embedding that the reference's attention classes apply one after the other
- * (diffusion/model/norms.py:182-231, diffusion/model/nets/sana_blocks.py:1572-1582).  In 32 bits, angles in 64, rounded once; into the cache from the unrounded key.
+ * For the streams of the decayed and the window attention above.  The q/k RMSNorm and the rotary embedding of the reference's attention classes
+ * (diffusion/model/norms.py:182-231, diffusion/model/nets/sana_blocks.py:1572-1582) are other functions, which this call does not replace: that norm is over
+ * all channels, in front of the heads, and that rotation by a table of angles for each token.  In 32 bits, angles in 64, rounded once; into
+ * the cache from the unrounded key.
  *   q, q_out  [B][N][H*d] views (NULL and H = 0: keys alone), k, v, k_out [B][N][Hkv*d] views, bf16 or f16, each its own strides (batch, token);
  *             q_out may be q itself and k_out k (with its strides), else they must not overlap the inputs
  *   k_out     may be NULL where there is a cache

@@ -275,7 +275,7 @@ int launch_heads(const sana_heads_args& a, hipStream_t s) {
 // 43.7 / 42.9 (48.3 / 49.6), 16 + 16 of 72 48.2 / 55.4 (54.0 / 64.1), 96 44.6 / 46.9 (52.1 / 52.8), 112 43.6 / 45.4 (48.5 / 49.3), but of 128 42.6 / 42.2
 // (42.5 / 43.3), of 16 69 / 27, and with fewer groups 16 + 4 of 72 46.9 / 46.0 (57.2 / 53.3), 4 + 4 47.5 / 33.6.  With a cache its rows of codes, which lie
 // by head, outweigh that up to 64 channels and from 112: 32 85.0 / 75.1, 48 84.1 / 78.0, 64 68.1 / 62.8, 72 80.9 / 91.0, 80 71.8 / 77.4, 96 72.7 / 75.9, 104
-// 62.1 / 65.6, 112 65.3 / 67.2 and 52.5 / 51.3, 128 47.0 / 48.6 and 60 / 56.
+// 62.1 / 65.6, 112 65.3 / 67.2 and 52.5 / 51.3 (of two sizes: 3 % either way), 128 47.0 / 48.6 and 60 / 56.
 template <typename T, int LPH>
 int heads_as(const sana_heads_args& a, hipStream_t s) {
   constexpr int AT_ONCE = 64 / LPH;

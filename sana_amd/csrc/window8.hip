@@ -36,13 +36,14 @@ __device__ __forceinline__ u32x4_t codes16(uint32_t lo, uint32_t hi) {
 // memory as the operand it is (16 channels a lane, two products), V through the wave's own LDS as bf16 to be transposed; its scale goes to the probability, and both as
 // the sum of two bf16 numbers into the product.  (bf16 for f16 too: a value's scale may be of any size.)
 // A probability is 2^(score - reference), and the reference moves only where a score is 8 above it.  It lies 48 above the scores of a tile with a value's scale over
-// 2^80, so that sums of up to 2^30 rows, of 2^8 times 127 times any scale each, stay below 2^127; 48 below those of a tile whose values' scales are all under 2^-64,
-// so that neither bf16 number is a subnormal one; weights and sums of parts are relative to their reference, whatever it is.
-// Every compute unit busy, memory bounds it: 64 streams x 8196 rows x 8 key heads of 128, 1.06 GB 164 us = 6.4 TB/s, reads alone (179 with loads that stay in the
-// caches; 4, 6, 12 waves 169, 175, 173; 64 rows a wave 185).  One stream of 131136 rows 277 MB in 32 parts 49 us with the join (25 parts 55, 48 parts 60: a part
-// a compute unit).  A short cache is what one compute unit takes in, 37 bytes a ns at most whatever is asked for (two tiles ahead no faster) behind
-// 6 us of launch, first loads and the waves' sum, so the values' channels go to several: 16 key heads of 72 x 1028 rows 11.3 us whole, 9.0 by three.  Products of
-// 8-bit numbers in the place of the conversions (q in three slices): 4 % less for a cache that one compute unit takes, nothing elsewhere.
+// 2^80, so that sums of up to 2^30 rows, of 2^-40 times 127 times any scale each, stay below 2^127; 48 below those of a tile whose values' scales are all under
+// 2^-64, so that neither bf16 number is a subnormal one.  Sums of waves and of parts are relative to their reference, whatever it is.
+// Every compute unit busy, memory bounds it: 64 streams x 8196 rows x 8 key heads of 128, 1.05 GB 166 us = 6.3 TB/s, reads alone (179 with loads that stay in
+// the caches; 4, 6, 12 waves 169, 175, 173; 64 rows a wave 185).  One stream of 131136 rows, 277 MB in 32 parts: 48 - 49 us a call in a long run over rotating
+// caches, 45 - 48 of them this kernel = 6 TB/s (25 parts 55, 48 parts 60: a part a compute unit), but 61 over the first milliseconds of a run, 56 of them this one.
+// A short cache is what one compute unit takes in, 37 bytes a ns at most whatever is asked for (two tiles ahead no faster) behind 6 us of launch, first loads and
+// the waves' sum, so the values' channels go to several: 16 key heads of 72 x 1028 rows 11.3 us whole, 9.0 by three.  Products of 8-bit numbers in the place of
+// the conversions (q in three slices): 4 % less for a cache that one compute unit takes, nothing elsewhere.
 template <typename T, int P, int VP, int NW, int RT>
 __global__ __launch_bounds__(64 * NW) void window_q8_kernel(const Window8Args x) {
   const WindowArgs& a = x.w;
